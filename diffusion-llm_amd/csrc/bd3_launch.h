@@ -148,6 +148,63 @@ struct GlueArgs {
   int row0;                   // first row of the launch (rows: the one past its last)
 };
 
+constexpr int kPagedMaxKeys = 1 << 30;  // of a sequence: key positions stay below 2^31 when rounded up to a block
+struct PagedArgs {
+  const uint16_t* q;        // (tokens, heads, 64)
+  const uint16_t* k;        // (pages, kv_heads, page, 64)
+  const uint16_t* v;
+  uint16_t* o;              // (tokens, heads, 64)
+  const int32_t* table;     // (seqs, width) page numbers
+  const int32_t* q_starts;  // (seqs + 1)
+  const int32_t* kv_lens;   // (seqs)
+  float* part_o;            // (seqs * kv_heads, q_slots, n_splits, 32, 64) fp32, or null
+  float* part_lse;          // (seqs * kv_heads, q_slots, n_splits, 32) log2 LSE, or null
+  int64_t sq_t, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, so_t, so_h, table_s;  // element strides
+  int seqs, tokens, kv_heads, group, pages, page, page_shift;
+  int max_kv;     // most keys of a sequence: the caller's bound, at most the table's
+  int bs;
+  int tile;       // query rows per workgroup
+  int q_tiles;    // tiles of the longest chunk
+  int q_slots;    // its 32-row partial slots
+  int n_splits;   // most key ranges of a tile
+  int split_len;  // most keys of a range
+  int unit;       // ranges are whole units of keys
+  float scale_log2;
+};
+
+struct PagedRopeArgs {
+  const uint16_t* qkv;  // (tokens, (heads + 2 kv_heads) * 64), last stride 1
+  const float* sin_t;   // (max_pos, 32) fp32
+  const float* cos_t;
+  uint16_t* q;          // (tokens, heads, 64)
+  uint16_t* k;          // (pages, kv_heads, page, 64)
+  uint16_t* v;
+  const int32_t* table;
+  const int32_t* q_starts;
+  const int32_t* kv_lens;
+  int64_t sx_t, sq_t, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, table_s;
+  int seqs, tokens, heads, kv_heads, pages, page, page_shift, width, max_pos;
+  int64_t total;  // tokens * (heads + 2 kv_heads) * 4 work items (< 2^31)
+};
+
+constexpr int kLogitSlice = 2048;  // tokens of the vocabulary per workgroup of adjust_logits
+struct LogitArgs {
+  const void* logits;       // (batch, rows, vocab), fp32 or bf16
+  void* out;
+  const int64_t* tokens;    // (batch, history) or null
+  const int32_t* lengths;   // (batch) or null: all of the history
+  const float* repetition_p;  // (batch) each, or null: the scalar
+  const float* frequency_p;
+  const float* presence_p;
+  const float* bias;        // (vocab) or (batch, vocab), or null
+  const int32_t* allowed;   // bits, (words), (batch, words) or (batch, rows, words), or null
+  int64_t in_b, in_r, out_b, out_r, tokens_s, bias_s, allowed_b, allowed_r;  // element strides
+  int fp32;
+  int batch, rows, vocab, history;
+  float repetition, frequency, presence, fill;
+  int slices, row_parts, part_rows;  // workgroups: vocabulary slices x parts of a sequence's rows x batch
+};
+
 // Launch shape of the kernels that walk rows (ln_modulate, the fused one), for
 // each launch of `rows` rows (the last may have fewer).
 struct GlueGrid {
@@ -166,6 +223,9 @@ hipError_t launch_prefill(const DecodeArgs& a, hipStream_t stream);
 hipError_t launch_qkv_rope(const QkvRopeArgs& a, hipStream_t stream);
 hipError_t launch_kv_write(const KvWriteArgs& a, hipStream_t stream);
 hipError_t launch_subs_sample(const SubsArgs& a, hipStream_t stream);
+hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream);
+hipError_t launch_paged_rope(const PagedRopeArgs& a, hipStream_t stream);
+hipError_t launch_adjust_logits(const LogitArgs& a, hipStream_t stream);
 hipError_t launch_ln_modulate(const GlueArgs& a, hipStream_t stream);
 hipError_t launch_gate_residual_ln_modulate(const GlueArgs& a, hipStream_t stream);
 hipError_t launch_gate_residual(const GlueArgs& a, hipStream_t stream);

@@ -844,6 +844,273 @@ int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t
 
 namespace {
 
+// What every paged call checks of its pool, table and batch.
+int check_paged(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                int32_t page_size, int32_t table_width, const int32_t* table, const int32_t* q_starts,
+                const int32_t* kv_lens, const int64_t* strides) {
+  if (seqs < 0 || tokens < 0) return fail(BD3_EINVAL, "seqs and tokens must be >= 0");
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0)
+    return fail(BD3_EINVAL, "heads (%d) must be a positive multiple of kv_heads (%d)", heads, kv_heads);
+  if (head_dim != bd3::kHeadDim) return fail(BD3_EINVAL, "head_dim must be 64, got %d", head_dim);
+  if (pages < 1 || table_width < 1) return fail(BD3_EINVAL, "need at least one page and one table entry a sequence");
+  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0)
+    return fail(BD3_EINVAL, "page_size must be a power of two in [16, 1024], got %d", page_size);
+  if ((int64_t)table_width * page_size > bd3::kPagedMaxKeys)
+    return fail(BD3_EINVAL, "a sequence's table must cover at most 2^30 keys");
+  if (strides == nullptr) return fail(BD3_EINVAL, "strides is NULL");
+  if (seqs > 0 && (table == nullptr || q_starts == nullptr || kv_lens == nullptr))
+    return fail(BD3_EINVAL, "page_table, q_starts and kv_lens must be non-NULL");
+  return BD3_OK;
+}
+
+// The token and page tensors: 16-byte rows.
+int check_rows(const void* p, const int64_t* st, int n, const char* name) {
+  if (p == nullptr || !aligned16(p)) return fail(BD3_EINVAL, "%s must be a 16-byte aligned device pointer", name);
+  for (int i = 0; i < n; ++i)
+    if (st[i] % 8 != 0 || st[i] < 0)
+      return fail(BD3_EINVAL, "%s stride[%d]=%lld must be a non-negative multiple of 8", name, i, (long long)st[i]);
+  return BD3_OK;
+}
+
+int log2_of(int32_t x) {
+  int s = 0;
+  while ((1 << s) < x) ++s;
+  return s;
+}
+
+// What a paged attention call runs: rows per workgroup, tiles and partial slots
+// of the longest chunk, key ranges.
+struct PagedPlan {
+  int tile, q_tiles, q_slots, n_splits, split_len, unit;
+};
+
+PagedPlan paged_plan(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
+                     int64_t total_kv) {
+  PagedPlan p;
+  const int64_t rows = (int64_t)max_q * (heads / kv_heads);
+  p.tile = 32;
+  p.unit = 32;
+  p.q_tiles = (int)((rows + p.tile - 1) / p.tile);
+  p.q_slots = (int)((rows + 31) / 32);
+  const int64_t work = std::min(total_kv, (int64_t)seqs * max_kv) * kv_heads * p.q_tiles;
+  int64_t len = std::max<int64_t>(256, work / 512);
+  len = std::max<int64_t>(len, (max_kv + 63) / 64);
+  len = (len + p.unit - 1) / p.unit * p.unit;
+  p.n_splits = (int)std::max<int64_t>(1, (max_kv + len - 1) / len);
+  p.split_len = (int)std::min<int64_t>(len, INT32_MAX);
+  return p;
+}
+
+size_t paged_part_rows(const PagedPlan& p, int32_t seqs, int32_t kv_heads) {
+  return p.n_splits > 1 ? (size_t)seqs * kv_heads * p.q_slots * p.n_splits * 32 : 0;
+}
+
+bool paged_bounds_ok(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv, int64_t total_kv) {
+  return seqs >= 1 && kv_heads >= 1 && heads >= kv_heads && max_q >= 1 && max_kv >= 1 &&
+         max_kv <= bd3::kPagedMaxKeys && total_kv >= 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
+                                      int64_t total_kv) {
+  if (!paged_bounds_ok(seqs, heads, kv_heads, max_q, max_kv, total_kv)) return 0;
+  const size_t rows = paged_part_rows(paged_plan(seqs, heads, kv_heads, max_q, max_kv, total_kv), seqs, kv_heads);
+  return rows == 0 ? 0 : align256(rows * bd3::kHeadDim * 4) + rows * 4;
+}
+
+int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
+                   const int32_t* q_starts, const int32_t* kv_lens, int32_t seqs, int32_t tokens, int32_t heads,
+                   int32_t kv_heads, int32_t head_dim, int32_t pages, int32_t page_size, int32_t table_width,
+                   int32_t max_q, int32_t max_kv, int64_t total_kv, int32_t block_size, const int64_t* strides,
+                   float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int st = check_paged(seqs, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, page_table,
+                           q_starts, kv_lens, strides))
+    return st;
+  if (block_size < 1) return fail(BD3_EINVAL, "block_size must be >= 1");
+  if (max_q < 0 || max_kv < 0 || total_kv < 0) return fail(BD3_EINVAL, "max_q, max_kv and total_kv must be >= 0");
+  if (max_kv > (int64_t)table_width * page_size)
+    return fail(BD3_EINVAL, "max_kv (%d) exceeds the page table's %lld keys a sequence", max_kv,
+                (long long)table_width * page_size);
+  if (int st = check_scale(scale)) return st;
+  if (seqs == 0 || tokens == 0 || max_q == 0) return BD3_OK;
+  if (max_kv == 0) max_kv = 1;  // chunks without keys: their rows are 0
+  max_q = std::min(max_q, tokens);
+  if (int st = check_rows(q, strides, 2, "q")) return st;
+  if (int st = check_rows(k_pages, strides + 2, 3, "k_pages")) return st;
+  if (int st = check_rows(v_pages, strides + 5, 3, "v_pages")) return st;
+  if (int st = check_rows(o, strides + 8, 2, "o")) return st;
+  // a tile's rows are addressed by 32-bit byte offsets from a page slot
+  if (strides[4] >= kMaxDmaSeqStride || strides[7] >= kMaxDmaSeqStride)
+    return fail(BD3_EINVAL, "page slot strides must be < 2^24 elements");
+  if (strides[10] < 0) return fail(BD3_EINVAL, "page_table stride must be >= 0");
+  const PagedPlan plan = paged_plan(seqs, heads, kv_heads, max_q, max_kv, total_kv);
+  const size_t rows = paged_part_rows(plan, seqs, kv_heads);
+  const size_t po_bytes = align256(rows * bd3::kHeadDim * 4);
+  const size_t need = rows == 0 ? 0 : po_bytes + rows * 4;
+  if (workspace_bytes < need) return fail(BD3_EINVAL, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace)))
+    return fail(BD3_EINVAL, "workspace must be a 16-byte aligned device pointer");
+  if ((int64_t)seqs * kv_heads * std::max((int64_t)plan.q_tiles * plan.n_splits, (int64_t)plan.q_slots) >=
+      ((int64_t)1 << 22))
+    return fail(BD3_EINVAL, "seqs * kv_heads * tiles * ranges too large (limit 2^22 workgroups)");
+  bd3::PagedArgs a = {};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k_pages);
+  a.v = static_cast<const uint16_t*>(v_pages);
+  a.o = static_cast<uint16_t*>(o);
+  a.table = page_table;
+  a.q_starts = q_starts;
+  a.kv_lens = kv_lens;
+  if (need > 0) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + po_bytes);
+  }
+  a.sq_t = strides[0];
+  a.sq_h = strides[1];
+  a.sk_p = strides[2];
+  a.sk_h = strides[3];
+  a.sk_s = strides[4];
+  a.sv_p = strides[5];
+  a.sv_h = strides[6];
+  a.sv_s = strides[7];
+  a.so_t = strides[8];
+  a.so_h = strides[9];
+  a.table_s = strides[10];
+  a.seqs = seqs;
+  a.tokens = tokens;
+  a.kv_heads = kv_heads;
+  a.group = heads / kv_heads;
+  a.pages = pages;
+  a.page = page_size;
+  a.page_shift = log2_of(page_size);
+  a.max_kv = max_kv;
+  a.bs = std::min(block_size, bd3::kPagedMaxKeys);  // as good as any larger one
+  a.tile = plan.tile;
+  a.q_tiles = plan.q_tiles;
+  a.q_slots = plan.q_slots;
+  a.n_splits = plan.n_splits;
+  a.split_len = plan.split_len;
+  a.unit = plan.unit;
+  a.scale_log2 = scale * bd3::kLog2e;
+  return hip_status(bd3::launch_paged_attn(a, static_cast<hipStream_t>(stream)), "paged_attn launch");
+}
+
+int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos_table, int32_t max_pos, void* q_out,
+                       void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* q_starts,
+                       const int32_t* kv_lens, int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads,
+                       int32_t head_dim, int32_t pages, int32_t page_size, int32_t table_width,
+                       const int64_t* strides, void* stream) {
+  if (int st = check_paged(seqs, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, page_table,
+                           q_starts, kv_lens, strides))
+    return st;
+  if (max_pos < 1) return fail(BD3_EINVAL, "max_pos must be >= 1");
+  if (seqs == 0 || tokens == 0) return BD3_OK;
+  if (sin_table == nullptr || cos_table == nullptr || !aligned16(sin_table) || !aligned16(cos_table))
+    return fail(BD3_EINVAL, "sin_table and cos_table must be 16-byte aligned device pointers");
+  if (int st = check_rows(qkv, strides, 1, "qkv")) return st;
+  if (int st = check_rows(q_out, strides + 1, 2, "q_out")) return st;
+  if (int st = check_rows(k_pages, strides + 3, 3, "k_pages")) return st;
+  if (int st = check_rows(v_pages, strides + 6, 3, "v_pages")) return st;
+  if (strides[9] < 0) return fail(BD3_EINVAL, "page_table stride must be >= 0");
+  bd3::PagedRopeArgs a = {};
+  a.qkv = static_cast<const uint16_t*>(qkv);
+  a.sin_t = sin_table;
+  a.cos_t = cos_table;
+  a.q = static_cast<uint16_t*>(q_out);
+  a.k = static_cast<uint16_t*>(k_pages);
+  a.v = static_cast<uint16_t*>(v_pages);
+  a.table = page_table;
+  a.q_starts = q_starts;
+  a.kv_lens = kv_lens;
+  a.sx_t = strides[0];
+  a.sq_t = strides[1];
+  a.sq_h = strides[2];
+  a.sk_p = strides[3];
+  a.sk_h = strides[4];
+  a.sk_s = strides[5];
+  a.sv_p = strides[6];
+  a.sv_h = strides[7];
+  a.sv_s = strides[8];
+  a.table_s = strides[9];
+  a.seqs = seqs;
+  a.tokens = tokens;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.pages = pages;
+  a.page = page_size;
+  a.page_shift = log2_of(page_size);
+  a.width = table_width;
+  a.max_pos = max_pos;
+  a.total = (int64_t)tokens * (heads + 2 * (int64_t)kv_heads) * 4;
+  if (a.total >= ((int64_t)1 << 31))
+    return fail(BD3_EINVAL, "tokens * heads too large (%lld work items, limit 2^31)", (long long)a.total);
+  return hip_status(bd3::launch_paged_rope(a, static_cast<hipStream_t>(stream)), "paged_qkv_rope launch");
+}
+
+int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_t batch, int32_t rows, int32_t vocab,
+                      const int64_t* tokens, int32_t history, const int32_t* lengths, const float* penalties,
+                      const float* repetition, const float* frequency, const float* presence, const float* bias,
+                      const int32_t* allowed, float fill, const int64_t* strides, void* stream) {
+  if (batch < 0 || rows < 0 || history < 0) return fail(BD3_EINVAL, "batch, rows and history must be >= 0");
+  if (vocab < 1) return fail(BD3_EINVAL, "vocab must be >= 1, got %d", vocab);
+  if (logits_fp32 != 0 && logits_fp32 != 1) return fail(BD3_EINVAL, "logits_fp32 must be 0 (bf16) or 1 (fp32)");
+  if (strides == nullptr || penalties == nullptr) return fail(BD3_EINVAL, "strides and penalties must be non-NULL");
+  for (int i = 0; i < 8; ++i)
+    if (strides[i] < 0) return fail(BD3_EINVAL, "stride[%d]=%lld must be >= 0", i, (long long)strides[i]);
+  if (!std::isfinite(penalties[0]) || !(penalties[0] > 0.f))
+    return fail(BD3_EINVAL, "repetition must be finite and > 0, got %g", (double)penalties[0]);
+  if (!std::isfinite(penalties[1]) || !std::isfinite(penalties[2]))
+    return fail(BD3_EINVAL, "frequency and presence must be finite");
+  if (!std::isfinite(fill)) return fail(BD3_EINVAL, "fill must be finite");
+  if (batch == 0 || rows == 0) return BD3_OK;
+  if (logits == nullptr || out == nullptr) return fail(BD3_EINVAL, "logits and out must be non-NULL");
+  const int el = logits_fp32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) % el != 0)
+    return fail(BD3_EINVAL, "logits and out must be aligned to their elements");
+  if (tokens != nullptr && reinterpret_cast<uintptr_t>(tokens) % 8 != 0)
+    return fail(BD3_EINVAL, "tokens must be aligned to 8 bytes");
+  bd3::LogitArgs a = {};
+  a.logits = logits;
+  a.out = out;
+  a.tokens = history > 0 ? tokens : nullptr;
+  a.lengths = lengths;
+  a.repetition_p = repetition;
+  a.frequency_p = frequency;
+  a.presence_p = presence;
+  a.bias = bias;
+  a.allowed = allowed;
+  a.in_b = strides[0];
+  a.in_r = strides[1];
+  a.out_b = strides[2];
+  a.out_r = strides[3];
+  a.tokens_s = strides[4];
+  a.bias_s = strides[5];
+  a.allowed_b = strides[6];
+  a.allowed_r = strides[7];
+  a.fp32 = logits_fp32;
+  a.batch = batch;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.history = history;
+  a.repetition = penalties[0];
+  a.frequency = penalties[1];
+  a.presence = penalties[2];
+  a.fill = fill;
+  a.slices = (vocab + bd3::kLogitSlice - 1) / bd3::kLogitSlice;
+  a.part_rows = rows;
+  a.row_parts = 1;
+  if ((int64_t)a.slices * a.row_parts * batch >= ((int64_t)1 << 23))
+    return fail(BD3_EINVAL, "batch * vocab too large (limit 2^23 workgroups)");
+  return hip_status(bd3::launch_adjust_logits(a, static_cast<hipStream_t>(stream)), "adjust_logits launch");
+}
+
+}  // extern "C"
+
+namespace {
+
 // Slices a row of the sampling scan may be cut into (1: one workgroup per
 // row): each takes at least 2048 of the row's elements (one pair per thread),
 // and 16 of them put 16 rows on every CU (8, 16 and 24 take 12.5, 12.3 and 14.9

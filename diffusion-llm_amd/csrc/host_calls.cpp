@@ -51,6 +51,10 @@ struct Library {
   decltype(&bd3_qkv_rope) qkv_rope;
   decltype(&bd3_subs_sample_ws) subs_sample_ws;
   decltype(&bd3_subs_sample_workspace_bytes) subs_sample_workspace_bytes;
+  decltype(&bd3_paged_attn_workspace_bytes) paged_attn_workspace_bytes;
+  decltype(&bd3_paged_attn) paged_attn;
+  decltype(&bd3_paged_qkv_rope) paged_qkv_rope;
+  decltype(&bd3_adjust_logits) adjust_logits;
   decltype(&bd3_ln_modulate) ln_modulate;
   decltype(&bd3_gate_residual) gate_residual;
   decltype(&bd3_gate_residual_ln_modulate) gate_residual_ln_modulate;
@@ -356,6 +360,207 @@ int32_t is_f32(const Tensor& t) {
   throw Refused{PyExc_KeyError, std::string("bf16 or fp32 tensors only, got ") + c10::toString(t.scalar_type())};
 }
 
+// The tensors that describe a ragged batch and its pool, checked (the kernels take
+// their addresses and sizes as they are).
+struct PagedBatch {
+  Tensor k, v, table, starts, lens;
+  int32_t seqs, pages, kv_heads, page, width;
+  PagedBatch(Args& a) : k(a.tensor()), v(a.tensor()), table(a.tensor()), starts(a.tensor()), lens(a.tensor()) {}
+  void check(const Tensor& first, int64_t heads) {
+    on_one_gpu(first, k, v, table, starts, lens);
+    require(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16, "bf16 inputs only");
+    require(k.dim() == 4 && k.sizes() == v.sizes() && k.size(3) == kHeadDim,
+            "k_pages and v_pages must be (pages, kv_heads, page_size, 64)");
+    require(vec_ready(k) && vec_ready(v), "k_pages and v_pages must have 16-byte aligned rows (they are not copied)");
+    require(k.size(1) >= 1 && heads % k.size(1) == 0, "heads must be a multiple of k_pages' kv_heads");
+    require(table.scalar_type() == at::kInt && starts.scalar_type() == at::kInt && lens.scalar_type() == at::kInt,
+            "page_table, q_starts and kv_lens must be int32");
+    require(table.dim() == 2 && (table.size(1) == 1 || table.stride(1) == 1),
+            "page_table must be (seqs, width) with last stride 1");
+    require(starts.dim() == 1 && lens.dim() == 1 && starts.size(0) == table.size(0) + 1 &&
+                lens.size(0) == table.size(0) && starts.is_contiguous() && lens.is_contiguous(),
+            "q_starts must be (seqs + 1) and kv_lens (seqs), contiguous");
+    require(table.size(0) <= INT32_MAX - 1 && table.size(1) <= INT32_MAX && k.size(0) <= INT32_MAX,
+            "batch or pool too large");
+    seqs = dim32(table, 0);
+    width = dim32(table, 1);
+    pages = dim32(k, 0);
+    kv_heads = dim32(k, 1);
+    page = k.size(2) <= INT32_MAX ? dim32(k, 2) : 0;
+  }
+  const int32_t* table_p() const { return static_cast<const int32_t*>(ptr(table)); }
+  const int32_t* starts_p() const { return static_cast<const int32_t*>(ptr(starts)); }
+  const int32_t* lens_p() const { return static_cast<const int32_t*>(ptr(lens)); }
+};
+
+// (tokens, heads, 64) result: the caller's, or a new one.
+Tensor token_rows(const Tensor& out, int64_t tokens, int64_t heads, const Tensor& like) {
+  if (!out.defined()) return at::empty({tokens, heads, kHeadDim}, like.options());
+  require(out.dim() == 3 && out.size(0) == tokens && out.size(1) == heads && out.size(2) == kHeadDim &&
+              out.scalar_type() == at::kBFloat16 && out.device() == like.device() && vec_ready(out),
+          "out must be a (tokens, heads, 64) bf16 tensor with 16-byte aligned rows");
+  return out;
+}
+
+// paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv, total_kv,
+// out or None) -> O; max_kv, total_kv < 0: the table's, seqs * max_kv
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] {
+    Args a(args, n, 11);
+    Tensor q = a.tensor();
+    PagedBatch b(a);
+    const int32_t bs = a.int32(), max_q = a.int32();
+    int32_t max_kv = a.int32();
+    int64_t total = a.integer();
+    Tensor out = a.maybe_tensor();
+    require(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(2) == kHeadDim,
+            "q must be a (tokens, heads, 64) bf16 tensor");
+    require(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX, "q is too large");
+    b.check(q, q.size(1));
+    {
+      NoGil nogil;
+      const c10::DeviceGuard device(q.device());
+      q = ready(q);
+      const int32_t T = dim32(q, 0), H = dim32(q, 1);
+      out = token_rows(out, T, H, q);
+      if (max_kv < 0) max_kv = (int32_t)std::min<int64_t>((int64_t)b.width * b.page, INT32_MAX);
+      if (total < 0) total = (int64_t)b.seqs * max_kv;
+      const int32_t mq = std::min(max_q, T);
+      const size_t bytes = g_lib.paged_attn_workspace_bytes(b.seqs, H, b.kv_heads, mq, std::max(max_kv, 1), total);
+      const Tensor ws = bytes ? workspace(bytes, q) : Tensor();
+      const int64_t st[11] = {q.stride(0),   q.stride(1),   b.k.stride(0),   b.k.stride(1),   b.k.stride(2), b.v.stride(0),
+                              b.v.stride(1), b.v.stride(2), out.stride(0), out.stride(1), b.table.stride(0)};
+      check(g_lib.paged_attn(ptr(q), ptr(b.k), ptr(b.v), ptr(out), b.table_p(), b.starts_p(), b.lens_p(), b.seqs, T, H,
+                             b.kv_heads, kHeadDim, b.pages, b.page, b.width, max_q, max_kv, total, bs, st, kScale,
+                             ptr(ws), bytes, stream_of(q)));
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// paged_attention_inputs(qkv, heads, sin, cos, k_pages, v_pages, page_table, q_starts, kv_lens, out or None) -> q
+PyObject* paged_attention_inputs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] {
+    Args a(args, n, 10);
+    Tensor qkv = a.tensor();
+    const int32_t heads = a.int32();
+    Tensor sin = a.tensor(), cos = a.tensor();
+    PagedBatch b(a);
+    Tensor out = a.maybe_tensor();
+    require(qkv.dim() == 2 && qkv.scalar_type() == at::kBFloat16, "qkv must be a (tokens, width) bf16 tensor");
+    require(heads >= 1, "n_heads must be >= 1");
+    b.check(qkv, heads);
+    on_one_gpu(qkv, sin, cos);
+    require(qkv.size(1) == ((int64_t)heads + 2 * (int64_t)b.kv_heads) * kHeadDim,
+            "projection width must be (n_heads + 2 * kv_heads) * 64");
+    require(qkv.size(0) <= INT32_MAX, "qkv is too large");
+    require(sin.dim() == 2 && sin.sizes() == cos.sizes() && sin.size(1) == kHeadDim / 2 &&
+                sin.scalar_type() == at::kFloat && cos.scalar_type() == at::kFloat && sin.size(0) <= INT32_MAX,
+            "RoPE tables must be (max_seq_len, 32) float32");
+    {
+      NoGil nogil;
+      const c10::DeviceGuard device(qkv.device());
+      qkv = ready(qkv);
+      sin = ready(sin.contiguous());
+      cos = ready(cos.contiguous());
+      out = token_rows(out, qkv.size(0), heads, qkv);
+      const int64_t st[10] = {qkv.stride(0), out.stride(0), out.stride(1), b.k.stride(0), b.k.stride(1), b.k.stride(2),
+                              b.v.stride(0), b.v.stride(1), b.v.stride(2), b.table.stride(0)};
+      check(g_lib.paged_qkv_rope(ptr(qkv), static_cast<const float*>(ptr(sin)), static_cast<const float*>(ptr(cos)),
+                                 dim32(sin, 0), ptr(out), ptr(b.k), ptr(b.v), b.table_p(), b.starts_p(), b.lens_p(),
+                                 b.seqs, dim32(qkv, 0), heads, b.kv_heads, kHeadDim, b.pages, b.page, b.width, st,
+                                 stream_of(qkv)));
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// A penalty: one number, or a (batch) float32 tensor.
+struct Penalty {
+  float one;
+  Tensor each;
+  Penalty(Args& a, float neutral) : one(neutral) {
+    if (THPVariable_Check(a.a[a.at]))
+      each = a.tensor();
+    else
+      one = (float)a.real();
+  }
+  const float* p() const { return static_cast<const float*>(ptr(each)); }
+};
+
+// adjust_logits(logits (batch, rows, vocab), tokens or None, lengths or None, repetition, frequency, presence, bias or
+// None, allowed or None, fill, out or None) -> out
+PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] {
+    Args a(args, n, 10);
+    Tensor x = a.tensor(), tokens = a.maybe_tensor(), lengths = a.maybe_tensor();
+    Penalty rep(a, 1.f), freq(a, 0.f), pres(a, 0.f);
+    Tensor bias = a.maybe_tensor(), allowed = a.maybe_tensor();
+    const double fill = a.real();
+    Tensor out = a.maybe_tensor();
+    on_one_gpu(x, tokens, lengths, rep.each, freq.each, pres.each, bias, allowed, out);
+    require(x.dim() == 3, "logits must be (batch, rows, vocab)");
+    const int64_t B = x.size(0), R = x.size(1), V = x.size(2);
+    require(B <= INT32_MAX && R <= INT32_MAX && V <= INT32_MAX && V >= 1, "logits are too large");
+    const int32_t fp32 = is_f32(x);
+    int64_t history = 0;
+    if (tokens.defined()) {
+      require(tokens.dim() == 2 && tokens.size(0) == B && tokens.scalar_type() == at::kLong,
+              "tokens must be (batch, history) int64");
+      history = tokens.size(1);
+      require(history <= INT32_MAX, "the history is too long");
+    }
+    if (lengths.defined())
+      require(tokens.defined() && lengths.dim() == 1 && lengths.size(0) == B && lengths.scalar_type() == at::kInt,
+              "lengths must be (batch) int32, with tokens");
+    for (Penalty* p : {&rep, &freq, &pres})
+      if (p->each.defined())
+        require(p->each.dim() == 1 && p->each.size(0) == B && p->each.scalar_type() == at::kFloat,
+                "a penalty must be a number or a (batch) float32 tensor");
+    if (bias.defined())
+      require(bias.scalar_type() == at::kFloat && bias.size(-1) == V && bias.dim() <= 2 &&
+                  (bias.dim() == 1 || bias.size(0) == B),
+              "bias must be (vocab) or (batch, vocab) float32");
+    if (allowed.defined())
+      require(allowed.scalar_type() == at::kInt && allowed.dim() >= 1 && allowed.dim() <= 3 &&
+                  allowed.size(-1) == (V + 31) / 32 && (allowed.dim() == 1 || allowed.size(0) == B) &&
+                  (allowed.dim() < 3 || allowed.size(1) == R),
+              "allowed must be int32 words, (ceil(vocab / 32)) for all, each sequence or each row");
+    {
+      NoGil nogil;
+      const c10::DeviceGuard device(x.device());
+      if (x.stride(2) != 1 && V > 1) x = x.contiguous();
+      auto rows = [](Tensor& t) {
+        if (t.defined() && t.dim() > 0 && t.stride(-1) != 1) t = t.contiguous();
+      };
+      rows(tokens);
+      rows(bias);
+      rows(allowed);
+      if (lengths.defined()) lengths = lengths.contiguous();
+      for (Penalty* p : {&rep, &freq, &pres})
+        if (p->each.defined()) p->each = p->each.contiguous();
+      if (!out.defined()) out = at::empty({B, R, V}, x.options());
+      require(out.scalar_type() == x.scalar_type() && out.sizes() == x.sizes() && (V == 1 || out.stride(2) == 1),
+              "out must have the logits' shape and dtype, with last stride 1");
+      const float penalties[3] = {rep.one, freq.one, pres.one};
+      const int64_t st[8] = {x.stride(0),
+                             x.stride(1),
+                             out.stride(0),
+                             out.stride(1),
+                             tokens.defined() ? tokens.stride(0) : 0,
+                             bias.defined() && bias.dim() == 2 ? bias.stride(0) : 0,
+                             allowed.defined() && allowed.dim() > 1 ? allowed.stride(0) : 0,
+                             allowed.defined() && allowed.dim() > 2 ? allowed.stride(1) : 0};
+      check(g_lib.adjust_logits(ptr(x), fp32, ptr(out), (int32_t)B, (int32_t)R, (int32_t)V,
+                                static_cast<const int64_t*>(ptr(tokens)), (int32_t)history,
+                                static_cast<const int32_t*>(ptr(lengths)), penalties, rep.p(), freq.p(), pres.p(),
+                                static_cast<const float*>(ptr(bias)), static_cast<const int32_t*>(ptr(allowed)),
+                                (float)fill, st, stream_of(x)));
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
 // A (batch, d) or (batch, 1, d) modulation vector as (batch, d).
 Tensor vec(Tensor t) {
   if (t.dim() == 3) {
@@ -488,6 +693,10 @@ PyObject* bind(PyObject*, PyObject* dict) {
     set("bd3_qkv_rope", l.qkv_rope);
     set("bd3_subs_sample_ws", l.subs_sample_ws);
     set("bd3_subs_sample_workspace_bytes", l.subs_sample_workspace_bytes);
+    set("bd3_paged_attn_workspace_bytes", l.paged_attn_workspace_bytes);
+    set("bd3_paged_attn", l.paged_attn);
+    set("bd3_paged_qkv_rope", l.paged_qkv_rope);
+    set("bd3_adjust_logits", l.adjust_logits);
     set("bd3_ln_modulate", l.ln_modulate);
     set("bd3_gate_residual", l.gate_residual);
     set("bd3_gate_residual_ln_modulate", l.gate_residual_ln_modulate);
@@ -504,6 +713,9 @@ PyMethodDef methods[] = {
     BD3_FAST(decode),
     BD3_FAST(qkv_rope),
     BD3_FAST(subs_sample),
+    BD3_FAST(paged_attention),
+    BD3_FAST(paged_attention_inputs),
+    BD3_FAST(adjust_logits),
     BD3_FAST(ln_modulate),
     BD3_FAST(gate_residual),
     BD3_FAST(gate_residual_ln_modulate),

@@ -1,0 +1,395 @@
+// paged.hip - attention of ragged batches over a paged KV cache, and the
+// attention inputs written into its pages.
+//
+// Sequence b owns the packed tokens q_starts[b] .. q_starts[b + 1] - 1 (n of
+// them) and kv = kv_lens[b] keys, the chunk's own included; key j lies in slot
+// j % page of page page_table[b][j / page]. Token i is at position p = kv - n + i
+// and sees keys j < min((p / bs + 1) * bs, kv), none if p < 0. `group` query heads
+// share a KV head: their rows are one matrix of n * group rows, row r token
+// r / group of head h * group + r % group, so a page is read once for all of them.
+//
+// The lengths and the table are device data, so the grid is sized by the
+// caller's bounds and workgroups without rows or keys leave at once. Everything
+// read through device data is bounded: token ranges by the tokens there are,
+// lengths by the table and the caller's bound, page numbers by the pages there
+// are. Keys of an entry outside [0, pages) are not seen (their rows come from
+// a zero row, their scores are masked); keys past the length re-read the last one.
+#include "bd3_device.h"
+#include "bd3_launch.h"
+
+namespace bd3 {
+namespace {
+
+constexpr int kQT = 32;       // rows per partial slot
+constexpr int kSub = 32;      // keys per wave step
+constexpr int kStride = 72;   // padded LDS row (bf16)
+constexpr int kMergeRow = kHeadDim + 4;
+
+__device__ __attribute__((aligned(128))) uint16_t zero_row[kHeadDim];
+
+typedef const __attribute__((address_space(1))) u32x4 global_u32x4;
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+
+// One sequence's share of the batch, bounded (see above).
+struct PagedSeq {
+  int q0, n, kv, rows;
+  __device__ __forceinline__ PagedSeq(const PagedArgs& a, int b) {
+    q0 = wave_uniform(clampi(a.q_starts[b], 0, a.tokens));
+    n = wave_uniform(clampi(a.q_starts[b + 1], q0, a.tokens)) - q0;
+    kv = wave_uniform(clampi(a.kv_lens[b], 0, a.max_kv));
+    rows = n * a.group;
+  }
+  // Keys that token i sees: [0, key_end).
+  __device__ __forceinline__ int key_end(const PagedArgs& a, int i) const {
+    const int p = kv - n + i;
+    const int e = (p / a.bs + 1) * a.bs;
+    return p < 0 ? 0 : (e < kv ? e : kv);
+  }
+  // One past the last key of the tile of `tile` rows at row r0 (r0 < rows).
+  __device__ __forceinline__ int tile_end(const PagedArgs& a, int r0) const {
+    const int last = (r0 + a.tile < rows ? r0 + a.tile : rows) - 1;
+    return wave_uniform(key_end(a, last / a.group));
+  }
+};
+
+// The key ranges of a tile that sees `keys` keys: `n` of `len` keys, equal ones.
+struct PagedSplit {
+  int n, len;
+  __device__ __forceinline__ PagedSplit(const PagedArgs& a, int keys) {
+    const int want = keys > a.split_len ? (keys + a.split_len - 1) / a.split_len : 1;
+    len = ((keys + want - 1) / want + a.unit - 1) / a.unit * a.unit;
+    n = keys > 0 ? (keys + len - 1) / len : 1;
+  }
+};
+
+template <int NW>
+struct MergeLds {
+  float o[NW][kQT][kMergeRow];  // unnormalised
+  float m[NW][kQT];
+  float l[NW][kQT];
+};
+template <int NW>
+constexpr size_t paged32_smem() {
+  constexpr size_t v = sizeof(__bf16) * NW * 2 * kSub * kStride;
+  return v > sizeof(MergeLds<NW>) ? v : sizeof(MergeLds<NW>);
+}
+
+// NW waves share the key chunks of one (range, 32-row tile, sequence * KV head).
+template <int NW>
+__global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[paged32_smem<NW>()];
+  const int tid = wi_x();
+  const int lane = tid & 63;
+  const int wave = wave_uniform(tid >> 6);
+  const int l32 = lane & 31;
+  const int g = lane >> 5;
+  __bf16* ks = reinterpret_cast<__bf16*>(smem) + wave * 2 * kSub * kStride;
+  __bf16* vs = ks + kSub * kStride;
+
+  const int id = wg_x();
+  const int split = id % a.n_splits;
+  const int qt = id / a.n_splits % a.q_tiles;
+  const int bh = id / a.n_splits / a.q_tiles;
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  const PagedSeq sq(a, b);
+  const int r0 = qt * kQT;
+  if (r0 >= sq.rows) return;
+  const int key_end = sq.tile_end(a, r0);
+  const PagedSplit sp(a, key_end);
+  if (split >= sp.n) return;
+
+  // Q^T B operand: lane holds row r0 + l32 (clamped), d = 16c + 8g .. +7.
+  const int row = r0 + l32 < sq.rows ? r0 + l32 : sq.rows - 1;
+  const int tok = row / a.group;
+  const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(h * a.group + row - tok * a.group) * a.sq_h;
+  bf16x8 qreg[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) qreg[c] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * c + 8 * g));
+  const int khi = sq.key_end(a, tok);
+  const int kfull = wave_uniform(sq.key_end(a, r0 / a.group));  // every row of the tile sees these
+
+  const int lo = split * sp.len;
+  const int hi = lo + sp.len < key_end ? lo + sp.len : key_end;
+  const int n_chunks = hi > lo ? (hi - lo + kSub - 1) / kSub : 0;
+
+  // Page entries of the wave's next 32 chunks: lane 2 i + half holds that of the
+  // half's 16 keys (a page holds at least 16) of the wave's (base + i)-th chunk.
+  const int32_t* table = a.table + (int64_t)b * a.table_s;
+  int ids = 0;
+  uint64_t ok = 0;
+  auto window = [&](int base) {
+    const int key = lo + (wave + NW * (base + (lane >> 1))) * kSub + 16 * (lane & 1);
+    ids = key < hi ? table[key >> a.page_shift] : -1;
+    ok = __ballot((unsigned)ids < (unsigned)a.pages);
+  };
+  u32x4 kr[4], vr[4];  // lane + 64 j -> key row 8 j + lane / 8 of the chunk, 16-byte part lane % 8
+  uint32_t okc = 0;    // halves of the chunk whose page exists
+  auto load = [&](int i) {  // the wave's i-th chunk
+    const int c0 = lo + (wave + NW * i) * kSub;
+    okc = 0;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int at = 2 * (i & 31) + hh;
+      const int key = c0 + 16 * hh;
+      const bool there = (ok >> at) & 1;
+      const int64_t page = __builtin_amdgcn_readlane(ids, at);
+      const int64_t slot = key & (a.page - 1);
+      const uint64_t kb = there ? (uint64_t)(uintptr_t)(a.k + page * a.sk_p + h * a.sk_h + slot * a.sk_s)
+                                : (uint64_t)(uintptr_t)zero_row;
+      const uint64_t vb = there ? (uint64_t)(uintptr_t)(a.v + page * a.sv_p + h * a.sv_h + slot * a.sv_s)
+                                : (uint64_t)(uintptr_t)zero_row;
+      okc |= there ? 1u << hh : 0u;
+      const int lim = there ? hi - 1 - key : 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int rr = (lane >> 3) + 8 * j;
+        const int rl = rr < lim ? rr : lim;
+        kr[2 * hh + j] = __builtin_nontemporal_load((global_u32x4*)(kb + 2 * ((int64_t)rl * a.sk_s + 8 * (lane & 7))));
+        vr[2 * hh + j] = __builtin_nontemporal_load((global_u32x4*)(vb + 2 * ((int64_t)rl * a.sv_s + 8 * (lane & 7))));
+      }
+    }
+  };
+
+  f32x16 oacc[2] = {};
+  float m = -INFINITY, lsum = 0.f;
+  const int tr_row = (lane & 15) >> 2;
+  const int tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const int mine = n_chunks > wave ? (n_chunks - wave + NW - 1) / NW : 0;
+  if (mine > 0) {
+    window(0);
+    load(0);
+  }
+  for (int i = 0; i < mine; ++i) {
+    const int c0 = lo + (wave + NW * i) * kSub;
+    const uint32_t there = okc;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int off = ((lane >> 3) + 8 * j) * kStride + 8 * (lane & 7);
+      *reinterpret_cast<u32x4*>(&ks[off]) = kr[j];
+      *reinterpret_cast<u32x4*>(&vs[off]) = vr[j];
+    }
+    if (i + 1 < mine) {
+      if (((i + 1) & 31) == 0) window(i + 1);
+      load(i + 1);
+    }
+    // S^T (32 keys x 32 rows): A = K rows from the tile (lane: key l32, d 16c + 8g .. +7).
+    f32x16 s = {};
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      s = mfma32(*reinterpret_cast<const bf16x8*>(&ks[l32 * kStride + 16 * c + 8 * g]), qreg[c], s);
+    if (c0 + kSub > kfull || c0 + kSub > hi || there != 3) {
+      const int lim = khi < hi ? khi : hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = c0 + 8 * (r >> 2) + 4 * g + (r & 3);
+        s[r] = key < lim && ((there >> (r >> 3)) & 1) ? s[r] : -INFINITY;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = max_xor32(mx);
+    const float mt = mx * a.scale_log2;
+    if (__ballot(mt > m) != 0) {
+      const float mn = fmaxf(m, mt);
+      const float alpha = (mn == -INFINITY) ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      lsum *= alpha;
+      oacc[0] *= alpha;
+      oacc[1] *= alpha;
+    }
+    const float m_use = (m == -INFINITY) ? 0.f : m;
+    float p[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      p[r] = fast_exp2(fmaf(s[r], a.scale_log2, -m_use));
+      lsum += p[r];
+    }
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+      const bf16x8 pop = to_bf16x8(p[8 * kc], p[8 * kc + 1], p[8 * kc + 2], p[8 * kc + 3],
+                                   p[8 * kc + 4], p[8 * kc + 5], p[8 * kc + 6], p[8 * kc + 7]);
+      const int vrow = 16 * kc + 4 * g + tr_row;
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        const bf16x8 va = cat8(lds_read_tr(&vs[vrow * kStride + 32 * db + tr_col]),
+                               lds_read_tr(&vs[(vrow + 8) * kStride + 32 * db + tr_col]));
+        oacc[db] = mfma32(va, pop, oacc[db]);
+      }
+    }
+  }
+
+  // Merge the waves' states.
+  lsum = sum_xor32(lsum);
+  __syncthreads();  // the tiles are reused below
+  MergeLds<NW>* ml = reinterpret_cast<MergeLds<NW>*>(smem);
+#pragma unroll
+  for (int db = 0; db < 2; ++db)
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg)
+      *reinterpret_cast<f32x4*>(&ml->o[wave][l32][32 * db + 8 * rg + 4 * g]) =
+          f32x4{oacc[db][4 * rg], oacc[db][4 * rg + 1], oacc[db][4 * rg + 2], oacc[db][4 * rg + 3]};
+  if (g == 0) {
+    ml->m[wave][l32] = m;
+    ml->l[wave][l32] = lsum;
+  }
+  __syncthreads();
+
+  const int64_t slot = ((int64_t)bh * a.q_tiles + qt) * a.n_splits + split;
+#pragma unroll
+  for (int t0 = 0; t0 < kQT; t0 += NW * 4) {
+    const int rt = t0 + (tid >> 4), d = 4 * (tid & 15);
+    float mw[NW], mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      mw[w] = ml->m[w][rt];
+      mm = fmaxf(mm, mw[w]);
+    }
+    const float mu = (mm == -INFINITY) ? 0.f : mm;
+    float lt = 0.f;
+    f32x4 ot = {};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float wgt = fast_exp2(mw[w] - mu);
+      lt += wgt * ml->l[w][rt];
+      ot += wgt * *reinterpret_cast<const f32x4*>(&ml->o[w][rt][d]);
+    }
+    const float inv = lt > 0.f ? 1.f / lt : 0.f;  // a row that sees no key: 0
+    if (sp.n == 1) {
+      if (r0 + rt < sq.rows) {
+        const int t = (r0 + rt) / a.group;
+        *reinterpret_cast<bf16x4*>(a.o + (int64_t)(sq.q0 + t) * a.so_t +
+                                   (int64_t)(h * a.group + r0 + rt - t * a.group) * a.so_h + d) =
+            to_bf16x4(ot[0] * inv, ot[1] * inv, ot[2] * inv, ot[3] * inv);
+      }
+    } else {
+      *reinterpret_cast<f32x4*>(&a.part_o[(slot * kQT + rt) * kHeadDim + d]) = ot * inv;
+      if (d == 0) a.part_lse[slot * kQT + rt] = lt > 0.f ? mm + fast_log2(lt) : -INFINITY;
+    }
+  }
+}
+
+// Merges the ranges of the tiles that were cut: weights exp2(lse_s - max lse), 16
+// threads a row, 4 outputs each; the loads of 8 ranges are issued before their
+// first use. Grid: (32-row slots, sequence * KV head).
+__global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
+  const int qt = wg_x() % a.q_slots;
+  const int bh = wg_x() / a.q_slots;
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  const PagedSeq sq(a, b);
+  const int row = qt * kQT + (wi_x() >> 4);
+  if (qt * kQT >= sq.rows) return;
+  const PagedSplit sp(a, sq.tile_end(a, qt * kQT / a.tile * a.tile));
+  if (sp.n <= 1 || row >= sq.rows) return;
+  const int d0 = 4 * (wi_x() & 15);
+  const int64_t slot0 = ((int64_t)bh * a.q_slots + qt) * a.n_splits;
+  const float* lp = a.part_lse + slot0 * kQT + (wi_x() >> 4);
+  const float* pp = a.part_o + (slot0 * kQT + (wi_x() >> 4)) * kHeadDim + d0;
+  constexpr int kG = 8;
+  float mm = -INFINITY, wt = 0.f;
+  f32x4 acc = {};
+  for (int s0 = 0; s0 < sp.n; s0 += kG) {
+    float l[kG];
+    f32x4 po[kG];
+#pragma unroll
+    for (int k = 0; k < kG; ++k) {
+      l[k] = s0 + k < sp.n ? lp[(s0 + k) * kQT] : -INFINITY;
+      po[k] = s0 + k < sp.n ? *reinterpret_cast<const f32x4*>(pp + (int64_t)(s0 + k) * kQT * kHeadDim) : f32x4{};
+    }
+    float mg = mm;
+#pragma unroll
+    for (int k = 0; k < kG; ++k) mg = fmaxf(mg, l[k]);
+    const float base = mg == -INFINITY ? 0.f : mg;
+    const float old = fast_exp2(mm - base);  // 0 while no key was met
+    wt *= old;
+    acc *= old;
+    mm = mg;
+#pragma unroll
+    for (int k = 0; k < kG; ++k) {
+      const float w = fast_exp2(l[k] - base);
+      wt += w;
+      acc += w * po[k];
+    }
+  }
+  const float inv = wt > 0.f ? 1.f / wt : 0.f;
+  const int t = row / a.group;
+  *reinterpret_cast<bf16x4*>(a.o + (int64_t)(sq.q0 + t) * a.so_t + (int64_t)(h * a.group + row - t * a.group) * a.so_h +
+                             d0) = to_bf16x4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+}
+
+// Rotary embedding of q and k at each token's position, q to packed tokens, k and
+// v into the pages. y1 = x1 c - x2 s, y2 = x1 s + x2 c on the halves of a head
+// row, in fp32 with the fp32 tables and rounded once (qkv_rope.hip instead repeats
+// an eager bf16 path's five roundings, which no caller of pages has to match).
+// Work item: (token, head of q | k | v, j): coordinate pairs (8j + i, 32 + 8j + i).
+__global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {
+  const uint32_t e0 = (uint32_t)wg_x() * 256u, e = e0 + wi_x();
+  const uint32_t per_tok = 4u * (uint32_t)(a.heads + 2 * a.kv_heads);
+  // The sequence of the workgroup's first token: those that end before it.
+  const int tok0 = (int)(e0 / per_tok);
+  int b = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    const int s = s0 + (wi_x() & 63);
+    b += __popcll(__ballot(s < a.seqs && a.q_starts[s + 1] <= tok0));
+  }
+  if (e >= (uint32_t)a.total) return;
+  const int tok = (int)(e / per_tok);
+  const int r = (int)(e - (uint32_t)tok * per_tok);
+  const int hh = r >> 2, j = r & 3;
+  while (b < a.seqs && a.q_starts[b + 1] <= tok) ++b;
+  if (b >= a.seqs || a.q_starts[b] > tok) return;  // behind the last sequence
+  const int end = a.q_starts[b + 1] < a.tokens ? a.q_starts[b + 1] : a.tokens;
+  const int64_t pos = (int64_t)a.kv_lens[b] - (end - tok);
+
+  const uint16_t* src = a.qkv + (int64_t)tok * a.sx_t + hh * kHeadDim + 8 * j;
+  u32x4 x1 = ld16(src), x2 = ld16(src + kHeadDim / 2);
+  uint16_t* dst;
+  if (hh < a.heads) {
+    dst = a.q + (int64_t)tok * a.sq_t + (int64_t)hh * a.sq_h;
+  } else {
+    // Nothing is written where the table has no page for the position.
+    if (pos < 0 || (pos >> a.page_shift) >= a.width) return;
+    const int page = a.table[(int64_t)b * a.table_s + (pos >> a.page_shift)];
+    if ((unsigned)page >= (unsigned)a.pages) return;
+    const int64_t slot = pos & (a.page - 1);
+    const int kh = hh - a.heads;
+    dst = kh < a.kv_heads ? a.k + (int64_t)page * a.sk_p + (int64_t)kh * a.sk_h + slot * a.sk_s
+                          : a.v + (int64_t)page * a.sv_p + (int64_t)(kh - a.kv_heads) * a.sv_h + slot * a.sv_s;
+  }
+  if (hh < a.heads + a.kv_heads) {
+    const int64_t tp = pos < 0 ? 0 : (pos >= a.max_pos ? a.max_pos - 1 : pos);
+    const float* cp = a.cos_t + tp * (kHeadDim / 2) + 8 * j;
+    const float* sp = a.sin_t + tp * (kHeadDim / 2) + 8 * j;
+    bf16x8 b1 = __builtin_bit_cast(bf16x8, x1), b2 = __builtin_bit_cast(bf16x8, x2), y1, y2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f1 = (float)b1[i], f2 = (float)b2[i], c = cp[i], s = sp[i];
+      y1[i] = (__bf16)(f1 * c - f2 * s);
+      y2[i] = (__bf16)(f1 * s + f2 * c);
+    }
+    x1 = __builtin_bit_cast(u32x4, y1);
+    x2 = __builtin_bit_cast(u32x4, y2);
+  }
+  st16(dst + 8 * j, x1);
+  st16(dst + 8 * j + kHeadDim / 2, x2);
+}
+
+}  // namespace
+
+hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream) {
+  const int64_t bh = (int64_t)a.seqs * a.kv_heads;
+  const dim3 grid((unsigned)(bh * a.q_tiles * a.n_splits));
+  hipLaunchKernelGGL(paged32_kernel<4>, grid, dim3(256), 0, stream, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.n_splits == 1) return e;
+  hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)(bh * a.q_slots)), dim3(512), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_rope(const PagedRopeArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL(paged_rope_kernel, dim3((unsigned)((a.total + 255) / 256)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace bd3

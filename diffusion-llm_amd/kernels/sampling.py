@@ -10,6 +10,9 @@ bd3_subs_sample_ws does it without writing any (rows, vocab)
 intermediate (the reference materialises the log-probs, the carry tensor,
 q, the uniforms and the noise, several of them in float64).
 
+`adjust_logits` applies penalties for repeated tokens, biases and grammar masks
+to the logits before that step (no reference counterpart).
+
 Noise: pass `u` (float64, the shape of the logits; e.g. torch.rand_like's
 draw) to reproduce the reference's arithmetic on the same uniforms, or let
 the kernel draw them from a counter-based Philox4x32-10 stream
@@ -71,3 +74,38 @@ def subs_sample_step(
         gen = generator or default_stream()
         seed, offset = gen.seed, gen.next_offset()
     return host().subs_sample(logits, block, mask_index, keep, u, seed, offset)
+
+
+def adjust_logits(
+    logits: Tensor,                 # (batch, rows, vocab) or (batch, vocab), bf16 or fp32
+    tokens: Tensor | None = None,   # (batch, history) int64: what each sequence holds so far
+    lengths: Tensor | None = None,  # (batch) int32: how much of it counts (default: all)
+    repetition: float | Tensor = 1.0,
+    frequency: float | Tensor = 0.0,
+    presence: float | Tensor = 0.0,
+    bias: Tensor | None = None,     # (vocab) or (batch, vocab) float32
+    allowed: Tensor | None = None,  # int32 words of bits, (words), (batch, words) or (batch, rows, words)
+    fill: float = -1e6,
+    out: Tensor | None = None,
+) -> Tensor:
+    """Penalties for tokens a sequence already holds, biases and a grammar mask,
+    for the logits that subs_sample_step draws from.
+
+    With c the number of times a token occurs in the first lengths[b] of
+    tokens[b]: where c > 0 its logit x becomes x / repetition (x * repetition if
+    x <= 0) minus frequency * c + presence; then bias is added; then tokens whose
+    bit (bit v % 32 of word v // 32) is 0 are set to `fill`, which SUBS's own
+    [MASK] logit (-1e6, model/subs.py:8) is by default: finite, as the draw wants
+    it, also in a row whose mask allows nothing. In fp32, rounded once. The
+    penalties are numbers or (batch) float32 tensors; tokens outside the
+    vocabulary count for nothing. `out=logits` works in place."""
+    assert logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32), \
+        "logits must be bf16 or fp32 CUDA tensors"
+    assert logits.dim() in (2, 3), "logits must be (batch, rows, vocab) or (batch, vocab)"
+    if logits.dim() == 3:
+        return host().adjust_logits(logits, tokens, lengths, repetition, frequency, presence, bias, allowed, fill, out)
+    assert allowed is None or allowed.dim() <= 2, "allowed must be (words) or (batch, words) for (batch, vocab) logits"
+    assert out is None or out.shape == logits.shape, "out must have the logits' shape and dtype, with last stride 1"
+    r = host().adjust_logits(logits.unsqueeze(1), tokens, lengths, repetition, frequency, presence, bias, allowed, fill,
+                             None if out is None else out.unsqueeze(1))
+    return r.squeeze(1)

@@ -7,7 +7,9 @@
  *     under the BD3-LM block-diffusion mask;
  *   - block-sparse decode attention of the last q_len positions over a
  *     KV cache of kv_len positions (block-causal);
- *   - split-KV decode attention (partials + LSE merge).
+ *   - split-KV decode attention (partials + LSE merge);
+ *   - attention of ragged batches over a paged KV cache, with the inputs written
+ *     into its pages, and penalties, biases and grammar masks on the logits.
  *
  * Conventions shared by every entry point:
  *   - All tensor pointers are DEVICE pointers to bf16 data (uint16 bit
@@ -316,6 +318,98 @@ int bd3_qkv_rope(const void* qkv, const int64_t* qkv_strides, int32_t batch, int
 int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t batch,
                  int32_t heads, int32_t seq, int32_t head_dim, const int64_t* strides,
                  void* stream);
+
+/*
+ * Attention of a ragged batch over a paged KV cache. Sequence b owns the packed
+ * tokens q_starts[b] .. q_starts[b + 1] - 1 (n of them, its newest) and
+ * kv_lens[b] keys, the chunk's own among them; key j is slot j % page_size of page
+ * page_table[b][j / page_size]. Token i of the chunk is at position p =
+ * kv_lens[b] - n + i and sees keys j < min((p / block_size + 1) * block_size,
+ * kv_lens[b]) (the rule of bd3_decode; block_size 1 is causal); a token that sees
+ * no key gets 0. heads / kv_heads query heads share a KV head (query head h
+ * reads h / (heads / kv_heads)). n may be 1 (single-token decoding), a block, a
+ * chunk of a prompt, or 0, and differ between sequences.
+ *   q, o: (tokens, heads, 64); rows of o that belong to no sequence are left as
+ *     they are. k_pages, v_pages: (pages, kv_heads, page_size, 64).
+ *   page_table: device int32 (seqs, table_width); q_starts: device int32 (seqs +
+ *     1), ascending; kv_lens: device int32 (seqs).
+ *   max_q, max_kv: the host's bounds of a chunk's tokens and a sequence's keys
+ *     (max_kv <= table_width * page_size). They size the launch: tokens beyond
+ *     max_q may be left out and keys beyond max_kv are not seen.
+ *   total_kv: about the sum of kv_lens, 0 .. seqs * max_kv: chooses how the keys
+ *     are cut over workgroups, not what is computed.
+ *   strides: 11 int64 element strides: q (token, head), k_pages (page, head,
+ *     slot), v_pages (page, head, slot), o (token, head), page_table (row); last
+ *     strides 1, all but the table's multiples of 8, slot strides < 2^24.
+ * Device data is not trusted with addresses: token ranges are cut to [0, tokens),
+ * lengths to [0, max_kv], and keys whose table entry lies outside [0, pages) are
+ * not seen. Table entries beyond a sequence's keys are not read.
+ * Preconditions: page_size a power of two in [16, 1024], head_dim == 64, heads a
+ * multiple of kv_heads. The same call may be captured into a graph: its launches
+ * depend on the arguments alone, and lengths, tables and starts may change
+ * between replays within max_q and max_kv. No reference counterpart.
+ */
+size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q,
+                                      int32_t max_kv, int64_t total_kv);
+int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* o,
+                   const int32_t* page_table, const int32_t* q_starts, const int32_t* kv_lens,
+                   int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                   int32_t pages, int32_t page_size, int32_t table_width, int32_t max_q,
+                   int32_t max_kv, int64_t total_kv, int32_t block_size, const int64_t* strides,
+                   float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention inputs of a ragged batch: q and k of every token rotated at its
+ * position (kv_lens[b] - n + i, kv_lens counting the new tokens), q written to
+ * q_out, k and v into the pages. The batch and the pool are described as for
+ * bd3_paged_attn.
+ *   qkv: (tokens, (heads + 2 * kv_heads) * 64): the query heads, then the key
+ *     heads, then the value heads.
+ *   sin_table, cos_table: device fp32 (max_pos, 32) (sin / cos of p *
+ *     theta^(-2k/64)); positions outside are clamped to them.
+ *   strides: 10 int64 element strides: qkv (token), q_out (token, head), k_pages
+ *     (page, head, slot), v_pages (page, head, slot), page_table (row).
+ * The rotation is computed in fp32 and rounded once (bd3_qkv_rope repeats the
+ * eager bf16 path's roundings instead). Tokens of no sequence are left out: their
+ * rows of q_out stay as they are. Nothing is written for a position before 0, past
+ * the table or whose entry lies outside [0, pages). No reference counterpart.
+ */
+int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos_table,
+                       int32_t max_pos, void* q_out, void* k_pages, void* v_pages,
+                       const int32_t* page_table, const int32_t* q_starts, const int32_t* kv_lens,
+                       int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads,
+                       int32_t head_dim, int32_t pages, int32_t page_size, int32_t table_width,
+                       const int64_t* strides, void* stream);
+
+/*
+ * Penalties for repeated tokens, biases and a grammar mask on logits before the
+ * draw. For logit x of token v in a row of sequence b, with c the count of v
+ * among tokens[b][0 .. lengths[b]):
+ *   if c > 0: x = x > 0 ? x / repetition : x * repetition,
+ *             x -= frequency * c + presence
+ *   x += bias[v];   x = fill where v's bit of the mask is 0
+ * in fp32, rounded once to the logits' type.
+ *   logits, out: (batch, rows, vocab) bf16 (logits_fp32 = 0) or fp32 (1), last
+ *     stride 1; out may be logits itself, and overlap it in no other way.
+ *   tokens: device int64 (batch, history), or NULL for no penalties; values
+ *     outside [0, vocab) count for nothing. lengths: device int32 (batch), cut to
+ *     [0, history]; NULL: all of history.
+ *   penalties: host {repetition, frequency, presence}; repetition, frequency,
+ *     presence: device fp32 (batch) in place of the one number, or NULL.
+ *   bias: device fp32 (vocab) (batch stride 0) or (batch, vocab), or NULL.
+ *   allowed: device int32 words, bit v % 32 of word v / 32 set where token v is
+ *     allowed, one set for all (strides 0), for each sequence or each row; NULL.
+ *   fill: finite, so that a row whose mask allows nothing stays finite (every
+ *     token the same).
+ *   strides: 8 int64 element strides: logits (batch, row), out (batch, row),
+ *     tokens (batch), bias (batch), allowed (batch, row).
+ * No reference counterpart.
+ */
+int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_t batch,
+                      int32_t rows, int32_t vocab, const int64_t* tokens, int32_t history,
+                      const int32_t* lengths, const float* penalties, const float* repetition,
+                      const float* frequency, const float* presence, const float* bias,
+                      const int32_t* allowed, float fill, const int64_t* strides, void* stream);
 
 /*
  * One ancestral denoising step of BD3-LM sampling for `rows` token
