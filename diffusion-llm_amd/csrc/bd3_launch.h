@@ -164,6 +164,7 @@ struct PagedArgs {
   int max_kv;     // most keys of a sequence: the caller's bound, at most the table's
   int bs;
   int tile;       // query rows per workgroup
+  int subs;       // sets of 4 waves per workgroup: 1, 2 or 4 (128-row tiles)
   int q_tiles;    // tiles of the longest chunk
   int q_slots;    // its 32-row partial slots
   int n_splits;   // most key ranges of a tile

@@ -881,15 +881,16 @@ int log2_of(int32_t x) {
 // What a paged attention call runs: rows per workgroup, tiles and partial slots
 // of the longest chunk, key ranges.
 struct PagedPlan {
-  int tile, q_tiles, q_slots, n_splits, split_len, unit;
+  int tile, subs, q_tiles, q_slots, n_splits, split_len, unit;
 };
 
 PagedPlan paged_plan(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
                      int64_t total_kv) {
   PagedPlan p;
   const int64_t rows = (int64_t)max_q * (heads / kv_heads);
-  p.tile = 32;
-  p.unit = 32;
+  p.tile = rows <= 64 ? 32 : 128;
+  p.unit = rows <= 64 ? 32 : 64;
+  p.subs = 1;
   p.q_tiles = (int)((rows + p.tile - 1) / p.tile);
   p.q_slots = (int)((rows + 31) / 32);
   const int64_t work = std::min(total_kv, (int64_t)seqs * max_kv) * kv_heads * p.q_tiles;
@@ -989,6 +990,7 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.max_kv = max_kv;
   a.bs = std::min(block_size, bd3::kPagedMaxKeys);  // as good as any larger one
   a.tile = plan.tile;
+  a.subs = plan.subs;
   a.q_tiles = plan.q_tiles;
   a.q_slots = plan.q_slots;
   a.n_splits = plan.n_splits;

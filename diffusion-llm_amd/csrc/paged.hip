@@ -16,6 +16,7 @@
 // a zero row, their scores are masked); keys past the length re-read the last one.
 #include "bd3_device.h"
 #include "bd3_launch.h"
+#include "bd3_swz.h"
 
 namespace bd3 {
 namespace {
@@ -270,6 +271,247 @@ __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
   }
 }
 
+// Chunks of more than 64 rows: 128-row tiles, four waves of 32 rows that share each
+// 64-key K / V tile, which goes from the page to LDS directly (bd3_swz.h; two
+// stages: the next tile loads during the current one). A wave loads 16 keys of a
+// tile, which lie in one page, so its source is one scalar base and the same lane
+// offsets for every full tile. SUBS sets of four waves take the tiles in turn, each
+// through a ring of its own, and add up at the end: few, long items.
+// S^T (keys x rows) = K Q^T, O^T += V^T P^T with P^T taken from the S^T registers;
+// a wave skips tiles past its last row's keys and masks only those that its
+// first row does not see whole. The running maximum is updated when it grew by
+// more than kRescale (log2): a stale one leaves O / l exact and bounds P by 2^8.
+constexpr float kRescale = 8.0f;
+
+template <int SUBS>
+__global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
+  __shared__ __attribute__((aligned(1024))) __bf16 smem_all[SUBS][2][2][kSwTile];  // [set][stage][K | V]
+  const int tid = wi_x();
+  const int lane = tid & 63;
+  const int wave = wave_uniform((tid >> 6) & 3);  // in its set
+  const int sub = SUBS == 1 ? 0 : wave_uniform(tid >> 8);
+  auto& smem = smem_all[sub];
+  const int l32 = lane & 31;
+  const int g = lane >> 5;
+
+  // Longest tiles of every sequence first; its KV heads side by side.
+  const int bhs = a.seqs * a.kv_heads;
+  const int bh = wg_x() % bhs;
+  const int split = wg_x() / bhs % a.n_splits;
+  const int rank = wg_x() / bhs / a.n_splits;
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  const PagedSeq sq(a, b);
+  const int qt = (sq.rows + 127) / 128 - 1 - rank;
+  if (qt < 0) return;
+  const int r0 = 128 * qt;
+  const int key_end = sq.tile_end(a, r0);
+  const PagedSplit sp(a, key_end);
+  if (split >= sp.n) return;
+  const int lo = split * sp.len;
+  const int hi = lo + sp.len < key_end ? lo + sp.len : key_end;
+  const int n_tiles = (hi - lo + kSwRows - 1) / kSwRows;  // 0: a tile that sees no key
+  const int n_mine = n_tiles > sub ? (n_tiles - sub + SUBS - 1) / SUBS : 0;
+
+  const int qrow0 = r0 + 32 * wave;
+  const int myr = qrow0 + l32;
+  const int row = myr < sq.rows ? myr : sq.rows - 1;
+  const int tok = row / a.group;
+  const int64_t head = h * a.group + row - tok * a.group;
+  const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + head * a.sq_h;
+  bf16x8 qreg[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) qreg[c] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * c + 8 * g));
+
+  // Page entries of the set's next 16 tiles: lane 4 i + w holds that of wave w's keys
+  // of the (base + i)-th one.
+  const int32_t* table = a.table + (int64_t)b * a.table_s;
+  auto entries = [&](int base) {
+    const int key = lo + (sub + SUBS * (base + (lane >> 2))) * kSwRows + 16 * (lane & 3);
+    return key < hi ? table[key >> a.page_shift] : -1;
+  };
+  int ids = entries(0), ids_next = -1;
+  uint64_t ok = __ballot((unsigned)ids < (unsigned)a.pages);
+
+  uint32_t koff[2], voff[2];
+  int lrow[2], lch[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    lrow[j] = 8 * j + (lane >> 3);
+    lch[j] = 8 * ((lane & 7) ^ swz(16 * wave + lrow[j]));
+    koff[j] = (uint32_t)(2 * (lrow[j] * (int)a.sk_s + lch[j]));
+    voff[j] = (uint32_t)(2 * (lrow[j] * (int)a.sv_s + lch[j]));
+  }
+  const uint32_t lds_w = lds_addr(&smem[0][0][0]) + (uint32_t)wave * 2048u;
+  const uint16_t* kh = a.k + h * a.sk_h;
+  const uint16_t* vh = a.v + h * a.sv_h;
+  uint32_t there = 0;  // quarters of the tile requested last whose page exists
+  auto issue = [&](int i) {  // the set's i-th tile
+    if ((i & 15) == 0 && i > 0) {
+      ids = ids_next;
+      ok = __ballot((unsigned)ids < (unsigned)a.pages);
+    }
+    if ((i & 15) == 8) ids_next = entries((i | 15) + 1);
+    const int at = 4 * (i & 15) + wave;
+    const int key = lo + (sub + SUBS * i) * kSwRows + 16 * wave;
+    there = (uint32_t)(ok >> (4 * (i & 15))) & 15u;
+    const uint32_t dst = lds_w + (uint32_t)(i & 1) * 16384u;
+    const int lim = (ok >> at) & 1 ? sq.kv - 1 - key : -1;  // the last of its 16 rows that is a key
+    const int64_t page = __builtin_amdgcn_readlane(ids, at);
+    const int64_t slot = key & (a.page - 1);
+    const void* kb = lim >= 0 ? kh + page * a.sk_p + slot * a.sk_s : zero_row;
+    const void* vb = lim >= 0 ? vh + page * a.sv_p + slot * a.sv_s : zero_row;
+    if (lim >= 15) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) dma16(kb, koff[j], dst + 1024u * j);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) dma16(vb, voff[j], dst + 8192u + 1024u * j);
+    } else {  // rows past the last key re-read it
+      const int top = lim < 0 ? 0 : lim;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = lrow[j] < top ? lrow[j] : top;
+        dma16(kb, (uint32_t)(2 * (r * (int)a.sk_s + lch[j])), dst + 1024u * j);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = lrow[j] < top ? lrow[j] : top;
+        dma16(vb, (uint32_t)(2 * (r * (int)a.sv_s + lch[j])), dst + 8192u + 1024u * j);
+      }
+    }
+  };
+  if (n_mine > 0) issue(0);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) asm volatile("" ::"v"(qreg[c]));  // waits for Q here, not in the loop
+
+  const int khi = sq.key_end(a, tok);  // the lane's row sees [0, khi)
+  const int wave_last = qrow0 + 31 < sq.rows ? qrow0 + 31 : sq.rows - 1;
+  const int emax = qrow0 < sq.rows ? wave_uniform(sq.key_end(a, wave_last / a.group)) : 0;
+  const int emin = qrow0 < sq.rows ? wave_uniform(sq.key_end(a, qrow0 / a.group)) : 0;
+
+  f32x16 o[2] = {};  // O^T [d block]
+  float mref = 0.f, lsum = 0.f;
+  bool valid = false;  // the row has met a key
+  const float c2 = a.scale_log2;
+  auto step = [&](int k0, uint32_t seen, const __bf16* ks, const __bf16* vs) {
+    f32x16 s[2];
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb) s[sb] = mfma32(sw_row_op(ks, 32 * sb, 0, lane), qreg[0], f32x16{});
+#pragma unroll
+    for (int c = 1; c < 4; ++c)
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb) s[sb] = mfma32(sw_row_op(ks, 32 * sb, c, lane), qreg[c], s[sb]);
+    if (k0 + kSwRows > emin || seen != 15u) {
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = k0 + 32 * sb + 8 * (r >> 2) + 4 * g + (r & 3);
+          s[sb][r] = key < khi && ((seen >> (2 * sb + (r >> 3))) & 1) ? s[sb][r] : -INFINITY;
+        }
+    }
+    float mrow = -INFINITY;
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) mrow = fmaxf(fmaxf(mrow, s[sb][r]), s[sb][r + 1]);
+    const float mt = fmaf(max_xor32(mrow), c2, -mref);
+    if (__ballot(!valid || mt > kRescale) != 0) {
+      const float delta = valid ? fmaxf(mt, 0.f) : (mt == -INFINITY ? 0.f : mt);
+      const float alpha = valid ? fast_exp2(-delta) : 1.f;
+      valid = valid || mt != -INFINITY;
+      mref += delta;
+      lsum *= alpha;
+      o[0] *= alpha;
+      o[1] *= alpha;
+    }
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb) {
+      float p[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r] = fast_exp2(fmaf(s[sb][r], c2, -mref));
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc) {
+        const bf16x8 pop = to_bf16x8(p[8 * kc], p[8 * kc + 1], p[8 * kc + 2], p[8 * kc + 3], p[8 * kc + 4],
+                                     p[8 * kc + 5], p[8 * kc + 6], p[8 * kc + 7]);
+        lsum += ((p[8 * kc] + p[8 * kc + 1]) + (p[8 * kc + 2] + p[8 * kc + 3])) +
+                ((p[8 * kc + 4] + p[8 * kc + 5]) + (p[8 * kc + 6] + p[8 * kc + 7]));
+#pragma unroll
+        for (int db = 0; db < 2; ++db) o[db] = mfma32(sw_tr_op(vs, 32 * sb + 16 * kc, 32 * db, lane), pop, o[db]);
+      }
+    }
+  };
+
+  uint32_t seen = there;
+  vm_wait_barrier<0>();
+  const int steps = (n_tiles + SUBS - 1) / SUBS;  // of the set with the most tiles
+  for (int i = 0; i < steps; ++i) {
+    if (i + 1 < n_mine) issue(i + 1);
+    const int k0 = lo + (sub + SUBS * i) * kSwRows;
+    if (i < n_mine && k0 < emax) step(k0, seen, smem[i & 1][0], smem[i & 1][1]);
+    seen = there;
+    // The next tile is there, and this wave's reads of this one are done before
+    // any wave requests the tile after it into the same stage.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    vm_wait_barrier<0>();
+  }
+
+  float ltot = sum_xor32(lsum);
+  if constexpr (SUBS > 1) {
+    // The other sets hand their state to set 0 through LDS (every wave is past its
+    // last read of the rings); a set that met no key of a row has l = 0.
+    constexpr int kWave = 34 * 64, kSet = 4 * kWave;
+    static_assert((SUBS - 1) * kSet * 4 <= (int)sizeof(smem_all), "hand-over fits the rings");
+    float* ex = reinterpret_cast<float*>(&smem_all[0][0][0][0]) + wave * kWave + lane;
+    if (sub > 0) {
+      float* my = ex + (sub - 1) * kSet;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        my[r * 64] = o[0][r];
+        my[(16 + r) * 64] = o[1][r];
+      }
+      my[32 * 64] = mref;
+      my[33 * 64] = ltot;
+    }
+    __syncthreads();
+    if (sub > 0) return;
+#pragma unroll
+    for (int t = 0; t < SUBS - 1; ++t, ex += kSet) {
+      const float m1 = ex[32 * 64], l1 = ex[33 * 64];
+      const float m = l1 > 0.f ? (ltot > 0.f ? fmaxf(mref, m1) : m1) : mref;
+      const float w0 = ltot > 0.f ? fast_exp2(mref - m) : 0.f, w1 = l1 > 0.f ? fast_exp2(m1 - m) : 0.f;
+      mref = m;
+      ltot = ltot * w0 + l1 * w1;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        o[0][r] = o[0][r] * w0 + ex[r * 64] * w1;
+        o[1][r] = o[1][r] * w0 + ex[(16 + r) * 64] * w1;
+      }
+    }
+  }
+  if (myr >= sq.rows) return;
+  const bool any = ltot > 0.f;
+  const float inv = any ? 1.f / ltot : 0.f;
+  if (sp.n == 1) {
+    uint16_t* op = a.o + (int64_t)(sq.q0 + tok) * a.so_t + head * a.so_h;
+#pragma unroll
+    for (int db = 0; db < 2; ++db)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<bf16x4*>(op + 32 * db + 8 * q4 + 4 * g) =
+            to_bf16x4(o[db][4 * q4] * inv, o[db][4 * q4 + 1] * inv, o[db][4 * q4 + 2] * inv, o[db][4 * q4 + 3] * inv);
+  } else {
+    const int64_t slot = ((int64_t)bh * a.q_slots + (qrow0 >> 5)) * a.n_splits + split;
+    float* po = a.part_o + (slot * kQT + l32) * kHeadDim;
+#pragma unroll
+    for (int db = 0; db < 2; ++db)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<f32x4*>(po + 32 * db + 8 * q4 + 4 * g) =
+            f32x4{o[db][4 * q4] * inv, o[db][4 * q4 + 1] * inv, o[db][4 * q4 + 2] * inv, o[db][4 * q4 + 3] * inv};
+    if (g == 0) a.part_lse[slot * kQT + l32] = any ? mref + fast_log2(ltot) : -INFINITY;
+  }
+}
+
 // Merges the ranges of the tiles that were cut: weights exp2(lse_s - max lse), 16
 // threads a row, 4 outputs each; the loads of 8 ranges are issued before their
 // first use. Grid: (32-row slots, sequence * KV head).
@@ -380,7 +622,16 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {
 hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream) {
   const int64_t bh = (int64_t)a.seqs * a.kv_heads;
   const dim3 grid((unsigned)(bh * a.q_tiles * a.n_splits));
-  hipLaunchKernelGGL(paged32_kernel<4>, grid, dim3(256), 0, stream, a);
+  if (a.tile == 128) {
+    if (a.subs == 4)
+      hipLaunchKernelGGL(paged128_kernel<4>, grid, dim3(1024), 0, stream, a);
+    else if (a.subs == 2)
+      hipLaunchKernelGGL(paged128_kernel<2>, grid, dim3(512), 0, stream, a);
+    else
+      hipLaunchKernelGGL(paged128_kernel<1>, grid, dim3(256), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL(paged32_kernel<4>, grid, dim3(256), 0, stream, a);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.n_splits == 1) return e;
   hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)(bh * a.q_slots)), dim3(512), 0, stream, a);
