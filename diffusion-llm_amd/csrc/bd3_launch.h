@@ -161,10 +161,11 @@ struct PagedArgs {
   float* part_lse;          // (seqs * kv_heads, q_slots, n_splits, 32) log2 LSE, or null
   int64_t sq_t, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, so_t, so_h, table_s;  // element strides
   int seqs, tokens, kv_heads, group, pages, page, page_shift;
+  int max_q;      // most tokens of a chunk: the caller's bound
   int max_kv;     // most keys of a sequence: the caller's bound, at most the table's
   int bs;
   int tile;       // query rows per workgroup
-  int subs;       // sets of 4 waves per workgroup: 1, 2 or 4 (128-row tiles)
+  int subs;       // sets of 4 waves per workgroup: 1, 2 or (128-row tiles) 4
   int q_tiles;    // tiles of the longest chunk
   int q_slots;    // its 32-row partial slots
   int n_splits;   // most key ranges of a tile

@@ -888,7 +888,7 @@ PagedPlan paged_plan(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_
                      int64_t total_kv) {
   PagedPlan p;
   const int64_t rows = (int64_t)max_q * (heads / kv_heads);
-  p.tile = rows <= 64 ? 32 : 128;
+  p.tile = rows <= 16 ? 16 : rows <= 64 ? 32 : 128;
   p.unit = rows <= 64 ? 32 : 64;
   p.subs = 1;
   p.q_tiles = (int)((rows + p.tile - 1) / p.tile);
@@ -987,6 +987,7 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.pages = pages;
   a.page = page_size;
   a.page_shift = log2_of(page_size);
+  a.max_q = max_q;
   a.max_kv = max_kv;
   a.bs = std::min(block_size, bd3::kPagedMaxKeys);  // as good as any larger one
   a.tile = plan.tile;
@@ -1102,8 +1103,12 @@ int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_
   a.presence = penalties[2];
   a.fill = fill;
   a.slices = (vocab + bd3::kLogitSlice - 1) / bd3::kLogitSlice;
-  a.part_rows = rows;
-  a.row_parts = 1;
+  // Eight rows to a workgroup, which counts the history for them once, and fewer
+  // while there is not one for every CU.
+  const int64_t few = 256 / ((int64_t)a.slices * batch);
+  a.row_parts = (int)std::min<int64_t>(rows, std::max<int64_t>((rows + 7) / 8, few));
+  a.part_rows = (rows + a.row_parts - 1) / a.row_parts;
+  a.row_parts = (rows + a.part_rows - 1) / a.part_rows;
   if ((int64_t)a.slices * a.row_parts * batch >= ((int64_t)1 << 23))
     return fail(BD3_EINVAL, "batch * vocab too large (limit 2^23 workgroups)");
   return hip_status(bd3::launch_adjust_logits(a, static_cast<hipStream_t>(stream)), "adjust_logits launch");

@@ -39,7 +39,7 @@ struct PagedSeq {
     q0 = wave_uniform(clampi(a.q_starts[b], 0, a.tokens));
     n = wave_uniform(clampi(a.q_starts[b + 1], q0, a.tokens)) - q0;
     kv = wave_uniform(clampi(a.kv_lens[b], 0, a.max_kv));
-    rows = n * a.group;
+    rows = (n < a.max_q ? n : a.max_q) * a.group;  // what the launch and its partials have room for
   }
   // Keys that token i sees: [0, key_end).
   __device__ __forceinline__ int key_end(const PagedArgs& a, int i) const {
@@ -64,22 +64,131 @@ struct PagedSplit {
   }
 };
 
+// The 32-key chunks of one key range that one of NW waves takes in turn (chunks
+// wave, wave + NW, ...): from the pages to registers, the next chunk's loads in
+// flight while the last one, staged in the wave's LDS tiles, is computed.
 template <int NW>
-struct MergeLds {
-  float o[NW][kQT][kMergeRow];  // unnormalised
-  float m[NW][kQT];
-  float l[NW][kQT];
+struct ChunkStream {
+  const PagedArgs& a;
+  const int32_t* table;
+  const uint16_t *kh, *vh;  // the head's rows of page 0
+  int lo, hi, wave, lane, mine;
+  int ids;        // lane 2 i + half: page of the half's 16 keys (a page holds at least 16) of chunk base + i
+  uint64_t ok;    // which of them exist
+  u32x4 kr[4], vr[4];  // lane + 64 j -> key row 8 j + lane / 8 of the chunk, 16-byte part lane % 8
+  uint32_t there;      // halves of the loaded chunk whose page exists
+
+  __device__ __forceinline__ ChunkStream(const PagedArgs& a_, int b, int h, int lo_, int hi_, int wave_, int lane_)
+      : a(a_), lo(lo_), hi(hi_), wave(wave_), lane(lane_), there(0) {
+    table = a.table + (int64_t)b * a.table_s;
+    kh = a.k + h * a.sk_h;
+    vh = a.v + h * a.sv_h;
+    const int n = hi > lo ? (hi - lo + kSub - 1) / kSub : 0;
+    mine = n > wave ? (n - wave + NW - 1) / NW : 0;
+  }
+  __device__ __forceinline__ int first_key(int i) const { return lo + (wave + NW * i) * kSub; }
+  __device__ __forceinline__ void load(int i) {
+    if ((i & 31) == 0) {
+      const int key = first_key(i + (lane >> 1)) + 16 * (lane & 1);
+      ids = key < hi ? table[key >> a.page_shift] : -1;
+      ok = __ballot((unsigned)ids < (unsigned)a.pages);
+    }
+    there = (uint32_t)(ok >> (2 * (i & 31))) & 3u;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int at = 2 * (i & 31) + hh;
+      const int key = first_key(i) + 16 * hh;
+      const bool is = (there >> hh) & 1;
+      const int64_t page = __builtin_amdgcn_readlane(ids, at);
+      const int64_t slot = key & (a.page - 1);
+      const uint64_t kb = (uint64_t)(uintptr_t)(is ? kh + page * a.sk_p + slot * a.sk_s : zero_row);
+      const uint64_t vb = (uint64_t)(uintptr_t)(is ? vh + page * a.sv_p + slot * a.sv_s : zero_row);
+      const int last = is ? hi - 1 - key : 0;  // rows past the range's end re-read its last one
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = (lane >> 3) + 8 * j < last ? (lane >> 3) + 8 * j : last;
+        kr[2 * hh + j] = __builtin_nontemporal_load(
+            (global_u32x4*)(kb + (uint32_t)(2 * (r * (int)a.sk_s + 8 * (lane & 7)))));
+        vr[2 * hh + j] = __builtin_nontemporal_load(
+            (global_u32x4*)(vb + (uint32_t)(2 * (r * (int)a.sv_s + 8 * (lane & 7)))));
+      }
+    }
+  }
+  __device__ __forceinline__ void stage(__bf16* ks, __bf16* vs) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int off = ((lane >> 3) + 8 * j) * kStride + 8 * (lane & 7);
+      *reinterpret_cast<u32x4*>(&ks[off]) = kr[j];
+      *reinterpret_cast<u32x4*>(&vs[off]) = vr[j];
+    }
+  }
 };
-template <int NW>
-constexpr size_t paged32_smem() {
+
+// The workgroup's item of a 16- or 32-row launch: (range, row tile, sequence * KV head).
+struct PagedItem {
+  int split, qt, bh, b, h;
+  __device__ __forceinline__ PagedItem(const PagedArgs& a) {
+    const int id = wg_x();
+    split = id % a.n_splits;
+    qt = id / a.n_splits % a.q_tiles;
+    bh = id / a.n_splits / a.q_tiles;
+    b = bh / a.kv_heads;
+    h = bh - b * a.kv_heads;
+  }
+};
+
+// The waves' states, unnormalised, merged by threads of 4 d each (16 a row): to the
+// result where the tile has one range, else to its partial.
+template <int NW, int ROWS>
+struct MergeLds {
+  float o[NW][ROWS][kMergeRow];
+  float m[NW][ROWS];
+  float l[NW][ROWS];
+  __device__ __forceinline__ void write_row(const PagedArgs& a, const PagedSeq& sq, const PagedSplit& sp,
+                                            const PagedItem& it, int rt, int d) const {
+    float mw[NW], mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      mw[w] = m[w][rt];
+      mm = fmaxf(mm, mw[w]);
+    }
+    const float mu = (mm == -INFINITY) ? 0.f : mm;
+    float lt = 0.f;
+    f32x4 ot = {};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float wgt = fast_exp2(mw[w] - mu);
+      lt += wgt * l[w][rt];
+      ot += wgt * *reinterpret_cast<const f32x4*>(&o[w][rt][d]);
+    }
+    const float inv = lt > 0.f ? 1.f / lt : 0.f;  // a row that sees no key: 0
+    if (sp.n == 1) {
+      const int row = it.qt * ROWS + rt;
+      if (row < sq.rows) {
+        const int t = row / a.group;
+        *reinterpret_cast<bf16x4*>(a.o + (int64_t)(sq.q0 + t) * a.so_t +
+                                   (int64_t)(it.h * a.group + row - t * a.group) * a.so_h + d) =
+            to_bf16x4(ot[0] * inv, ot[1] * inv, ot[2] * inv, ot[3] * inv);
+      }
+    } else {
+      const int64_t slot = ((int64_t)it.bh * a.q_slots + it.qt) * a.n_splits + it.split;
+      *reinterpret_cast<f32x4*>(&a.part_o[(slot * kQT + rt) * kHeadDim + d]) = ot * inv;
+      if (d == 0) a.part_lse[slot * kQT + rt] = lt > 0.f ? mm + fast_log2(lt) : -INFINITY;
+    }
+  }
+};
+template <int NW, int ROWS>
+constexpr size_t chunk_smem() {
   constexpr size_t v = sizeof(__bf16) * NW * 2 * kSub * kStride;
-  return v > sizeof(MergeLds<NW>) ? v : sizeof(MergeLds<NW>);
+  return v > sizeof(MergeLds<NW, ROWS>) ? v : sizeof(MergeLds<NW, ROWS>);
 }
 
-// NW waves share the key chunks of one (range, 32-row tile, sequence * KV head).
+// Up to 64 rows: 32-row tiles, NW waves share the key chunks of a range. S^T (32
+// keys x 32 rows) = K Q^T on v_mfma_f32_32x32x16_bf16 with the K tile's rows as A
+// operands; O^T += V^T P^T with V read transposed.
 template <int NW>
 __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[paged32_smem<NW>()];
+  __shared__ __attribute__((aligned(16))) char smem[chunk_smem<NW, kQT>()];
   const int tid = wi_x();
   const int lane = tid & 63;
   const int wave = wave_uniform(tid >> 6);
@@ -88,103 +197,48 @@ __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
   __bf16* ks = reinterpret_cast<__bf16*>(smem) + wave * 2 * kSub * kStride;
   __bf16* vs = ks + kSub * kStride;
 
-  const int id = wg_x();
-  const int split = id % a.n_splits;
-  const int qt = id / a.n_splits % a.q_tiles;
-  const int bh = id / a.n_splits / a.q_tiles;
-  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  const PagedSeq sq(a, b);
-  const int r0 = qt * kQT;
+  const PagedItem it(a);
+  const PagedSeq sq(a, it.b);
+  const int r0 = it.qt * kQT;
   if (r0 >= sq.rows) return;
   const int key_end = sq.tile_end(a, r0);
   const PagedSplit sp(a, key_end);
-  if (split >= sp.n) return;
+  if (it.split >= sp.n) return;
+  const int lo = it.split * sp.len;
+  const int hi = lo + sp.len < key_end ? lo + sp.len : key_end;
+  ChunkStream<NW> kv(a, it.b, it.h, lo, hi, wave, lane);
+  if (kv.mine > 0) kv.load(0);
 
   // Q^T B operand: lane holds row r0 + l32 (clamped), d = 16c + 8g .. +7.
   const int row = r0 + l32 < sq.rows ? r0 + l32 : sq.rows - 1;
   const int tok = row / a.group;
-  const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(h * a.group + row - tok * a.group) * a.sq_h;
+  const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(it.h * a.group + row - tok * a.group) * a.sq_h;
   bf16x8 qreg[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) qreg[c] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * c + 8 * g));
-  const int khi = sq.key_end(a, tok);
+  const int ends = sq.key_end(a, tok);
+  const int khi = ends < hi ? ends : hi;
   const int kfull = wave_uniform(sq.key_end(a, r0 / a.group));  // every row of the tile sees these
-
-  const int lo = split * sp.len;
-  const int hi = lo + sp.len < key_end ? lo + sp.len : key_end;
-  const int n_chunks = hi > lo ? (hi - lo + kSub - 1) / kSub : 0;
-
-  // Page entries of the wave's next 32 chunks: lane 2 i + half holds that of the
-  // half's 16 keys (a page holds at least 16) of the wave's (base + i)-th chunk.
-  const int32_t* table = a.table + (int64_t)b * a.table_s;
-  int ids = 0;
-  uint64_t ok = 0;
-  auto window = [&](int base) {
-    const int key = lo + (wave + NW * (base + (lane >> 1))) * kSub + 16 * (lane & 1);
-    ids = key < hi ? table[key >> a.page_shift] : -1;
-    ok = __ballot((unsigned)ids < (unsigned)a.pages);
-  };
-  u32x4 kr[4], vr[4];  // lane + 64 j -> key row 8 j + lane / 8 of the chunk, 16-byte part lane % 8
-  uint32_t okc = 0;    // halves of the chunk whose page exists
-  auto load = [&](int i) {  // the wave's i-th chunk
-    const int c0 = lo + (wave + NW * i) * kSub;
-    okc = 0;
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int at = 2 * (i & 31) + hh;
-      const int key = c0 + 16 * hh;
-      const bool there = (ok >> at) & 1;
-      const int64_t page = __builtin_amdgcn_readlane(ids, at);
-      const int64_t slot = key & (a.page - 1);
-      const uint64_t kb = there ? (uint64_t)(uintptr_t)(a.k + page * a.sk_p + h * a.sk_h + slot * a.sk_s)
-                                : (uint64_t)(uintptr_t)zero_row;
-      const uint64_t vb = there ? (uint64_t)(uintptr_t)(a.v + page * a.sv_p + h * a.sv_h + slot * a.sv_s)
-                                : (uint64_t)(uintptr_t)zero_row;
-      okc |= there ? 1u << hh : 0u;
-      const int lim = there ? hi - 1 - key : 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int rr = (lane >> 3) + 8 * j;
-        const int rl = rr < lim ? rr : lim;
-        kr[2 * hh + j] = __builtin_nontemporal_load((global_u32x4*)(kb + 2 * ((int64_t)rl * a.sk_s + 8 * (lane & 7))));
-        vr[2 * hh + j] = __builtin_nontemporal_load((global_u32x4*)(vb + 2 * ((int64_t)rl * a.sv_s + 8 * (lane & 7))));
-      }
-    }
-  };
 
   f32x16 oacc[2] = {};
   float m = -INFINITY, lsum = 0.f;
   const int tr_row = (lane & 15) >> 2;
   const int tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-  const int mine = n_chunks > wave ? (n_chunks - wave + NW - 1) / NW : 0;
-  if (mine > 0) {
-    window(0);
-    load(0);
-  }
-  for (int i = 0; i < mine; ++i) {
-    const int c0 = lo + (wave + NW * i) * kSub;
-    const uint32_t there = okc;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int off = ((lane >> 3) + 8 * j) * kStride + 8 * (lane & 7);
-      *reinterpret_cast<u32x4*>(&ks[off]) = kr[j];
-      *reinterpret_cast<u32x4*>(&vs[off]) = vr[j];
-    }
-    if (i + 1 < mine) {
-      if (((i + 1) & 31) == 0) window(i + 1);
-      load(i + 1);
-    }
-    // S^T (32 keys x 32 rows): A = K rows from the tile (lane: key l32, d 16c + 8g .. +7).
+  for (int i = 0; i < kv.mine; ++i) {
+    const int c0 = kv.first_key(i);
+    const uint32_t there = kv.there;
+    kv.stage(ks, vs);
+    if (i + 1 < kv.mine) kv.load(i + 1);
+    // A = K rows from the tile (lane: key l32, d 16c + 8g .. +7).
     f32x16 s = {};
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       s = mfma32(*reinterpret_cast<const bf16x8*>(&ks[l32 * kStride + 16 * c + 8 * g]), qreg[c], s);
     if (c0 + kSub > kfull || c0 + kSub > hi || there != 3) {
-      const int lim = khi < hi ? khi : hi;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = c0 + 8 * (r >> 2) + 4 * g + (r & 3);
-        s[r] = key < lim && ((there >> (r >> 3)) & 1) ? s[r] : -INFINITY;
+        s[r] = key < khi && ((there >> (r >> 3)) & 1) ? s[r] : -INFINITY;
       }
     }
     float mx = -INFINITY;
@@ -200,11 +254,11 @@ __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
       oacc[0] *= alpha;
       oacc[1] *= alpha;
     }
-    const float m_use = (m == -INFINITY) ? 0.f : m;
+    const float mu = (m == -INFINITY) ? 0.f : m;
     float p[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      p[r] = fast_exp2(fmaf(s[r], a.scale_log2, -m_use));
+      p[r] = fast_exp2(fmaf(s[r], a.scale_log2, -mu));
       lsum += p[r];
     }
 #pragma unroll
@@ -221,10 +275,9 @@ __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
     }
   }
 
-  // Merge the waves' states.
   lsum = sum_xor32(lsum);
   __syncthreads();  // the tiles are reused below
-  MergeLds<NW>* ml = reinterpret_cast<MergeLds<NW>*>(smem);
+  auto* ml = reinterpret_cast<MergeLds<NW, kQT>*>(smem);
 #pragma unroll
   for (int db = 0; db < 2; ++db)
 #pragma unroll
@@ -236,39 +289,115 @@ __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
     ml->l[wave][l32] = lsum;
   }
   __syncthreads();
+#pragma unroll
+  for (int t0 = 0; t0 < kQT; t0 += NW * 4) ml->write_row(a, sq, sp, it, t0 + (tid >> 4), 4 * (tid & 15));
+}
 
-  const int64_t slot = ((int64_t)bh * a.q_tiles + qt) * a.n_splits + split;
+// Up to 16 rows (a block of 16, a few tokens of shared heads, one token): the same
+// on v_mfma_f32_16x16x32_bf16, so no MFMA row or softmax lane is spent on absent
+// rows. S^T of 16 keys x 16 rows: A = K read from the tile (lane: key 16 kb + lane %
+// 16, d 32 c + 8 hq .. +7, hq = lane / 16), B = Q^T; result lane (row lane % 16, hq)
+// holds keys 16 kb + 4 hq + r. O^T (16 d x 16 rows) += V^T P^T over the 32 keys.
+template <int NW>
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 4 : 2) void paged16_kernel(PagedArgs a) {
+  constexpr int kRows = 16;
+  __shared__ __attribute__((aligned(16))) char smem[chunk_smem<NW, kRows>()];
+  const int tid = wi_x();
+  const int lane = tid & 63;
+  const int wave = wave_uniform(tid >> 6);
+  const int l16 = lane & 15;
+  const int hq = lane >> 4;
+  __bf16* ks = reinterpret_cast<__bf16*>(smem) + wave * 2 * kSub * kStride;
+  __bf16* vs = ks + kSub * kStride;
+
+  const PagedItem it(a);
+  const PagedSeq sq(a, it.b);
+  if (it.qt * kRows >= sq.rows) return;
+  const int key_end = sq.tile_end(a, 0);
+  const PagedSplit sp(a, key_end);
+  if (it.split >= sp.n) return;
+  const int lo = it.split * sp.len;
+  const int hi = lo + sp.len < key_end ? lo + sp.len : key_end;
+  ChunkStream<NW> kv(a, it.b, it.h, lo, hi, wave, lane);
+  if (kv.mine > 0) kv.load(0);
+
+  const int row = l16 < sq.rows ? l16 : sq.rows - 1;
+  const int tok = row / a.group;
+  const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(it.h * a.group + row - tok * a.group) * a.sq_h;
+  bf16x8 qreg[2];
 #pragma unroll
-  for (int t0 = 0; t0 < kQT; t0 += NW * 4) {
-    const int rt = t0 + (tid >> 4), d = 4 * (tid & 15);
-    float mw[NW], mm = -INFINITY;
+  for (int c = 0; c < 2; ++c) qreg[c] = __builtin_bit_cast(bf16x8, ld16(qp + 32 * c + 8 * hq));
+  const int ends = sq.key_end(a, tok);
+  const int khi = ends < hi ? ends : hi;
+  const int kfull = wave_uniform(sq.key_end(a, 0));  // every row sees these
+
+  f32x4 o[4] = {};  // O^T [16-d block]: lane (row l16, hq) holds d 16 db + 4 hq + r
+  float m = -INFINITY, lsum = 0.f;
+  const int tr_row = l16 >> 2;
+  const int tr_col = 4 * (lane & 3);
+  for (int i = 0; i < kv.mine; ++i) {
+    const int c0 = kv.first_key(i);
+    const uint32_t there = kv.there;
+    kv.stage(ks, vs);
+    if (i + 1 < kv.mine) kv.load(i + 1);
+    f32x4 s[2];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      mw[w] = ml->m[w][rt];
-      mm = fmaxf(mm, mw[w]);
+    for (int kb = 0; kb < 2; ++kb) {
+      const __bf16* kt = &ks[(16 * kb + l16) * kStride + 8 * hq];
+      s[kb] = mfma16(*reinterpret_cast<const bf16x8*>(kt), qreg[0], f32x4{});
+      s[kb] = mfma16(*reinterpret_cast<const bf16x8*>(kt + 32), qreg[1], s[kb]);
     }
-    const float mu = (mm == -INFINITY) ? 0.f : mm;
-    float lt = 0.f;
-    f32x4 ot = {};
+    if (c0 + kSub > kfull || c0 + kSub > hi || there != 3) {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float wgt = fast_exp2(mw[w] - mu);
-      lt += wgt * ml->l[w][rt];
-      ot += wgt * *reinterpret_cast<const f32x4*>(&ml->o[w][rt][d]);
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[kb][r] = c0 + 16 * kb + 4 * hq + r < khi && ((there >> kb) & 1) ? s[kb][r] : -INFINITY;
     }
-    const float inv = lt > 0.f ? 1.f / lt : 0.f;  // a row that sees no key: 0
-    if (sp.n == 1) {
-      if (r0 + rt < sq.rows) {
-        const int t = (r0 + rt) / a.group;
-        *reinterpret_cast<bf16x4*>(a.o + (int64_t)(sq.q0 + t) * a.so_t +
-                                   (int64_t)(h * a.group + r0 + rt - t * a.group) * a.so_h + d) =
-            to_bf16x4(ot[0] * inv, ot[1] * inv, ot[2] * inv, ot[3] * inv);
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mx = fmaxf(mx, shfl_xor(mx, 16));
+    mx = max_xor32(mx);
+    const float mt = mx * a.scale_log2;
+    if (__ballot(mt > m) != 0) {
+      const float mn = fmaxf(m, mt);
+      const float alpha = (mn == -INFINITY) ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db) o[db] *= alpha;
+    }
+    const float mu = (m == -INFINITY) ? 0.f : m;
+    float p[2][4];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[kb][r] = fast_exp2(fmaf(s[kb][r], a.scale_log2, -mu));
+        lsum += p[kb][r];
       }
-    } else {
-      *reinterpret_cast<f32x4*>(&a.part_o[(slot * kQT + rt) * kHeadDim + d]) = ot * inv;
-      if (d == 0) a.part_lse[slot * kQT + rt] = lt > 0.f ? mm + fast_log2(lt) : -INFINITY;
+    const bf16x8 pop = to_bf16x8(p[0][0], p[0][1], p[0][2], p[0][3], p[1][0], p[1][1], p[1][2], p[1][3]);
+    const int vrow = 4 * hq + tr_row;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+      const bf16x8 va = cat8(lds_read_tr(&vs[vrow * kStride + 16 * db + tr_col]),
+                             lds_read_tr(&vs[(vrow + 16) * kStride + 16 * db + tr_col]));
+      o[db] = mfma16(va, pop, o[db]);
     }
   }
+
+  lsum += shfl_xor(lsum, 16);
+  lsum = sum_xor32(lsum);
+  __syncthreads();  // the tiles are reused below
+  auto* ml = reinterpret_cast<MergeLds<NW, kRows>*>(smem);
+#pragma unroll
+  for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(&ml->o[wave][l16][16 * db + 4 * hq]) = o[db];
+  if (hq == 0) {
+    ml->m[wave][l16] = m;
+    ml->l[wave][l16] = lsum;
+  }
+  __syncthreads();
+  if (tid < 16 * kRows) ml->write_row(a, sq, sp, it, tid >> 4, 4 * (tid & 15));
 }
 
 // Chunks of more than 64 rows: 128-row tiles, four waves of 32 rows that share each
@@ -630,7 +759,14 @@ hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream) {
     else
       hipLaunchKernelGGL(paged128_kernel<1>, grid, dim3(256), 0, stream, a);
   } else {
-    hipLaunchKernelGGL(paged32_kernel<4>, grid, dim3(256), 0, stream, a);
+    if (a.tile == 16 && a.subs == 2)
+      hipLaunchKernelGGL(paged16_kernel<8>, grid, dim3(512), 0, stream, a);
+    else if (a.tile == 16)
+      hipLaunchKernelGGL(paged16_kernel<4>, grid, dim3(256), 0, stream, a);
+    else if (a.subs == 2)
+      hipLaunchKernelGGL(paged32_kernel<8>, grid, dim3(512), 0, stream, a);
+    else
+      hipLaunchKernelGGL(paged32_kernel<4>, grid, dim3(256), 0, stream, a);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.n_splits == 1) return e;

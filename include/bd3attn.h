@@ -334,8 +334,8 @@ int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t
  *   page_table: device int32 (seqs, table_width); q_starts: device int32 (seqs +
  *     1), ascending; kv_lens: device int32 (seqs).
  *   max_q, max_kv: the host's bounds of a chunk's tokens and a sequence's keys
- *     (max_kv <= table_width * page_size). They size the launch: tokens beyond
- *     max_q may be left out and keys beyond max_kv are not seen.
+ *     (max_kv <= table_width * page_size). They size the launch: a chunk's
+ *     tokens beyond max_q are left out and keys beyond max_kv are not seen.
  *   total_kv: about the sum of kv_lens, 0 .. seqs * max_kv: chooses how the keys
  *     are cut over workgroups, not what is computed.
  *   strides: 11 int64 element strides: q (token, head), k_pages (page, head,
