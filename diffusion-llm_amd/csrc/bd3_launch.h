@@ -148,6 +148,19 @@ struct GlueArgs {
   int row0;                   // first row of the launch (rows: the one past its last)
 };
 
+// Division of 0 <= n < 2^31 by a number d known at the launch: the upper word of n
+// times m = floor(2^(31 + s) / d) + 1, 2^(s - 1) < d <= 2^s, exceeds n / d by n e / (d
+// 2^(31 + s)) with 0 < e <= d <= 2^s, less than 1 / d, so its floor is exact.
+struct FastDiv {
+  uint32_t m;
+  int s;  // -1: d is 1
+  static FastDiv of(int d) {
+    int s = 0;
+    while (((int64_t)1 << s) < d) ++s;
+    return s == 0 ? FastDiv{0, -1} : FastDiv{(uint32_t)(((uint64_t)1 << (31 + s)) / (uint32_t)d + 1), s - 1};
+  }
+};
+
 constexpr int kPagedMaxKeys = 1 << 30;  // of a sequence: key positions stay below 2^31 when rounded up to a block
 struct PagedArgs {
   const uint16_t* q;        // (tokens, heads, 64)
@@ -164,13 +177,17 @@ struct PagedArgs {
   int max_q;      // most tokens of a chunk: the caller's bound
   int max_kv;     // most keys of a sequence: the caller's bound, at most the table's
   int bs;
+  FastDiv bs_div, group_div, kv_heads_div;
   int tile;       // query rows per workgroup
   int subs;       // sets of 4 waves per workgroup: 1, 2 or (128-row tiles) 4
   int q_tiles;    // tiles of the longest chunk
   int q_slots;    // its 32-row partial slots
   int n_splits;   // most key ranges of a tile
-  int split_len;  // most keys of a range
-  int unit;       // ranges are whole units of keys
+  int split_shift;  // log2 of a range's keys
+  int workgroups;
+  // 128-row tiles: the most that all chunks together have, and the order of TileItem.
+  int tiles, levels;
+  FastDiv level_div;
   float scale_log2;
 };
 

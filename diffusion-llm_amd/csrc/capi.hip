@@ -878,27 +878,74 @@ int log2_of(int32_t x) {
   return s;
 }
 
-// What a paged attention call runs: rows per workgroup, tiles and partial slots
-// of the longest chunk, key ranges.
+// What a paged attention call runs: rows per workgroup, sets of four waves that
+// share an item, tiles and partial slots of the longest chunk, key ranges.
 struct PagedPlan {
-  int tile, subs, q_tiles, q_slots, n_splits, split_len, unit;
+  int tile, subs, q_tiles, q_slots, n_splits, split_shift;
 };
 
-PagedPlan paged_plan(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
+// Estimated us of a plan, to choose the sets and the length of the key ranges: the
+// longest item's chain of 64-key steps against the load per CU, then the merge
+// launch. Fitted to 2100 timings of 450 batches drawn over 1-64 sequences, 1-3000
+// tokens a chunk, 20-10000 keys, 1-16 KV heads and groups of 1-12 (rms error 7-11%).
+double paged_us(int tile, int subs, double longest, double keys, double items, bool split) {
+  struct Cost {
+    double chain0, chain, load0, load, item, merge, merge_item;
+  };
+  static constexpr Cost kRows16 = {4.7, 0.37, 2.8, 0.62, 1.4, 2.9, 0.0};  // two sets
+  static constexpr Cost kRows32[2] = {{4.8, 0.67, 4.1, 0.63, 0.74, 2.8, 0.79}, {5.6, 0.35, 2.0, 0.58, 4.4, 3.4, 0.0}};
+  static constexpr Cost kRows128[3] = {{4.3, 1.05, 5.8, 0.56, 1.8, 4.3, 1.85},
+                                       {4.6, 0.71, 6.0, 0.57, 3.2, 3.9, 1.88},
+                                       {8.4, 0.53, 0.0, 0.59, 9.8, 0.0, 0.0}};  // four sets: never with ranges
+  const Cost& c = tile == 16 ? kRows16 : tile == 32 ? kRows32[subs - 1] : kRows128[subs >> 1];
+  const double chain = c.chain0 + c.chain * longest / 64.0;
+  const double load = c.load0 + c.load * keys / (64.0 * 256.0) + c.item * items / 256.0;
+  return std::cbrt(chain * chain * chain + load * load * load) + (split ? c.merge + c.merge_item * items / 256.0 : 0.0);
+}
+
+// The cheapest plan of the sets and ranges (256 keys and longer, at most 64 of a
+// sequence) for what the host knows: bounds, tokens and the keys in all. Ranges pay
+// where a few long sequences would leave the chip idle. Of 150 batches of each
+// tile the plan takes 0.7% (16 rows), 2% and 1.5% more than the best one. us, whole
+// items -> plan: 12 heads, 16 over 3600 keys 24.7 -> 11.7; 32 sequences of
+// 100-8192 keys 65.7 -> 51.3; 8 chunks of 66-524 tokens over 200-4000 44.5 (one set,
+// 512-key ranges) -> 31.6 (four sets).
+PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
                      int64_t total_kv) {
   PagedPlan p;
-  const int64_t rows = (int64_t)max_q * (heads / kv_heads);
+  const int64_t group = heads / kv_heads, rows = (int64_t)max_q * group;
   p.tile = rows <= 16 ? 16 : rows <= 64 ? 32 : 128;
-  p.unit = rows <= 64 ? 32 : 64;
-  p.subs = 1;
   p.q_tiles = (int)((rows + p.tile - 1) / p.tile);
   p.q_slots = (int)((rows + 31) / 32);
-  const int64_t work = std::min(total_kv, (int64_t)seqs * max_kv) * kv_heads * p.q_tiles;
-  int64_t len = std::max<int64_t>(256, work / 512);
-  len = std::max<int64_t>(len, (max_kv + 63) / 64);
-  len = (len + p.unit - 1) / p.unit * p.unit;
-  p.n_splits = (int)std::max<int64_t>(1, (max_kv + len - 1) / len);
-  p.split_len = (int)std::min<int64_t>(len, INT32_MAX);
+  const double total = (double)std::min(total_kv, (int64_t)seqs * max_kv), bh = (double)seqs * kv_heads;
+  double units = bh * p.q_tiles, seen = total / seqs;  // items without ranges, keys that one sees
+  if (p.tile == 128) {
+    units = std::min(units, kv_heads * ((double)tokens * (double)group / 128.0 + 0.5 * seqs));
+    seen = std::max(1.0, seen - 0.5 * tokens / seqs);
+  }
+  double best = INFINITY;
+  p.subs = 0;
+  p.n_splits = 1;
+  p.split_shift = 30;
+  for (int subs = p.tile == 16 ? 2 : 1; subs <= (p.tile == 128 ? 4 : 2); subs *= 2) {
+    const double whole = paged_us(p.tile, subs, max_kv, units * seen, units, false);
+    if (whole < best) {
+      best = whole;
+      p.subs = subs;
+      p.split_shift = 30;
+    }
+    for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
+      if (max_kv >> shift > 64) continue;
+      const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
+      const double us = paged_us(p.tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items, true);
+      if (us < best) {
+        best = us;
+        p.subs = subs;
+        p.split_shift = shift;
+      }
+    }
+  }
+  p.n_splits = std::max(1, (int)(((int64_t)max_kv + ((int64_t)1 << p.split_shift >> 1)) >> p.split_shift));
   return p;
 }
 
@@ -906,19 +953,18 @@ size_t paged_part_rows(const PagedPlan& p, int32_t seqs, int32_t kv_heads) {
   return p.n_splits > 1 ? (size_t)seqs * kv_heads * p.q_slots * p.n_splits * 32 : 0;
 }
 
-bool paged_bounds_ok(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv, int64_t total_kv) {
-  return seqs >= 1 && kv_heads >= 1 && heads >= kv_heads && max_q >= 1 && max_kv >= 1 &&
-         max_kv <= bd3::kPagedMaxKeys && total_kv >= 0;
-}
-
 }  // namespace
 
 extern "C" {
 
-size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
-                                      int64_t total_kv) {
-  if (!paged_bounds_ok(seqs, heads, kv_heads, max_q, max_kv, total_kv)) return 0;
-  const size_t rows = paged_part_rows(paged_plan(seqs, heads, kv_heads, max_q, max_kv, total_kv), seqs, kv_heads);
+size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q,
+                                      int32_t max_kv, int64_t total_kv) {
+  if (seqs < 1 || tokens < 1 || kv_heads < 1 || heads < kv_heads || max_q < 1 || max_kv < 0 ||
+      max_kv > bd3::kPagedMaxKeys || total_kv < 0)
+    return 0;
+  max_q = std::min(max_q, tokens);
+  max_kv = std::max(max_kv, 1);
+  const size_t rows = paged_part_rows(paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv), seqs, kv_heads);
   return rows == 0 ? 0 : align256(rows * bd3::kHeadDim * 4) + rows * 4;
 }
 
@@ -947,15 +993,15 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   if (strides[4] >= kMaxDmaSeqStride || strides[7] >= kMaxDmaSeqStride)
     return fail(BD3_EINVAL, "page slot strides must be < 2^24 elements");
   if (strides[10] < 0) return fail(BD3_EINVAL, "page_table stride must be >= 0");
-  const PagedPlan plan = paged_plan(seqs, heads, kv_heads, max_q, max_kv, total_kv);
+  const PagedPlan plan = paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
   const size_t rows = paged_part_rows(plan, seqs, kv_heads);
   const size_t po_bytes = align256(rows * bd3::kHeadDim * 4);
   const size_t need = rows == 0 ? 0 : po_bytes + rows * 4;
   if (workspace_bytes < need) return fail(BD3_EINVAL, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
   if (need > 0 && (workspace == nullptr || !aligned16(workspace)))
     return fail(BD3_EINVAL, "workspace must be a 16-byte aligned device pointer");
-  if ((int64_t)seqs * kv_heads * std::max((int64_t)plan.q_tiles * plan.n_splits, (int64_t)plan.q_slots) >=
-      ((int64_t)1 << 22))
+  const int64_t most = (int64_t)seqs * kv_heads * plan.q_tiles * plan.n_splits;
+  if (std::max(most, (int64_t)seqs * kv_heads * plan.q_slots) >= ((int64_t)1 << 22))
     return fail(BD3_EINVAL, "seqs * kv_heads * tiles * ranges too large (limit 2^22 workgroups)");
   bd3::PagedArgs a = {};
   a.q = static_cast<const uint16_t*>(q);
@@ -995,8 +1041,19 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.q_tiles = plan.q_tiles;
   a.q_slots = plan.q_slots;
   a.n_splits = plan.n_splits;
-  a.split_len = plan.split_len;
-  a.unit = plan.unit;
+  a.split_shift = plan.split_shift;
+  a.bs_div = bd3::FastDiv::of(a.bs);
+  a.group_div = bd3::FastDiv::of(a.group);
+  a.kv_heads_div = bd3::FastDiv::of(kv_heads);
+  if (plan.tile < 128) {  // about as many as there are items
+    a.workgroups = (int)std::min(most, ((total_kv >> plan.split_shift) + seqs) * kv_heads * plan.q_tiles);
+  } else {
+    a.tiles = (int)std::min((int64_t)seqs * plan.q_tiles, (int64_t)tokens * a.group / 128 + seqs);
+    const int unit = std::max(1, 128 / a.group);
+    a.level_div = bd3::FastDiv::of(unit);
+    a.levels = max_kv / unit + 1 + plan.q_tiles;
+    a.workgroups = a.tiles * kv_heads * plan.n_splits;
+  }
   a.scale_log2 = scale * bd3::kLog2e;
   return hip_status(bd3::launch_paged_attn(a, static_cast<hipStream_t>(stream)), "paged_attn launch");
 }

@@ -425,8 +425,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       out = token_rows(out, T, H, q);
       if (max_kv < 0) max_kv = (int32_t)std::min<int64_t>((int64_t)b.width * b.page, INT32_MAX);
       if (total < 0) total = (int64_t)b.seqs * max_kv;
-      const int32_t mq = std::min(max_q, T);
-      const size_t bytes = g_lib.paged_attn_workspace_bytes(b.seqs, H, b.kv_heads, mq, std::max(max_kv, 1), total);
+      const size_t bytes = g_lib.paged_attn_workspace_bytes(b.seqs, T, H, b.kv_heads, max_q, max_kv, total);
       const Tensor ws = bytes ? workspace(bytes, q) : Tensor();
       const int64_t st[11] = {q.stride(0),   q.stride(1),   b.k.stride(0),   b.k.stride(1),   b.k.stride(2), b.v.stride(0),
                               b.v.stride(1), b.v.stride(2), out.stride(0), out.stride(1), b.table.stride(0)};

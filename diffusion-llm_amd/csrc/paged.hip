@@ -32,37 +32,47 @@ typedef const __attribute__((address_space(1))) u32x4 global_u32x4;
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
+__device__ __forceinline__ int fast_div(int n, FastDiv d) {
+  return d.s < 0 ? n : (int)(__umulhi((uint32_t)n, d.m) >> d.s);
+}
+
 // One sequence's share of the batch, bounded (see above).
 struct PagedSeq {
   int q0, n, kv, rows;
+  PagedSeq() = default;
   __device__ __forceinline__ PagedSeq(const PagedArgs& a, int b) {
-    q0 = wave_uniform(clampi(a.q_starts[b], 0, a.tokens));
-    n = wave_uniform(clampi(a.q_starts[b + 1], q0, a.tokens)) - q0;
-    kv = wave_uniform(clampi(a.kv_lens[b], 0, a.max_kv));
+    q0 = clampi(a.q_starts[b], 0, a.tokens);
+    n = clampi(a.q_starts[b + 1], q0, a.tokens) - q0;
+    kv = clampi(a.kv_lens[b], 0, a.max_kv);
     rows = (n < a.max_q ? n : a.max_q) * a.group;  // what the launch and its partials have room for
+  }
+  __device__ __forceinline__ PagedSeq of_lane(int lane) const {
+    PagedSeq r;
+    r.q0 = __builtin_amdgcn_readlane(q0, lane);
+    r.n = __builtin_amdgcn_readlane(n, lane);
+    r.kv = __builtin_amdgcn_readlane(kv, lane);
+    r.rows = __builtin_amdgcn_readlane(rows, lane);
+    return r;
   }
   // Keys that token i sees: [0, key_end).
   __device__ __forceinline__ int key_end(const PagedArgs& a, int i) const {
     const int p = kv - n + i;
-    const int e = (p / a.bs + 1) * a.bs;
+    const int e = (fast_div(p < 0 ? 0 : p, a.bs_div) + 1) * a.bs;
     return p < 0 ? 0 : (e < kv ? e : kv);
   }
   // One past the last key of the tile of `tile` rows at row r0 (r0 < rows).
   __device__ __forceinline__ int tile_end(const PagedArgs& a, int r0) const {
     const int last = (r0 + a.tile < rows ? r0 + a.tile : rows) - 1;
-    return wave_uniform(key_end(a, last / a.group));
+    return wave_uniform(key_end(a, fast_div(last, a.group_div)));
   }
 };
 
-// The key ranges of a tile that sees `keys` keys: `n` of `len` keys, equal ones.
-struct PagedSplit {
-  int n, len;
-  __device__ __forceinline__ PagedSplit(const PagedArgs& a, int keys) {
-    const int want = keys > a.split_len ? (keys + a.split_len - 1) / a.split_len : 1;
-    len = ((keys + want - 1) / want + a.unit - 1) / a.unit * a.unit;
-    n = keys > 0 ? (keys + len - 1) / len : 1;
-  }
-};
+// Ranges of 2^split_shift keys that `keys` keys are cut into; what is left over, up to
+// half a range, goes to the last one.
+__device__ __forceinline__ int key_ranges(const PagedArgs& a, int keys) {
+  const int n = (keys + (1 << a.split_shift >> 1)) >> a.split_shift;
+  return n > 1 ? n : 1;
+}
 
 // The 32-key chunks of one key range that one of NW waves takes in turn (chunks
 // wave, wave + NW, ...): from the pages to registers, the next chunk's loads in
@@ -124,16 +134,118 @@ struct ChunkStream {
   }
 };
 
-// The workgroup's item of a 16- or 32-row launch: (range, row tile, sequence * KV head).
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+  return v;
+}
+
+// Item `id` of the 16- and 32-row launches: KV head (fastest), row tile, range, in the
+// order of the sequences. Every sequence has items of its own number, so the list
+// is made here from the lengths, a lane a sequence: a launch of the most items that
+// the bounds allow spent about 1 ns on each empty workgroup (32 sequences of
+// 100-8192 keys, 12 heads: 67 us at the best range length, 55 with the list).
 struct PagedItem {
-  int split, qt, bh, b, h;
-  __device__ __forceinline__ PagedItem(const PagedArgs& a) {
-    const int id = wg_x();
-    split = id % a.n_splits;
-    qt = id / a.n_splits % a.q_tiles;
-    bh = id / a.n_splits / a.q_tiles;
-    b = bh / a.kv_heads;
-    h = bh - b * a.kv_heads;
+  int b, h, qt, split;
+  PagedSeq sq;
+  int total;  // items of all, or (more than 64 sequences) INT_MAX while not known
+  bool found;
+  __device__ __forceinline__ PagedItem(const PagedArgs& a, int id) {
+    const int lane = wi_x() & 63;
+    const int j = wave_uniform(fast_div(id, a.kv_heads_div));
+    h = id - j * a.kv_heads;
+    found = false;
+    int before = 0;  // items of the sequences up to s0, of one head
+    for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+      PagedSeq mine = {};
+      int items = 0, tiles = 0;
+      if (s0 + lane < a.seqs) {
+        mine = PagedSeq(a, s0 + lane);
+        tiles = (mine.rows + a.tile - 1) / a.tile;
+        items = tiles * key_ranges(a, mine.kv);
+      }
+      const int upto = wave_scan(items);
+      const int at = __popcll(__ballot(before + upto <= j));
+      total = s0 + 64 < a.seqs ? INT32_MAX : (before + __builtin_amdgcn_readlane(upto, 63)) * a.kv_heads;
+      if (at < 64) {
+        int rem = j - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(items, at));
+        const int t = __builtin_amdgcn_readlane(tiles, at);
+        b = s0 + at;
+        sq = mine.of_lane(at);
+        for (split = 0; rem >= t; rem -= t) ++split;
+        qt = rem;
+        found = true;
+        return;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+};
+
+// Tile `j` of all sequences' 128-row tiles of one head, those that see most keys
+// first (up to 64 sequences; beyond, in the order of the sequences). A sequence's
+// tiles, last one first, see kv, kv - u, kv - 2 u, ... keys (u tokens a tile), so its
+// r-th one belongs to level (max_kv - kv) / u + r, and the tiles below level l number
+// the sum of clamp(l - first level, 0, tiles): a binary search finds j's level, a
+// lane a sequence.
+struct TileItem {
+  int b, rank;
+  PagedSeq sq;
+  bool found;
+  __device__ __forceinline__ TileItem(const PagedArgs& a, int j) {
+    const int lane = wi_x() & 63;
+    found = false;
+    if (a.seqs <= 64) {
+      PagedSeq mine = {};
+      if (lane < a.seqs) mine = PagedSeq(a, lane);
+      const int tiles = (mine.rows + 127) / 128;
+      const int first = fast_div(a.max_kv - mine.kv, a.level_div);
+      auto below = [&](int level) {
+        const int c = level - first < tiles ? level - first : tiles;
+        return __builtin_amdgcn_readlane(wave_scan(c > 0 ? c : 0), 63);
+      };
+      int lo = 0, hi = a.levels;  // below(lo) <= j < below(hi)
+      if (j >= below(hi)) return;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (below(mid) <= j)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const int nth = j - below(lo);  // of the level's tiles (found with every lane active: the sum is over all)
+      const bool live = lo >= first && lo < first + tiles;
+      const uint64_t all = __ballot(live);
+      const int mine_th = __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+      const uint64_t it = __ballot(live && mine_th == nth);
+      if (it == 0) return;
+      b = __builtin_ctzll(it);
+      sq = mine.of_lane(b);
+      rank = lo - __builtin_amdgcn_readlane(first, b);
+      found = true;
+      return;
+    }
+    int before = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+      PagedSeq mine = {};
+      if (s0 + lane < a.seqs) mine = PagedSeq(a, s0 + lane);
+      const int tiles = (mine.rows + 127) / 128;
+      const int upto = wave_scan(tiles);
+      const int at = __popcll(__ballot(before + upto <= j));
+      if (at < 64) {
+        rank = j - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(tiles, at));
+        b = s0 + at;
+        sq = mine.of_lane(at);
+        found = true;
+        return;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
   }
 };
 
@@ -144,8 +256,8 @@ struct MergeLds {
   float o[NW][ROWS][kMergeRow];
   float m[NW][ROWS];
   float l[NW][ROWS];
-  __device__ __forceinline__ void write_row(const PagedArgs& a, const PagedSeq& sq, const PagedSplit& sp,
-                                            const PagedItem& it, int rt, int d) const {
+  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const PagedItem& it, int rt,
+                                            int d) const {
     float mw[NW], mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
@@ -162,16 +274,16 @@ struct MergeLds {
       ot += wgt * *reinterpret_cast<const f32x4*>(&o[w][rt][d]);
     }
     const float inv = lt > 0.f ? 1.f / lt : 0.f;  // a row that sees no key: 0
-    if (sp.n == 1) {
+    if (ranges == 1) {
       const int row = it.qt * ROWS + rt;
-      if (row < sq.rows) {
-        const int t = row / a.group;
-        *reinterpret_cast<bf16x4*>(a.o + (int64_t)(sq.q0 + t) * a.so_t +
+      if (row < it.sq.rows) {
+        const int t = fast_div(row, a.group_div);
+        *reinterpret_cast<bf16x4*>(a.o + (int64_t)(it.sq.q0 + t) * a.so_t +
                                    (int64_t)(it.h * a.group + row - t * a.group) * a.so_h + d) =
             to_bf16x4(ot[0] * inv, ot[1] * inv, ot[2] * inv, ot[3] * inv);
       }
     } else {
-      const int64_t slot = ((int64_t)it.bh * a.q_slots + it.qt) * a.n_splits + it.split;
+      const int64_t slot = (((int64_t)it.b * a.kv_heads + it.h) * a.q_slots + it.qt) * a.n_splits + it.split;
       *reinterpret_cast<f32x4*>(&a.part_o[(slot * kQT + rt) * kHeadDim + d]) = ot * inv;
       if (d == 0) a.part_lse[slot * kQT + rt] = lt > 0.f ? mm + fast_log2(lt) : -INFINITY;
     }
@@ -187,8 +299,7 @@ constexpr size_t chunk_smem() {
 // keys x 32 rows) = K Q^T on v_mfma_f32_32x32x16_bf16 with the K tile's rows as A
 // operands; O^T += V^T P^T with V read transposed.
 template <int NW>
-__global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[chunk_smem<NW, kQT>()];
+__device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem& it, char* smem) {
   const int tid = wi_x();
   const int lane = tid & 63;
   const int wave = wave_uniform(tid >> 6);
@@ -197,28 +308,26 @@ __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
   __bf16* ks = reinterpret_cast<__bf16*>(smem) + wave * 2 * kSub * kStride;
   __bf16* vs = ks + kSub * kStride;
 
-  const PagedItem it(a);
-  const PagedSeq sq(a, it.b);
+  const PagedSeq& sq = it.sq;
   const int r0 = it.qt * kQT;
-  if (r0 >= sq.rows) return;
   const int key_end = sq.tile_end(a, r0);
-  const PagedSplit sp(a, key_end);
-  if (it.split >= sp.n) return;
-  const int lo = it.split * sp.len;
-  const int hi = lo + sp.len < key_end ? lo + sp.len : key_end;
+  const int ranges = key_ranges(a, key_end);
+  if (it.split >= ranges) return;
+  const int lo = it.split << a.split_shift;
+  const int hi = it.split + 1 < ranges ? (it.split + 1) << a.split_shift : key_end;
   ChunkStream<NW> kv(a, it.b, it.h, lo, hi, wave, lane);
   if (kv.mine > 0) kv.load(0);
 
   // Q^T B operand: lane holds row r0 + l32 (clamped), d = 16c + 8g .. +7.
   const int row = r0 + l32 < sq.rows ? r0 + l32 : sq.rows - 1;
-  const int tok = row / a.group;
+  const int tok = fast_div(row, a.group_div);
   const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(it.h * a.group + row - tok * a.group) * a.sq_h;
   bf16x8 qreg[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) qreg[c] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * c + 8 * g));
   const int ends = sq.key_end(a, tok);
   const int khi = ends < hi ? ends : hi;
-  const int kfull = wave_uniform(sq.key_end(a, r0 / a.group));  // every row of the tile sees these
+  const int kfull = wave_uniform(sq.key_end(a, fast_div(r0, a.group_div)));  // every row of the tile sees these
 
   f32x16 oacc[2] = {};
   float m = -INFINITY, lsum = 0.f;
@@ -290,7 +399,7 @@ __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
   }
   __syncthreads();
 #pragma unroll
-  for (int t0 = 0; t0 < kQT; t0 += NW * 4) ml->write_row(a, sq, sp, it, t0 + (tid >> 4), 4 * (tid & 15));
+  for (int t0 = 0; t0 < kQT; t0 += NW * 4) ml->write_row(a, ranges, it, t0 + (tid >> 4), 4 * (tid & 15));
 }
 
 // Up to 16 rows (a block of 16, a few tokens of shared heads, one token): the same
@@ -299,9 +408,8 @@ __global__ __launch_bounds__(NW * 64) void paged32_kernel(PagedArgs a) {
 // 16, d 32 c + 8 hq .. +7, hq = lane / 16), B = Q^T; result lane (row lane % 16, hq)
 // holds keys 16 kb + 4 hq + r. O^T (16 d x 16 rows) += V^T P^T over the 32 keys.
 template <int NW>
-__global__ __launch_bounds__(NW * 64, NW == 4 ? 4 : 2) void paged16_kernel(PagedArgs a) {
+__device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem& it, char* smem) {
   constexpr int kRows = 16;
-  __shared__ __attribute__((aligned(16))) char smem[chunk_smem<NW, kRows>()];
   const int tid = wi_x();
   const int lane = tid & 63;
   const int wave = wave_uniform(tid >> 6);
@@ -310,19 +418,17 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 4 : 2) void paged16_kernel(Paged
   __bf16* ks = reinterpret_cast<__bf16*>(smem) + wave * 2 * kSub * kStride;
   __bf16* vs = ks + kSub * kStride;
 
-  const PagedItem it(a);
-  const PagedSeq sq(a, it.b);
-  if (it.qt * kRows >= sq.rows) return;
+  const PagedSeq& sq = it.sq;
   const int key_end = sq.tile_end(a, 0);
-  const PagedSplit sp(a, key_end);
-  if (it.split >= sp.n) return;
-  const int lo = it.split * sp.len;
-  const int hi = lo + sp.len < key_end ? lo + sp.len : key_end;
+  const int ranges = key_ranges(a, key_end);
+  if (it.split >= ranges) return;
+  const int lo = it.split << a.split_shift;
+  const int hi = it.split + 1 < ranges ? (it.split + 1) << a.split_shift : key_end;
   ChunkStream<NW> kv(a, it.b, it.h, lo, hi, wave, lane);
   if (kv.mine > 0) kv.load(0);
 
   const int row = l16 < sq.rows ? l16 : sq.rows - 1;
-  const int tok = row / a.group;
+  const int tok = fast_div(row, a.group_div);
   const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(it.h * a.group + row - tok * a.group) * a.sq_h;
   bf16x8 qreg[2];
 #pragma unroll
@@ -397,7 +503,24 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 4 : 2) void paged16_kernel(Paged
     ml->l[wave][l16] = lsum;
   }
   __syncthreads();
-  if (tid < 16 * kRows) ml->write_row(a, sq, sp, it, tid >> 4, 4 * (tid & 15));
+  if (tid < 16 * kRows) ml->write_row(a, ranges, it, tid >> 4, 4 * (tid & 15));
+}
+
+template <int NW, int ROWS>
+__global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void paged_rows_kernel(PagedArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[chunk_smem<NW, ROWS>()];
+  // The launch has about as many workgroups as there are items; those left over
+  // (lengths that the caller's total did not tell) are taken in turn.
+  for (int id = wg_x();; id += a.workgroups) {
+    const PagedItem it(a, id);
+    if (!it.found) return;
+    if constexpr (ROWS == 16)
+      paged16_item<NW>(a, it, smem);
+    else
+      paged32_item<NW>(a, it, smem);
+    if (id + a.workgroups >= it.total) return;
+    __syncthreads();
+  }
 }
 
 // Chunks of more than 64 rows: 128-row tiles, four waves of 32 rows that share each
@@ -423,28 +546,29 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   const int l32 = lane & 31;
   const int g = lane >> 5;
 
-  // Longest tiles of every sequence first; its KV heads side by side.
-  const int bhs = a.seqs * a.kv_heads;
-  const int bh = wg_x() % bhs;
-  const int split = wg_x() / bhs % a.n_splits;
-  const int rank = wg_x() / bhs / a.n_splits;
-  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  const PagedSeq sq(a, b);
-  const int qt = (sq.rows + 127) / 128 - 1 - rank;
-  if (qt < 0) return;
+  const int per_split = a.tiles * a.kv_heads;
+  const int split = wg_x() / per_split;
+  const int e = wg_x() - split * per_split;
+  const int j = wave_uniform(fast_div(e, a.kv_heads_div));
+  const int h = e - j * a.kv_heads;
+  const TileItem it(a, j);
+  if (!it.found) return;
+  const PagedSeq& sq = it.sq;
+  const int b = it.b, bh = b * a.kv_heads + h;
+  const int qt = (sq.rows + 127) / 128 - 1 - it.rank;
   const int r0 = 128 * qt;
   const int key_end = sq.tile_end(a, r0);
-  const PagedSplit sp(a, key_end);
-  if (split >= sp.n) return;
-  const int lo = split * sp.len;
-  const int hi = lo + sp.len < key_end ? lo + sp.len : key_end;
+  const int ranges = key_ranges(a, key_end);
+  if (split >= ranges) return;
+  const int lo = split << a.split_shift;
+  const int hi = split + 1 < ranges ? (split + 1) << a.split_shift : key_end;
   const int n_tiles = (hi - lo + kSwRows - 1) / kSwRows;  // 0: a tile that sees no key
   const int n_mine = n_tiles > sub ? (n_tiles - sub + SUBS - 1) / SUBS : 0;
 
   const int qrow0 = r0 + 32 * wave;
   const int myr = qrow0 + l32;
   const int row = myr < sq.rows ? myr : sq.rows - 1;
-  const int tok = row / a.group;
+  const int tok = fast_div(row, a.group_div);
   const int64_t head = h * a.group + row - tok * a.group;
   const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + head * a.sq_h;
   bf16x8 qreg[4];
@@ -514,8 +638,8 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
 
   const int khi = sq.key_end(a, tok);  // the lane's row sees [0, khi)
   const int wave_last = qrow0 + 31 < sq.rows ? qrow0 + 31 : sq.rows - 1;
-  const int emax = qrow0 < sq.rows ? wave_uniform(sq.key_end(a, wave_last / a.group)) : 0;
-  const int emin = qrow0 < sq.rows ? wave_uniform(sq.key_end(a, qrow0 / a.group)) : 0;
+  const int emax = qrow0 < sq.rows ? wave_uniform(sq.key_end(a, fast_div(wave_last, a.group_div))) : 0;
+  const int emin = qrow0 < sq.rows ? wave_uniform(sq.key_end(a, fast_div(qrow0, a.group_div))) : 0;
 
   f32x16 o[2] = {};  // O^T [d block]
   float mref = 0.f, lsum = 0.f;
@@ -620,7 +744,7 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   if (myr >= sq.rows) return;
   const bool any = ltot > 0.f;
   const float inv = any ? 1.f / ltot : 0.f;
-  if (sp.n == 1) {
+  if (ranges == 1) {
     uint16_t* op = a.o + (int64_t)(sq.q0 + tok) * a.so_t + head * a.so_h;
 #pragma unroll
     for (int db = 0; db < 2; ++db)
@@ -648,11 +772,11 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
   const int qt = wg_x() % a.q_slots;
   const int bh = wg_x() / a.q_slots;
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  const PagedSeq sq(a, b);
+  const PagedSeq sq = PagedSeq(a, b).of_lane(0);
   const int row = qt * kQT + (wi_x() >> 4);
   if (qt * kQT >= sq.rows) return;
-  const PagedSplit sp(a, sq.tile_end(a, qt * kQT / a.tile * a.tile));
-  if (sp.n <= 1 || row >= sq.rows) return;
+  const int ranges = key_ranges(a, sq.tile_end(a, qt * kQT / a.tile * a.tile));
+  if (ranges <= 1 || row >= sq.rows) return;
   const int d0 = 4 * (wi_x() & 15);
   const int64_t slot0 = ((int64_t)bh * a.q_slots + qt) * a.n_splits;
   const float* lp = a.part_lse + slot0 * kQT + (wi_x() >> 4);
@@ -660,13 +784,13 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
   constexpr int kG = 8;
   float mm = -INFINITY, wt = 0.f;
   f32x4 acc = {};
-  for (int s0 = 0; s0 < sp.n; s0 += kG) {
+  for (int s0 = 0; s0 < ranges; s0 += kG) {
     float l[kG];
     f32x4 po[kG];
 #pragma unroll
     for (int k = 0; k < kG; ++k) {
-      l[k] = s0 + k < sp.n ? lp[(s0 + k) * kQT] : -INFINITY;
-      po[k] = s0 + k < sp.n ? *reinterpret_cast<const f32x4*>(pp + (int64_t)(s0 + k) * kQT * kHeadDim) : f32x4{};
+      l[k] = s0 + k < ranges ? lp[(s0 + k) * kQT] : -INFINITY;
+      po[k] = s0 + k < ranges ? *reinterpret_cast<const f32x4*>(pp + (int64_t)(s0 + k) * kQT * kHeadDim) : f32x4{};
     }
     float mg = mm;
 #pragma unroll
@@ -684,7 +808,7 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
     }
   }
   const float inv = wt > 0.f ? 1.f / wt : 0.f;
-  const int t = row / a.group;
+  const int t = fast_div(row, a.group_div);
   *reinterpret_cast<bf16x4*>(a.o + (int64_t)(sq.q0 + t) * a.so_t + (int64_t)(h * a.group + row - t * a.group) * a.so_h +
                              d0) = to_bf16x4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
 }
@@ -750,7 +874,7 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {
 
 hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream) {
   const int64_t bh = (int64_t)a.seqs * a.kv_heads;
-  const dim3 grid((unsigned)(bh * a.q_tiles * a.n_splits));
+  const dim3 grid((unsigned)a.workgroups);
   if (a.tile == 128) {
     if (a.subs == 4)
       hipLaunchKernelGGL(paged128_kernel<4>, grid, dim3(1024), 0, stream, a);
@@ -759,14 +883,12 @@ hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream) {
     else
       hipLaunchKernelGGL(paged128_kernel<1>, grid, dim3(256), 0, stream, a);
   } else {
-    if (a.tile == 16 && a.subs == 2)
-      hipLaunchKernelGGL(paged16_kernel<8>, grid, dim3(512), 0, stream, a);
-    else if (a.tile == 16)
-      hipLaunchKernelGGL(paged16_kernel<4>, grid, dim3(256), 0, stream, a);
+    if (a.tile == 16)
+      hipLaunchKernelGGL((paged_rows_kernel<8, 16>), grid, dim3(512), 0, stream, a);
     else if (a.subs == 2)
-      hipLaunchKernelGGL(paged32_kernel<8>, grid, dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((paged_rows_kernel<8, 32>), grid, dim3(512), 0, stream, a);
     else
-      hipLaunchKernelGGL(paged32_kernel<4>, grid, dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((paged_rows_kernel<4, 32>), grid, dim3(256), 0, stream, a);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.n_splits == 1) return e;

@@ -349,8 +349,8 @@ int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t
  * depend on the arguments alone, and lengths, tables and starts may change
  * between replays within max_q and max_kv. No reference counterpart.
  */
-size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q,
-                                      int32_t max_kv, int64_t total_kv);
+size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                      int32_t max_q, int32_t max_kv, int64_t total_kv);
 int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* o,
                    const int32_t* page_table, const int32_t* q_starts, const int32_t* kv_lens,
                    int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,

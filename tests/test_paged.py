@@ -200,14 +200,15 @@ def test_no_work_is_no_launch(lib):
 
 def test_workspace(lib):
     size = lib.bd3_paged_attn_workspace_bytes
-    assert size(2, 4, 2, 4, 64, 100) == 0  # nothing to cut
-    need = size(1, 12, 12, 16, 8192, 8192)
+    assert size(2, 8, 4, 2, 4, 64, 100) == 0  # nothing to cut
+    need = size(1, 16, 12, 12, 16, 8192, 8192)
     assert need > 0 and need % 4 == 0
     kw = dict(seqs=1, heads=12, kv_heads=12, tokens=16, max_q=16, width=512, max_kv=8192, total=8192)
     assert attn(lib, **kw, ws=P, ws_bytes=need - 1) == _native.BD3_EINVAL and "too small" in _native.last_error()
     assert attn(lib, **kw, ws=None, ws_bytes=need) == _native.BD3_EINVAL and "aligned" in _native.last_error()
-    for bad in ((0, 12, 12, 16, 8192, 1), (1, 0, 0, 16, 8192, 1), (1, 12, 12, 0, 8192, 1), (1, 12, 12, 16, 0, 1),
-                (1, 12, 12, 16, (1 << 30) + 1, 1), (1, 12, 12, 16, 8192, -1)):
+    for bad in ((0, 16, 12, 12, 16, 8192, 1), (1, 0, 12, 12, 16, 8192, 1), (1, 16, 0, 0, 16, 8192, 1),
+                (1, 16, 12, 12, 0, 8192, 1), (1, 16, 12, 12, 16, -1, 1), (1, 16, 12, 12, 16, (1 << 30) + 1, 1),
+                (1, 16, 12, 12, 16, 8192, -1)):
         assert size(*bad) == 0
 
 
