@@ -170,8 +170,8 @@ struct PagedArgs {
   const int32_t* table;     // (seqs, width) page numbers
   const int32_t* q_starts;  // (seqs + 1)
   const int32_t* kv_lens;   // (seqs)
-  float* part_o;            // (seqs * kv_heads, q_slots, n_splits, 32, 64) fp32, or null
-  float* part_lse;          // (seqs * kv_heads, q_slots, n_splits, 32) log2 LSE, or null
+  float* part_o;            // (seqs * kv_heads, q_slots, n_splits, slot_rows, 64) fp32, or null
+  float* part_lse;          // (seqs * kv_heads, q_slots, n_splits, slot_rows) log2 LSE, or null
   int64_t sq_t, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, so_t, so_h, table_s;  // element strides
   int seqs, tokens, kv_heads, group, pages, page, page_shift;
   int max_q;      // most tokens of a chunk: the caller's bound
@@ -182,6 +182,7 @@ struct PagedArgs {
   int subs;       // sets of 4 waves per workgroup: 1, 2 or (128-row tiles) 4
   int q_tiles;    // tiles of the longest chunk
   int q_slots;    // its 32-row partial slots
+  int slot_rows;  // 32, or the rows there are where the longest chunk has fewer
   int n_splits;   // most key ranges of a tile
   int split_shift;  // log2 of a range's keys
   int workgroups;

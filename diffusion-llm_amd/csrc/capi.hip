@@ -881,7 +881,7 @@ int log2_of(int32_t x) {
 // What a paged attention call runs: rows per workgroup, sets of four waves that
 // share an item, tiles and partial slots of the longest chunk, key ranges.
 struct PagedPlan {
-  int tile, subs, q_tiles, q_slots, n_splits, split_shift;
+  int tile, subs, q_tiles, q_slots, slot_rows, n_splits, split_shift;
 };
 
 // Estimated us of a plan, to choose the sets and the length of the key ranges: the
@@ -917,6 +917,7 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
   p.tile = rows <= 16 ? 16 : rows <= 64 ? 32 : 128;
   p.q_tiles = (int)((rows + p.tile - 1) / p.tile);
   p.q_slots = (int)((rows + 31) / 32);
+  p.slot_rows = (int)std::min<int64_t>(rows, 32);
   const double total = (double)std::min(total_kv, (int64_t)seqs * max_kv), bh = (double)seqs * kv_heads;
   double units = bh * p.q_tiles, seen = total / seqs;  // items without ranges, keys that one sees
   if (p.tile == 128) {
@@ -950,7 +951,7 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
 }
 
 size_t paged_part_rows(const PagedPlan& p, int32_t seqs, int32_t kv_heads) {
-  return p.n_splits > 1 ? (size_t)seqs * kv_heads * p.q_slots * p.n_splits * 32 : 0;
+  return p.n_splits > 1 ? (size_t)seqs * kv_heads * p.q_slots * p.n_splits * p.slot_rows : 0;
 }
 
 }  // namespace
@@ -1040,6 +1041,7 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.subs = plan.subs;
   a.q_tiles = plan.q_tiles;
   a.q_slots = plan.q_slots;
+  a.slot_rows = plan.slot_rows;
   a.n_splits = plan.n_splits;
   a.split_shift = plan.split_shift;
   a.bs_div = bd3::FastDiv::of(a.bs);
@@ -1115,7 +1117,7 @@ int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_
                       const float* repetition, const float* frequency, const float* presence, const float* bias,
                       const int32_t* allowed, float fill, const int64_t* strides, void* stream) {
   if (batch < 0 || rows < 0 || history < 0) return fail(BD3_EINVAL, "batch, rows and history must be >= 0");
-  if (vocab < 1) return fail(BD3_EINVAL, "vocab must be >= 1, got %d", vocab);
+  if (vocab < 1 || vocab > (1 << 30)) return fail(BD3_EINVAL, "vocab must lie in [1, 2^30], got %d", vocab);
   if (logits_fp32 != 0 && logits_fp32 != 1) return fail(BD3_EINVAL, "logits_fp32 must be 0 (bf16) or 1 (fp32)");
   if (strides == nullptr || penalties == nullptr) return fail(BD3_EINVAL, "strides and penalties must be non-NULL");
   for (int i = 0; i < 8; ++i)
@@ -1124,7 +1126,9 @@ int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_
     return fail(BD3_EINVAL, "repetition must be finite and > 0, got %g", (double)penalties[0]);
   if (!std::isfinite(penalties[1]) || !std::isfinite(penalties[2]))
     return fail(BD3_EINVAL, "frequency and presence must be finite");
-  if (!std::isfinite(fill)) return fail(BD3_EINVAL, "fill must be finite");
+  // 3.3961775e38: from there on a number rounds to an infinite bf16
+  if (!std::isfinite(fill) || (!logits_fp32 && std::fabs(fill) >= 3.3961775e38f))
+    return fail(BD3_EINVAL, "fill must be finite in the logits' type, got %g", (double)fill);
   if (batch == 0 || rows == 0) return BD3_OK;
   if (logits == nullptr || out == nullptr) return fail(BD3_EINVAL, "logits and out must be non-NULL");
   const int el = logits_fp32 ? 4 : 2;

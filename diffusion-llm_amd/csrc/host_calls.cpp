@@ -19,6 +19,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -393,11 +394,14 @@ struct PagedBatch {
   const int32_t* lens_p() const { return static_cast<const int32_t*>(ptr(lens)); }
 };
 
+// Written tensors: no element twice (an expanded one would be a race).
+bool writable(const Tensor& t) { return at::has_internal_overlap(t) != at::MemOverlap::Yes; }
+
 // (tokens, heads, 64) result: the caller's, or a new one.
 Tensor token_rows(const Tensor& out, int64_t tokens, int64_t heads, const Tensor& like) {
   if (!out.defined()) return at::empty({tokens, heads, kHeadDim}, like.options());
   require(out.dim() == 3 && out.size(0) == tokens && out.size(1) == heads && out.size(2) == kHeadDim &&
-              out.scalar_type() == at::kBFloat16 && out.device() == like.device() && vec_ready(out),
+              out.scalar_type() == at::kBFloat16 && out.device() == like.device() && vec_ready(out) && writable(out),
           "out must be a (tokens, heads, 64) bf16 tensor with 16-byte aligned rows");
   return out;
 }
@@ -450,6 +454,7 @@ PyObject* paged_attention_inputs(PyObject*, PyObject* const* args, Py_ssize_t n)
     require(heads >= 1, "n_heads must be >= 1");
     b.check(qkv, heads);
     on_one_gpu(qkv, sin, cos);
+    require(writable(b.k) && writable(b.v), "k_pages and v_pages are written: no element may occur twice");
     require(qkv.size(1) == ((int64_t)heads + 2 * (int64_t)b.kv_heads) * kHeadDim,
             "projection width must be (n_heads + 2 * kv_heads) * 64");
     require(qkv.size(0) <= INT32_MAX, "qkv is too large");
@@ -539,7 +544,8 @@ PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
       for (Penalty* p : {&rep, &freq, &pres})
         if (p->each.defined()) p->each = p->each.contiguous();
       if (!out.defined()) out = at::empty({B, R, V}, x.options());
-      require(out.scalar_type() == x.scalar_type() && out.sizes() == x.sizes() && (V == 1 || out.stride(2) == 1),
+      require(out.scalar_type() == x.scalar_type() && out.sizes() == x.sizes() && (V == 1 || out.stride(2) == 1) &&
+                  writable(out),
               "out must have the logits' shape and dtype, with last stride 1");
       const float penalties[3] = {rep.one, freq.one, pres.one};
       const int64_t st[8] = {x.stride(0),

@@ -21,7 +21,7 @@
 namespace bd3 {
 namespace {
 
-constexpr int kQT = 32;       // rows per partial slot
+constexpr int kQT = 32;       // rows of the 32-row tile and of a partial slot (128-row tiles have four)
 constexpr int kSub = 32;      // keys per wave step
 constexpr int kStride = 72;   // padded LDS row (bf16)
 constexpr int kMergeRow = kHeadDim + 4;
@@ -283,9 +283,10 @@ struct MergeLds {
             to_bf16x4(ot[0] * inv, ot[1] * inv, ot[2] * inv, ot[3] * inv);
       }
     } else {
+      if (rt >= a.slot_rows) return;
       const int64_t slot = (((int64_t)it.b * a.kv_heads + it.h) * a.q_slots + it.qt) * a.n_splits + it.split;
-      *reinterpret_cast<f32x4*>(&a.part_o[(slot * kQT + rt) * kHeadDim + d]) = ot * inv;
-      if (d == 0) a.part_lse[slot * kQT + rt] = lt > 0.f ? mm + fast_log2(lt) : -INFINITY;
+      *reinterpret_cast<f32x4*>(&a.part_o[(slot * a.slot_rows + rt) * kHeadDim + d]) = ot * inv;
+      if (d == 0) a.part_lse[slot * a.slot_rows + rt] = lt > 0.f ? mm + fast_log2(lt) : -INFINITY;
     }
   }
 };
@@ -779,8 +780,8 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
   if (ranges <= 1 || row >= sq.rows) return;
   const int d0 = 4 * (wi_x() & 15);
   const int64_t slot0 = ((int64_t)bh * a.q_slots + qt) * a.n_splits;
-  const float* lp = a.part_lse + slot0 * kQT + (wi_x() >> 4);
-  const float* pp = a.part_o + (slot0 * kQT + (wi_x() >> 4)) * kHeadDim + d0;
+  const float* lp = a.part_lse + slot0 * a.slot_rows + (wi_x() >> 4);
+  const float* pp = a.part_o + (slot0 * a.slot_rows + (wi_x() >> 4)) * kHeadDim + d0;
   constexpr int kG = 8;
   float mm = -INFINITY, wt = 0.f;
   f32x4 acc = {};
@@ -789,8 +790,8 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
     f32x4 po[kG];
 #pragma unroll
     for (int k = 0; k < kG; ++k) {
-      l[k] = s0 + k < ranges ? lp[(s0 + k) * kQT] : -INFINITY;
-      po[k] = s0 + k < ranges ? *reinterpret_cast<const f32x4*>(pp + (int64_t)(s0 + k) * kQT * kHeadDim) : f32x4{};
+      l[k] = s0 + k < ranges ? lp[(s0 + k) * a.slot_rows] : -INFINITY;
+      po[k] = s0 + k < ranges ? *reinterpret_cast<const f32x4*>(pp + (int64_t)(s0 + k) * a.slot_rows * kHeadDim) : f32x4{};
     }
     float mg = mm;
 #pragma unroll

@@ -13,6 +13,11 @@ carries its backward (register_autograd).
         n_splits 0: the library's automatic split (bd3_decode), -1: the reference's split
         rule (ceil(kv_len / 256), split_kv_decode_attention's default), > 0: at most that
         many (split_kv_decode_attention); token_major: O is a view of (batch, q_len, heads, head_dim) memory
+    torch.ops.bd3.paged_qkv_rope(qkv, n_heads, sin, cos, k_pages, v_pages, page_table, q_starts, kv_lens) -> q
+        kernels.paged.paged_attention_inputs; writes k_pages and v_pages
+    torch.ops.bd3.paged_attn(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv=-1,
+                             total_kv=-1) -> O
+        kernels.paged.paged_attention; -1: the defaults
 """
 from __future__ import annotations
 
@@ -100,4 +105,30 @@ def _decode_fake(q, k, v, block_size, n_splits, token_major=False):
     if token_major:
         B, H, S, Dh = q.shape
         return q.new_empty((B, S, H, Dh)).transpose(1, 2)
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("bd3::paged_qkv_rope", mutates_args=("k_pages", "v_pages"))
+def paged_qkv_rope(qkv: Tensor, n_heads: int, sin_table: Tensor, cos_table: Tensor, k_pages: Tensor, v_pages: Tensor,
+                   page_table: Tensor, q_starts: Tensor, kv_lens: Tensor) -> Tensor:
+    """The attention inputs of a ragged batch, keys and values into their pages."""
+    return host().paged_attention_inputs(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, page_table, q_starts,
+                                         kv_lens, None)
+
+
+@paged_qkv_rope.register_fake
+def _paged_qkv_rope_fake(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, page_table, q_starts, kv_lens):
+    return qkv.new_empty((qkv.shape[0], n_heads, D))
+
+
+@torch.library.custom_op("bd3::paged_attn", mutates_args=())
+def paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, q_starts: Tensor, kv_lens: Tensor,
+               block_size: int, max_q: int, max_kv: int = -1, total_kv: int = -1) -> Tensor:
+    """Attention of a ragged batch over its pages."""
+    return host().paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv,
+                                  total_kv, None)
+
+
+@paged_attn.register_fake
+def _paged_attn_fake(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv=-1, total_kv=-1):
     return q.new_empty(q.shape)

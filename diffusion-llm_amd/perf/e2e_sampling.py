@@ -1,6 +1,7 @@
 """end-to-end BD3-LM block sampling with this library's kernels.
 
     python diffusion-llm_amd/perf/e2e_sampling.py [--blocks 64] [--check-steps 4]
+    python diffusion-llm_amd/perf/e2e_sampling.py --serve
 
 A minimal restatement of the reference's inference model and sampler, used
 only to measure the attention path in place (it is a benchmark workload,
@@ -30,6 +31,9 @@ each block's backbone captured once as a HIP graph and replayed per step,
 and with plain launches), the eager sampler's tokens/s over the first
 blocks, and the logits' max-abs difference between the two backbones at
 sampled denoising steps (same tokens, same committed prefix).
+
+With --serve: the same backbone over a paged cache (`serve`), sequences of
+different lengths in one batch that join and leave as the pool's pages allow.
 """
 from __future__ import annotations
 
@@ -285,6 +289,121 @@ def generate(cfg, p, tables, batch, n_blocks, steps, backend, check=None, graph=
     return x
 
 
+# ---------------------------------------------------------------------------
+# serving: sequences of different lengths in one batch, their cache in pages
+
+
+def backbone_paged(cfg, p, tables, tokens, batch, ada):
+    """Logits (tokens, vocab) of a ragged batch's packed tokens (kernels.paged.
+    PagedBatch); their keys and values go to the batch's pages. `ada`:
+    ada_params for one sequence (the conditioning is the same for all)."""
+    from kernels.dit_glue import gate_residual_ln_modulate, ln_modulate
+    T = tokens.shape[0]
+    ada_layers, ada_final = ada
+    layers = p["layers"]
+    x = p["emb"][tokens][None]
+    h = ln_modulate(x, layers[0]["ln1"], ada_layers[0][0], ada_layers[0][1], cfg.eps)
+    for li, L in enumerate(layers):
+        _, _, g1, sh2, sc2, g2 = ada_layers[li]
+        q = batch.attention_inputs(linear(h[0], L["qkv"]), cfg.heads, *tables, li)
+        o = batch.attention(q, li, cfg.bs).view(1, T, cfg.d)
+        x, h = gate_residual_ln_modulate(x, g1, linear(o, L["out"]), L["ln2"], sh2, sc2, cfg.eps)
+        y = linear(F.gelu(linear(h, L["fc1"]), approximate="tanh"), L["fc2"])
+        if li + 1 < len(layers):
+            w_next, (sh_next, sc_next) = layers[li + 1]["ln1"], ada_layers[li + 1][:2]
+        else:
+            w_next, (sh_next, sc_next) = p["f_ln"], ada_final
+        x, h = gate_residual_ln_modulate(x, g2, y, w_next, sh_next, sc_next, cfg.eps)
+    return linear(h[0], p["lm_head"])
+
+
+def serve(cfg, p, tables, prompts, n_blocks, steps, n_pages, page_size=64, repetition=1.0, allowed=None, seed=0,
+          check=None):
+    """Continue each prompt (1-D token tensors of whole blocks) by n_blocks[i]
+    blocks, as many sequences at a time as the pool of n_pages holds: a waiting
+    one joins as soon as the pages it will need are free. Every round runs one
+    prefill of the prompts that join, `steps` denoising steps of the next block of
+    all live sequences, with a repetition penalty over what each holds so far
+    and a mask of allowed tokens, and the pass that commits the block. `check`:
+    optional callback(tokens before the block, block, logits) of each sequence's
+    first step. Returns the sequences' tokens."""
+    from kernels.paged import PagedKVCache
+    from kernels.sampling import PhiloxStream, adjust_logits, subs_sample_step
+    device = p["emb"].device
+    cache = PagedKVCache(cfg.layers, n_pages, cfg.heads, page_size, device=device)
+    gen = PhiloxStream(seed=seed)
+    ada = ada_params(cfg, p, 1, device)
+    assert all(len(t) % cfg.bs == 0 for t in prompts), "prompts must be whole blocks"
+    need = [-(-(len(t) + n * cfg.bs) // page_size) for t, n in zip(prompts, n_blocks)]
+    assert max(need, default=0) <= n_pages, "a sequence does not fit the pool"
+    waiting, live, reserved = list(range(len(prompts))), {}, 0  # live: index -> [sequence, blocks left]
+    out = [t.to(device) for t in prompts]
+    while waiting or live:
+        joined = []
+        while waiting and reserved + need[waiting[0]] <= n_pages:
+            i = waiting.pop(0)
+            reserved += need[i]
+            live[i] = [cache.add(), n_blocks[i]]
+            if len(out[i]):
+                joined.append(i)
+        if joined:
+            batch = cache.batch([live[i][0] for i in joined], [len(out[i]) for i in joined])
+            backbone_paged(cfg, p, tables, torch.cat([out[i] for i in joined]), batch, ada)
+            batch.commit()
+        for i in [i for i, (_, left) in live.items() if left == 0]:
+            cache.free(live.pop(i)[0])
+            reserved -= need[i]
+        if not live:
+            continue
+        ids = list(live)
+        batch = cache.batch([live[i][0] for i in ids], [cfg.bs] * len(ids))
+        lengths = torch.tensor([len(out[i]) for i in ids], device=device, dtype=torch.int32)
+        history = torch.nn.utils.rnn.pad_sequence([out[i] for i in ids], batch_first=True, padding_value=-1)
+        block = torch.full((len(ids), cfg.bs), cfg.mask, device=device, dtype=torch.long)
+        for step in range(steps):
+            t, s = 1 - step / steps, 1 - (step + 1) / steps
+            logits = backbone_paged(cfg, p, tables, block.flatten(), batch, ada).view(len(ids), cfg.bs, -1)
+            if check is not None and step == 0:
+                for k, i in enumerate(ids):
+                    check(out[i], block[k], logits[k])
+            logits = adjust_logits(logits, history, lengths, repetition=repetition, allowed=allowed)
+            block = subs_sample_step(logits, block, cfg.mask, s / t, generator=gen)
+        backbone_paged(cfg, p, tables, block.flatten(), batch, ada)
+        batch.commit()
+        for i, new in zip(ids, block):
+            out[i] = torch.cat([out[i], new])
+            live[i][1] -= 1
+    assert cache.free_pages == n_pages
+    return out
+
+
+def run_serving(sequences: int = 32, steps: int = 8, seed: int = 0) -> dict:
+    """Tokens/s of `serve`: prompts of 32 to 1024 tokens, each continued by 4 to
+    16 blocks of 32, through a pool of half the pages that all of them need."""
+    import random
+    from kernels.kv_cache import rope_tables
+    cfg = Cfg()
+    device = torch.device("cuda:0")
+    p = init_params(cfg, seed, device)
+    tables = rope_tables(cfg.d // cfg.heads, cfg.max_seq, device=device)
+    rng = random.Random(seed)
+    g = torch.Generator(device=device).manual_seed(seed)
+    prompts = [torch.randint(0, cfg.mask, (cfg.bs * rng.randint(1, 32),), generator=g, device=device)
+               for _ in range(sequences)]
+    n_blocks = [rng.randint(4, 16) for _ in prompts]
+    pages = sum(-(-(len(t) + n * cfg.bs) // 64) for t, n in zip(prompts, n_blocks)) // 2
+    with torch.no_grad():
+        serve(cfg, p, tables, prompts[:2], [1, 1], 2, pages)  # warm-up
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        serve(cfg, p, tables, prompts, n_blocks, steps, pages, repetition=1.1)
+        torch.cuda.synchronize()
+        seconds = time.perf_counter() - t0
+    return {"workload": f"{sequences} prompts of 32-1024 tokens continued by 4-16 blocks of {cfg.bs}, {steps} steps per "
+                        f"block, 12L / 768 / 12H, vocab 50258, paged cache of {pages} x 64 tokens (random init)",
+            "tokens_per_s": sum(n_blocks) * cfg.bs / seconds, "seconds": seconds}
+
+
 def run(blocks: int = 64, eager_blocks: int = 2, check_steps: int = 4, batch: int = 8, seed: int = 0) -> dict:
     import kernels.ops  # noqa: F401
     from kernels.kv_cache import rope_tables
@@ -366,7 +485,11 @@ def main(argv=None) -> int:
     ap.add_argument("--blocks", type=int, default=64)
     ap.add_argument("--eager-blocks", type=int, default=2)
     ap.add_argument("--check-steps", type=int, default=4)
+    ap.add_argument("--serve", action="store_true", help="the ragged serving loop instead")
     args = ap.parse_args(argv)
+    if args.serve:
+        print(json.dumps(run_serving()), flush=True)
+        return 0
     print(json.dumps(run(args.blocks, args.eager_blocks, args.check_steps)), flush=True)
     return 0
 

@@ -341,7 +341,8 @@ int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t
  *   strides: 11 int64 element strides: q (token, head), k_pages (page, head,
  *     slot), v_pages (page, head, slot), o (token, head), page_table (row); last
  *     strides 1, all but the table's multiples of 8, slot strides < 2^24.
- * Device data is not trusted with addresses: token ranges are cut to [0, tokens),
+ * o overlaps none of the inputs. Pages may be shared by sequences (a common
+ * prefix). Device data is not trusted with addresses: token ranges are cut to [0, tokens),
  * lengths to [0, max_kv], and keys whose table entry lies outside [0, pages) are
  * not seen. Table entries beyond a sequence's keys are not read.
  * Preconditions: page_size a power of two in [16, 1024], head_dim == 64, heads a
@@ -372,7 +373,8 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
  * The rotation is computed in fp32 and rounded once (bd3_qkv_rope repeats the
  * eager bf16 path's roundings instead). Tokens of no sequence are left out: their
  * rows of q_out stay as they are. Nothing is written for a position before 0, past
- * the table or whose entry lies outside [0, pages). No reference counterpart.
+ * the table or whose entry lies outside [0, pages). No two tokens may have the
+ * same slot. No reference counterpart.
  */
 int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos_table,
                        int32_t max_pos, void* q_out, void* k_pages, void* v_pages,
@@ -399,7 +401,7 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
  *   bias: device fp32 (vocab) (batch stride 0) or (batch, vocab), or NULL.
  *   allowed: device int32 words, bit v % 32 of word v / 32 set where token v is
  *     allowed, one set for all (strides 0), for each sequence or each row; NULL.
- *   fill: finite, so that a row whose mask allows nothing stays finite (every
+ *   fill: finite in the logits' type, so that a row whose mask allows nothing stays finite (every
  *     token the same).
  *   strides: 8 int64 element strides: logits (batch, row), out (batch, row),
  *     tokens (batch), bias (batch), allowed (batch, row).

@@ -176,3 +176,37 @@ def test_graph_and_draw(cuda):
         assert torch.equal(out, want)
         drawn = subs_sample_step(out, block, MASK, 0.0, generator=PhiloxStream(rep)).cpu()
         assert all(yes[b, t] for b in range(B) for t in drawn[b].tolist())
+
+
+@pytest.mark.gpu
+def test_refusals(cuda):
+    x = torch.zeros(2, 3, 100, device=cuda)
+    t = torch.zeros(2, 5, dtype=torch.long, device=cuda)
+    for args, kw, text in [
+            ((x.half(),), {}, "bf16 or fp32"), ((x[0, 0],), {}, "batch, rows, vocab"), ((x, t.int()), {}, "int64"),
+            ((x, t[:1]), {}, "tokens must"), ((x, None, torch.zeros(2, dtype=torch.int32, device=cuda)), {}, "with tokens"),
+            ((x, t, torch.zeros(2, dtype=torch.long, device=cuda)), {}, "int32"), ((x, t), {"repetition": 0.0}, "repetition"),
+            ((x, t), {"frequency": torch.zeros(3, device=cuda)}, "penalty"), ((x,), {"bias": torch.zeros(99, device=cuda)}, "bias"),
+            ((x,), {"bias": torch.zeros(2, 100, device=cuda, dtype=BF)}, "float32"),
+            ((x,), {"allowed": torch.zeros(2, 3, dtype=torch.int32, device=cuda)}, "allowed"),
+            ((x,), {"allowed": torch.zeros(2, 4, dtype=torch.long, device=cuda)}, "allowed"), ((x,), {"fill": float("-inf")}, "fill"),
+            ((x.to(BF),), {"fill": -3.4e38}, "fill"), ((x,), {"out": torch.zeros(2, 3, 100, device=cuda, dtype=BF)}, "out must"),
+            ((x,), {"out": torch.zeros(1, 3, 100, device=cuda).expand(2, 3, 100)}, "out must"),
+            ((x, t.cpu()), {}, "one device"),
+            ((x[:, 0],), {"allowed": torch.zeros(2, 1, 4, dtype=torch.int32, device=cuda)}, "allowed")]:
+        with pytest.raises(AssertionError, match=text):
+            adjust_logits(*args, **kw)
+
+
+@pytest.mark.gpu
+def test_other_streams_agree(cuda):
+    x, kw = case(4, 9, 5001, BF, 300, "each", 2, 3, seed=9)
+    xd, d = x.to(cuda), dev(kw, cuda)
+    want = adjust_logits(xd, **d)
+    torch.cuda.synchronize()
+    outs = []
+    for s in [torch.cuda.Stream() for _ in range(3)]:
+        with torch.cuda.stream(s):
+            outs += [adjust_logits(xd, **d) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)

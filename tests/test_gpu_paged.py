@@ -62,6 +62,36 @@ def test_attention_matches_definition(cuda, record_error, lens, heads, kv_heads,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [64, 65, 130])
+@pytest.mark.parametrize("chunk,heads,kv_heads", [(1, 2, 1), (16, 2, 2), (32, 1, 1), (70, 1, 1), (25, 6, 1)])
+def test_many_sequences(cuda, record_error, seqs, chunk, heads, kv_heads):
+    """More sequences than a wave has lanes; some without tokens, some without keys."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = [(int(n), int(x)) for n, x in zip(torch.randint(0, chunk + 1, (seqs,), generator=g),
+                                             torch.randint(0, 400, (seqs,), generator=g))]
+    lens[3], lens[seqs - 1] = (0, 0), (chunk, 900)
+    c = paged_case(lens, heads, kv_heads, 16, seed=seqs)
+    ref, tol = attention_reference(c, 16)
+    for total in (0, c["total"], 10 ** 7):
+        o = attend(on(c, cuda), 16, total_kv=total, max_q=chunk)
+        record_error("paged attention / bound", worst(o, ref, tol), 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk,bound", [(16, 5), (32, 20), (64, 33), (300, 130)])
+def test_tokens_beyond_max_q_are_left_out(cuda, record_error, chunk, bound):
+    """A chunk longer than the bound: its first tokens as ever, the rest as they were."""
+    c = paged_case([(chunk, 800), (3, 50)], 2, 2, 16, seed=8)
+    ref, tol = attention_reference(c, 16)
+    for total in (0, c["total"]):
+        out = torch.full_like(c["q"], 7.0).to(cuda)
+        attend(on(c, cuda), 16, out=out, max_q=bound, total_kv=total)
+        assert (out[bound:chunk] == 7.0).all()
+        kept = torch.cat([torch.arange(bound), torch.arange(chunk, chunk + 3)])
+        record_error("paged attention / bound", worst(out[kept.to(cuda)], ref[kept], tol[kept]), 1.0)
+
+
+@pytest.mark.gpu
 def test_large_scores(cuda, record_error):
     """Scores of +-100: a row's weight sits on few keys, whichever range holds them."""
     c = paged_case([(16, 700), (1, 2000), (100, 100)], 2, 2, 64, seed=3, q_scale=8.0)
@@ -249,6 +279,67 @@ def test_other_streams_and_repeats_agree(cuda):
             outs += [attend(c, 16, total_kv=0) for _ in range(5)]
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.gpu
+def test_shared_prefix_pages(cuda, record_error):
+    """Two sequences whose tables begin with the same pages."""
+    c = paged_case([(16, 496), (16, 240)], 2, 2, 16, seed=12)
+    c["table"][1, :15] = c["table"][0, :15]
+    ref, tol = attention_reference(c, 16)
+    record_error("paged attention / bound", worst(attend(on(c, cuda), 16), ref, tol), 1.0)
+
+
+@pytest.mark.gpu
+def test_compile_paged_no_graph_break(cuda):
+    """The custom ops under torch.compile: the same bits, one graph, pages written."""
+    import kernels.ops  # noqa: F401
+    c = on(inputs_case([(16, 100), (5, 30)], 4, 2, 16, seed=1), cuda)
+    batch = (c["table"], c["starts"], c["kv"])
+
+    def layer(qkv, k, v):
+        q = torch.ops.bd3.paged_qkv_rope(qkv * 2, 4, c["sin"], c["cos"], k, v, *batch)
+        return torch.ops.bd3.paged_attn(q, k, v, *batch, 16, 16) + 1
+
+    k1, v1, k2, v2 = c["k"].clone(), c["v"].clone(), c["k"].clone(), c["v"].clone()
+    want = layer(c["qkv"], k1, v1)
+    got = torch.compile(layer, backend="aot_eager", fullgraph=True, dynamic=True)(c["qkv"], k2, v2)
+    assert torch.equal(got, want) and torch.equal(k1, k2) and torch.equal(v1, v2)
+    assert not torch.equal(k1, c["k"])
+
+
+@pytest.mark.gpu
+def test_refusals(cuda):
+    c = on(paged_case([(4, 20)], 4, 2, 16), cuda)
+    ok = dict(q=c["q"], k=c["k"], v=c["v"], table=c["table"], starts=c["starts"], kv=c["kv"])
+
+    def call(**kw):
+        d = {**c, **ok, **kw}
+        return paged_attention(d["q"], d["k"], d["v"], d["table"], d["starts"], d["kv"], 4, max_q=4,
+                               out=kw.get("out"))
+
+    for kw, text in [
+            (dict(q=c["q"].float()), "bf16"), (dict(q=c["q"][:, :3]), "multiple"), (dict(k=c["k"].float()), "bf16"),
+            (dict(v=c["v"][:-1]), "k_pages and v_pages"), (dict(k=c["k"][..., :32], v=c["v"][..., :32]), "64"),
+            (dict(table=c["table"].long()), "int32"), (dict(table=c["table"][:, ::2]), "last stride 1"),
+            (dict(starts=c["starts"][:1]), "q_starts"), (dict(kv=c["kv"].repeat(2)), "kv_lens"),
+            (dict(kv=c["kv"].cpu()), "one device"), (dict(out=torch.empty(4, 4, 32, device=cuda, dtype=BF)), "out must"),
+            (dict(out=torch.empty(4, 4, D, device=cuda)), "out must"),
+            (dict(out=torch.empty(4, 1, D, device=cuda, dtype=BF).expand(4, 4, D)), "out must"),
+            (dict(k=torch.empty(c["k"].numel() + 1, device=cuda, dtype=BF)[1:].view_as(c["k"])), "16-byte")]:
+        with pytest.raises(AssertionError, match=text):
+            call(**kw)
+    with pytest.raises(AssertionError, match="exceeds"):
+        paged_attention(c["q"], c["k"], c["v"], c["table"], c["starts"], c["kv"], 4, max_q=4, max_kv=10 ** 6)
+    sin, cos = (t.to(cuda) for t in rope_tables(D, 64))
+    qkv = torch.zeros(4, 8 * D, device=cuda, dtype=BF)
+    with pytest.raises(AssertionError, match="no element may occur twice"):
+        one = c["k"][:1].expand(3, -1, -1, -1)
+        paged_attention_inputs(qkv, 4, sin, cos, one, one, c["table"], c["starts"], c["kv"])
+    with pytest.raises(AssertionError, match="projection width"):
+        paged_attention_inputs(qkv[:, :-D], 4, sin, cos, c["k"], c["v"], c["table"], c["starts"], c["kv"])
+    with pytest.raises(AssertionError, match="RoPE tables"):
+        paged_attention_inputs(qkv, 4, sin.double(), cos.double(), c["k"], c["v"], c["table"], c["starts"], c["kv"])
 
 
 # ---------------------------------------------------------------------------

@@ -115,6 +115,19 @@ def test_cache_bookkeeping():
     assert empty.page_table.shape == (0, 1) and empty.max_q == 0
 
 
+def test_custom_ops_fake_shapes():
+    import kernels.ops  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        k = torch.empty(9, 2, 16, 64, dtype=BF)
+        i = torch.empty(3, dtype=torch.int32)
+        q = torch.ops.bd3.paged_qkv_rope(torch.empty(7, 8 * 64, dtype=BF), 4, torch.empty(9, 32), torch.empty(9, 32), k, k,
+                                         i[None], i, i)
+        assert q.shape == (7, 4, 64) and q.dtype == BF
+        o = torch.ops.bd3.paged_attn(q, k, k, i[None], i, i, 16, 4)
+        assert o.shape == q.shape and o.dtype == BF
+
+
 def test_cpu_tensors_raise(lib):
     c = paged_case([(4, 8)], 2, 2, 16)
     with pytest.raises(AssertionError, match="CUDA"):
@@ -213,10 +226,10 @@ def test_workspace(lib):
 
 
 @pytest.mark.parametrize("kw,text", [
-    (dict(batch=-1), ">= 0"), (dict(vocab=0), "vocab"), (dict(fp32=2), "logits_fp32"), (dict(x=None), "non-NULL"),
+    (dict(batch=-1), ">= 0"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 30) + 1), "vocab"), (dict(fp32=2), "logits_fp32"), (dict(x=None), "non-NULL"),
     (dict(out=P + 1), "aligned to their elements"), (dict(tokens=P + 4), "8 bytes"), (dict(pen=[0.0, 0, 0]), "repetition"),
     (dict(pen=[float("inf"), 0, 0]), "repetition"), (dict(pen=[1.0, float("nan"), 0]), "frequency"), (dict(pen=None), "penalties"),
-    (dict(fill=float("-inf")), "fill"), (dict(st=[-1] + [0] * 7), "stride[0]"), (dict(st=None), "strides"),
+    (dict(fill=float("-inf")), "fill"), (dict(fill=-3.4e38), "fill"), (dict(st=[-1] + [0] * 7), "stride[0]"), (dict(st=None), "strides"),
     (dict(batch=1 << 22, vocab=1 << 20), "too large")])
 def test_logits_refusals(lib, kw, text):
     a = dict(x=P, fp32=0, out=P, batch=2, rows=3, vocab=100, tokens=P, history=5, lens=None, pen=[1.0, 0.0, 0.0],
