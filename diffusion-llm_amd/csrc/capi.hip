@@ -886,30 +886,34 @@ struct PagedPlan {
 
 // Estimated us of a plan, to choose the sets and the length of the key ranges: the
 // longest item's chain of 64-key steps against the load per CU, then the merge
-// launch. Fitted to 2100 timings of 450 batches drawn over 1-64 sequences, 1-3000
-// tokens a chunk, 20-10000 keys, 1-16 KV heads and groups of 1-12 (rms error 7-11%).
-double paged_us(int tile, int subs, double longest, double keys, double items, bool split) {
+// launch. Lengths that differ leave the longest item to the end of the 16- and
+// 32-row launches (items in the order of the sequences), so there the two nearly add
+// up; the 128-row launch takes the longest first. Fitted to 8200 timings of 1500
+// batches drawn over 1-64 sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV
+// heads and groups of 1-12 (rms error 8-10%).
+double paged_us(int tile, int subs, double longest, double keys, double items, bool split, bool even) {
   struct Cost {
     double chain0, chain, load0, load, item, merge, merge_item;
   };
-  static constexpr Cost kRows16 = {4.7, 0.37, 2.8, 0.62, 1.4, 2.9, 0.0};  // two sets
-  static constexpr Cost kRows32[2] = {{4.8, 0.67, 4.1, 0.63, 0.74, 2.8, 0.79}, {5.6, 0.35, 2.0, 0.58, 4.4, 3.4, 0.0}};
+  static constexpr Cost kRows16 = {5.7, 0.32, 0.0, 0.64, 1.6, 3.1, 0.0};  // two sets
+  static constexpr Cost kRows32[2] = {{5.6, 0.64, 0.2, 0.56, 1.7, 3.1, 0.37}, {5.9, 0.33, 0.1, 0.51, 4.7, 3.5, 0.0}};
   static constexpr Cost kRows128[3] = {{4.3, 1.05, 5.8, 0.56, 1.8, 4.3, 1.85},
                                        {4.6, 0.71, 6.0, 0.57, 3.2, 3.9, 1.88},
                                        {8.4, 0.53, 0.0, 0.59, 9.8, 0.0, 0.0}};  // four sets: never with ranges
   const Cost& c = tile == 16 ? kRows16 : tile == 32 ? kRows32[subs - 1] : kRows128[subs >> 1];
   const double chain = c.chain0 + c.chain * longest / 64.0;
   const double load = c.load0 + c.load * keys / (64.0 * 256.0) + c.item * items / 256.0;
-  return std::cbrt(chain * chain * chain + load * load * load) + (split ? c.merge + c.merge_item * items / 256.0 : 0.0);
+  const double e = even || tile == 128 ? 3.0 : 1.5;
+  return std::pow(std::pow(chain, e) + std::pow(load, e), 1.0 / e) +
+         (split ? c.merge + c.merge_item * items / 256.0 : 0.0);
 }
 
 // The cheapest plan of the sets and ranges (256 keys and longer, at most 64 of a
 // sequence) for what the host knows: bounds, tokens and the keys in all. Ranges pay
-// where a few long sequences would leave the chip idle. Of 150 batches of each
-// tile the plan takes 0.7% (16 rows), 2% and 1.5% more than the best one. us, whole
-// items -> plan: 12 heads, 16 over 3600 keys 24.7 -> 11.7; 32 sequences of
-// 100-8192 keys 65.7 -> 51.3; 8 chunks of 66-524 tokens over 200-4000 44.5 (one set,
-// 512-key ranges) -> 31.6 (four sets).
+// where a few long sequences would leave the chip idle. Over 500 batches of each tile
+// the plan takes 0.5% (16 rows) and 1.5% more than the best one. us, whole items ->
+// plan: 12 heads, 16 over 3600 keys 24.7 -> 10.8; 32 sequences of 100-8192 keys 66 ->
+// 51; 32 rows over 2000 keys of 8 sequences 17.3 -> 14.6.
 PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
                      int64_t total_kv) {
   PagedPlan p;
@@ -924,12 +928,13 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
     units = std::min(units, kv_heads * ((double)tokens * (double)group / 128.0 + 0.5 * seqs));
     seen = std::max(1.0, seen - 0.5 * tokens / seqs);
   }
+  const bool even = (double)max_kv * seqs < 1.5 * total;
   double best = INFINITY;
   p.subs = 0;
   p.n_splits = 1;
   p.split_shift = 30;
   for (int subs = p.tile == 16 ? 2 : 1; subs <= (p.tile == 128 ? 4 : 2); subs *= 2) {
-    const double whole = paged_us(p.tile, subs, max_kv, units * seen, units, false);
+    const double whole = paged_us(p.tile, subs, max_kv, units * seen, units, false, even);
     if (whole < best) {
       best = whole;
       p.subs = subs;
@@ -938,7 +943,7 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
     for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
       if (max_kv >> shift > 64) continue;
       const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
-      const double us = paged_us(p.tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items, true);
+      const double us = paged_us(p.tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items, true, even);
       if (us < best) {
         best = us;
         p.subs = subs;
