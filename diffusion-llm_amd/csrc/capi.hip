@@ -884,22 +884,22 @@ struct PagedPlan {
   int tile, subs, q_tiles, q_slots, slot_rows, n_splits, split_shift;
 };
 
-// Estimated us of a plan, to choose the sets and the length of the key ranges: the
+// Estimated us of a plan, to choose tile, sets and the length of the key ranges: the
 // longest item's chain of 64-key steps against the load per CU, then the merge
 // launch. Lengths that differ leave the longest item to the end of the 16- and
 // 32-row launches (items in the order of the sequences), so there the two nearly add
-// up; the 128-row launch takes the longest first. Fitted to 8200 timings of 1500
+// up; the 128-row launch takes the longest first. Fitted to 9100 timings of 2000
 // batches drawn over 1-64 sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV
-// heads and groups of 1-12 (rms error 8-10%).
+// heads and groups of 1-12 (rms error 7-12%).
 double paged_us(int tile, int subs, double longest, double keys, double items, bool split, bool even) {
   struct Cost {
     double chain0, chain, load0, load, item, merge, merge_item;
   };
   static constexpr Cost kRows16 = {5.7, 0.32, 0.0, 0.64, 1.6, 3.1, 0.0};  // two sets
-  static constexpr Cost kRows32[2] = {{5.6, 0.64, 0.2, 0.56, 1.7, 3.1, 0.37}, {5.9, 0.33, 0.1, 0.51, 4.7, 3.5, 0.0}};
-  static constexpr Cost kRows128[3] = {{4.3, 1.05, 5.8, 0.56, 1.8, 4.3, 1.85},
-                                       {4.6, 0.71, 6.0, 0.57, 3.2, 3.9, 1.88},
-                                       {8.4, 0.53, 0.0, 0.59, 9.8, 0.0, 0.0}};  // four sets: never with ranges
+  static constexpr Cost kRows32[2] = {{5.7, 0.62, 1.1, 0.54, 1.7, 3.1, 0.37}, {5.9, 0.33, 0.5, 0.52, 4.7, 3.6, 0.0}};
+  static constexpr Cost kRows128[3] = {{4.6, 1.0, 5.2, 0.68, 1.4, 3.2, 1.7},
+                                       {5.5, 0.66, 4.8, 0.70, 2.9, 3.2, 1.9},
+                                       {8.0, 0.52, 0.0, 0.69, 9.5, 0.0, 0.0}};  // four sets: never with ranges
   const Cost& c = tile == 16 ? kRows16 : tile == 32 ? kRows32[subs - 1] : kRows128[subs >> 1];
   const double chain = c.chain0 + c.chain * longest / 64.0;
   const double load = c.load0 + c.load * keys / (64.0 * 256.0) + c.item * items / 256.0;
@@ -908,49 +908,49 @@ double paged_us(int tile, int subs, double longest, double keys, double items, b
          (split ? c.merge + c.merge_item * items / 256.0 : 0.0);
 }
 
-// The cheapest plan of the sets and ranges (256 keys and longer, at most 64 of a
-// sequence) for what the host knows: bounds, tokens and the keys in all. Ranges pay
-// where a few long sequences would leave the chip idle. Over 500 batches of each tile
-// the plan takes 0.5% (16 rows) and 1.5% more than the best one. us, whole items ->
-// plan: 12 heads, 16 over 3600 keys 24.7 -> 10.8; 32 sequences of 100-8192 keys 66 ->
-// 51; 32 rows over 2000 keys of 8 sequences 17.3 -> 14.6.
+// The cheapest plan of the tiles (16 rows where they are enough, else 32 up to 256
+// rows or 128), sets and ranges (256 keys and longer, at most 64 of a sequence) for
+// what the host knows: bounds, tokens and the keys in all. Ranges pay where a few
+// long sequences would leave the chip idle; 32-row tiles re-read the keys for
+// every tile but start and step faster. Over 500 batches each of up to 16, 17-64,
+// 17-300 and 65-3000 rows the plan takes 0.5%, 2%, 3% and 1.5% more than the best one.
+// us, whole items -> plan: 12 heads, 16 over 3600 keys 24.7 -> 10.8; 32 sequences of
+// 100-8192 keys 66 -> 51; 32 rows over 2000 keys of 8 sequences 17.3 -> 14.6; 32-row
+// tiles -> plan: 50 rows over 1000 keys of 32 sequences 24.4 -> 19.1; 128-row tiles ->
+// plan: 96 rows over 800 keys of 4 sequences, 4 KV heads 12.5 -> 8.7.
 PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
                      int64_t total_kv) {
-  PagedPlan p;
   const int64_t group = heads / kv_heads, rows = (int64_t)max_q * group;
-  p.tile = rows <= 16 ? 16 : rows <= 64 ? 32 : 128;
-  p.q_tiles = (int)((rows + p.tile - 1) / p.tile);
-  p.q_slots = (int)((rows + 31) / 32);
-  p.slot_rows = (int)std::min<int64_t>(rows, 32);
-  const double total = (double)std::min(total_kv, (int64_t)seqs * max_kv), bh = (double)seqs * kv_heads;
-  double units = bh * p.q_tiles, seen = total / seqs;  // items without ranges, keys that one sees
-  if (p.tile == 128) {
-    units = std::min(units, kv_heads * ((double)tokens * (double)group / 128.0 + 0.5 * seqs));
-    seen = std::max(1.0, seen - 0.5 * tokens / seqs);
-  }
+  const double total = (double)std::min(total_kv, (int64_t)seqs * max_kv);
+  const double seen = std::max(1.0, (total - 0.5 * tokens) / seqs);  // keys that a tile sees, about
   const bool even = (double)max_kv * seqs < 1.5 * total;
+  PagedPlan p = {};
   double best = INFINITY;
-  p.subs = 0;
-  p.n_splits = 1;
-  p.split_shift = 30;
-  for (int subs = p.tile == 16 ? 2 : 1; subs <= (p.tile == 128 ? 4 : 2); subs *= 2) {
-    const double whole = paged_us(p.tile, subs, max_kv, units * seen, units, false, even);
-    if (whole < best) {
-      best = whole;
+  for (int tile : {16, 32, 128}) {
+    if (tile == 16 ? rows > 16 : rows <= 16 || (tile == 32 && rows > 256)) continue;
+    const int q_tiles = (int)((rows + tile - 1) / tile);
+    // items without ranges: not every chunk is as long as the longest
+    const double units = kv_heads * std::max(1.0, std::min((double)seqs * q_tiles,
+                                                           (double)tokens * (double)group / tile + 0.5 * seqs));
+    const auto take = [&](double us, int subs, int shift) {
+      if (!(us < best)) return;
+      best = us;
+      p.tile = tile;
+      p.q_tiles = q_tiles;
       p.subs = subs;
-      p.split_shift = 30;
-    }
-    for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
-      if (max_kv >> shift > 64) continue;
-      const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
-      const double us = paged_us(p.tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items, true, even);
-      if (us < best) {
-        best = us;
-        p.subs = subs;
-        p.split_shift = shift;
+      p.split_shift = shift;
+    };
+    for (int subs = tile == 16 ? 2 : 1; subs <= (tile == 128 ? 4 : 2); subs *= 2) {
+      take(paged_us(tile, subs, max_kv, units * seen, units, false, even), subs, 30);
+      for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
+        if (max_kv >> shift > 64) continue;
+        const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
+        take(paged_us(tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items, true, even), subs, shift);
       }
     }
   }
+  p.q_slots = (int)((rows + 31) / 32);
+  p.slot_rows = (int)std::min<int64_t>(rows, 32);
   p.n_splits = std::max(1, (int)(((int64_t)max_kv + ((int64_t)1 << p.split_shift >> 1)) >> p.split_shift));
   return p;
 }

@@ -296,7 +296,7 @@ constexpr size_t chunk_smem() {
   return v > sizeof(MergeLds<NW, ROWS>) ? v : sizeof(MergeLds<NW, ROWS>);
 }
 
-// Up to 64 rows: 32-row tiles, NW waves share the key chunks of a range. S^T (32
+// 32-row tiles: NW waves share the key chunks of a range. S^T (32
 // keys x 32 rows) = K Q^T on v_mfma_f32_32x32x16_bf16 with the K tile's rows as A
 // operands; O^T += V^T P^T with V read transposed.
 template <int NW>
@@ -524,7 +524,7 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
   }
 }
 
-// Chunks of more than 64 rows: 128-row tiles, four waves of 32 rows that share each
+// 128-row tiles: four waves of 32 rows that share each
 // 64-key K / V tile, which goes from the page to LDS directly (bd3_swz.h; two
 // stages: the next tile loads during the current one). A wave loads 16 keys of a
 // tile, which lie in one page, so its source is one scalar base and the same lane
@@ -755,14 +755,14 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
             to_bf16x4(o[db][4 * q4] * inv, o[db][4 * q4 + 1] * inv, o[db][4 * q4 + 2] * inv, o[db][4 * q4 + 3] * inv);
   } else {
     const int64_t slot = ((int64_t)bh * a.q_slots + (qrow0 >> 5)) * a.n_splits + split;
-    float* po = a.part_o + (slot * kQT + l32) * kHeadDim;
+    float* po = a.part_o + (slot * a.slot_rows + l32) * kHeadDim;
 #pragma unroll
     for (int db = 0; db < 2; ++db)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4)
         *reinterpret_cast<f32x4*>(po + 32 * db + 8 * q4 + 4 * g) =
             f32x4{o[db][4 * q4] * inv, o[db][4 * q4 + 1] * inv, o[db][4 * q4 + 2] * inv, o[db][4 * q4 + 3] * inv};
-    if (g == 0) a.part_lse[slot * kQT + l32] = any ? mref + fast_log2(ltot) : -INFINITY;
+    if (g == 0) a.part_lse[slot * a.slot_rows + l32] = any ? mref + fast_log2(ltot) : -INFINITY;
   }
 }
 

@@ -344,7 +344,7 @@ int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t
  * o overlaps none of the inputs. Pages may be shared by sequences (a common
  * prefix). Device data is not trusted with addresses: token ranges are cut to [0, tokens),
  * lengths to [0, max_kv], and keys whose table entry lies outside [0, pages) are
- * not seen. Table entries beyond a sequence's keys are not read.
+ * not seen. Table entries beyond a sequence's keys are not used.
  * Preconditions: page_size a power of two in [16, 1024], head_dim == 64, heads a
  * multiple of kv_heads. The same call may be captured into a graph: its launches
  * depend on the arguments alone, and lengths, tables and starts may change
