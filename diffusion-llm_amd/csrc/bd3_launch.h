@@ -184,10 +184,11 @@ struct PagedArgs {
   int q_slots;    // its 32-row partial slots
   int slot_rows;  // 32, or the rows there are where the longest chunk has fewer
   int n_splits;   // most key ranges of a tile
-  int split_shift;  // log2 of a range's keys
+  int split_shift;  // log2 of about a range's keys
   int workgroups;
-  // 128-row tiles: the most that all chunks together have, and the order of TileItem.
-  int tiles, levels;
+  // 128-row tiles, not cut: taken in the order of TileItem. level_step: 64^k levels
+  // to a lane, so that 64 lanes cover them all.
+  int sorted, level_step;
   FastDiv level_div;
   float scale_log2;
 };

@@ -1052,14 +1052,17 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.bs_div = bd3::FastDiv::of(a.bs);
   a.group_div = bd3::FastDiv::of(a.group);
   a.kv_heads_div = bd3::FastDiv::of(kv_heads);
-  if (plan.tile < 128) {  // about as many as there are items
-    a.workgroups = (int)std::min(most, ((total_kv >> plan.split_shift) + seqs) * kv_heads * plan.q_tiles);
-  } else {
-    a.tiles = (int)std::min((int64_t)seqs * plan.q_tiles, (int64_t)tokens * a.group / 128 + seqs);
-    const int unit = std::max(1, 128 / a.group);
+  if (plan.tile == 128) {  // the most tiles and ranges that the chunks can have
+    const int64_t tiles = std::min((int64_t)seqs * plan.q_tiles, (int64_t)tokens * a.group / 128 + seqs);
+    a.workgroups = (int)(tiles * plan.n_splits * kv_heads);
+    const int unit = std::max(1, 128 / a.group);  // tokens of a tile
+    const int64_t levels = (int64_t)max_kv / unit + plan.q_tiles;
+    a.sorted = plan.n_splits == 1 && seqs <= 64 && levels < (1 << 24);
     a.level_div = bd3::FastDiv::of(unit);
-    a.levels = max_kv / unit + 1 + plan.q_tiles;
-    a.workgroups = a.tiles * kv_heads * plan.n_splits;
+    a.level_step = 1;
+    while (a.sorted && a.level_step * (int64_t)64 <= levels) a.level_step *= 64;
+  } else {  // about as many as there are items; each takes more if need be
+    a.workgroups = (int)std::min(most, ((total_kv >> plan.split_shift) + seqs) * kv_heads * plan.q_tiles);
   }
   a.scale_log2 = scale * bd3::kLog2e;
   return hip_status(bd3::launch_paged_attn(a, static_cast<hipStream_t>(stream)), "paged_attn launch");

@@ -67,12 +67,37 @@ struct PagedSeq {
   }
 };
 
-// Ranges of 2^split_shift keys that `keys` keys are cut into; what is left over, up to
-// half a range, goes to the last one.
-__device__ __forceinline__ int key_ranges(const PagedArgs& a, int keys) {
-  const int n = (keys + (1 << a.split_shift >> 1)) >> a.split_shift;
-  return n > 1 ? n : 1;
-}
+// How a sequence of kv keys is cut into ranges of `len` keys; a tile that sees only
+// some of the keys has fewer of them.
+// Plain (16- and 32-row tiles): 2^split_shift keys, up to half a range more in the last one.
+// EVEN (128-row tiles): about 2^split_shift keys, whole 64-key tiles, as many in every
+// range but the last: the plain form let the longest items end 4 us after the others
+// (96 rows over 500-4000 keys of 24 sequences, 512-key ranges: 30 us, 24 so). The
+// shorter launches lose 0.5 us to its arithmetic and gain nothing. Its quotients are
+// products with a reciprocal, made exact where it matters.
+template <bool EVEN>
+struct KeySplit {
+  int len, shift;
+  __device__ __forceinline__ KeySplit(const PagedArgs& a, int kv) : len(1 << a.split_shift), shift(a.split_shift) {
+    if constexpr (EVEN) {
+      const int n = (kv + (1 << shift >> 1)) >> shift;
+      len = kv;
+      // at least kv / n: 2^-20 more than covers the reciprocal's and the product's errors
+      if (n > 1) len = (int)((float)kv * __builtin_amdgcn_rcpf((float)n) * 1.000001f) + 1;
+      len = (len + kSwRows - 1) & -kSwRows;
+    }
+  }
+  __device__ __forceinline__ int ranges(int keys) const {  // at least 1
+    if constexpr (EVEN) {  // ceil(keys / len): the estimate's floor is at most two below it
+      int q = (int)((float)keys * __builtin_amdgcn_rcpf((float)(len > 1 ? len : 1)));
+      q += q * len < keys;
+      q += q * len < keys;
+      return q > 1 ? q : 1;
+    }
+    const int q = (keys + (1 << shift >> 1)) >> shift;
+    return q > 1 ? q : 1;
+  }
+};
 
 // The 32-key chunks of one key range that one of NW waves takes in turn (chunks
 // wave, wave + NW, ...): from the pages to registers, the next chunk's loads in
@@ -145,11 +170,12 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// Item `id` of the 16- and 32-row launches: KV head (fastest), row tile, range, in the
+// Item `id` of the list: KV head (fastest), row tile, range, in the
 // order of the sequences. Every sequence has items of its own number, so the list
 // is made here from the lengths, a lane a sequence: a launch of the most items that
 // the bounds allow spent about 1 ns on each empty workgroup (32 sequences of
 // 100-8192 keys, 12 heads: 67 us at the best range length, 55 with the list).
+template <bool EVEN>
 struct PagedItem {
   int b, h, qt, split;
   PagedSeq sq;
@@ -167,7 +193,7 @@ struct PagedItem {
       if (s0 + lane < a.seqs) {
         mine = PagedSeq(a, s0 + lane);
         tiles = (mine.rows + a.tile - 1) / a.tile;
-        items = tiles * key_ranges(a, mine.kv);
+        items = tiles * KeySplit<EVEN>(a, mine.kv).ranges(mine.kv);
       }
       const int upto = wave_scan(items);
       const int at = __popcll(__ballot(before + upto <= j));
@@ -188,11 +214,10 @@ struct PagedItem {
 };
 
 // Tile `j` of all sequences' 128-row tiles of one head, those that see most keys
-// first (up to 64 sequences; beyond, in the order of the sequences). A sequence's
-// tiles, last one first, see kv, kv - u, kv - 2 u, ... keys (u tokens a tile), so its
-// r-th one belongs to level (max_kv - kv) / u + r, and the tiles below level l number
-// the sum of clamp(l - first level, 0, tiles): a binary search finds j's level, a
-// lane a sequence.
+// first (up to 64 sequences). A sequence's tiles, last one first, see kv, kv - u, kv
+// - 2 u, ... keys (u tokens a tile), so its r-th one belongs to level (max_kv - kv) /
+// u + r, and the tiles below level l number the sum of clamp(l - first level, 0,
+// tiles). Each lane forms that sum for a level of its own, 64 levels at a time.
 struct TileItem {
   int b, rank;
   PagedSeq sq;
@@ -200,52 +225,36 @@ struct TileItem {
   __device__ __forceinline__ TileItem(const PagedArgs& a, int j) {
     const int lane = wi_x() & 63;
     found = false;
-    if (a.seqs <= 64) {
-      PagedSeq mine = {};
-      if (lane < a.seqs) mine = PagedSeq(a, lane);
-      const int tiles = (mine.rows + 127) / 128;
-      const int first = fast_div(a.max_kv - mine.kv, a.level_div);
-      auto below = [&](int level) {
-        const int c = level - first < tiles ? level - first : tiles;
-        return __builtin_amdgcn_readlane(wave_scan(c > 0 ? c : 0), 63);
-      };
-      int lo = 0, hi = a.levels;  // below(lo) <= j < below(hi)
-      if (j >= below(hi)) return;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (below(mid) <= j)
-          lo = mid;
-        else
-          hi = mid;
+    PagedSeq mine = {};
+    if (lane < a.seqs) mine = PagedSeq(a, lane);
+    const int tiles = (mine.rows + 127) / 128;
+    const int first = fast_div(a.max_kv - mine.kv, a.level_div);
+    auto below = [&](int level) {  // every lane for its own level
+      int sum = 0;
+      for (int s = 0; s < a.seqs; ++s) {
+        const int c = level - __builtin_amdgcn_readlane(first, s), t = __builtin_amdgcn_readlane(tiles, s);
+        sum += c < 0 ? 0 : (c < t ? c : t);
       }
-      const int nth = j - below(lo);  // of the level's tiles (found with every lane active: the sum is over all)
-      const bool live = lo >= first && lo < first + tiles;
-      const uint64_t all = __ballot(live);
-      const int mine_th = __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
-      const uint64_t it = __ballot(live && mine_th == nth);
-      if (it == 0) return;
-      b = __builtin_ctzll(it);
-      sq = mine.of_lane(b);
-      rank = lo - __builtin_amdgcn_readlane(first, b);
-      found = true;
-      return;
+      return sum;
+    };
+    // The last level with at most j tiles below it: `step` levels to a lane, then 1.
+    int at = 0, before = 0;
+    for (int step = a.level_step; step > 0; step >>= 6) {
+      const int sum = below(at + step * lane);
+      const int n = __popcll(__ballot(sum <= j)) - 1;  // lane 0's sum is at most j
+      at += step * n;
+      before = __builtin_amdgcn_readlane(sum, n);
     }
-    int before = 0;
-    for (int s0 = 0; s0 < a.seqs; s0 += 64) {
-      PagedSeq mine = {};
-      if (s0 + lane < a.seqs) mine = PagedSeq(a, s0 + lane);
-      const int tiles = (mine.rows + 127) / 128;
-      const int upto = wave_scan(tiles);
-      const int at = __popcll(__ballot(before + upto <= j));
-      if (at < 64) {
-        rank = j - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(tiles, at));
-        b = s0 + at;
-        sq = mine.of_lane(at);
-        found = true;
-        return;
-      }
-      before += __builtin_amdgcn_readlane(upto, 63);
-    }
+    const int nth = j - before;  // of the level's tiles
+    const bool live = at >= first && at < first + tiles;
+    const uint64_t all = __ballot(live);
+    const int mine_th = __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+    const uint64_t it = __ballot(live && mine_th == nth);
+    if (it == 0) return;  // j is past the last tile
+    b = __builtin_ctzll(it);
+    sq = mine.of_lane(b);
+    rank = at - __builtin_amdgcn_readlane(first, b);
+    found = true;
   }
 };
 
@@ -256,7 +265,7 @@ struct MergeLds {
   float o[NW][ROWS][kMergeRow];
   float m[NW][ROWS];
   float l[NW][ROWS];
-  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const PagedItem& it, int rt,
+  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const PagedItem<false>& it, int rt,
                                             int d) const {
     float mw[NW], mm = -INFINITY;
 #pragma unroll
@@ -300,7 +309,7 @@ constexpr size_t chunk_smem() {
 // keys x 32 rows) = K Q^T on v_mfma_f32_32x32x16_bf16 with the K tile's rows as A
 // operands; O^T += V^T P^T with V read transposed.
 template <int NW>
-__device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem& it, char* smem) {
+__device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem<false>& it, char* smem) {
   const int tid = wi_x();
   const int lane = tid & 63;
   const int wave = wave_uniform(tid >> 6);
@@ -312,10 +321,11 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
   const PagedSeq& sq = it.sq;
   const int r0 = it.qt * kQT;
   const int key_end = sq.tile_end(a, r0);
-  const int ranges = key_ranges(a, key_end);
+  const KeySplit<false> cut(a, sq.kv);
+  const int ranges = cut.ranges(key_end);
   if (it.split >= ranges) return;
-  const int lo = it.split << a.split_shift;
-  const int hi = it.split + 1 < ranges ? (it.split + 1) << a.split_shift : key_end;
+  const int lo = it.split << cut.shift;
+  const int hi = it.split + 1 < ranges ? lo + cut.len : key_end;
   ChunkStream<NW> kv(a, it.b, it.h, lo, hi, wave, lane);
   if (kv.mine > 0) kv.load(0);
 
@@ -409,7 +419,7 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
 // 16, d 32 c + 8 hq .. +7, hq = lane / 16), B = Q^T; result lane (row lane % 16, hq)
 // holds keys 16 kb + 4 hq + r. O^T (16 d x 16 rows) += V^T P^T over the 32 keys.
 template <int NW>
-__device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem& it, char* smem) {
+__device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem<false>& it, char* smem) {
   constexpr int kRows = 16;
   const int tid = wi_x();
   const int lane = tid & 63;
@@ -421,10 +431,11 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
 
   const PagedSeq& sq = it.sq;
   const int key_end = sq.tile_end(a, 0);
-  const int ranges = key_ranges(a, key_end);
+  const KeySplit<false> cut(a, sq.kv);
+  const int ranges = cut.ranges(key_end);
   if (it.split >= ranges) return;
-  const int lo = it.split << a.split_shift;
-  const int hi = it.split + 1 < ranges ? (it.split + 1) << a.split_shift : key_end;
+  const int lo = it.split << cut.shift;
+  const int hi = it.split + 1 < ranges ? lo + cut.len : key_end;
   ChunkStream<NW> kv(a, it.b, it.h, lo, hi, wave, lane);
   if (kv.mine > 0) kv.load(0);
 
@@ -513,7 +524,7 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
   // The launch has about as many workgroups as there are items; those left over
   // (lengths that the caller's total did not tell) are taken in turn.
   for (int id = wg_x();; id += a.workgroups) {
-    const PagedItem it(a, id);
+    const PagedItem<false> it(a, id);
     if (!it.found) return;
     if constexpr (ROWS == 16)
       paged16_item<NW>(a, it, smem);
@@ -547,24 +558,45 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   const int l32 = lane & 31;
   const int g = lane >> 5;
 
-  const int per_split = a.tiles * a.kv_heads;
-  const int split = wg_x() / per_split;
-  const int e = wg_x() - split * per_split;
-  const int j = wave_uniform(fast_div(e, a.kv_heads_div));
-  const int h = e - j * a.kv_heads;
-  const TileItem it(a, j);
-  if (!it.found) return;
-  const PagedSeq& sq = it.sq;
-  const int b = it.b, bh = b * a.kv_heads + h;
-  const int qt = (sq.rows + 127) / 128 - 1 - it.rank;
+  // One item a workgroup; the launch has the most there can be, those without one at its end.
+  int b, h, qt, split = 0;
+  PagedSeq sq;
+  if (a.sorted) {
+    const int j = wave_uniform(fast_div(wg_x(), a.kv_heads_div));
+    h = wg_x() - j * a.kv_heads;
+    const TileItem it(a, j);
+    if (!it.found) return;
+    b = it.b;
+    sq = it.sq;
+    qt = (sq.rows + 127) / 128 - 1 - it.rank;
+  } else {
+    const PagedItem<true> it(a, wg_x());
+    if (!it.found) return;
+    b = it.b;
+    h = it.h;
+    sq = it.sq;
+    qt = it.qt;
+    split = it.split;
+  }
+  const int bh = b * a.kv_heads + h;
   const int r0 = 128 * qt;
   const int key_end = sq.tile_end(a, r0);
-  const int ranges = key_ranges(a, key_end);
+  const KeySplit<true> cut(a, sq.kv);
+  const int ranges = wave_uniform(cut.ranges(key_end));
   if (split >= ranges) return;
-  const int lo = split << a.split_shift;
-  const int hi = split + 1 < ranges ? (split + 1) << a.split_shift : key_end;
+  const int lo = wave_uniform(split * cut.len);
+  const int hi = split + 1 < ranges ? wave_uniform(lo + cut.len) : key_end;
   const int n_tiles = (hi - lo + kSwRows - 1) / kSwRows;  // 0: a tile that sees no key
   const int n_mine = n_tiles > sub ? (n_tiles - sub + SUBS - 1) / SUBS : 0;
+
+  // Page entries of the set's next 16 tiles: lane 4 i + w holds that of wave w's keys
+  // of the (base + i)-th one.
+  const int32_t* table = a.table + (int64_t)b * a.table_s;
+  auto entries = [&](int base) {
+    const int key = lo + (sub + SUBS * (base + (lane >> 2))) * kSwRows + 16 * (lane & 3);
+    return key < hi ? table[key >> a.page_shift] : -1;
+  };
+  int ids = entries(0), ids_next = -1;
 
   const int qrow0 = r0 + 32 * wave;
   const int myr = qrow0 + l32;
@@ -576,14 +608,6 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) qreg[c] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * c + 8 * g));
 
-  // Page entries of the set's next 16 tiles: lane 4 i + w holds that of wave w's keys
-  // of the (base + i)-th one.
-  const int32_t* table = a.table + (int64_t)b * a.table_s;
-  auto entries = [&](int base) {
-    const int key = lo + (sub + SUBS * (base + (lane >> 2))) * kSwRows + 16 * (lane & 3);
-    return key < hi ? table[key >> a.page_shift] : -1;
-  };
-  int ids = entries(0), ids_next = -1;
   uint64_t ok = __ballot((unsigned)ids < (unsigned)a.pages);
 
   uint32_t koff[2], voff[2];
@@ -776,7 +800,8 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
   const PagedSeq sq = PagedSeq(a, b).of_lane(0);
   const int row = qt * kQT + (wi_x() >> 4);
   if (qt * kQT >= sq.rows) return;
-  const int ranges = key_ranges(a, sq.tile_end(a, qt * kQT / a.tile * a.tile));
+  const int keys = sq.tile_end(a, qt * kQT / a.tile * a.tile);
+  const int ranges = a.tile == 128 ? KeySplit<true>(a, sq.kv).ranges(keys) : KeySplit<false>(a, sq.kv).ranges(keys);
   if (ranges <= 1 || row >= sq.rows) return;
   const int d0 = 4 * (wi_x() & 15);
   const int64_t slot0 = ((int64_t)bh * a.q_slots + qt) * a.n_splits;
