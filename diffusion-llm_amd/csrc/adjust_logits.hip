@@ -13,8 +13,8 @@
 // not matter), keeps what depends on the token alone in registers (8 tokens a
 // thread) and walks the rows, one 16-byte read and write a thread and row, four
 // rows in flight. With no row loop's reads in flight and the bias and history
-// requested one after another the same took 61 us instead of 40 (32 x 32 rows of
-// 50258 bf16 logits: a large copy's rate) and 13 instead of 10 (64 fp32 rows, a bias and a mask each).
+// requested one after another the same took 61 us instead of 46 (32 x 32 rows of
+// 50258 bf16 logits; 40.7 now, a large copy's rate) and 13 instead of 10 (64 fp32 rows, a bias and a mask each).
 #include "bd3_device.h"
 #include "bd3_launch.h"
 
@@ -31,7 +31,11 @@ typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // Eight logits of a row as they lie in memory: loads of several rows are in flight
-// before the first is unpacked.
+// before the first is unpacked. bf16 logits are read once, non-temporally: their
+// reads are not to push the result, which the draw reads next, out of the caches
+// (32 x 32 rows of 50258: 46.2 us with plain reads, 40.8 so; 45.5 with non-temporal
+// writes too). fp32 ones take two reads of a cache line, so plain ones (64 rows 10.0
+// us, non-temporal 10.7).
 template <typename T>
 struct Row8;
 template <>
@@ -39,7 +43,7 @@ struct Row8<uint16_t> {
   u32x4 w;
   __device__ __forceinline__ void load(const uint16_t* p, int left) {
     if (left >= kCols) {
-      w = (u32x4)*reinterpret_cast<const u32x4_a2*>(p);
+      w = (u32x4)__builtin_nontemporal_load(reinterpret_cast<const u32x4_a2*>(p));
     } else {
       w = u32x4{};
 #pragma unroll
@@ -131,10 +135,19 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitArgs a) {
     add[i] = 0.f;
   }
   if (a.bias != nullptr && left > 0) {
-    Row8<float> w;
-    w.load(a.bias + (int64_t)b * a.bias_s + col, left);
+    const float* bp = a.bias + (int64_t)b * a.bias_s + col;
+    if (left >= kCols) {
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) add[i] = w.get(i);
+      for (int i = 0; i < kCols; i += 4) {
+        const f32x4 w = *reinterpret_cast<const f32x4_a4*>(bp + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) add[i + k] = w[k];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCols; ++i)
+        if (i < left) add[i] = bp[i];
+    }
   }
   if (a.tokens != nullptr) {
     constexpr int kFlight = 8;  // tokens requested by a thread before the first is counted
