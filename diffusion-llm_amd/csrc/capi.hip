@@ -888,10 +888,13 @@ struct PagedPlan {
 // longest item's chain of 64-key steps against the load per CU, then the merge
 // launch. Lengths that differ leave the longest item to the end of the 16- and
 // 32-row launches (items in the order of the sequences), so there the two nearly add
-// up; the 128-row launch takes the longest first. Fitted to 9100 timings of 2000
-// batches drawn over 1-64 sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV
-// heads and groups of 1-12 (rms error 7-12%).
-double paged_us(int tile, int subs, double longest, double keys, double items, bool split, bool even) {
+// up; the 128-row launch takes the longest first. busiest: the keys of the CU that
+// gets most of evenly long items, which bounds the 16-row launches: 264 items of 4860
+// keys leave two on 8 CUs and take 75 us whole, 60 in ranges of 1024 (the same 22
+// sequences of 12 heads over 6004 keys 92, 71). Fitted to batches drawn over 1-64
+// sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV heads and groups of 1-12;
+// over 1700 others the rms error is 9% for 16 rows, 12-15% for more.
+double paged_us(int tile, int subs, double longest, double keys, double items, double busiest, bool split, bool even) {
   struct Cost {
     double chain0, chain, load0, load, item, merge, merge_item;
   };
@@ -901,7 +904,8 @@ double paged_us(int tile, int subs, double longest, double keys, double items, b
                                        {5.5, 0.66, 4.8, 0.70, 2.9, 3.2, 1.9},
                                        {8.0, 0.52, 0.0, 0.69, 9.5, 0.0, 0.0}};  // four sets: never with ranges
   const Cost& c = tile == 16 ? kRows16 : tile == 32 ? kRows32[subs - 1] : kRows128[subs >> 1];
-  const double chain = c.chain0 + c.chain * longest / 64.0;
+  const double chain =
+      c.chain0 + std::max(c.chain * longest, tile == 16 && even ? 0.36 * busiest : 0.0) / 64.0;
   const double load = c.load0 + c.load * keys / (64.0 * 256.0) + c.item * items / 256.0;
   const double e = even || tile == 128 ? 3.0 : 1.5;
   return std::pow(std::pow(chain, e) + std::pow(load, e), 1.0 / e) +
@@ -912,10 +916,11 @@ double paged_us(int tile, int subs, double longest, double keys, double items, b
 // rows or 128), sets and ranges (256 keys and longer, at most 64 of a sequence) for
 // what the host knows: bounds, tokens and the keys in all. Ranges pay where a few
 // long sequences would leave the chip idle; 32-row tiles re-read the keys for
-// every tile but start and step faster. Over 500 batches each of up to 16, 17-64,
-// 17-300 and 65-3000 rows the plan takes 0.5%, 2%, 3% and 1.5% more than the best one.
+// every tile but start and step faster. Over 500 batches of up to 16 rows, 600 of
+// 17-300 and 600 of 65-3000 the plan takes 1%, 2% and 1% more than the best of all
+// plans on average, at worst 33%, 44% and 31%.
 // us, whole items -> plan: 12 heads, 16 over 3600 keys 24.7 -> 10.8; 32 sequences of
-// 100-8192 keys 66 -> 51; 32 rows over 2000 keys of 8 sequences 17.3 -> 14.6; 32-row
+// 100-8192 keys 66 -> 51; 32 rows over 500-2000 keys of 8 sequences 17.3 -> 14.6; 32-row
 // tiles -> plan: 50 rows over 1000 keys of 32 sequences 24.4 -> 19.1; 128-row tiles ->
 // plan: 96 rows over 800 keys of 4 sequences, 4 KV heads 12.5 -> 8.7.
 PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
@@ -932,6 +937,9 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
     // items without ranges: not every chunk is as long as the longest
     const double units = kv_heads * std::max(1.0, std::min((double)seqs * q_tiles,
                                                            (double)tokens * (double)group / tile + 0.5 * seqs));
+    const auto busiest = [&](double ranges) {
+      return std::ceil((double)seqs * kv_heads * ranges / 256.0) * max_kv / ranges;
+    };
     const auto take = [&](double us, int subs, int shift) {
       if (!(us < best)) return;
       best = us;
@@ -941,11 +949,13 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
       p.split_shift = shift;
     };
     for (int subs = tile == 16 ? 2 : 1; subs <= (tile == 128 ? 4 : 2); subs *= 2) {
-      take(paged_us(tile, subs, max_kv, units * seen, units, false, even), subs, 30);
+      take(paged_us(tile, subs, max_kv, units * seen, units, busiest(1), false, even), subs, 30);
       for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
         if (max_kv >> shift > 64) continue;
         const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
-        take(paged_us(tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items, true, even), subs, shift);
+        take(paged_us(tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items,
+                      busiest(std::max(1.0, std::floor(max_kv / len + 0.5))), true, even),
+             subs, shift);
       }
     }
   }
