@@ -8,12 +8,22 @@
 // share a KV head: their rows are one matrix of n * group rows, row r token
 // r / group of head h * group + r % group, so a page is read once for all of them.
 //
-// The lengths and the table are device data, so the grid is sized by the
-// caller's bounds and workgroups without rows or keys leave at once. Everything
-// read through device data is bounded: token ranges by the tokens there are,
-// lengths by the table and the caller's bound, page numbers by the pages there
-// are. Keys of an entry outside [0, pages) are not seen (their rows come from
-// a zero row, their scores are masked); keys past the length re-read the last one.
+// O = softmax(q K^T * scale) V over the keys seen, in one pass over the pages with a
+// running maximum and sum (fp32, base 2) per row; probabilities are rounded to bf16
+// for the second product (relative 2^-8 each, as in every attention kernel here),
+// the result once. Long sequences are cut into key ranges whose fp32 partials a
+// second launch merges.
+//
+// The lengths and the table are device data, so workgroups find their items from
+// them (PagedItem, TileItem). Everything read through device data is bounded: token
+// ranges by the tokens there are, lengths by the table and the caller's bound, page
+// numbers by the pages there are. Keys of an entry outside [0, pages) are not seen
+// (their rows come from a zero row, their scores are masked); keys past the length
+// re-read the last one, so nothing that a page holds behind it comes in.
+//
+// Pages cost 11% against a contiguous cache in full launches: 32 sequences x 12 heads,
+// 16 rows over 4112 keys, 70 us at 16- to 256-key pages (5.8 TB/s) against 63; short
+// ones pay two dependent reads (lengths, table entries) before the first key.
 #include "bd3_device.h"
 #include "bd3_launch.h"
 #include "bd3_swz.h"
@@ -305,9 +315,13 @@ constexpr size_t chunk_smem() {
   return v > sizeof(MergeLds<NW, ROWS>) ? v : sizeof(MergeLds<NW, ROWS>);
 }
 
-// 32-row tiles: NW waves share the key chunks of a range. S^T (32
-// keys x 32 rows) = K Q^T on v_mfma_f32_32x32x16_bf16 with the K tile's rows as A
-// operands; O^T += V^T P^T with V read transposed.
+// 32-row tiles: NW waves share the key chunks of a range. S^T (32 keys x 32 rows) =
+// K Q^T on v_mfma_f32_32x32x16_bf16 with the K tile's rows as A operands; O^T += V^T
+// P^T with V read transposed. Eight waves for few items (one workgroup a CU at 160
+// registers), four for many (three a CU), each at its best ranges: 32 rows over 500-2000
+// keys of 8 sequences 14.6 us against 15.4; 32 sequences of 100-8000 keys 43.3, 41.6. At four waves per
+// SIMD it spills (43 -> 50 us). Full launches are bound by HBM (32 sequences x 4128 keys
+// 73 us, 5.6 TB/s; contiguous 65).
 template <int NW>
 __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem<false>& it, char* smem) {
   const int tid = wi_x();
@@ -418,6 +432,11 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
 // rows. S^T of 16 keys x 16 rows: A = K read from the tile (lane: key 16 kb + lane %
 // 16, d 32 c + 8 hq .. +7, hq = lane / 16), B = Q^T; result lane (row lane % 16, hq)
 // holds keys 16 kb + 4 hq + r. O^T (16 d x 16 rows) += V^T P^T over the 32 keys.
+// Eight waves always: four took 8.4 us for 6.8 over 600 keys and 52.2 for 51.3 of a full
+// launch (100-8192 keys). Few workgroups are bound by latency: over 3600 keys of one sequence
+// lengths are there after 0.5 us, the first chunk is staged after 2.8, done after 3.4,
+// merged and written after 4.6 of the kernel's 7.8 us. Many are bound by HBM: 32
+// sequences of 100-8192 keys 48 us, 5.5 TB/s.
 template <int NW>
 __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem<false>& it, char* smem) {
   constexpr int kRows = 16;
@@ -535,16 +554,21 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
   }
 }
 
-// 128-row tiles: four waves of 32 rows that share each
-// 64-key K / V tile, which goes from the page to LDS directly (bd3_swz.h; two
-// stages: the next tile loads during the current one). A wave loads 16 keys of a
-// tile, which lie in one page, so its source is one scalar base and the same lane
-// offsets for every full tile. SUBS sets of four waves take the tiles in turn, each
-// through a ring of its own, and add up at the end: few, long items.
+// 128-row tiles: four waves of 32 rows that share each 64-key K / V tile, which goes
+// from the page to LDS directly (bd3_swz.h; two stages: the next tile loads during
+// the current one). A wave loads 16 keys of a tile, which lie in one page, so its
+// source is one scalar base and the same lane offsets for every full tile. SUBS sets
+// of four waves take the tiles in turn, each through a ring of its own, and add up at
+// the end: few, long items.
 // S^T (keys x rows) = K Q^T, O^T += V^T P^T with P^T taken from the S^T registers;
 // a wave skips tiles past its last row's keys and masks only those that its
 // first row does not see whole. The running maximum is updated when it grew by
 // more than kRescale (log2): a stale one leaves O / l exact and bounds P by 2^8.
+// Full launches are bound by the softmax's VALU work beside the products (8 prompts
+// of 2048 tokens, 12 heads: 72 us), short ones by a tile's own
+// chain, ~1 us for a workgroup alone on its CU: three and four stages only cost
+// occupancy (83 -> 95-107 us for prompts of 1500-4034 tokens, 28 -> 31-37 for 96 rows over
+// 500-4000 keys).
 constexpr float kRescale = 8.0f;
 
 template <int SUBS>
@@ -843,6 +867,8 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
 // v into the pages. y1 = x1 c - x2 s, y2 = x1 s + x2 c on the halves of a head
 // row, in fp32 with the fp32 tables and rounded once (qkv_rope.hip instead repeats
 // an eager bf16 path's five roundings, which no caller of pages has to match).
+// Bound by HBM: 24 chunks of 100-2000 tokens, 16 + 2 x 4 heads, 19.9 us, 4.95 TB/s read
+// and written (a large copy: 5.1); a denoising step's 1024 tokens take 4.4 us.
 // Work item: (token, head of q | k | v, j): coordinate pairs (8j + i, 32 + 8j + i).
 __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {
   const uint32_t e0 = (uint32_t)wg_x() * 256u, e = e0 + wi_x();

@@ -8,6 +8,8 @@ gfx950 kernels implement, so tests can check the kernels against them:
     oracle.attention  the eager fp32 masked attention, its autograd
                       gradients, the decode attention and the split-KV
                       LSE merge (torch on the CPU)
+    oracle.serving    attention over a paged cache, its inputs and adjusted
+                      logits, in float64 (no reference counterpart)
 
 Only tests/, __graft_entry__.smoke() and bench.py's cpu_baseline leg may
 import it, and only as the checker (or, for bench.py, as the timed CPU
