@@ -1136,6 +1136,8 @@ int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_
                       const int32_t* allowed, float fill, const int64_t* strides, void* stream) {
   if (batch < 0 || rows < 0 || history < 0) return fail(BD3_EINVAL, "batch, rows and history must be >= 0");
   if (vocab < 1 || vocab > (1 << 30)) return fail(BD3_EINVAL, "vocab must lie in [1, 2^30], got %d", vocab);
+  // 32-bit indices run up to a workgroup's worth past the last row and token of the history
+  if (rows > (1 << 30) || history > (1 << 30)) return fail(BD3_EINVAL, "rows and history must be at most 2^30");
   if (logits_fp32 != 0 && logits_fp32 != 1) return fail(BD3_EINVAL, "logits_fp32 must be 0 (bf16) or 1 (fp32)");
   if (strides == nullptr || penalties == nullptr) return fail(BD3_EINVAL, "strides and penalties must be non-NULL");
   for (int i = 0; i < 8; ++i)

@@ -405,7 +405,7 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
  *     token the same).
  *   strides: 8 int64 element strides: logits (batch, row), out (batch, row),
  *     tokens (batch), bias (batch), allowed (batch, row).
- * No reference counterpart.
+ * vocab, rows and history at most 2^30. No reference counterpart.
  */
 int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_t batch,
                       int32_t rows, int32_t vocab, const int64_t* tokens, int32_t history,

@@ -240,3 +240,16 @@ def test_logits_refusals(lib, kw, text):
     assert lib.bd3_adjust_logits(a["x"], a["fp32"], a["out"], a["batch"], a["rows"], a["vocab"], a["tokens"], a["history"],
                                  a["lens"], pen, None, None, None, None, None, a["fill"], st, None) == _native.BD3_EINVAL
     assert text in _native.last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(history=(1 << 31) - 1), dict(history=(1 << 30) + 1), dict(rows=(1 << 31) - 1, vocab=1),
+                                dict(rows=(1 << 30) + 1, vocab=1), dict(rows=1 << 30, vocab=1)])
+def test_logits_sizes_whose_indices_would_wrap(lib, kw):
+    """Indices into the history and the rows are 32 bits wide and run up to a
+    workgroup's worth past the last one."""
+    a = dict(batch=1, rows=3, vocab=100, history=5)
+    a.update(kw)
+    pen, st = (ctypes.c_float * 3)(1.0, 0.0, 0.0), (ctypes.c_int64 * 8)(300, 100, 300, 100, 5, 0, 0, 0)
+    assert lib.bd3_adjust_logits(P, 0, P, a["batch"], a["rows"], a["vocab"], P, a["history"], None, pen, None, None, None,
+                                 None, None, -1e6, st, None) == _native.BD3_EINVAL
+    assert "2^30" in _native.last_error() or "too large" in _native.last_error()
