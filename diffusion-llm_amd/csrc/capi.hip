@@ -965,6 +965,11 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
   return p;
 }
 
+// Rows of the longest chunk that the plan's numbers hold (2^22 tiles of 128 at most).
+bool paged_fits(int32_t heads, int32_t kv_heads, int32_t max_q) {
+  return (int64_t)max_q * (heads / kv_heads) < ((int64_t)1 << 29);
+}
+
 size_t paged_part_rows(const PagedPlan& p, int32_t seqs, int32_t kv_heads) {
   return p.n_splits > 1 ? (size_t)seqs * kv_heads * p.q_slots * p.n_splits * p.slot_rows : 0;
 }
@@ -979,6 +984,7 @@ size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t tokens, int32_t head
       max_kv > bd3::kPagedMaxKeys || total_kv < 0)
     return 0;
   max_q = std::min(max_q, tokens);
+  if (!paged_fits(heads, kv_heads, max_q)) return 0;
   max_kv = std::max(max_kv, 1);
   const size_t rows = paged_part_rows(paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv), seqs, kv_heads);
   return rows == 0 ? 0 : align256(rows * bd3::kHeadDim * 4) + rows * 4;
@@ -1009,6 +1015,8 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   if (strides[4] >= kMaxDmaSeqStride || strides[7] >= kMaxDmaSeqStride)
     return fail(BD3_EINVAL, "page slot strides must be < 2^24 elements");
   if (strides[10] < 0) return fail(BD3_EINVAL, "page_table stride must be >= 0");
+  if (!paged_fits(heads, kv_heads, max_q))
+    return fail(BD3_EINVAL, "max_q * heads / kv_heads too large (limit 2^29 rows a chunk)");
   const PagedPlan plan = paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
   const size_t rows = paged_part_rows(plan, seqs, kv_heads);
   const size_t po_bytes = align256(rows * bd3::kHeadDim * 4);

@@ -253,3 +253,12 @@ def test_logits_sizes_whose_indices_would_wrap(lib, kw):
     assert lib.bd3_adjust_logits(P, 0, P, a["batch"], a["rows"], a["vocab"], P, a["history"], None, pen, None, None, None,
                                  None, None, -1e6, st, None) == _native.BD3_EINVAL
     assert "2^30" in _native.last_error() or "too large" in _native.last_error()
+
+
+def test_attention_rows_beyond_32_bits(lib):
+    """max_q * heads / kv_heads rows of 2^32 and more do not fit the tile numbers."""
+    kw = dict(seqs=1, tokens=1 << 30, heads=1 << 24, kv_heads=1, max_q=1 << 30, total=64)
+    assert attn(lib, **kw) == _native.BD3_EINVAL
+    assert "too large" in _native.last_error()
+    assert lib.bd3_paged_attn_workspace_bytes(1, 1 << 30, 1 << 24, 1, 1 << 30, 64, 64) == 0
+    assert lib.bd3_paged_attn_workspace_bytes(1, 1 << 30, 1 << 24, 1, 1 << 30, 1 << 20, 1 << 20) == 0
