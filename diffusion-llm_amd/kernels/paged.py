@@ -50,7 +50,8 @@ def paged_attention(
     """Attention of each sequence's chunk over its pages: (tokens, heads, 64).
     A token that sees no key gets 0. Rows of `out` behind the last sequence are
     left as they are (without `out` they are undefined). Keys of table entries
-    that are no page (negative, or past the pool) are not seen."""
+    that are no page (negative, or past the pool) are not seen. `out` overlaps no
+    input."""
     return host().paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q,
                                   -1 if max_kv is None else max_kv, -1 if total_kv is None else total_kv, out)
 
@@ -71,7 +72,8 @@ def paged_attention_inputs(
     their slots in the pages. Computed in fp32 and rounded once, so a key
     differs from kv_cache.attention_inputs' (which repeats the eager path's bf16
     roundings) by up to two of its last bits. Positions beyond the RoPE tables
-    use their last row; nothing is written where the table has no page."""
+    use their last row; nothing is written where the table has no page. qkv, out,
+    k_pages and v_pages do not overlap."""
     return host().paged_attention_inputs(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, page_table, q_starts,
                                          kv_lens, out)
 

@@ -210,3 +210,15 @@ def test_other_streams_agree(cuda):
             outs += [adjust_logits(xd, **d) for _ in range(3)]
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.gpu
+def test_overlapping_out_is_refused(cuda):
+    """In place is fine, any other overlap has no defined result."""
+    flat = torch.randn(2 * 3 * 100 + 100, device=cuda)
+    x = flat[:600].view(2, 3, 100)
+    for out in (flat[100:].view(2, 3, 100), flat[:600].view(3, 2, 100).transpose(0, 1)):
+        with pytest.raises(AssertionError, match="overlap"):
+            adjust_logits(x, bias=torch.ones(100, device=cuda), out=out)
+    want = x + 1
+    assert torch.equal(adjust_logits(x, bias=torch.ones(100, device=cuda), out=x), want)

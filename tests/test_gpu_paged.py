@@ -465,3 +465,37 @@ def test_cache_steps_equal_one_pass(cuda, record_error):
         # each within HALF (|o| + sum p |v|), |v| < 6, of the same value
         record_error("chunks vs whole", float((a - b).abs().max()), 2 * HALF * 12)
         record_error("blocks vs whole", float((a - c).abs().max()), 2 * HALF * 12)
+
+
+@pytest.mark.gpu
+def test_overlapping_tensors_are_refused(cuda):
+    """What a workgroup writes while another still reads it has no defined result.
+    Apart, the halves of one buffer are fine, and so are interleaved k and v pools."""
+    c = on(paged_case([(4, 20)], 4, 2, 16), cuda)
+    batch = (c["table"], c["starts"], c["kv"])
+    flat = torch.zeros(2 * c["q"].numel(), device=cuda, dtype=BF)
+    n = c["q"].numel()
+    q = flat[:n].view_as(c["q"]).copy_(c["q"])
+    want = paged_attention(c["q"], c["k"], c["v"], *batch, 4, max_q=4)
+    for out in (q, flat[64:n + 64].view_as(q), c["k"].view(-1)[:n].view_as(q), c["v"].view(-1)[:n].view_as(q)):
+        with pytest.raises(AssertionError, match="overlap"):
+            paged_attention(q, c["k"], c["v"], *batch, 4, max_q=4, out=out)
+    assert torch.equal(paged_attention(q, c["k"], c["v"], *batch, 4, max_q=4, out=flat[n:].view_as(q)), want)
+
+    sin, cos = (t.to(cuda) for t in rope_tables(D, 64))
+    buf = torch.ones(4 * 8 * D, device=cuda, dtype=BF)
+    qkv = buf.view(4, 8 * D)
+
+    def inputs(k, v, out=None):
+        return paged_attention_inputs(qkv, 4, sin, cos, k, v, *batch, out=out)
+
+    pool = torch.zeros(c["k"].numel() + 64, device=cuda, dtype=BF)
+    k = pool[:-64].view_as(c["k"])
+    for kw in (dict(k=k, v=k), dict(k=k, v=pool[64:].view_as(k)), dict(k=k, v=c["v"], out=buf[:n].view_as(q)),
+               dict(k=k, v=c["v"], out=k.view(-1)[:n].view_as(q))):
+        with pytest.raises(AssertionError, match="overlap"):
+            inputs(**kw)
+    both = torch.zeros(2, *c["k"].shape, device=cuda, dtype=BF)
+    woven = torch.zeros(c["k"].shape[0], 2, *c["k"].shape[1:], device=cuda, dtype=BF)
+    a, b = inputs(both[0], both[1]), inputs(woven[:, 0], woven[:, 1])
+    assert torch.equal(a, b) and torch.equal(both, woven.transpose(0, 1)) and both.abs().sum() > 0
