@@ -180,8 +180,8 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// Item `id` of the list: KV head (fastest), row tile, range, in the
-// order of the sequences. Every sequence has items of its own number, so the list
+// Item `id` of the list: KV head (fastest), row tile, range, in the order of the
+// sequences. Every sequence has items of its own number, so the list
 // is made here from the lengths, a lane a sequence: a launch of the most items that
 // the bounds allow spent about 1 ns on each empty workgroup (32 sequences of
 // 100-8192 keys, 12 heads: 67 us at the best range length, 55 with the list).
@@ -319,9 +319,9 @@ constexpr size_t chunk_smem() {
 // K Q^T on v_mfma_f32_32x32x16_bf16 with the K tile's rows as A operands; O^T += V^T
 // P^T with V read transposed. Eight waves for few items (one workgroup a CU at 160
 // registers), four for many (three a CU), each at its best ranges: 32 rows over 500-2000
-// keys of 8 sequences 14.6 us against 15.4; 32 sequences of 100-8000 keys 43.3, 41.6. At four waves per
-// SIMD it spills (43 -> 50 us). Full launches are bound by HBM (32 sequences x 4128 keys
-// 73 us, 5.6 TB/s; contiguous 65).
+// keys of 8 sequences 14.6 us against 15.4; 32 sequences of 100-8000 keys 43.3, 41.6.
+// At four waves per SIMD it spills (43 -> 50 us). Full launches are bound by HBM (32
+// sequences x 4128 keys 73 us, 5.6 TB/s; contiguous 65).
 template <int NW>
 __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem<false>& it, char* smem) {
   const int tid = wi_x();
@@ -567,8 +567,8 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
 // Full launches are bound by the softmax's VALU work beside the products (8 prompts
 // of 2048 tokens, 12 heads: 72 us), short ones by a tile's own
 // chain, ~1 us for a workgroup alone on its CU: three and four stages only cost
-// occupancy (83 -> 95-107 us for prompts of 1500-4034 tokens, 28 -> 31-37 for 96 rows over
-// 500-4000 keys).
+// occupancy (84 -> 95-107 us for prompts of 1507-4034 tokens, 28.5 -> 31-37 for 96 rows
+// over 727-3871 keys).
 constexpr float kRescale = 8.0f;
 
 template <int SUBS>

@@ -50,8 +50,10 @@ def paged_attention(
     """Attention of each sequence's chunk over its pages: (tokens, heads, 64).
     A token that sees no key gets 0. Rows of `out` behind the last sequence are
     left as they are (without `out` they are undefined). Keys of table entries
-    that are no page (negative, or past the pool) are not seen. `out` overlaps no
-    input."""
+    that are no page (negative, or past the pool) are not seen. Slots past a
+    sequence's keys may hold anything; its keys and values themselves must be
+    finite, also those that only later tokens of the chunk see (their weights are
+    zeros that multiply them). `out` overlaps no input."""
     return host().paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q,
                                   -1 if max_kv is None else max_kv, -1 if total_kv is None else total_kv, out)
 

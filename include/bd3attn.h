@@ -342,9 +342,11 @@ int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t
  *     slot), v_pages (page, head, slot), o (token, head), page_table (row); last
  *     strides 1, all but the table's multiples of 8, slot strides < 2^24.
  * o overlaps none of the inputs. Pages may be shared by sequences (a common
- * prefix). Device data is not trusted with addresses: token ranges are cut to [0, tokens),
- * lengths to [0, max_kv], and keys whose table entry lies outside [0, pages) are
- * not seen. Table entries beyond a sequence's keys are not used.
+ * prefix). Device data is not trusted with addresses: token ranges are cut to
+ * [0, tokens), lengths to [0, max_kv], and keys whose table entry lies outside
+ * [0, pages) are not seen. Table entries beyond a sequence's keys are not used, and slots beyond
+ * them may hold anything; the keys and values of a sequence must be finite, also those
+ * that only later tokens of its chunk see (zero weights multiply them).
  * Preconditions: page_size a power of two in [16, 1024], head_dim == 64, heads a
  * multiple of kv_heads. The same call may be captured into a graph: its launches
  * depend on the arguments alone, and lengths, tables and starts may change
@@ -401,8 +403,8 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
  *   bias: device fp32 (vocab) (batch stride 0) or (batch, vocab), or NULL.
  *   allowed: device int32 words, bit v % 32 of word v / 32 set where token v is
  *     allowed, one set for all (strides 0), for each sequence or each row; NULL.
- *   fill: finite in the logits' type, so that a row whose mask allows nothing stays finite (every
- *     token the same).
+ *   fill: finite in the logits' type, so that a row whose mask allows nothing stays
+ *     finite (every token the same).
  *   strides: 8 int64 element strides: logits (batch, row), out (batch, row),
  *     tokens (batch), bias (batch), allowed (batch, row).
  * vocab, rows and history at most 2^30. No reference counterpart.
