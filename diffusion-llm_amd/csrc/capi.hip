@@ -893,7 +893,7 @@ struct PagedPlan {
 // keys leave two on 8 CUs and take 75 us whole, 60 in ranges of 1024 (the same 22
 // sequences of 12 heads over 6004 keys 92, 71). Fitted to batches drawn over 1-64
 // sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV heads and groups of 1-12;
-// over 1700 others the rms error is 9% for 16 rows, 12-15% for more.
+// over 1751 others the rms error is 9% for 16 rows, 15% for 17-300, 12% for more.
 double paged_us(int tile, int subs, double longest, double keys, double items, double busiest, bool split, bool even) {
   struct Cost {
     double chain0, chain, load0, load, item, merge, merge_item;
@@ -916,9 +916,9 @@ double paged_us(int tile, int subs, double longest, double keys, double items, d
 // rows or 128), sets and ranges (256 keys and longer, at most 64 of a sequence) for
 // what the host knows: bounds, tokens and the keys in all. Ranges pay where a few
 // long sequences would leave the chip idle; 32-row tiles re-read the keys for
-// every tile but start and step faster. Over 500 batches of up to 16 rows, 600 of
-// 17-300 and 600 of 65-3000 the plan takes 1%, 2% and 1% more than the best of all
-// plans on average, at worst 33%, 44% and 31%.
+// every tile but start and step faster. Over 500 batches of up to 16 rows, 800 of
+// 17-300 and 451 of 257 and more the plan takes 1%, 3% and 2% more than the best of
+// all plans on average, at worst 33%, 47% and 36%.
 // us, whole items -> plan: 12 heads, 16 over 3600 keys 24.7 -> 10.8; 32 sequences of
 // 100-8192 keys 66 -> 51; 32 rows over 500-2000 keys of 8 sequences 17.3 -> 14.6; 32-row
 // tiles -> plan: 50 rows over 1000 keys of 32 sequences 24.4 -> 19.1; 128-row tiles ->
