@@ -926,7 +926,7 @@ double paged_us(int tile, int subs, double longest, double keys, double items, d
 PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
                      int64_t total_kv) {
   const int64_t group = heads / kv_heads, rows = (int64_t)max_q * group;
-  const double total = (double)std::min(total_kv, (int64_t)seqs * max_kv);
+  const double total = (double)total_kv;
   const double seen = std::max(1.0, (total - 0.5 * tokens) / seqs);  // keys that a tile sees, about
   const bool even = (double)max_kv * seqs < 1.5 * total;
   PagedPlan p = {};
@@ -986,6 +986,7 @@ size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t tokens, int32_t head
   max_q = std::min(max_q, tokens);
   if (!paged_fits(heads, kv_heads, max_q)) return 0;
   max_kv = std::max(max_kv, 1);
+  total_kv = std::min(total_kv, (int64_t)seqs * max_kv);
   const size_t rows = paged_part_rows(paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv), seqs, kv_heads);
   return rows == 0 ? 0 : align256(rows * bd3::kHeadDim * 4) + rows * 4;
 }
@@ -1007,6 +1008,7 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   if (seqs == 0 || tokens == 0 || max_q == 0) return BD3_OK;
   if (max_kv == 0) max_kv = 1;  // chunks without keys: their rows are 0
   max_q = std::min(max_q, tokens);
+  total_kv = std::min(total_kv, (int64_t)seqs * max_kv);  // any larger one says no more
   if (int st = check_rows(q, strides, 2, "q")) return st;
   if (int st = check_rows(k_pages, strides + 2, 3, "k_pages")) return st;
   if (int st = check_rows(v_pages, strides + 5, 3, "v_pages")) return st;

@@ -336,8 +336,8 @@ int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t
  *   max_q, max_kv: the host's bounds of a chunk's tokens and a sequence's keys
  *     (max_kv <= table_width * page_size). They size the launch: a chunk's
  *     tokens beyond max_q are left out and keys beyond max_kv are not seen.
- *   total_kv: about the sum of kv_lens, 0 .. seqs * max_kv: chooses how the keys
- *     are cut over workgroups, not what is computed.
+ *   total_kv: about the sum of kv_lens (>= 0; more than seqs * max_kv counts as that):
+ *     chooses how the keys are cut over workgroups, not what is computed.
  *   strides: 11 int64 element strides: q (token, head), k_pages (page, head,
  *     slot), v_pages (page, head, slot), o (token, head), page_table (row); last
  *     strides 1, all but the table's multiples of 8, slot strides < 2^24.

@@ -499,3 +499,15 @@ def test_overlapping_tensors_are_refused(cuda):
     woven = torch.zeros(c["k"].shape[0], 2, *c["k"].shape[1:], device=cuda, dtype=BF)
     a, b = inputs(both[0], both[1]), inputs(woven[:, 0], woven[:, 1])
     assert torch.equal(a, b) and torch.equal(both, woven.transpose(0, 1)) and both.abs().sum() > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk,heads,kv_heads", [(1, 2, 2), (16, 4, 2), (50, 160, 40), (200, 2, 2)])
+def test_any_total_is_a_hint(cuda, record_error, chunk, heads, kv_heads):
+    """total_kv up to the largest integer: the launch it shapes stays that of the
+    batch (2^63 - 1 wrapped the number of workgroups)."""
+    c = paged_case([(chunk, 900), (1, 30)], heads, kv_heads, 16, seed=chunk)
+    ref, tol = attention_reference(c, 16)
+    d = on(c, cuda)
+    for total in (2 * c["max_kv"], 1 << 40, 2 ** 63 - 1):
+        record_error("paged attention / bound", worst(attend(d, 16, total_kv=total), ref, tol), 1.0)

@@ -262,3 +262,12 @@ def test_attention_rows_beyond_32_bits(lib):
     assert "too large" in _native.last_error()
     assert lib.bd3_paged_attn_workspace_bytes(1, 1 << 30, 1 << 24, 1, 1 << 30, 64, 64) == 0
     assert lib.bd3_paged_attn_workspace_bytes(1, 1 << 30, 1 << 24, 1, 1 << 30, 1 << 20, 1 << 20) == 0
+
+
+def test_totals_beyond_the_bound_are_the_bound(lib):
+    size = lib.bd3_paged_attn_workspace_bytes
+    for seqs, tokens, heads, kv_heads, max_q, max_kv in ((1, 16, 12, 12, 16, 8192), (2, 32, 12, 12, 16, 8192)):
+        most = size(seqs, tokens, heads, kv_heads, max_q, max_kv, seqs * max_kv)
+        assert most > 0
+        for total in (seqs * max_kv + 1, 1 << 40, 2 ** 63 - 1):
+            assert size(seqs, tokens, heads, kv_heads, max_q, max_kv, total) == most
