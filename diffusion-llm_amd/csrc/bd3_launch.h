@@ -170,8 +170,8 @@ struct PagedArgs {
   const int32_t* table;     // (seqs, width) page numbers
   const int32_t* q_starts;  // (seqs + 1)
   const int32_t* kv_lens;   // (seqs)
-  float* part_o;            // (seqs * kv_heads, q_slots, n_splits, slot_rows, 64) fp32, or null
-  float* part_lse;          // (seqs * kv_heads, q_slots, n_splits, slot_rows) log2 LSE, or null
+  float* part_o;            // (kv_heads, part_rows, n_splits, 64) fp32, or null
+  float* part_lse;          // (kv_heads, part_rows, n_splits) log2 LSE, or null
   int64_t sq_t, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, so_t, so_h, table_s;  // element strides
   int seqs, tokens, kv_heads, group, pages, page, page_shift;
   int max_q;      // most tokens of a chunk: the caller's bound
@@ -181,9 +181,9 @@ struct PagedArgs {
   int tile;       // query rows per workgroup
   int subs;       // sets of 4 waves per workgroup: 1, 2 or (128-row tiles) 4
   int q_tiles;    // tiles of the longest chunk
-  int q_slots;    // its 32-row partial slots
-  int slot_rows;  // 32, or the rows there are where the longest chunk has fewer
-  int n_splits;   // most key ranges of a tile
+  int part_slots;  // workgroups of the merge for a KV head: 32 of its part_rows each
+  int part_rows;   // tokens * group: the packed rows of a KV head, row q0 * group + r that of row r of a chunk at q0
+  int n_splits;    // most key ranges of a tile
   int split_shift;  // log2 of about a range's keys
   int workgroups;
   // 128-row tiles, not cut: taken in the order of TileItem. level_step: 64^k levels

@@ -879,10 +879,20 @@ int log2_of(int32_t x) {
 }
 
 // What a paged attention call runs: rows per workgroup, sets of four waves that
-// share an item, tiles and partial slots of the longest chunk, key ranges.
+// share an item, tiles of the longest chunk, key ranges.
 struct PagedPlan {
-  int tile, subs, q_tiles, q_slots, slot_rows, n_splits, split_shift;
+  int tile, subs, q_tiles, n_splits, split_shift;
 };
+
+// Partials of a call that cuts its keys: a row of 64 outputs and its LSE, in fp32, for
+// every query row of the batch and range, and at most this many bytes of them, which
+// a captured graph keeps. The bound leaves 14 ranges to 2175 tokens of 32 heads and 2
+// to 16000; more rows than that are enough items without ranges. (Slots for every
+// 32 rows of the longest chunk in every sequence took 3.3 GB for 63 single tokens over
+// 100-8192 keys beside a prompt of 2048, 12 heads, and 146 us with their merge; 53 MB, 85 us so.)
+constexpr int64_t kPagedPartBytes = (int64_t)256 << 20;
+constexpr int64_t kPagedPartRows = kPagedPartBytes / ((bd3::kHeadDim + 1) * 4);
+static_assert(kPagedPartRows * bd3::kHeadDim <= INT32_MAX, "32-bit indices of the partials");
 
 // Estimated us of a plan, to choose tile, sets and the length of the key ranges: the
 // longest item's chain of 64-key steps against the load per CU, then the merge
@@ -912,6 +922,11 @@ double paged_us(int tile, int subs, double longest, double keys, double items, d
          (split ? c.merge + c.merge_item * items / 256.0 : 0.0);
 }
 
+// Ranges of a sequence of max_kv keys.
+int paged_ranges(int32_t max_kv, int shift) {
+  return std::max(1, (int)(((int64_t)max_kv + ((int64_t)1 << shift >> 1)) >> shift));
+}
+
 // The cheapest plan of the tiles (16 rows where they are enough, else 32 up to 256
 // rows or 128), sets and ranges (256 keys and longer, at most 64 of a sequence) for
 // what the host knows: bounds, tokens and the keys in all. Ranges pay where a few
@@ -929,6 +944,7 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
   const double total = (double)total_kv;
   const double seen = std::max(1.0, (total - 0.5 * tokens) / seqs);  // keys that a tile sees, about
   const bool even = (double)max_kv * seqs < 1.5 * total;
+  const int64_t part_rows = std::min((int64_t)tokens * heads, kPagedPartRows + 1);  // more than the bound is as much
   PagedPlan p = {};
   double best = INFINITY;
   for (int tile : {16, 32, 128}) {
@@ -952,6 +968,7 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
       take(paged_us(tile, subs, max_kv, units * seen, units, busiest(1), false, even), subs, 30);
       for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
         if (max_kv >> shift > 64) continue;
+        if (part_rows * paged_ranges(max_kv, shift) > kPagedPartRows) continue;
         const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
         take(paged_us(tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items,
                       busiest(std::max(1.0, std::floor(max_kv / len + 0.5))), true, even),
@@ -959,9 +976,7 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
       }
     }
   }
-  p.q_slots = (int)((rows + 31) / 32);
-  p.slot_rows = (int)std::min<int64_t>(rows, 32);
-  p.n_splits = std::max(1, (int)(((int64_t)max_kv + ((int64_t)1 << p.split_shift >> 1)) >> p.split_shift));
+  p.n_splits = paged_ranges(max_kv, p.split_shift);
   return p;
 }
 
@@ -970,8 +985,8 @@ bool paged_fits(int32_t heads, int32_t kv_heads, int32_t max_q) {
   return (int64_t)max_q * (heads / kv_heads) < ((int64_t)1 << 29);
 }
 
-size_t paged_part_rows(const PagedPlan& p, int32_t seqs, int32_t kv_heads) {
-  return p.n_splits > 1 ? (size_t)seqs * kv_heads * p.q_slots * p.n_splits * p.slot_rows : 0;
+size_t paged_part_rows(const PagedPlan& p, int32_t tokens, int32_t heads) {
+  return p.n_splits > 1 ? (size_t)tokens * heads * p.n_splits : 0;
 }
 
 }  // namespace
@@ -987,7 +1002,7 @@ size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t tokens, int32_t head
   if (!paged_fits(heads, kv_heads, max_q)) return 0;
   max_kv = std::max(max_kv, 1);
   total_kv = std::min(total_kv, (int64_t)seqs * max_kv);
-  const size_t rows = paged_part_rows(paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv), seqs, kv_heads);
+  const size_t rows = paged_part_rows(paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv), tokens, heads);
   return rows == 0 ? 0 : align256(rows * bd3::kHeadDim * 4) + rows * 4;
 }
 
@@ -1020,14 +1035,14 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   if (!paged_fits(heads, kv_heads, max_q))
     return fail(BD3_EINVAL, "max_q * heads / kv_heads too large (limit 2^29 rows a chunk)");
   const PagedPlan plan = paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
-  const size_t rows = paged_part_rows(plan, seqs, kv_heads);
+  const size_t rows = paged_part_rows(plan, tokens, heads);
   const size_t po_bytes = align256(rows * bd3::kHeadDim * 4);
   const size_t need = rows == 0 ? 0 : po_bytes + rows * 4;
   if (workspace_bytes < need) return fail(BD3_EINVAL, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
   if (need > 0 && (workspace == nullptr || !aligned16(workspace)))
     return fail(BD3_EINVAL, "workspace must be a 16-byte aligned device pointer");
   const int64_t most = (int64_t)seqs * kv_heads * plan.q_tiles * plan.n_splits;
-  if (std::max(most, (int64_t)seqs * kv_heads * plan.q_slots) >= ((int64_t)1 << 22))
+  if (most >= ((int64_t)1 << 22))
     return fail(BD3_EINVAL, "seqs * kv_heads * tiles * ranges too large (limit 2^22 workgroups)");
   bd3::PagedArgs a = {};
   a.q = static_cast<const uint16_t*>(q);
@@ -1065,9 +1080,11 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.tile = plan.tile;
   a.subs = plan.subs;
   a.q_tiles = plan.q_tiles;
-  a.q_slots = plan.q_slots;
-  a.slot_rows = plan.slot_rows;
   a.n_splits = plan.n_splits;
+  if (plan.n_splits > 1) {
+    a.part_rows = tokens * a.group;  // bounded by kPagedPartRows
+    a.part_slots = (a.part_rows + 31) / 32;
+  }
   a.split_shift = plan.split_shift;
   a.bs_div = bd3::FastDiv::of(a.bs);
   a.group_div = bd3::FastDiv::of(a.group);

@@ -31,7 +31,7 @@
 namespace bd3 {
 namespace {
 
-constexpr int kQT = 32;       // rows of the 32-row tile and of a partial slot (128-row tiles have four)
+constexpr int kQT = 32;       // rows of the 32-row tile and of a workgroup of the merge
 constexpr int kSub = 32;      // keys per wave step
 constexpr int kStride = 72;   // padded LDS row (bf16)
 constexpr int kMergeRow = kHeadDim + 4;
@@ -63,6 +63,14 @@ struct PagedSeq {
     r.kv = __builtin_amdgcn_readlane(kv, lane);
     r.rows = __builtin_amdgcn_readlane(rows, lane);
     return r;
+  }
+  // Place of a row's partial of one range: the packed rows of a KV head after those of
+  // the head before it, a row's ranges side by side. So partials take what the
+  // tokens there are need, however long the longest chunk is. (With the ranges outermost
+  // 32 sequences of 16 rows took 52.0 us for 51.4: writes 128 KB apart.) At most 2^20
+  // places: kPagedPartRows.
+  __device__ __forceinline__ int part_row(const PagedArgs& a, int h, int split, int r0) const {
+    return (h * a.part_rows + q0 * a.group + r0) * a.n_splits + split;
   }
   // Keys that token i sees: [0, key_end).
   __device__ __forceinline__ int key_end(const PagedArgs& a, int i) const {
@@ -293,8 +301,8 @@ struct MergeLds {
       ot += wgt * *reinterpret_cast<const f32x4*>(&o[w][rt][d]);
     }
     const float inv = lt > 0.f ? 1.f / lt : 0.f;  // a row that sees no key: 0
+    const int row = it.qt * ROWS + rt;
     if (ranges == 1) {
-      const int row = it.qt * ROWS + rt;
       if (row < it.sq.rows) {
         const int t = fast_div(row, a.group_div);
         *reinterpret_cast<bf16x4*>(a.o + (int64_t)(it.sq.q0 + t) * a.so_t +
@@ -302,10 +310,10 @@ struct MergeLds {
             to_bf16x4(ot[0] * inv, ot[1] * inv, ot[2] * inv, ot[3] * inv);
       }
     } else {
-      if (rt >= a.slot_rows) return;
-      const int64_t slot = (((int64_t)it.b * a.kv_heads + it.h) * a.q_slots + it.qt) * a.n_splits + it.split;
-      *reinterpret_cast<f32x4*>(&a.part_o[(slot * a.slot_rows + rt) * kHeadDim + d]) = ot * inv;
-      if (d == 0) a.part_lse[slot * a.slot_rows + rt] = lt > 0.f ? mm + fast_log2(lt) : -INFINITY;
+      if (row >= it.sq.rows) return;
+      const int at = it.sq.part_row(a, it.h, it.split, row);
+      *reinterpret_cast<f32x4*>(&a.part_o[at * kHeadDim + d]) = ot * inv;
+      if (d == 0) a.part_lse[at] = lt > 0.f ? mm + fast_log2(lt) : -INFINITY;
     }
   }
 };
@@ -602,7 +610,6 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     qt = it.qt;
     split = it.split;
   }
-  const int bh = b * a.kv_heads + h;
   const int r0 = 128 * qt;
   const int key_end = sq.tile_end(a, r0);
   const KeySplit<true> cut(a, sq.kv);
@@ -802,35 +809,58 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
         *reinterpret_cast<bf16x4*>(op + 32 * db + 8 * q4 + 4 * g) =
             to_bf16x4(o[db][4 * q4] * inv, o[db][4 * q4 + 1] * inv, o[db][4 * q4 + 2] * inv, o[db][4 * q4 + 3] * inv);
   } else {
-    const int64_t slot = ((int64_t)bh * a.q_slots + (qrow0 >> 5)) * a.n_splits + split;
-    float* po = a.part_o + (slot * a.slot_rows + l32) * kHeadDim;
+    const int at = sq.part_row(a, h, split, myr);
+    float* po = a.part_o + at * kHeadDim;
 #pragma unroll
     for (int db = 0; db < 2; ++db)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4)
         *reinterpret_cast<f32x4*>(po + 32 * db + 8 * q4 + 4 * g) =
             f32x4{o[db][4 * q4] * inv, o[db][4 * q4 + 1] * inv, o[db][4 * q4 + 2] * inv, o[db][4 * q4 + 3] * inv};
-    if (g == 0) a.part_lse[slot * a.slot_rows + l32] = any ? mref + fast_log2(ltot) : -INFINITY;
+    if (g == 0) a.part_lse[at] = any ? mref + fast_log2(ltot) : -INFINITY;
   }
 }
 
 // Merges the ranges of the tiles that were cut: weights exp2(lse_s - max lse), 16
 // threads a row, 4 outputs each; the loads of 8 ranges are issued before their
-// first use. Grid: (32-row slots, sequence * KV head).
+// first use. Grid: (32 packed rows, KV head).
 __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
-  const int qt = wg_x() % a.q_slots;
-  const int bh = wg_x() / a.q_slots;
-  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  const PagedSeq sq = PagedSeq(a, b).of_lane(0);
-  const int row = qt * kQT + (wi_x() >> 4);
-  if (qt * kQT >= sq.rows) return;
-  const int keys = sq.tile_end(a, qt * kQT / a.tile * a.tile);
+  const int h = wg_x() / a.part_slots;
+  const int at = (wg_x() - h * a.part_slots) * kQT + (wi_x() >> 4);
+  const int lane = wi_x() & 63;
+  const int tok = fast_div(at, a.group_div);
+  // The share that holds the row's token, from the lane that has it: a lane a
+  // sequence, four rows to a wave. Every lane stays in the loop, it holds a share.
+  PagedSeq sq = {};
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    PagedSeq mine = {};
+    if (s0 + lane < a.seqs) mine = PagedSeq(a, s0 + lane);
+    int from = -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = __builtin_amdgcn_readlane(tok, 16 * k);
+      const uint64_t has = __ballot(mine.q0 <= t && t - mine.q0 < mine.n);
+      if ((lane >> 4) == k && has != 0) from = __builtin_ctzll(has);
+    }
+    const int q0 = __builtin_amdgcn_ds_bpermute(4 * from, mine.q0), n = __builtin_amdgcn_ds_bpermute(4 * from, mine.n);
+    const int kv = __builtin_amdgcn_ds_bpermute(4 * from, mine.kv), rows = __builtin_amdgcn_ds_bpermute(4 * from, mine.rows);
+    if (from >= 0 && sq.n == 0) {
+      sq.q0 = q0;
+      sq.n = n;
+      sq.kv = kv;
+      sq.rows = rows;
+    }
+  }
+  const int row = at - sq.q0 * a.group;
+  if (row >= sq.rows) return;  // of no sequence, or past the caller's bound
+  const int r0 = row & -a.tile;
+  const int keys = sq.key_end(a, fast_div((r0 + a.tile < sq.rows ? r0 + a.tile : sq.rows) - 1, a.group_div));
   const int ranges = a.tile == 128 ? KeySplit<true>(a, sq.kv).ranges(keys) : KeySplit<false>(a, sq.kv).ranges(keys);
-  if (ranges <= 1 || row >= sq.rows) return;
+  if (ranges <= 1) return;
   const int d0 = 4 * (wi_x() & 15);
-  const int64_t slot0 = ((int64_t)bh * a.q_slots + qt) * a.n_splits;
-  const float* lp = a.part_lse + slot0 * a.slot_rows + (wi_x() >> 4);
-  const float* pp = a.part_o + (slot0 * a.slot_rows + (wi_x() >> 4)) * kHeadDim + d0;
+  const int part0 = (h * a.part_rows + at) * a.n_splits;
+  const float* lp = a.part_lse + part0;
+  const float* pp = a.part_o + part0 * kHeadDim + d0;
   constexpr int kG = 8;
   float mm = -INFINITY, wt = 0.f;
   f32x4 acc = {};
@@ -839,8 +869,8 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
     f32x4 po[kG];
 #pragma unroll
     for (int k = 0; k < kG; ++k) {
-      l[k] = s0 + k < ranges ? lp[(s0 + k) * a.slot_rows] : -INFINITY;
-      po[k] = s0 + k < ranges ? *reinterpret_cast<const f32x4*>(pp + (int64_t)(s0 + k) * a.slot_rows * kHeadDim) : f32x4{};
+      l[k] = s0 + k < ranges ? lp[s0 + k] : -INFINITY;
+      po[k] = s0 + k < ranges ? *reinterpret_cast<const f32x4*>(pp + (s0 + k) * kHeadDim) : f32x4{};
     }
     float mg = mm;
 #pragma unroll
@@ -858,9 +888,8 @@ __global__ __launch_bounds__(512) void paged_combine_kernel(PagedArgs a) {
     }
   }
   const float inv = wt > 0.f ? 1.f / wt : 0.f;
-  const int t = fast_div(row, a.group_div);
-  *reinterpret_cast<bf16x4*>(a.o + (int64_t)(sq.q0 + t) * a.so_t + (int64_t)(h * a.group + row - t * a.group) * a.so_h +
-                             d0) = to_bf16x4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+  *reinterpret_cast<bf16x4*>(a.o + (int64_t)tok * a.so_t + (int64_t)(h * a.group + at - tok * a.group) * a.so_h + d0) =
+      to_bf16x4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
 }
 
 // Rotary embedding of q and k at each token's position, q to packed tokens, k and
@@ -925,7 +954,6 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {
 }  // namespace
 
 hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream) {
-  const int64_t bh = (int64_t)a.seqs * a.kv_heads;
   const dim3 grid((unsigned)a.workgroups);
   if (a.tile == 128) {
     if (a.subs == 4)
@@ -944,7 +972,7 @@ hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream) {
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.n_splits == 1) return e;
-  hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)(bh * a.q_slots)), dim3(512), 0, stream, a);
+  hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)(a.kv_heads * a.part_slots)), dim3(512), 0, stream, a);
   return hipGetLastError();
 }
 

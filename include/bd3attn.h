@@ -347,6 +347,8 @@ int bd3_kv_write(const void* k, const void* v, void* k_dst, void* v_dst, int32_t
  * [0, pages) are not seen. Table entries beyond a sequence's keys are not used, and slots beyond
  * them may hold anything; the keys and values of a sequence must be finite, also those
  * that only later tokens of its chunk see (zero weights multiply them).
+ *   workspace: bd3_paged_attn_workspace_bytes of the same arguments: 260 bytes for each
+ *     token, head and key range where a call cuts its keys, at most 256 MB; else 0.
  * Preconditions: page_size a power of two in [16, 1024], head_dim == 64, heads a
  * multiple of kv_heads. The same call may be captured into a graph: its launches
  * depend on the arguments alone, and lengths, tables and starts may change

@@ -511,3 +511,45 @@ def test_any_total_is_a_hint(cuda, record_error, chunk, heads, kv_heads):
     d = on(c, cuda)
     for total in (2 * c["max_kv"], 1 << 40, 2 ** 63 - 1):
         record_error("paged attention / bound", worst(attend(d, 16, total_kv=total), ref, tol), 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("singles,chunk,ctx,heads,kv_heads", [
+    (90, 300, 900, 2, 2), (63, 700, 100, 4, 1), (70, 40, 1500, 2, 2), (130, 12, 1200, 6, 3), (5, 33, 3000, 2, 1)])
+def test_a_chunk_beside_single_tokens(cuda, record_error, singles, chunk, ctx, heads, kv_heads):
+    """A prompt chunk in the middle of sequences of one token, some without any: the
+    keys of both in ranges, whose partials lie packed, 32 rows of several sequences to
+    a workgroup of the merge."""
+    from kernels import _native
+    g = torch.Generator().manual_seed(singles)
+    lens = [(int(n), int(x)) for n, x in zip((torch.rand(singles, generator=g) < 0.8).int(),
+                                             torch.randint(0, 1700, (singles,), generator=g))]
+    lens.insert(singles // 2, (chunk, ctx))
+    c = paged_case(lens, heads, kv_heads, 16, seed=singles, extra_tokens=4)
+    T = int(c["starts"][-1])
+    ref, tol = attention_reference(c, 16)
+    d = on(c, cuda)
+    cut = 0
+    for total in (0, c["total"], 10 ** 7):
+        out = torch.full_like(d["q"], 7.0)
+        attend(d, 16, total_kv=total, out=out)
+        record_error("paged attention / bound", worst(out[:T], ref[:T], tol[:T]), 1.0)
+        assert (out[T:] == 7.0).all(), "rows behind the last sequence were written"
+        cut += _native.lib().bd3_paged_attn_workspace_bytes(len(lens), T + 4, heads, kv_heads, c["max_q"], c["max_kv"],
+                                                            total) > 0
+    assert cut, "no call cut its keys"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk", [1, 16, 40, 200])
+def test_partials_of_starts_that_do_not_ascend(cuda, chunk):
+    """Starts that run backwards are no batch; the rows of sequences that still own
+    tokens of their own come out as ever, and nothing else is touched."""
+    c = paged_case([(chunk, 1500), (chunk, 900), (chunk, 1200)], 2, 2, 16, seed=chunk)
+    d = on(c, cuda)
+    want = attend(d, 16, total_kv=0)
+    d["starts"] = torch.tensor([0, chunk, chunk - 1, -5], dtype=torch.int32, device=cuda)
+    out = torch.full_like(d["q"], 7.0)
+    attend(d, 16, total_kv=0, out=out)
+    assert torch.equal(out[:chunk], want[:chunk])
+    assert (out[chunk:] == 7.0).all()

@@ -271,3 +271,19 @@ def test_totals_beyond_the_bound_are_the_bound(lib):
         assert most > 0
         for total in (seqs * max_kv + 1, 1 << 40, 2 ** 63 - 1):
             assert size(seqs, tokens, heads, kv_heads, max_q, max_kv, total) == most
+
+
+def test_partials_follow_the_tokens(lib):
+    """Scratch memory goes by the query rows that there are, a row of 64 outputs and
+    an LSE for each and range, not by the longest chunk in every sequence: a prompt
+    chunk beside many single tokens took gigabytes."""
+    for singles, chunk, heads, kv_heads, max_kv, total in (
+            (63, 2048, 12, 12, 8192, 64 * 600), (63, 2048, 12, 12, 8192, 64 * 4000), (127, 2048, 12, 12, 32768, 128 * 600),
+            (31, 200, 12, 12, 8192, 32 * 600), (47, 2000, 12, 12, 8192, 50000), (127, 2048, 32, 8, 32768, 1 << 19),
+            (255, 2048, 32, 8, 16384, 1 << 19), (0, 1 << 17, 12, 12, 1 << 20, 1 << 20)):
+        tokens, ranges = singles + chunk, 65
+        need = lib.bd3_paged_attn_workspace_bytes(singles + 1, tokens, heads, kv_heads, chunk, max_kv, total)
+        assert need <= min(tokens * heads * ranges * 260, (256 << 20) + 256), (singles, chunk, need)
+    # and it is what the rows of the ranges take
+    need = lib.bd3_paged_attn_workspace_bytes(1, 16, 12, 12, 16, 8192, 8192)
+    assert need % (16 * 12 * 260) < 256 and need // (16 * 12 * 260) in range(2, 66)
