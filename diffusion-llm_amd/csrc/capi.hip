@@ -879,10 +879,14 @@ int log2_of(int32_t x) {
 }
 
 // What a paged attention call runs: rows per workgroup, sets of four waves that
-// share an item, tiles of the longest chunk, key ranges.
+// share an item (0 rows: nothing fits the launch), tiles of the longest chunk, the most
+// tiles of all chunks, key ranges.
 struct PagedPlan {
   int tile, subs, q_tiles, n_splits, split_shift;
+  int64_t tiles;
 };
+constexpr int kPagedWorkgroups = (1 << 22) - 1;  // of a launch
+constexpr int64_t kPagedItems = 1 << 30;         // that the kernels' 32-bit sums hold, whatever the starts are
 
 // Partials of a call that cuts its keys: a row of 64 outputs and its LSE, in fp32, for
 // every query row of the batch and range, and at most this many bytes of them, which
@@ -946,6 +950,7 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
   const bool even = (double)max_kv * seqs < 1.5 * total;
   const int64_t part_rows = std::min((int64_t)tokens * heads, kPagedPartRows + 1);  // more than the bound is as much
   PagedPlan p = {};
+  p.split_shift = 30;
   double best = INFINITY;
   for (int tile : {16, 32, 128}) {
     if (tile == 16 ? rows > 16 : rows <= 16 || (tile == 32 && rows > 256)) continue;
@@ -956,19 +961,28 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
     const auto busiest = [&](double ranges) {
       return std::ceil((double)seqs * kv_heads * ranges / 256.0) * max_kv / ranges;
     };
+    const int64_t tiles = std::min((int64_t)seqs * q_tiles, (int64_t)tokens * group / tile + seqs);
+    const auto fits = [&](int64_t ranges) {  // each product is below 2^63 where it is formed
+      const int64_t items = (int64_t)seqs * q_tiles;
+      if (items >= kPagedItems || items * ranges >= kPagedItems || items * ranges * kv_heads >= kPagedItems) return false;
+      return tile != 128 || tiles * ranges * kv_heads <= kPagedWorkgroups;  // the shorter tiles' workgroups take several
+    };
     const auto take = [&](double us, int subs, int shift) {
       if (!(us < best)) return;
       best = us;
       p.tile = tile;
       p.q_tiles = q_tiles;
+      p.tiles = tiles;
       p.subs = subs;
       p.split_shift = shift;
     };
+    if (!fits(1)) continue;
     for (int subs = tile == 16 ? 2 : 1; subs <= (tile == 128 ? 4 : 2); subs *= 2) {
       take(paged_us(tile, subs, max_kv, units * seen, units, busiest(1), false, even), subs, 30);
       for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
         if (max_kv >> shift > 64) continue;
-        if (part_rows * paged_ranges(max_kv, shift) > kPagedPartRows) continue;
+        const int ranges = paged_ranges(max_kv, shift);
+        if (part_rows * ranges > kPagedPartRows || !fits(ranges)) continue;
         const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
         take(paged_us(tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items,
                       busiest(std::max(1.0, std::floor(max_kv / len + 0.5))), true, even),
@@ -1024,6 +1038,11 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   if (max_kv == 0) max_kv = 1;  // chunks without keys: their rows are 0
   max_q = std::min(max_q, tokens);
   total_kv = std::min(total_kv, (int64_t)seqs * max_kv);  // any larger one says no more
+  if (!paged_fits(heads, kv_heads, max_q))
+    return fail(BD3_EINVAL, "max_q * heads / kv_heads too large (limit 2^29 rows a chunk)");
+  const PagedPlan plan = paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
+  if (plan.tile == 0)
+    return fail(BD3_EINVAL, "batch too large (limits: 2^22 workgroups, seqs * kv_heads * tiles of the longest chunk 2^30)");
   if (int st = check_rows(q, strides, 2, "q")) return st;
   if (int st = check_rows(k_pages, strides + 2, 3, "k_pages")) return st;
   if (int st = check_rows(v_pages, strides + 5, 3, "v_pages")) return st;
@@ -1032,18 +1051,12 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   if (strides[4] >= kMaxDmaSeqStride || strides[7] >= kMaxDmaSeqStride)
     return fail(BD3_EINVAL, "page slot strides must be < 2^24 elements");
   if (strides[10] < 0) return fail(BD3_EINVAL, "page_table stride must be >= 0");
-  if (!paged_fits(heads, kv_heads, max_q))
-    return fail(BD3_EINVAL, "max_q * heads / kv_heads too large (limit 2^29 rows a chunk)");
-  const PagedPlan plan = paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
   const size_t rows = paged_part_rows(plan, tokens, heads);
   const size_t po_bytes = align256(rows * bd3::kHeadDim * 4);
   const size_t need = rows == 0 ? 0 : po_bytes + rows * 4;
   if (workspace_bytes < need) return fail(BD3_EINVAL, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
   if (need > 0 && (workspace == nullptr || !aligned16(workspace)))
     return fail(BD3_EINVAL, "workspace must be a 16-byte aligned device pointer");
-  const int64_t most = (int64_t)seqs * kv_heads * plan.q_tiles * plan.n_splits;
-  if (most >= ((int64_t)1 << 22))
-    return fail(BD3_EINVAL, "seqs * kv_heads * tiles * ranges too large (limit 2^22 workgroups)");
   bd3::PagedArgs a = {};
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k_pages);
@@ -1090,8 +1103,7 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.group_div = bd3::FastDiv::of(a.group);
   a.kv_heads_div = bd3::FastDiv::of(kv_heads);
   if (plan.tile == 128) {  // the most tiles and ranges that the chunks can have
-    const int64_t tiles = std::min((int64_t)seqs * plan.q_tiles, (int64_t)tokens * a.group / 128 + seqs);
-    a.workgroups = (int)(tiles * plan.n_splits * kv_heads);
+    a.workgroups = (int)(plan.tiles * plan.n_splits * kv_heads);
     const int unit = std::max(1, 128 / a.group);  // tokens of a tile
     const int64_t levels = (int64_t)max_kv / unit + plan.q_tiles;
     a.sorted = plan.n_splits == 1 && seqs <= 64 && levels < (1 << 24);
@@ -1099,7 +1111,8 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
     a.level_step = 1;
     while (a.sorted && a.level_step * (int64_t)64 <= levels) a.level_step *= 64;
   } else {  // about as many as there are items; each takes more if need be
-    a.workgroups = (int)std::min(most, ((total_kv >> plan.split_shift) + seqs) * kv_heads * plan.q_tiles);
+    const int64_t items = ((total_kv >> plan.split_shift) + seqs) * kv_heads * plan.q_tiles;
+    a.workgroups = (int)std::min({items, plan.tiles * plan.n_splits * kv_heads, (int64_t)kPagedWorkgroups});
   }
   a.scale_log2 = scale * bd3::kLog2e;
   return hip_status(bd3::launch_paged_attn(a, static_cast<hipStream_t>(stream)), "paged_attn launch");

@@ -553,3 +553,18 @@ def test_partials_of_starts_that_do_not_ascend(cuda, chunk):
     attend(d, 16, total_kv=0, out=out)
     assert torch.equal(out[:chunk], want[:chunk])
     assert (out[chunk:] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,chunk", [(16, 2, 1024), (4, 2, 100), (4, 2, 3)])
+def test_thousands_of_sequences(cuda, record_error, heads, kv_heads, chunk):
+    """One chunk among 8192 sequences, most without tokens in this step: the launch
+    goes by the tokens."""
+    g = torch.Generator().manual_seed(1)
+    lens = [(int(n), int(x)) for n, x in zip((torch.rand(8191, generator=g) < 0.05).int(),
+                                             torch.randint(0, 40, (8191,), generator=g))]
+    lens.insert(5000, (chunk, 700))
+    c = paged_case(lens, heads, kv_heads, 64, seed=1)
+    ref, tol = attention_reference(c, 16)
+    for total in (0, c["total"]):
+        record_error("paged attention / bound", worst(attend(on(c, cuda), 16, total_kv=total), ref, tol), 1.0)

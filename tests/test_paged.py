@@ -287,3 +287,25 @@ def test_partials_follow_the_tokens(lib):
     # and it is what the rows of the ranges take
     need = lib.bd3_paged_attn_workspace_bytes(1, 16, 12, 12, 16, 8192, 8192)
     assert need % (16 * 12 * 260) < 256 and need // (16 * 12 * 260) in range(2, 66)
+
+
+def test_batches_are_refused_by_what_they_launch(lib):
+    """A long chunk beside many short ones: what counts is the tiles that the tokens
+    make, not the longest chunk's in every sequence. (An absent q shows that the
+    sizes were accepted, before anything could be launched.)"""
+    for singles, chunk, heads, kv_heads, max_kv in ((255, 16384, 32, 32, 16384), (511, 8192, 32, 8, 16384),
+                                                    (4095, 32768, 64, 8, 1 << 17), (8191, 1024, 16, 2, 1024)):
+        for total in (0, max_kv + 100 * singles, (singles + 1) * max_kv):
+            kw = dict(seqs=singles + 1, tokens=singles + chunk, heads=heads, kv_heads=kv_heads, max_q=chunk,
+                      width=max_kv // 16, max_kv=max_kv, total=total)
+            assert attn(lib, **kw, q=None) == _native.BD3_EINVAL
+            assert "q must" in _native.last_error(), (singles, chunk, _native.last_error())
+    # and products that would wrap are still refused
+    big = (1 << 31) - 1
+    for kw in (dict(seqs=big, tokens=big, max_q=1), dict(seqs=big, tokens=big, heads=big, kv_heads=big, max_q=1),
+               dict(seqs=1 << 20, tokens=1 << 30, max_q=4096), dict(seqs=1 << 24, tokens=1 << 24, heads=64, kv_heads=64),
+               dict(seqs=1, tokens=1 << 28, heads=4, kv_heads=2, max_q=1 << 28)):
+        assert attn(lib, **kw, q=None) == _native.BD3_EINVAL
+        assert "too large" in _native.last_error(), kw
+        n = {**dict(seqs=2, tokens=8, heads=4, kv_heads=2, max_q=4), **kw}
+        assert lib.bd3_paged_attn_workspace_bytes(n["seqs"], n["tokens"], n["heads"], n["kv_heads"], n["max_q"], 64, 100) == 0
