@@ -980,9 +980,8 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
     for (int subs = tile == 16 ? 2 : 1; subs <= (tile == 128 ? 4 : 2); subs *= 2) {
       take(paged_us(tile, subs, max_kv, units * seen, units, busiest(1), false, even), subs, 30);
       for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
-        if (max_kv >> shift > 64) continue;
         const int ranges = paged_ranges(max_kv, shift);
-        if (part_rows * ranges > kPagedPartRows || !fits(ranges)) continue;
+        if (ranges > 64 || part_rows * ranges > kPagedPartRows || !fits(ranges)) continue;
         const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
         take(paged_us(tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items,
                       busiest(std::max(1.0, std::floor(max_kv / len + 0.5))), true, even),

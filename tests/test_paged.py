@@ -309,3 +309,11 @@ def test_batches_are_refused_by_what_they_launch(lib):
         assert "too large" in _native.last_error(), kw
         n = {**dict(seqs=2, tokens=8, heads=4, kv_heads=2, max_q=4), **kw}
         assert lib.bd3_paged_attn_workspace_bytes(n["seqs"], n["tokens"], n["heads"], n["kv_heads"], n["max_q"], 64, 100) == 0
+
+
+def test_at_most_64_ranges(lib):
+    """Of a sequence, as rounded: 16540 keys are 65 ranges of about 256."""
+    size = lib.bd3_paged_attn_workspace_bytes
+    for max_kv in (16383, 16384, 16511, 16512, 16540, 16639, 16640, 33100, 66200, 1 << 20):
+        for total in (max_kv // 10, max_kv):
+            assert size(1, 1, 1, 1, 1, max_kv, total) <= 64 * 260 + 256, max_kv
