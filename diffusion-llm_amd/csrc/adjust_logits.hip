@@ -6,7 +6,9 @@
 //   c > 0: x = x > 0 ? x / repetition : x * repetition, then x -= frequency * c + presence
 //   x += bias[v];   x = fill where the mask's bit of v is 0
 // in fp32, rounded once to the logits' type. fill is finite, so a row whose mask
-// leaves nothing holds it everywhere.
+// leaves nothing holds it everywhere; and a finite logit stays finite, as the draw
+// wants it: what a penalty or bias takes past the type's range (the type's lowest value
+// times a repetition) becomes its largest of that sign.
 //
 // A workgroup takes 2048 tokens of the vocabulary for some of a sequence's rows:
 // it counts its tokens among the history in LDS (integer adds: the order does
@@ -14,8 +16,8 @@
 // thread) and walks the rows, one 16-byte read and write a thread and row, four
 // rows in flight. With no row loop's reads in flight and the bias and history
 // requested one after another the same took 61 us instead of 46 (32 x 32 rows of
-// 50258 bf16 logits; 40.8 now, 5.06 TB/s, a large copy's rate) and 13.5 instead of 10
-// (64 fp32 rows, a bias and a mask each).
+// 50258 bf16 logits; 41.3 now, 5.0 TB/s, a large copy's rate) and 13.5 instead of 10
+// (64 fp32 rows, a bias and a mask each; 10.2 now).
 #include "bd3_device.h"
 #include "bd3_launch.h"
 
@@ -26,6 +28,24 @@ constexpr int kCols = 8;                    // tokens per thread
 constexpr int kSlice = kLogitSlice;         // tokens per workgroup
 constexpr int kThreads = kSlice / kCols;
 static_assert(kThreads == 256, "one pass over a slice");
+
+// |x| as an integer. Behind an empty asm: this code is built without honour to NaNs, and
+// the compiler takes comparisons of plain bits back to such ones of floats, which a
+// NaN passes.
+__device__ __forceinline__ uint32_t magnitude(float x) {
+  uint32_t u = __float_as_uint(x);
+  asm("" : "+v"(u));
+  return u & 0x7fffffffu;
+}
+
+constexpr uint32_t kInf = 0x7f800000u;  // magnitude of an infinite one; a NaN's is larger
+
+// x, a result of a and b, or the largest number of its sign where x is infinite
+// and a and b are finite.
+__device__ __forceinline__ float finite(float x, float a, float b) {
+  const bool over = magnitude(x) == kInf && magnitude(a) < kInf && magnitude(b) < kInf;
+  return over ? __uint_as_float((__float_as_uint(x) & 0x80000000u) | (kInf - 1)) : x;
+}
 
 // Rows start at any element: 16-byte accesses of element alignment.
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -55,14 +75,33 @@ struct Row8<uint16_t> {
   __device__ __forceinline__ float get(int i) const {
     return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
   }
-  static __device__ __forceinline__ void store(uint16_t* p, const float (&x)[kCols], int left) {
+  __device__ __forceinline__ void set(const float (&x)[kCols]) {
+    w = __builtin_bit_cast(u32x4, to_bf16x8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]));
+  }
+  // Is any of them infinite (or NaN)?
+  __device__ __forceinline__ bool infinite() const {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+    return ((__builtin_bit_cast(uint32_t, m) + 0x00800080u) & 0x80008000u) != 0;
+  }
+  // The type's lowest or highest value for those that became infinite from finite ones.
+  __device__ __forceinline__ void limit(const Row8& x, const float (&add)[kCols]) {
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) {
+      const uint32_t u = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+      const bool over = (u & 0x7fffu) == 0x7f80u && magnitude(x.get(i)) < kInf && magnitude(add[i]) < kInf;
+      w[i >> 1] -= over ? 1u << (16 * (i & 1)) : 0u;
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* p, int left) const {
     if (left >= kCols) {
-      *reinterpret_cast<u32x4_a2*>(p) =
-          __builtin_bit_cast(u32x4, to_bf16x8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]));
+      *reinterpret_cast<u32x4_a2*>(p) = w;
     } else {
 #pragma unroll
       for (int i = 0; i < kCols; ++i)
-        if (i < left) p[i] = __builtin_bit_cast(uint16_t, (__bf16)x[i]);
+        if (i < left) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
     }
   }
 };
@@ -81,14 +120,28 @@ struct Row8<float> {
     }
   }
   __device__ __forceinline__ float get(int i) const { return w[i >> 2][i & 3]; }
-  static __device__ __forceinline__ void store(float* p, const float (&x)[kCols], int left) {
+  __device__ __forceinline__ void set(const float (&x)[kCols]) {
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) w[i >> 2][i & 3] = x[i];
+  }
+  __device__ __forceinline__ bool infinite() const {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) top = fmaxf(top, fabsf(get(i)));
+    return magnitude(top) >= kInf;
+  }
+  __device__ __forceinline__ void limit(const Row8& x, const float (&add)[kCols]) {
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) w[i >> 2][i & 3] = finite(get(i), x.get(i), add[i]);
+  }
+  __device__ __forceinline__ void store(float* p, int left) const {
     if (left >= kCols) {
-      *reinterpret_cast<f32x4_a4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<f32x4_a4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+      *reinterpret_cast<f32x4_a4*>(p) = w[0];
+      *reinterpret_cast<f32x4_a4*>(p + 4) = w[1];
     } else {
 #pragma unroll
       for (int i = 0; i < kCols; ++i)
-        if (i < left) p[i] = x[i];
+        if (i < left) p[i] = w[i >> 2][i & 3];
     }
   }
 };
@@ -174,7 +227,7 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitArgs a) {
       if (i0 > tid) request(i0);
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
-        const uint64_t at = (uint64_t)(t[k] - v0);
+        const uint64_t at = (uint64_t)t[k] - (uint64_t)v0;
         if (at < (uint64_t)kSlice && t[k] >= 0 && i0 + k * kThreads < n) atomicAdd(&count[at], 1u);
       }
     }
@@ -186,7 +239,8 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitArgs a) {
       if (c > 0) {
         up[i] = inv;
         down[i] = rep;
-        add[i] -= f * (float)c + g;
+        const float pen = finite(fmaf(f, (float)c, g), f, g);
+        add[i] = finite(add[i] - pen, add[i], pen);
       }
     }
   }
@@ -204,7 +258,17 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitArgs a) {
         x[i] = fmaf(x[i], x[i] > 0.f ? up[i] : down[i], add[i]);
         x[i] = (yes[k] >> i) & 1 ? x[i] : a.fill;
       }
-      Row8<T>::store(out + (int64_t)(r0 + k) * a.out_r, x, left);
+      // A row is looked at for infinite ones as a whole, 41.3 us; value by value, all of
+      // them always, 43.4.
+      Row8<T> y;
+      y.set(x);
+      if (__builtin_expect(__ballot(y.infinite()) != 0, 0)) {
+        // bf16: read again (the result may lie over it, but is not written yet), so that the
+        // row's registers are free before; with them kept there is a wave fewer per SIMD.
+        if constexpr (sizeof(T) == 2) v[k].load(in + (int64_t)(r0 + k) * a.in_r, left);
+        y.limit(v[k], add);
+      }
+      y.store(out + (int64_t)(r0 + k) * a.out_r, left);
     }
   }
 }

@@ -96,8 +96,10 @@ def adjust_logits(
     x <= 0) minus frequency * c + presence; then bias is added; then tokens whose
     bit (bit v % 32 of word v // 32) is 0 are set to `fill`, which SUBS's own
     [MASK] logit (-1e6, model/subs.py:8) is by default: finite, as the draw wants
-    it, also in a row whose mask allows nothing. In fp32, rounded once. The
-    penalties are numbers or (batch) float32 tensors; tokens outside the
+    it, also in a row whose mask allows nothing. In fp32, rounded once; what leaves
+    the dtype's range becomes its largest value of that sign, unless the logit or
+    its bias is infinite. The penalties are numbers or (batch) float32 tensors of
+    finite values (not looked at), repetition > 0; tokens outside the
     vocabulary count for nothing. `out=logits` works in place."""
     assert logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32), \
         "logits must be bf16 or fp32 CUDA tensors"

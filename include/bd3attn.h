@@ -394,14 +394,16 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
  *   if c > 0: x = x > 0 ? x / repetition : x * repetition,
  *             x -= frequency * c + presence
  *   x += bias[v];   x = fill where v's bit of the mask is 0
- * in fp32, rounded once to the logits' type.
+ * in fp32, rounded once to the logits' type; a result past the type's range becomes its
+ * largest value of that sign unless the logit or the bias is infinite itself.
  *   logits, out: (batch, rows, vocab) bf16 (logits_fp32 = 0) or fp32 (1), last
  *     stride 1; out may be logits itself, and overlap it in no other way.
  *   tokens: device int64 (batch, history), or NULL for no penalties; values
  *     outside [0, vocab) count for nothing. lengths: device int32 (batch), cut to
  *     [0, history]; NULL: all of history.
- *   penalties: host {repetition, frequency, presence}; repetition, frequency,
- *     presence: device fp32 (batch) in place of the one number, or NULL.
+ *   penalties: host {repetition, frequency, presence}, finite, repetition > 0; repetition,
+ *     frequency, presence: device fp32 (batch) in place of the one number, or NULL; their
+ *     values must be such, too (they are not looked at).
  *   bias: device fp32 (vocab) (batch stride 0) or (batch, vocab), or NULL.
  *   allowed: device int32 words, bit v % 32 of word v / 32 set where token v is
  *     allowed, one set for all (strides 0), for each sequence or each row; NULL.

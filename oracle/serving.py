@@ -94,6 +94,9 @@ def adjust_logits(logits, tokens=None, lengths=None, repetition=1.0, frequency=0
                 x[b, :, t] -= of(frequency, b) * c + of(presence, b)
         if bias is not None:
             x[b] += (bias if bias.dim() == 1 else bias[b]).to(F64)
+        # finite terms: in the type's range
+        top = torch.finfo(logits.dtype).max
+        x[b] = torch.where(torch.isfinite(x[b]), x[b].clamp(-top, top), x[b])
         if allowed is not None:
             for r in range(R):
                 words = allowed if allowed.dim() == 1 else allowed[b] if allowed.dim() == 2 else allowed[b, r]

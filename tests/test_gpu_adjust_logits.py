@@ -222,3 +222,39 @@ def test_overlapping_out_is_refused(cuda):
             adjust_logits(x, bias=torch.ones(100, device=cuda), out=out)
     want = x + 1
     assert torch.equal(adjust_logits(x, bias=torch.ones(100, device=cuda), out=x), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("V", [40, 2051])
+def test_finite_logits_stay_finite(cuda, dtype, V):
+    """The type's lowest and highest values, as a caller bans or forces a token, under
+    penalties and biases that take them past its range: the value itself, not an
+    infinite one, so the draw that follows sees finite logits only. Infinite and nan
+    logits and biases go through."""
+    top, inf = torch.finfo(dtype).max, float("inf")
+    x = torch.zeros(3, 2, V, dtype=dtype)
+    x[:, :, 0::4], x[:, :, 1::4], x[:, :, 2::4] = -top, top, 1.5
+    tokens = torch.arange(V)[None].repeat(3, 1)
+    rep, freq = torch.tensor([1.3, 0.5, 1.0]), torch.tensor([0.5, 0.0, 1e38])
+    bias = torch.zeros(3, V)
+    bias[0, 0::4], bias[1, 1::4], bias[2, 0::8] = -3e38, 3e38, -3e38
+    kw = dict(repetition=rep, frequency=freq, presence=0.1, bias=bias)
+    ref = orc.adjust_logits(x, tokens, None, **kw)
+    assert torch.isfinite(ref).all() and ref.abs().max() == top
+    got = adjust_logits(x.to(cuda), tokens.to(cuda), **dev(kw, cuda)).cpu()
+    assert torch.isfinite(got).all()
+    # one rounding to the dtype and at most four fp32 ones of terms of the size of the result or of 3.4e38
+    tol = 1.001 * (torch.finfo(dtype).eps / 2 * ref.abs() + 4 * 2.0 ** -24 * 3.5e38 * (ref.abs() > 1e30)) + 1e-6
+    assert ((got.double() - ref).abs() <= tol).all()
+    assert (got[0, :, 0::4] == -top).all() and (got[1, :, 1::4] == top).all()
+
+    wild = x.clone()
+    wild[0, 0, 2], wild[0, 0, 6], wild[0, 1, 2] = -inf, inf, torch.nan
+    bias[1, 2] = -inf
+    out = adjust_logits(wild.to(cuda), tokens.to(cuda), **dev(kw, cuda)).cpu()
+    assert out[0, 0, 2] == -inf and out[0, 0, 6] == inf and torch.isnan(out[0, 1, 2]) and (out[1, :, 2] == -inf).all()
+    keep = torch.ones_like(wild, dtype=torch.bool)
+    keep[0, 0, 2] = keep[0, 0, 6] = keep[0, 1, 2] = False
+    keep[1, :, 2] = False
+    assert torch.equal(out[keep], got[keep])
