@@ -397,11 +397,17 @@ struct PagedBatch {
 // Written tensors: no element twice (an expanded one would be a race).
 bool writable(const Tensor& t) { return at::has_internal_overlap(t) != at::MemOverlap::Yes; }
 
-// A written tensor apart from what the same launch reads or writes elsewhere, as far as
-// that can be told (dense tensors; woven views are the caller's to keep apart).
-bool apart(const Tensor& written, const Tensor& other) {
+// A written tensor apart from all that the same launch reads or writes elsewhere, as far
+// as that can be told (dense tensors; woven views are the caller's to keep apart).
+// Absent and empty ones are.
+bool apart_from(const Tensor& written, const Tensor& other) {
+  if (!written.defined() || !other.defined() || written.numel() == 0 || other.numel() == 0) return true;
   const auto s = at::get_overlap_status(written, other);
   return s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial && written.data_ptr() != other.data_ptr();
+}
+template <class... T>
+bool apart(const Tensor& written, const T&... others) {
+  return (... && apart_from(written, others));
 }
 
 // (tokens, heads, 64) result: the caller's, or a new one.
@@ -434,7 +440,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       q = ready(q);
       const int32_t T = dim32(q, 0), H = dim32(q, 1);
       out = token_rows(out, T, H, q);
-      require(out.numel() == 0 || (apart(out, q) && apart(out, b.k) && apart(out, b.v)), "out must not overlap an input");
+      require(apart(out, q, b.k, b.v, b.table, b.starts, b.lens), "out must not overlap an input");
       if (max_kv < 0) max_kv = (int32_t)std::min<int64_t>((int64_t)b.width * b.page, INT32_MAX);
       if (total < 0) total = (int64_t)b.seqs * max_kv;
       const size_t bytes = g_lib.paged_attn_workspace_bytes(b.seqs, T, H, b.kv_heads, max_q, max_kv, total);
@@ -476,10 +482,10 @@ PyObject* paged_attention_inputs(PyObject*, PyObject* const* args, Py_ssize_t n)
       sin = ready(sin.contiguous());
       cos = ready(cos.contiguous());
       out = token_rows(out, qkv.size(0), heads, qkv);
-      require(qkv.numel() == 0 ||
-                  (apart(out, qkv) && apart(out, b.k) && apart(out, b.v) && apart(b.k, qkv) && apart(b.v, qkv) &&
-                   apart(b.k, b.v)),
+      require(qkv.numel() == 0 || (apart(out, qkv, b.k, b.v) && apart(b.k, qkv, b.v) && apart(b.v, qkv)),
               "qkv, out, k_pages and v_pages must not overlap");
+      for (const Tensor* t : {&out, &b.k, &b.v})
+        require(apart(*t, sin, cos, b.table, b.starts, b.lens), "out and the pages must not overlap an input");
       const int64_t st[10] = {qkv.stride(0), out.stride(0), out.stride(1), b.k.stride(0), b.k.stride(1), b.k.stride(2),
                               b.v.stride(0), b.v.stride(1), b.v.stride(2), b.table.stride(0)};
       check(g_lib.paged_qkv_rope(ptr(qkv), static_cast<const float*>(ptr(sin)), static_cast<const float*>(ptr(cos)),
@@ -561,6 +567,8 @@ PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
               "out must have the logits' shape and dtype, with last stride 1");
       require(at::get_overlap_status(out, x) != at::MemOverlapStatus::Partial,
               "out must be the logits themselves or not overlap them");
+      require(apart(out, tokens, lengths, rep.each, freq.each, pres.each, bias, allowed),
+              "out must not overlap an input other than the logits");
       const float penalties[3] = {rep.one, freq.one, pres.one};
       const int64_t st[8] = {x.stride(0),
                              x.stride(1),

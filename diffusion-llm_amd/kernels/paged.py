@@ -74,8 +74,8 @@ def paged_attention_inputs(
     their slots in the pages. Computed in fp32 and rounded once, so a key
     differs from kv_cache.attention_inputs' (which repeats the eager path's bf16
     roundings) by up to two of its last bits. Positions beyond the RoPE tables
-    use their last row; nothing is written where the table has no page. qkv, out,
-    k_pages and v_pages do not overlap."""
+    use their last row; nothing is written where the table has no page. out,
+    k_pages and v_pages overlap neither each other nor another argument."""
     return host().paged_attention_inputs(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, page_table, q_starts,
                                          kv_lens, out)
 

@@ -100,7 +100,8 @@ def adjust_logits(
     the dtype's range becomes its largest value of that sign, unless the logit or
     its bias is infinite. The penalties are numbers or (batch) float32 tensors of
     finite values (not looked at), repetition > 0; tokens outside the
-    vocabulary count for nothing. `out=logits` works in place."""
+    vocabulary count for nothing. `out=logits` works in place; out overlaps no
+    other argument."""
     assert logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32), \
         "logits must be bf16 or fp32 CUDA tensors"
     assert logits.dim() in (2, 3), "logits must be (batch, rows, vocab) or (batch, vocab)"

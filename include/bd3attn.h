@@ -378,7 +378,8 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
  * eager bf16 path's roundings instead). Tokens of no sequence are left out: their
  * rows of q_out stay as they are. Nothing is written for a position before 0, past
  * the table or whose entry lies outside [0, pages). No two tokens may have the
- * same slot. No reference counterpart.
+ * same slot; q_out, k_pages and v_pages overlap neither each other nor what is read.
+ * No reference counterpart.
  */
 int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos_table,
                        int32_t max_pos, void* q_out, void* k_pages, void* v_pages,
@@ -397,7 +398,8 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
  * in fp32, rounded once to the logits' type; a result past the type's range becomes its
  * largest value of that sign unless the logit or the bias is infinite itself.
  *   logits, out: (batch, rows, vocab) bf16 (logits_fp32 = 0) or fp32 (1), last
- *     stride 1; out may be logits itself, and overlap it in no other way.
+ *     stride 1; out may be logits itself, and overlaps it in no other way and no other
+ *     argument.
  *   tokens: device int64 (batch, history), or NULL for no penalties; values
  *     outside [0, vocab) count for nothing. lengths: device int32 (batch), cut to
  *     [0, history]; NULL: all of history.

@@ -258,3 +258,35 @@ def test_finite_logits_stay_finite(cuda, dtype, V):
     keep[0, 0, 2] = keep[0, 0, 6] = keep[0, 1, 2] = False
     keep[1, :, 2] = False
     assert torch.equal(out[keep], got[keep])
+
+
+@pytest.mark.gpu
+def test_out_over_another_input_is_refused(cuda):
+    """Every argument that the launch reads beside the logits: a bias inside the result,
+    a result over the mask, the history, the lengths or a penalty."""
+    B, R, V = 2, 3, 96
+    x = torch.randn(B, R, V, device=cuda)
+    buf = torch.zeros(B * R * V + 64, device=cuda)
+    out = buf[:B * R * V].view(B, R, V)
+
+    def inside(dtype, n):  # n numbers of dtype within out's memory
+        return buf[128:].view(dtype)[:n]
+
+    tokens = torch.zeros(B, 4, dtype=torch.long, device=cuda)
+    for kw in (dict(bias=inside(torch.float32, V)), dict(allowed=inside(torch.int32, 3)),
+               dict(tokens=inside(torch.long, B * 4).view(B, 4)), dict(tokens=tokens, lengths=inside(torch.int32, B)),
+               dict(tokens=tokens, repetition=inside(torch.float32, B)), dict(tokens=tokens, frequency=inside(torch.float32, B)),
+               dict(tokens=tokens, presence=buf[:B])):
+        with pytest.raises(AssertionError, match="overlap"):
+            adjust_logits(x, **kw, out=out)
+    bias = buf[B * R * V - V + 64:]  # ends behind the result, begins in it
+    with pytest.raises(AssertionError, match="overlap"):
+        adjust_logits(x, bias=bias, out=out)
+    assert (buf == 0).all()
+    # apart in the same memory, and empty ones
+    far = torch.zeros(B * R * V + V, device=cuda)
+    far[B * R * V:] = 1.0
+    assert torch.equal(adjust_logits(x, bias=far[B * R * V:], out=far[:B * R * V].view(B, R, V)), x + 1)
+    assert torch.equal(adjust_logits(x, tokens[:, :0], bias=far[B * R * V:], out=out), x + 1)
+    none = adjust_logits(x[:0], tokens[:0], bias=far[B * R * V:], out=torch.empty(0, R, V, device=cuda))
+    assert none.shape == (0, R, V)

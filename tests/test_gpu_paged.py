@@ -568,3 +568,43 @@ def test_thousands_of_sequences(cuda, record_error, heads, kv_heads, chunk):
     ref, tol = attention_reference(c, 16)
     for total in (0, c["total"]):
         record_error("paged attention / bound", worst(attend(on(c, cuda), 16, total_kv=total), ref, tol), 1.0)
+
+
+@pytest.mark.gpu
+def test_results_over_the_batch_s_arrays_are_refused(cuda):
+    """The table, starts and lengths, and RoPE tables, that a launch reads while it
+    writes its result or the pages."""
+    c = on(paged_case([(4, 20), (3, 2)], 4, 2, 16), cuda)
+    n = c["q"].numel()
+    buf = torch.zeros(n, device=cuda, dtype=BF)
+    out = buf.view_as(c["q"])
+    ints = buf.view(torch.int32)
+    same = dict(table=c["table"], starts=c["starts"], kv=c["kv"])
+
+    def inside(t):
+        return ints[8:8 + t.numel()].view_as(t).copy_(t)
+
+    sin, cos = (t.to(cuda) for t in rope_tables(D, 64))
+    qkv = torch.zeros(c["q"].shape[0], 8 * D, device=cuda, dtype=BF)
+    pool = torch.zeros(c["k"].numel(), device=cuda, dtype=BF).view_as(c["k"])
+    for name in same:
+        kw = {**same, name: inside(same[name])}
+        batch = (kw["table"], kw["starts"], kw["kv"])
+        with pytest.raises(AssertionError, match="overlap"):
+            paged_attention(c["q"], c["k"], c["v"], *batch, 4, max_q=4, out=out)
+        with pytest.raises(AssertionError, match="overlap"):
+            paged_attention_inputs(qkv, 4, sin, cos, c["k"], c["v"], *batch, out=out)
+        pool_ints = pool.view(-1).view(torch.int32)
+        kw[name] = pool_ints[:same[name].numel()].view_as(same[name]).copy_(same[name])
+        for k, v in ((pool, c["v"]), (c["k"], pool)):
+            with pytest.raises(AssertionError, match="overlap"):
+                paged_attention_inputs(qkv, 4, sin, cos, k, v, kw["table"], kw["starts"], kw["kv"])
+    wide = torch.zeros(4 * c["k"].numel(), device=cuda, dtype=BF)
+    pages = wide[:c["k"].numel()].view_as(c["k"])
+    rope = wide.view(torch.float32)[:32].view(1, 32)
+    for a, b in ((rope, cos[:1]), (sin[:1], rope)):
+        with pytest.raises(AssertionError, match="overlap"):
+            paged_attention_inputs(qkv, 4, a, b, pages, c["v"], *same.values())
+    batch = tuple(same.values())
+    assert torch.equal(paged_attention(c["q"], c["k"], c["v"], *batch, 4, max_q=4, out=out),
+                       paged_attention(c["q"], c["k"], c["v"], *batch, 4, max_q=4))
