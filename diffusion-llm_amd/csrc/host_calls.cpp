@@ -410,6 +410,14 @@ bool apart(const Tensor& written, const T&... others) {
   return (... && apart_from(written, others));
 }
 
+// Packed tokens, readable for the kernels. A single one counts as contiguous whatever
+// its stride is, and contiguous() hands it back; in ordinary use it is a row of a wider
+// tensor.
+Tensor ready_tokens(const Tensor& t) {
+  const Tensor c = ready(t);
+  return vec_ready(c) ? c : c.clone(at::MemoryFormat::Contiguous);
+}
+
 // (tokens, heads, 64) result: the caller's, or a new one.
 Tensor token_rows(const Tensor& out, int64_t tokens, int64_t heads, const Tensor& like) {
   if (!out.defined()) return at::empty({tokens, heads, kHeadDim}, like.options());
@@ -437,7 +445,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     {
       NoGil nogil;
       const c10::DeviceGuard device(q.device());
-      q = ready(q);
+      q = ready_tokens(q);
       const int32_t T = dim32(q, 0), H = dim32(q, 1);
       out = token_rows(out, T, H, q);
       require(apart(out, q, b.k, b.v, b.table, b.starts, b.lens), "out must not overlap an input");
@@ -478,7 +486,7 @@ PyObject* paged_attention_inputs(PyObject*, PyObject* const* args, Py_ssize_t n)
     {
       NoGil nogil;
       const c10::DeviceGuard device(qkv.device());
-      qkv = ready(qkv);
+      qkv = ready_tokens(qkv);
       sin = ready(sin.contiguous());
       cos = ready(cos.contiguous());
       out = token_rows(out, qkv.size(0), heads, qkv);

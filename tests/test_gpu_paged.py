@@ -608,3 +608,28 @@ def test_results_over_the_batch_s_arrays_are_refused(cuda):
     batch = tuple(same.values())
     assert torch.equal(paged_attention(c["q"], c["k"], c["v"], *batch, 4, max_q=4, out=out),
                        paged_attention(c["q"], c["k"], c["v"], *batch, 4, max_q=4))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 2])
+def test_rows_off_the_grid_are_copied(cuda, n):
+    """Tokens of a wider tensor whose rows are not multiples of 16 bytes, one of them
+    too (torch calls that one contiguous), and bases off the grid."""
+    c = on(inputs_case([(n, 100)], 4, 2, 16, seed=1), cuda)
+    want = attend(c, 16)
+    wide = torch.zeros((n, c["q"].numel() // n + 3), device=cuda, dtype=BF)
+    wide[:, :-3] = c["q"].view(n, -1)
+    flat = torch.zeros(c["q"].numel() + 1, device=cuda, dtype=BF)
+    flat[1:] = c["q"].view(-1)
+    for q in (wide[:, :-3].view(n, 4, D), flat[1:].view(n, 4, D)):
+        assert torch.equal(attend(dict(c, q=q), 16), want)
+    k1, v1 = c["k"].clone(), c["v"].clone()
+    rotated = put(dict(c, k=k1, v=v1), 4)
+    wide = torch.zeros((n, 8 * D + 5), device=cuda, dtype=BF)
+    wide[:, :-5] = c["qkv"]
+    flat = torch.zeros(c["qkv"].numel() + 3, device=cuda, dtype=BF)
+    flat[3:] = c["qkv"].view(-1)
+    for qkv in (wide[:, :-5], flat[3:].view(n, -1)):
+        k2, v2 = c["k"].clone(), c["v"].clone()
+        assert torch.equal(put(dict(c, qkv=qkv, k=k2, v=v2), 4), rotated)
+        assert torch.equal(k1, k2) and torch.equal(v1, v2)
