@@ -410,6 +410,15 @@ bool apart(const Tensor& written, const T&... others) {
   return (... && apart_from(written, others));
 }
 
+// Every element of one at the address of the other's (of the same sizes): strides of
+// dimensions of one do not matter.
+bool same_memory(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) != 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
 // Packed tokens, readable for the kernels. A single one counts as contiguous whatever
 // its stride is, and contiguous() hands it back; in ordinary use it is a row of a wider
 // tensor.
@@ -573,7 +582,7 @@ PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
       require(out.scalar_type() == x.scalar_type() && out.sizes() == x.sizes() && (V == 1 || out.stride(2) == 1) &&
                   writable(out),
               "out must have the logits' shape and dtype, with last stride 1");
-      require(at::get_overlap_status(out, x) != at::MemOverlapStatus::Partial,
+      require(same_memory(out, x) || at::get_overlap_status(out, x) != at::MemOverlapStatus::Partial,
               "out must be the logits themselves or not overlap them");
       require(apart(out, tokens, lengths, rep.each, freq.each, pres.each, bias, allowed),
               "out must not overlap an input other than the logits");

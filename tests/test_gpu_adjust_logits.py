@@ -290,3 +290,22 @@ def test_out_over_another_input_is_refused(cuda):
     assert torch.equal(adjust_logits(x, tokens[:, :0], bias=far[B * R * V:], out=out), x + 1)
     none = adjust_logits(x[:0], tokens[:0], bias=far[B * R * V:], out=torch.empty(0, R, V, device=cuda))
     assert none.shape == (0, R, V)
+
+
+@pytest.mark.gpu
+def test_in_place_whatever_a_single_row_s_stride_is(cuda):
+    """One sequence's last logits: a view of them by another way is the same memory,
+    although torch gives the dimension of one another stride."""
+    for batch, rows in ((1, 1), (1, 3), (3, 1)):
+        big = torch.randn(batch, rows + 2, 100, device=cuda)[:, 2:].contiguous()
+        x = big.as_strided((batch, rows, 100), (rows * 100 if batch > 1 else 7, 100 if rows > 1 else 3, 1))
+        want = big + 1
+        assert adjust_logits(x, bias=torch.ones(100, device=cuda), out=big) is not None
+        assert torch.equal(big, want)
+        adjust_logits(big, bias=torch.ones(100, device=cuda), out=x)
+        assert torch.equal(big, want + 1)
+    x = torch.randn(1, 5, 100, device=cuda)
+    last, same = x[:, -1], x[0, -1:]
+    want = last + 1
+    adjust_logits(last, bias=torch.ones(100, device=cuda), out=same)
+    assert torch.equal(x[:, -1], want)
