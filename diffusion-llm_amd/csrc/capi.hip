@@ -1181,8 +1181,9 @@ int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_
   if (strides == nullptr || penalties == nullptr) return fail(BD3_EINVAL, "strides and penalties must be non-NULL");
   for (int i = 0; i < 8; ++i)
     if (strides[i] < 0) return fail(BD3_EINVAL, "stride[%d]=%lld must be >= 0", i, (long long)strides[i]);
-  if (!std::isfinite(penalties[0]) || !(penalties[0] > 0.f))
-    return fail(BD3_EINVAL, "repetition must be finite and > 0, got %g", (double)penalties[0]);
+  // the kernel multiplies by its reciprocal, which is infinite for the smallest numbers
+  if (!std::isfinite(penalties[0]) || !(penalties[0] >= 0x1p-126f))
+    return fail(BD3_EINVAL, "repetition must be finite and at least 2^-126, got %g", (double)penalties[0]);
   if (!std::isfinite(penalties[1]) || !std::isfinite(penalties[2]))
     return fail(BD3_EINVAL, "frequency and presence must be finite");
   // 3.3961775e38: from there on a number rounds to an infinite bf16

@@ -99,7 +99,7 @@ def adjust_logits(
     it, also in a row whose mask allows nothing. In fp32, rounded once; what leaves
     the dtype's range becomes its largest value of that sign, unless the logit or
     its bias is infinite. The penalties are numbers or (batch) float32 tensors of
-    finite values (not looked at), repetition > 0; tokens outside the
+    finite values (not looked at), repetition at least 2^-126; tokens outside the
     vocabulary count for nothing. `out=logits` works in place; out overlaps no
     other argument."""
     assert logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32), \

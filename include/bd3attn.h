@@ -403,7 +403,7 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
  *   tokens: device int64 (batch, history), or NULL for no penalties; values
  *     outside [0, vocab) count for nothing. lengths: device int32 (batch), cut to
  *     [0, history]; NULL: all of history.
- *   penalties: host {repetition, frequency, presence}, finite, repetition > 0; repetition,
+ *   penalties: host {repetition, frequency, presence}, finite, repetition >= 2^-126; repetition,
  *     frequency, presence: device fp32 (batch) in place of the one number, or NULL; their
  *     values must be such, too (they are not looked at).
  *   bias: device fp32 (vocab) (batch stride 0) or (batch, vocab), or NULL.

@@ -317,3 +317,18 @@ def test_at_most_64_ranges(lib):
     for max_kv in (16383, 16384, 16511, 16512, 16540, 16639, 16640, 33100, 66200, 1 << 20):
         for total in (max_kv // 10, max_kv):
             assert size(1, 1, 1, 1, 1, max_kv, total) <= 64 * 260 + 256, max_kv
+
+
+def test_repetitions_without_a_reciprocal(lib):
+    """1 / 1e-39 is infinite in fp32: x / repetition would be, however small x is."""
+    st = (ctypes.c_int64 * 8)(300, 100, 300, 100, 5, 0, 0, 0)
+    for r in (1e-39, 1e-44, 2.0 ** -127):
+        pen = (ctypes.c_float * 3)(r, 0.0, 0.0)
+        assert pen[0] > 0
+        assert lib.bd3_adjust_logits(None, 0, None, 2, 3, 100, P, 5, None, pen, None, None, None, None, None, -1e6, st,
+                                     None) == _native.BD3_EINVAL
+        assert "repetition" in _native.last_error()
+    pen = (ctypes.c_float * 3)(2.0 ** -126, 0.0, 0.0)
+    assert lib.bd3_adjust_logits(None, 0, None, 2, 3, 100, P, 5, None, pen, None, None, None, None, None, -1e6, st,
+                                 None) == _native.BD3_EINVAL
+    assert "non-NULL" in _native.last_error()
