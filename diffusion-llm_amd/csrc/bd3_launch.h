@@ -161,6 +161,7 @@ struct FastDiv {
   }
 };
 
+constexpr int kMergeRows = 16;
 constexpr int kPagedMaxKeys = 1 << 30;  // of a sequence: key positions stay below 2^31 when rounded up to a block
 struct PagedArgs {
   const uint16_t* q;        // (tokens, heads, 64)
@@ -181,7 +182,7 @@ struct PagedArgs {
   int tile;       // query rows per workgroup
   int subs;       // sets of 4 waves per workgroup: 1, 2 or (128-row tiles) 4
   int q_tiles;    // tiles of the longest chunk
-  int part_slots;  // workgroups of the merge for a KV head: 32 of its part_rows each
+  int part_slots;  // workgroups of the merge for a KV head: kMergeRows of its part_rows each
   int part_rows;   // tokens * group: the packed rows of a KV head, row q0 * group + r that of row r of a chunk at q0
   int n_splits;    // most key ranges of a tile
   int split_shift;  // log2 of about a range's keys

@@ -1095,7 +1095,7 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.n_splits = plan.n_splits;
   if (plan.n_splits > 1) {
     a.part_rows = tokens * a.group;  // bounded by kPagedPartRows
-    a.part_slots = (a.part_rows + 31) / 32;
+    a.part_slots = (a.part_rows + bd3::kMergeRows - 1) / bd3::kMergeRows;
   }
   a.split_shift = plan.split_shift;
   a.bs_div = bd3::FastDiv::of(a.bs);

@@ -518,8 +518,8 @@ def test_any_total_is_a_hint(cuda, record_error, chunk, heads, kv_heads):
     (90, 300, 900, 2, 2), (63, 700, 100, 4, 1), (70, 40, 1500, 2, 2), (130, 12, 1200, 6, 3), (5, 33, 3000, 2, 1)])
 def test_a_chunk_beside_single_tokens(cuda, record_error, singles, chunk, ctx, heads, kv_heads):
     """A prompt chunk in the middle of sequences of one token, some without any: the
-    keys of both in ranges, whose partials lie packed, 32 rows of several sequences to
-    a workgroup of the merge."""
+    keys of both in ranges, whose partials lie packed, rows of several sequences to a
+    workgroup of the merge."""
     from kernels import _native
     g = torch.Generator().manual_seed(singles)
     lens = [(int(n), int(x)) for n, x in zip((torch.rand(singles, generator=g) < 0.8).int(),
