@@ -401,7 +401,9 @@ bool writable(const Tensor& t) { return at::has_internal_overlap(t) != at::MemOv
 // as that can be told (dense tensors; woven views are the caller's to keep apart).
 // Absent and empty ones are.
 bool apart_from(const Tensor& written, const Tensor& other) {
-  if (!written.defined() || !other.defined() || written.numel() == 0 || other.numel() == 0) return true;
+  if (!written.defined() || !other.defined() || written.storage().data() == nullptr ||
+      written.storage().data() != other.storage().data() || written.numel() == 0 || other.numel() == 0)
+    return true;
   const auto s = at::get_overlap_status(written, other);
   return s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial && written.data_ptr() != other.data_ptr();
 }
