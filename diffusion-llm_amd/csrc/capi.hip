@@ -904,10 +904,10 @@ static_assert(kPagedPartRows * bd3::kHeadDim <= INT32_MAX, "32-bit indices of th
 // 32-row launches (items in the order of the sequences), so there the two nearly add
 // up; the 128-row launch takes the longest first. busiest: the keys of the CU that
 // gets most of evenly long items, which bounds the 16-row launches: 264 items of 4860
-// keys leave two on 8 CUs and take 75 us whole, 60 in ranges of 1024 (the same 22
-// sequences of 12 heads over 6004 keys 92, 71). Fitted to batches drawn over 1-64
+// keys leave two on 8 CUs and take 75 us whole, 61 in ranges of 1024 (the same 22
+// sequences of 12 heads over 6004 keys 92, 76). Fitted to batches drawn over 1-64
 // sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV heads and groups of 1-12;
-// over 1751 others the rms error is 9% for 16 rows, 15% for 17-300, 12% for more.
+// over 1500 others the rms error is 9% for up to 16 rows, 12% for 17-256, 10% for more.
 double paged_us(int tile, int subs, double longest, double keys, double items, double busiest, bool split, bool even) {
   struct Cost {
     double chain0, chain, load0, load, item, merge, merge_item;
@@ -935,13 +935,13 @@ int paged_ranges(int32_t max_kv, int shift) {
 // rows or 128), sets and ranges (256 keys and longer, at most 64 of a sequence) for
 // what the host knows: bounds, tokens and the keys in all. Ranges pay where a few
 // long sequences would leave the chip idle; 32-row tiles re-read the keys for
-// every tile but start and step faster. Over 500 batches of up to 16 rows, 800 of
-// 17-300 and 451 of 257 and more the plan takes 1%, 3% and 2% more than the best of
-// all plans on average, at worst 33%, 47% and 36%.
-// us, whole items -> plan: 12 heads, 16 over 3600 keys 24.7 -> 10.8; 32 sequences of
-// 100-8192 keys 66 -> 51; 32 rows over 500-2000 keys of 8 sequences 17.3 -> 14.6; 32-row
-// tiles -> plan: 50 rows over 1000 keys of 32 sequences 24.4 -> 19.1; 128-row tiles ->
-// plan: 96 rows over 800 keys of 4 sequences, 4 KV heads 12.5 -> 8.7.
+// every tile but start and step faster. Over 500 batches of up to 16 rows, 600 of
+// 17-256 and 400 of 257 and more the plan takes 1%, 3% and 2% more than the best of
+// all plans on average, at worst 20%, 59% and 27%.
+// us, whole items -> plan: 12 heads, 16 over 3600 keys 25.6 -> 11.9; 32 sequences of
+// 100-8192 keys 67 -> 51; 32 rows over 500-2000 keys of 8 sequences 17.0 -> 14.5; 32-row
+// tiles -> plan: 50 rows over 150-1050 keys of 32 sequences 24.7 -> 19.8; 128-row tiles ->
+// plan: 96 rows over 232-832 keys of 4 sequences, 4 KV heads 12.6 -> 9.0.
 PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
                      int64_t total_kv) {
   const int64_t group = heads / kv_heads, rows = (int64_t)max_q * group;

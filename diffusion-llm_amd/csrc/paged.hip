@@ -67,7 +67,7 @@ struct PagedSeq {
   // Place of a row's partial of one range: the packed rows of a KV head after those of
   // the head before it, a row's ranges side by side. So partials take what the
   // tokens there are need, however long the longest chunk is. (With the ranges outermost
-  // 32 sequences of 16 rows took 52.0 us for 51.4: writes 128 KB apart.) At most 2^20
+  // 32 sequences of 16 rows took 0.6 us more: writes 128 KB apart.) At most 2^20
   // places: kPagedPartRows.
   __device__ __forceinline__ int part_row(const PagedArgs& a, int h, int split, int r0) const {
     return (h * a.part_rows + q0 * a.group + r0) * a.n_splits + split;
@@ -327,7 +327,7 @@ constexpr size_t chunk_smem() {
 // K Q^T on v_mfma_f32_32x32x16_bf16 with the K tile's rows as A operands; O^T += V^T
 // P^T with V read transposed. Eight waves for few items (one workgroup a CU at 160
 // registers), four for many (three a CU), each at its best ranges: 32 rows over 500-2000
-// keys of 8 sequences 14.6 us against 15.4; 32 sequences of 100-8000 keys 43.3, 41.6.
+// keys of 8 sequences 13.9 us against 15.1; over 4032 keys of 48 sequences 111, 104.
 // At four waves per SIMD it spills (43 -> 50 us). Full launches are bound by HBM (32
 // sequences x 4128 keys 73 us, 5.6 TB/s; contiguous 65).
 template <int NW>
@@ -573,7 +573,7 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
 // first row does not see whole. The running maximum is updated when it grew by
 // more than kRescale (log2): a stale one leaves O / l exact and bounds P by 2^8.
 // Full launches are bound by the softmax's VALU work beside the products (8 prompts
-// of 2048 tokens, 12 heads: 72 us), short ones by a tile's own
+// of 2048 tokens, 12 heads: 74 us), short ones by a tile's own
 // chain, ~1 us for a workgroup alone on its CU: three and four stages only cost
 // occupancy (84 -> 95-107 us for prompts of 1507-4034 tokens, 28.5 -> 31-37 for 96 rows
 // over 727-3871 keys).
@@ -907,7 +907,7 @@ __global__ __launch_bounds__(16 * kMergeRows) void paged_combine_kernel(PagedArg
 // v into the pages. y1 = x1 c - x2 s, y2 = x1 s + x2 c on the halves of a head
 // row, in fp32 with the fp32 tables and rounded once (qkv_rope.hip instead repeats
 // an eager bf16 path's five roundings, which no caller of pages has to match).
-// Bound by HBM: 24 chunks of 100-2000 tokens, 16 + 2 x 4 heads, 19.9 us, 4.95 TB/s read
+// Bound by HBM: 24 chunks of 100-2000 tokens, 16 + 2 x 4 heads, 20.0 us, 4.9 TB/s read
 // and written (a large copy: 5.1); a denoising step's 1024 tokens take 4.4 us.
 // Work item: (token, head of q | k | v, j): coordinate pairs (8j + i, 32 + 8j + i).
 __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {

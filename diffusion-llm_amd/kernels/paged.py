@@ -115,7 +115,8 @@ class PagedKVCache:
         return self._length[seq]
 
     def free(self, seq: int) -> None:
-        """Give a sequence's pages back to the pool."""
+        """Give a sequence's pages back to the pool. The next batch may take them: what
+        still runs on them must be before it in stream order."""
         self._free.extend(reversed(self._pages.pop(seq)))
         del self._length[seq]
 
