@@ -633,3 +633,40 @@ def test_rows_off_the_grid_are_copied(cuda, n):
         k2, v2 = c["k"].clone(), c["v"].clone()
         assert torch.equal(put(dict(c, qkv=qkv, k=k2, v=v2), 4), rotated)
         assert torch.equal(k1, k2) and torch.equal(v1, v2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first,heads,kv_heads", [([1, 1, 16, 0, 1], 4, 4), ([30, 1, 1, 40, 2], 4, 2),
+                                                  ([1, 300, 1, 7, 130], 2, 2)])
+def test_attention_graph_follows_the_starts(cuda, first, heads, kv_heads):
+    """Two captures in one memory pool, replayed in turn with tokens moved between the
+    sequences, eager calls between: the merge finds each row's sequence on the device."""
+    T, bound = sum(first), max(first)
+    kv = [1500, 700, 2100, 40, 900]
+    c = on(paged_case([(n, x - n if x > n else 0) for n, x in zip(first, kv)], heads, kv_heads, 16, seed=3, poison=False), cuda)
+    kw = {"max_q": bound, "max_kv": c["max_kv"], "total_kv": 0}
+    side, pool = torch.cuda.Stream(), torch.cuda.graph_pool_handle()
+    outs = [torch.zeros_like(c["q"]) for _ in range(2)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attend(c, 16, **kw)
+        torch.cuda.synchronize()
+        for graph, out in zip(graphs, outs):
+            with torch.cuda.graph(graph, stream=side, pool=pool):
+                attend(c, 16, out=out, **kw)
+    torch.cuda.synchronize()
+    for order in ([0, 1, 2, 3, 4], [4, 3, 2, 1, 0], [1, 4, 0, 2, 3], [2, 0, 3, 4, 1]):
+        n = [first[i] for i in order]
+        c["starts"].copy_(torch.tensor([sum(n[:b]) for b in range(6)], dtype=torch.int32))
+        assert int(c["starts"][-1]) == T
+        host = {k: t.cpu() if torch.is_tensor(t) else t for k, t in c.items()}
+        ref, tol = attention_reference(host, 16)
+        eager = attend(c, 16, **kw)
+        for graph, out in zip(graphs, outs):
+            out.fill_(5.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager), order
+        assert worst(eager, ref, tol) <= 1.0
