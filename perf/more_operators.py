@@ -271,7 +271,7 @@ def run(s):
             k, v = _own("values")(s["k_pages"], s["v_pages"], s["k_scales"], s["v_scales"])
             return q, k, v
         if kind == "select":
-            _own("bounds")(s["k_pages"], s["bounds"], *batch, k_scales=s["k_scales"])
+            _own("bounds")(s["k_pages"], s["bounds"], *batch, s["tokens"], k_scales=s["k_scales"])
             columns = _own("select")(s["q"], s["bounds"], *batch, s["bs"], s["page"], s["top"], max_q=s["max_q"],
                                      max_kv=s["max_kv"])
             return s["bounds"], columns
