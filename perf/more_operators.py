@@ -7,13 +7,13 @@ A case is a dict of plain values; `kind` names the operator:
 
   append     split + RoPE of the chunk's projection, keys and values written into
              pages of 8-bit codes with a scale for each 16 slots and head
-             (paged_attention_inputs with scales), and the pages read back
+             (paged_attention_inputs8), and the pages read back
              (page_values)
   cache8     attention of each sequence's chunk over such pages, block-causal
-             (paged_attention with scales)
+             (paged_attention_pool)
   select     the bounds of the pages that the chunk wrote (page_bounds) and the
              pages that each query's attention is to read (select_pages)
-  sparse     attention over the selected pages (paged_attention with columns)
+  sparse     attention over the selected pages (paged_attention_pool with columns)
 
 Chunks hold q_lo .. q_hi tokens and come after ctx_lo .. ctx_hi cached ones, a
 length per sequence, spread over their logarithm. Heads are 64 wide and queries
@@ -256,8 +256,8 @@ def _own(name):
         if pkg not in sys.path:
             sys.path.insert(0, pkg)
         from kernels import paged
-        _entry.update(inputs=paged.paged_attention_inputs, values=paged.page_values, attention=paged.paged_attention,
-                      bounds=paged.page_bounds, select=paged.select_pages)
+        _entry.update(inputs=paged.paged_attention_inputs8, values=paged.page_values,
+                      attention=paged.paged_attention_pool, bounds=paged.page_bounds, select=paged.select_pages)
     return _entry[name]
 
 
@@ -266,8 +266,8 @@ def run(s):
     if own:
         batch = s["page_table"], s["q_starts"], s["kv_lens"]
         if kind == "append":
-            q = _own("inputs")(s["qkv"], s["heads"], s["sin"], s["cos"], s["k_pages"], s["v_pages"], *batch,
-                               k_scales=s["k_scales"], v_scales=s["v_scales"])
+            q = _own("inputs")(s["qkv"], s["heads"], s["sin"], s["cos"], s["k_pages"], s["v_pages"], s["k_scales"],
+                               s["v_scales"], *batch)
             k, v = _own("values")(s["k_pages"], s["v_pages"], s["k_scales"], s["v_scales"])
             return q, k, v
         if kind == "select":
