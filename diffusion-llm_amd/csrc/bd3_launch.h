@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "bd3attn.h"
+
 namespace bd3 {
 
 constexpr int kHeadDim = 64;
@@ -163,18 +165,24 @@ struct FastDiv {
 
 constexpr int kMergeRows = 16;
 constexpr int kPagedMaxKeys = 1 << 30;  // of a sequence: key positions stay below 2^31 when rounded up to a block
+enum PoolType { kPoolBf16 = BD3_POOL_BF16, kPoolInt8 = BD3_POOL_INT8, kPoolE4m3 = BD3_POOL_E4M3 };
 struct PagedArgs {
   const uint16_t* q;        // (tokens, heads, 64)
-  const uint16_t* k;        // (pages, kv_heads, page, 64)
-  const uint16_t* v;
+  const void* k;            // (pages, kv_heads, page, 64) bf16 or codes
+  const void* v;
+  const float* k_scales;    // 8-bit pools: (pages, kv_heads, page / 16)
+  const float* v_scales;
+  const int32_t* columns;   // (tokens, kv_heads, top) columns of the table, or null: all keys
   uint16_t* o;              // (tokens, heads, 64)
   const int32_t* table;     // (seqs, width) page numbers
   const int32_t* q_starts;  // (seqs + 1)
   const int32_t* kv_lens;   // (seqs)
   float* part_o;            // (kv_heads, part_rows, n_splits, 64) fp32, or null
   float* part_lse;          // (kv_heads, part_rows, n_splits) log2 LSE, or null
-  int64_t sq_t, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, so_t, so_h, table_s;  // element strides
+  int64_t sq_t, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, so_t, so_h, table_s, sc_t, sc_h;  // element strides
   int seqs, tokens, kv_heads, group, pages, page, page_shift;
+  int top;          // entries of a list
+  int block_tiles;  // lists: tiles of a block of bs tokens
   int max_q;      // most tokens of a chunk: the caller's bound
   int max_kv;     // most keys of a sequence: the caller's bound, at most the table's
   int bs;
@@ -199,14 +207,39 @@ struct PagedRopeArgs {
   const float* sin_t;   // (max_pos, 32) fp32
   const float* cos_t;
   uint16_t* q;          // (tokens, heads, 64)
-  uint16_t* k;          // (pages, kv_heads, page, 64)
-  uint16_t* v;
+  void* k;              // (pages, kv_heads, page, 64) bf16 or codes
+  void* v;
+  float* k_scales;      // 8-bit pools: (pages, kv_heads, page / 16)
+  float* v_scales;
   const int32_t* table;
   const int32_t* q_starts;
   const int32_t* kv_lens;
   int64_t sx_t, sq_t, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, table_s;
   int seqs, tokens, heads, kv_heads, pages, page, page_shift, width, max_pos;
   int64_t total;  // tokens * (heads + 2 kv_heads) * 4 work items (< 2^31)
+  int blocks;     // 8-bit pools: most blocks of 16 slots that the chunks touch
+  FastDiv parts_div;
+};
+
+struct PageValuesArgs {
+  const void* codes[2];      // k, v: (pages, kv_heads, page, 64)
+  const float* scales[2];    // (pages, kv_heads, page / 16)
+  uint16_t* out[2];          // (pages, kv_heads, page, 64) bf16, contiguous
+  int64_t s_p[2], s_h[2], s_s[2];
+  int kv_heads, blocks;      // blocks of a page
+  int64_t total;             // blocks of 16 rows of one of the two
+};
+
+struct SelectArgs {
+  PagedArgs p;               // batch, pool (bounds) and queries (selection)
+  uint16_t* bounds;          // (pages, kv_heads, 2, 64): lowest and highest key
+  int32_t* out;              // (tokens, kv_heads, top)
+  int slots;                 // most pages that the chunks touch (bounds), most blocks of the chunks (selection)
+  int width;                 // columns within max_kv
+  int first, recent;         // columns always taken
+  float* scores;             // (slots, kv_heads, width)
+  float* error;              // (slots, kv_heads, ceil(width / 16)): bound of the scores' distance from the exact sums
+  double* sums;              // (slots, kv_heads, width)
 };
 
 constexpr int kLogitSlice = 2048;  // tokens of the vocabulary per workgroup of adjust_logits
@@ -246,7 +279,12 @@ hipError_t launch_qkv_rope(const QkvRopeArgs& a, hipStream_t stream);
 hipError_t launch_kv_write(const KvWriteArgs& a, hipStream_t stream);
 hipError_t launch_subs_sample(const SubsArgs& a, hipStream_t stream);
 hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t stream);
+hipError_t launch_paged_pool(const PagedArgs& a, int pool, hipStream_t stream);  // 8-bit pools, lists
 hipError_t launch_paged_rope(const PagedRopeArgs& a, hipStream_t stream);
+hipError_t launch_paged_rope8(const PagedRopeArgs& a, int pool, hipStream_t stream);
+hipError_t launch_page_values(const PageValuesArgs& a, int pool, hipStream_t stream);
+hipError_t launch_page_bounds(const SelectArgs& a, int pool, hipStream_t stream);
+hipError_t launch_select_pages(const SelectArgs& a, hipStream_t stream);
 hipError_t launch_adjust_logits(const LogitArgs& a, hipStream_t stream);
 hipError_t launch_ln_modulate(const GlueArgs& a, hipStream_t stream);
 hipError_t launch_gate_residual_ln_modulate(const GlueArgs& a, hipStream_t stream);

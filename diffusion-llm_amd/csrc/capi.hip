@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 #include <mutex>
 #include <string>
 
@@ -872,6 +873,20 @@ int check_rows(const void* p, const int64_t* st, int n, const char* name) {
   return BD3_OK;
 }
 
+// A pool's pages and their scales. 16-byte rows: 8 elements in bf16, 16 codes.
+int check_pool(const void* p, const float* scales, int32_t pool_type, const int64_t* st, const char* name) {
+  if (pool_type != BD3_POOL_BF16 && pool_type != BD3_POOL_INT8 && pool_type != BD3_POOL_E4M3)
+    return fail(BD3_EINVAL, "pool_type must be BD3_POOL_BF16, BD3_POOL_INT8 or BD3_POOL_E4M3, got %d", pool_type);
+  if ((scales != nullptr) != (pool_type != BD3_POOL_BF16))
+    return fail(BD3_EINVAL, "%s: 8-bit pools have scales, bf16 pools none", name);
+  if (reinterpret_cast<uintptr_t>(scales) % 4 != 0) return fail(BD3_EINVAL, "%s: scales must be 4-byte aligned", name);
+  if (int s = check_rows(p, st, 3, name)) return s;
+  for (int i = 0; i < 3; ++i)
+    if (pool_type != BD3_POOL_BF16 && st[i] % 16 != 0)
+      return fail(BD3_EINVAL, "%s stride[%d]=%lld must be a multiple of 16", name, i, (long long)st[i]);
+  return BD3_OK;
+}
+
 int log2_of(int32_t x) {
   int s = 0;
   while ((1 << s) < x) ++s;
@@ -885,6 +900,7 @@ struct PagedPlan {
   int tile, subs, q_tiles, n_splits, split_shift;
   int64_t tiles;
 };
+constexpr int kMaxWorkgroups = (1 << 24) - 1;    // of 256 threads: a launch has fewer than 2^32
 constexpr int kPagedWorkgroups = (1 << 22) - 1;  // of a launch
 constexpr int64_t kPagedItems = 1 << 30;         // that the kernels' 32-bit sums hold, whatever the starts are
 
@@ -942,8 +958,8 @@ int paged_ranges(int32_t max_kv, int shift) {
 // 100-8192 keys 67 -> 51; 32 rows over 500-2000 keys of 8 sequences 17.0 -> 14.5; 32-row
 // tiles -> plan: 50 rows over 150-1050 keys of 32 sequences 24.7 -> 19.8; 128-row tiles ->
 // plan: 96 rows over 232-832 keys of 4 sequences, 4 KV heads 12.6 -> 9.0.
-PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q, int32_t max_kv,
-                     int64_t total_kv) {
+PagedPlan paged_plan(int pool_type, int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q,
+                     int32_t max_kv, int64_t total_kv) {
   const int64_t group = heads / kv_heads, rows = (int64_t)max_q * group;
   const double total = (double)total_kv;
   const double seen = std::max(1.0, (total - 0.5 * tokens) / seqs);  // keys that a tile sees, about
@@ -953,7 +969,8 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
   p.split_shift = 30;
   double best = INFINITY;
   for (int tile : {16, 32, 128}) {
-    if (tile == 16 ? rows > 16 : rows <= 16 || (tile == 32 && rows > 256)) continue;
+    if (tile == 16 ? rows > 16 : rows <= 16 || (tile == 32 && rows > 256 && pool_type == BD3_POOL_BF16)) continue;
+    if (tile == 128 && pool_type != BD3_POOL_BF16) continue;
     const int q_tiles = (int)((rows + tile - 1) / tile);
     // items without ranges: not every chunk is as long as the longest
     const double units = kv_heads * std::max(1.0, std::min((double)seqs * q_tiles,
@@ -993,6 +1010,49 @@ PagedPlan paged_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_hea
   return p;
 }
 
+// The most blocks of bs positions that the batch's chunks can lie in.
+int64_t chunk_blocks(int64_t seqs, int64_t tokens, int64_t bs) { return std::min(tokens, tokens / bs + 2 * seqs); }
+
+// Keys of the longest list.
+int32_t listed_keys(int32_t page_size, int32_t max_kv, int32_t top) {
+  return (int32_t)std::min((int64_t)top * page_size, ((int64_t)max_kv + page_size - 1) / page_size * page_size);
+}
+
+// The plan over lists: tiles hold the rows of one block; ranges as above.
+PagedPlan columns_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t page_size, int32_t max_q,
+                       int32_t max_kv, int32_t block_size, int32_t top, int32_t* block_tiles) {
+  const int64_t group = heads / kv_heads, rows = std::min(block_size, max_q) * group;
+  const int32_t keys = listed_keys(page_size, max_kv, top);
+  PagedPlan p = {};
+  p.split_shift = 30;
+  const int tile = rows <= 16 ? 16 : 32;
+  *block_tiles = (int32_t)((rows + tile - 1) / tile);
+  const int64_t tiles = chunk_blocks(seqs, tokens, block_size) * *block_tiles;
+  const double units = (double)kv_heads * *block_tiles * std::max(1.0, std::min((double)tiles, (double)tokens / block_size + 0.5 * seqs));
+  const int64_t part_rows = std::min((int64_t)tokens * heads, kPagedPartRows + 1);
+  if (tiles >= kPagedItems || tiles * kv_heads >= kPagedItems) return p;
+  double best = INFINITY;
+  for (int subs = tile == 16 ? 2 : 1; subs <= 2; subs *= 2) {
+    const auto take = [&](double us, int shift) {
+      if (!(us < best)) return;
+      best = us;
+      p.tile = tile;
+      p.tiles = tiles;
+      p.subs = subs;
+      p.split_shift = shift;
+    };
+    const auto busiest = [&](double ranges) { return std::ceil(units * ranges / 256.0) * keys / ranges; };
+    take(paged_us(tile, subs, keys, units * keys, units, busiest(1), false, true), 30);
+    for (int shift = 8; 3 * ((int64_t)1 << shift) <= 2 * (int64_t)keys; ++shift) {
+      const int ranges = paged_ranges(keys, shift);
+      if (ranges > 64 || part_rows * ranges > kPagedPartRows || tiles * ranges * kv_heads >= kPagedItems) continue;
+      take(paged_us(tile, subs, 1.25 * (1 << shift), units * keys, units * ranges, busiest(ranges), true, true), shift);
+    }
+  }
+  p.n_splits = paged_ranges(keys, p.split_shift);
+  return p;
+}
+
 // Rows of the longest chunk that the plan's numbers hold (2^22 tiles of 128 at most).
 bool paged_fits(int32_t heads, int32_t kv_heads, int32_t max_q) {
   return (int64_t)max_q * (heads / kv_heads) < ((int64_t)1 << 29);
@@ -1006,28 +1066,41 @@ size_t paged_part_rows(const PagedPlan& p, int32_t tokens, int32_t heads) {
 
 extern "C" {
 
-size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q,
-                                      int32_t max_kv, int64_t total_kv) {
+size_t bd3_paged_attn_pool_workspace_bytes(int32_t pool_type, int32_t seqs, int32_t tokens, int32_t heads,
+                                           int32_t kv_heads, int32_t page_size, int32_t max_q, int32_t max_kv,
+                                           int64_t total_kv, int32_t block_size, int32_t top) {
   if (seqs < 1 || tokens < 1 || kv_heads < 1 || heads < kv_heads || max_q < 1 || max_kv < 0 ||
-      max_kv > bd3::kPagedMaxKeys || total_kv < 0)
+      max_kv > bd3::kPagedMaxKeys || total_kv < 0 || page_size < 1 || block_size < 1 || top < 0)
     return 0;
   max_q = std::min(max_q, tokens);
   if (!paged_fits(heads, kv_heads, max_q)) return 0;
   max_kv = std::max(max_kv, 1);
   total_kv = std::min(total_kv, (int64_t)seqs * max_kv);
-  const size_t rows = paged_part_rows(paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv), tokens, heads);
+  int32_t block_tiles;
+  const PagedPlan plan = top > 0 ? columns_plan(seqs, tokens, heads, kv_heads, page_size, max_q, max_kv,
+                                                std::min(block_size, bd3::kPagedMaxKeys), top, &block_tiles)
+                                 : paged_plan(pool_type, seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
+  const size_t rows = paged_part_rows(plan, tokens, heads);
   return rows == 0 ? 0 : align256(rows * bd3::kHeadDim * 4) + rows * 4;
 }
 
-int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
-                   const int32_t* q_starts, const int32_t* kv_lens, int32_t seqs, int32_t tokens, int32_t heads,
-                   int32_t kv_heads, int32_t head_dim, int32_t pages, int32_t page_size, int32_t table_width,
-                   int32_t max_q, int32_t max_kv, int64_t total_kv, int32_t block_size, const int64_t* strides,
-                   float scale, void* workspace, size_t workspace_bytes, void* stream) {
+size_t bd3_paged_attn_workspace_bytes(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t max_q,
+                                      int32_t max_kv, int64_t total_kv) {
+  return bd3_paged_attn_pool_workspace_bytes(BD3_POOL_BF16, seqs, tokens, heads, kv_heads, 16, max_q, max_kv, total_kv, 1, 0);
+}
+
+int bd3_paged_attn_pool(const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
+                        const float* v_scales, int32_t pool_type, void* o, const int32_t* page_table,
+                        const int32_t* q_starts, const int32_t* kv_lens, const int32_t* columns, int32_t top,
+                        int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                        int32_t page_size, int32_t table_width, int32_t max_q, int32_t max_kv, int64_t total_kv,
+                        int32_t block_size, const int64_t* strides, float scale, void* workspace,
+                        size_t workspace_bytes, void* stream) {
   if (int st = check_paged(seqs, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, page_table,
                            q_starts, kv_lens, strides))
     return st;
   if (block_size < 1) return fail(BD3_EINVAL, "block_size must be >= 1");
+  if (columns != nullptr && top < 1) return fail(BD3_EINVAL, "top must be >= 1");
   if (max_q < 0 || max_kv < 0 || total_kv < 0) return fail(BD3_EINVAL, "max_q, max_kv and total_kv must be >= 0");
   if (max_kv > (int64_t)table_width * page_size)
     return fail(BD3_EINVAL, "max_kv (%d) exceeds the page table's %lld keys a sequence", max_kv,
@@ -1039,13 +1112,19 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   total_kv = std::min(total_kv, (int64_t)seqs * max_kv);  // any larger one says no more
   if (!paged_fits(heads, kv_heads, max_q))
     return fail(BD3_EINVAL, "max_q * heads / kv_heads too large (limit 2^29 rows a chunk)");
-  const PagedPlan plan = paged_plan(seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
+  block_size = std::min(block_size, bd3::kPagedMaxKeys);  // as good as any larger one
+  int32_t block_tiles = 0;
+  const PagedPlan plan = columns != nullptr ? columns_plan(seqs, tokens, heads, kv_heads, page_size, max_q, max_kv,
+                                                           block_size, top, &block_tiles)
+                                            : paged_plan(pool_type, seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
   if (plan.tile == 0)
     return fail(BD3_EINVAL, "batch too large (limits: 2^22 workgroups, seqs * kv_heads * tiles of the longest chunk 2^30)");
   if (int st = check_rows(q, strides, 2, "q")) return st;
-  if (int st = check_rows(k_pages, strides + 2, 3, "k_pages")) return st;
-  if (int st = check_rows(v_pages, strides + 5, 3, "v_pages")) return st;
+  if (int st = check_pool(k_pages, k_scales, pool_type, strides + 2, "k_pages")) return st;
+  if (int st = check_pool(v_pages, v_scales, pool_type, strides + 5, "v_pages")) return st;
   if (int st = check_rows(o, strides + 8, 2, "o")) return st;
+  if (columns != nullptr && (strides[11] < 0 || strides[12] < 0 || reinterpret_cast<uintptr_t>(columns) % 4 != 0))
+    return fail(BD3_EINVAL, "columns must be 4-byte aligned, its strides >= 0");
   // a tile's rows are addressed by 32-bit byte offsets from a page slot
   if (strides[4] >= kMaxDmaSeqStride || strides[7] >= kMaxDmaSeqStride)
     return fail(BD3_EINVAL, "page slot strides must be < 2^24 elements");
@@ -1058,8 +1137,11 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
     return fail(BD3_EINVAL, "workspace must be a 16-byte aligned device pointer");
   bd3::PagedArgs a = {};
   a.q = static_cast<const uint16_t*>(q);
-  a.k = static_cast<const uint16_t*>(k_pages);
-  a.v = static_cast<const uint16_t*>(v_pages);
+  a.k = k_pages;
+  a.v = v_pages;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.columns = columns;
   a.o = static_cast<uint16_t*>(o);
   a.table = page_table;
   a.q_starts = q_starts;
@@ -1088,7 +1170,13 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
   a.page_shift = log2_of(page_size);
   a.max_q = max_q;
   a.max_kv = max_kv;
-  a.bs = std::min(block_size, bd3::kPagedMaxKeys);  // as good as any larger one
+  if (columns != nullptr) {
+    a.top = top;
+    a.block_tiles = block_tiles;
+    a.sc_t = strides[11];
+    a.sc_h = strides[12];
+  }
+  a.bs = block_size;
   a.tile = plan.tile;
   a.subs = plan.subs;
   a.q_tiles = plan.q_tiles;
@@ -1109,19 +1197,33 @@ int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void
     a.level_div = bd3::FastDiv::of(unit);
     a.level_step = 1;
     while (a.sorted && a.level_step * (int64_t)64 <= levels) a.level_step *= 64;
+  } else if (columns != nullptr) {
+    a.workgroups = (int)std::min(plan.tiles * plan.n_splits * kv_heads, (int64_t)kPagedWorkgroups);
   } else {  // about as many as there are items; each takes more if need be
     const int64_t items = ((total_kv >> plan.split_shift) + seqs) * kv_heads * plan.q_tiles;
     a.workgroups = (int)std::min({items, plan.tiles * plan.n_splits * kv_heads, (int64_t)kPagedWorkgroups});
   }
   a.scale_log2 = scale * bd3::kLog2e;
-  return hip_status(bd3::launch_paged_attn(a, static_cast<hipStream_t>(stream)), "paged_attn launch");
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  const bool plain = columns == nullptr && pool_type == BD3_POOL_BF16;
+  return hip_status(plain ? bd3::launch_paged_attn(a, on) : bd3::launch_paged_pool(a, pool_type, on), "paged_attn launch");
 }
 
-int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos_table, int32_t max_pos, void* q_out,
-                       void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* q_starts,
-                       const int32_t* kv_lens, int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads,
-                       int32_t head_dim, int32_t pages, int32_t page_size, int32_t table_width,
-                       const int64_t* strides, void* stream) {
+int bd3_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
+                   const int32_t* q_starts, const int32_t* kv_lens, int32_t seqs, int32_t tokens, int32_t heads,
+                   int32_t kv_heads, int32_t head_dim, int32_t pages, int32_t page_size, int32_t table_width,
+                   int32_t max_q, int32_t max_kv, int64_t total_kv, int32_t block_size, const int64_t* strides,
+                   float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  return bd3_paged_attn_pool(q, k_pages, v_pages, nullptr, nullptr, BD3_POOL_BF16, o, page_table, q_starts, kv_lens, nullptr,
+                             0, seqs, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, max_q, max_kv,
+                             total_kv, block_size, strides, scale, workspace, workspace_bytes, stream);
+}
+
+static int paged_rope(const void* qkv, const float* sin_table, const float* cos_table, int32_t max_pos, void* q_out,
+                      void* k_pages, void* v_pages, float* k_scales, float* v_scales, int32_t pool_type,
+                      const int32_t* page_table, const int32_t* q_starts, const int32_t* kv_lens, int32_t seqs,
+                      int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                      int32_t page_size, int32_t table_width, const int64_t* strides, void* stream) {
   if (int st = check_paged(seqs, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, page_table,
                            q_starts, kv_lens, strides))
     return st;
@@ -1131,16 +1233,18 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
     return fail(BD3_EINVAL, "sin_table and cos_table must be 16-byte aligned device pointers");
   if (int st = check_rows(qkv, strides, 1, "qkv")) return st;
   if (int st = check_rows(q_out, strides + 1, 2, "q_out")) return st;
-  if (int st = check_rows(k_pages, strides + 3, 3, "k_pages")) return st;
-  if (int st = check_rows(v_pages, strides + 6, 3, "v_pages")) return st;
+  if (int st = check_pool(k_pages, k_scales, pool_type, strides + 3, "k_pages")) return st;
+  if (int st = check_pool(v_pages, v_scales, pool_type, strides + 6, "v_pages")) return st;
   if (strides[9] < 0) return fail(BD3_EINVAL, "page_table stride must be >= 0");
   bd3::PagedRopeArgs a = {};
   a.qkv = static_cast<const uint16_t*>(qkv);
   a.sin_t = sin_table;
   a.cos_t = cos_table;
   a.q = static_cast<uint16_t*>(q_out);
-  a.k = static_cast<uint16_t*>(k_pages);
-  a.v = static_cast<uint16_t*>(v_pages);
+  a.k = k_pages;
+  a.v = v_pages;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
   a.table = page_table;
   a.q_starts = q_starts;
   a.kv_lens = kv_lens;
@@ -1166,8 +1270,195 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
   a.total = (int64_t)tokens * (heads + 2 * (int64_t)kv_heads) * 4;
   if (a.total >= ((int64_t)1 << 31))
     return fail(BD3_EINVAL, "tokens * heads too large (%lld work items, limit 2^31)", (long long)a.total);
-  return hip_status(bd3::launch_paged_rope(a, static_cast<hipStream_t>(stream)), "paged_qkv_rope launch");
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (pool_type == BD3_POOL_BF16) return hip_status(bd3::launch_paged_rope(a, on), "paged_qkv_rope launch");
+  a.blocks = (int)chunk_blocks(seqs, tokens, 16);
+  if (a.blocks * (int64_t)(heads + 2 * kv_heads) > 4 * (int64_t)kMaxWorkgroups)
+    return fail(BD3_EINVAL, "batch too large (limit 2^26 blocks of 16 slots and heads)");
+  a.parts_div = bd3::FastDiv::of(heads + 2 * kv_heads);
+  return hip_status(bd3::launch_paged_rope8(a, pool_type, on), "paged_qkv_rope8 launch");
 }
+
+int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos_table, int32_t max_pos, void* q_out,
+                       void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* q_starts,
+                       const int32_t* kv_lens, int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads,
+                       int32_t head_dim, int32_t pages, int32_t page_size, int32_t table_width,
+                       const int64_t* strides, void* stream) {
+  return paged_rope(qkv, sin_table, cos_table, max_pos, q_out, k_pages, v_pages, nullptr, nullptr, BD3_POOL_BF16, page_table,
+                    q_starts, kv_lens, seqs, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, strides,
+                    stream);
+}
+
+int bd3_paged_qkv_rope8(const void* qkv, const float* sin_table, const float* cos_table, int32_t max_pos, void* q_out,
+                        void* k_pages, void* v_pages, float* k_scales, float* v_scales, int32_t pool_type,
+                        const int32_t* page_table, const int32_t* q_starts, const int32_t* kv_lens, int32_t seqs,
+                        int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                        int32_t page_size, int32_t table_width, const int64_t* strides, void* stream) {
+  if (pool_type == BD3_POOL_BF16) return fail(BD3_EINVAL, "pool_type must be BD3_POOL_INT8 or BD3_POOL_E4M3");
+  return paged_rope(qkv, sin_table, cos_table, max_pos, q_out, k_pages, v_pages, k_scales, v_scales, pool_type, page_table,
+                    q_starts, kv_lens, seqs, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, strides,
+                    stream);
+}
+
+int bd3_page_values(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                    int32_t pool_type, void* k_out, void* v_out, int32_t pages, int32_t kv_heads, int32_t page_size,
+                    int32_t head_dim, const int64_t* strides, void* stream) {
+  if (pages < 0 || kv_heads < 1) return fail(BD3_EINVAL, "pages must be >= 0, kv_heads >= 1");
+  if (head_dim != bd3::kHeadDim) return fail(BD3_EINVAL, "head_dim must be 64, got %d", head_dim);
+  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0)
+    return fail(BD3_EINVAL, "page_size must be a power of two in [16, 1024], got %d", page_size);
+  if (strides == nullptr) return fail(BD3_EINVAL, "strides is NULL");
+  if (pool_type == BD3_POOL_BF16) return fail(BD3_EINVAL, "pool_type must be BD3_POOL_INT8 or BD3_POOL_E4M3");
+  if (pages == 0) return BD3_OK;
+  if (int st = check_pool(k_pages, k_scales, pool_type, strides, "k_pages")) return st;
+  if (int st = check_pool(v_pages, v_scales, pool_type, strides + 3, "v_pages")) return st;
+  if (k_out == nullptr || v_out == nullptr || !aligned16(k_out) || !aligned16(v_out))
+    return fail(BD3_EINVAL, "k_out and v_out must be 16-byte aligned device pointers");
+  bd3::PageValuesArgs a = {};
+  a.codes[0] = k_pages;
+  a.codes[1] = v_pages;
+  a.scales[0] = k_scales;
+  a.scales[1] = v_scales;
+  a.out[0] = static_cast<uint16_t*>(k_out);
+  a.out[1] = static_cast<uint16_t*>(v_out);
+  for (int i = 0; i < 2; ++i) {
+    a.s_p[i] = strides[3 * i];
+    a.s_h[i] = strides[3 * i + 1];
+    a.s_s[i] = strides[3 * i + 2];
+  }
+  a.kv_heads = kv_heads;
+  a.blocks = page_size / 16;
+  a.total = (int64_t)pages * kv_heads * a.blocks;
+  if (a.total > 2 * (int64_t)kMaxWorkgroups) return fail(BD3_EINVAL, "pool too large (limit 2^25 blocks of 16 slots and heads)");
+  return hip_status(bd3::launch_page_values(a, pool_type, static_cast<hipStream_t>(stream)), "page_values launch");
+}
+
+int bd3_page_bounds(const void* k_pages, const float* k_scales, int32_t pool_type, void* bounds,
+                    const int32_t* page_table, const int32_t* q_starts, const int32_t* kv_lens, int32_t seqs,
+                    int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t pages, int32_t page_size,
+                    int32_t table_width, const int64_t* strides, void* stream) {
+  if (int st = check_paged(seqs, tokens, kv_heads, kv_heads, head_dim, pages, page_size, table_width, page_table, q_starts,
+                           kv_lens, strides))
+    return st;
+  if (seqs == 0 || tokens == 0) return BD3_OK;
+  if (int st = check_pool(k_pages, k_scales, pool_type, strides, "k_pages")) return st;
+  if (strides[3] < 0) return fail(BD3_EINVAL, "page_table stride must be >= 0");
+  if (bounds == nullptr || !aligned16(bounds)) return fail(BD3_EINVAL, "bounds must be a 16-byte aligned device pointer");
+  bd3::SelectArgs a = {};
+  a.p.k = k_pages;
+  a.p.k_scales = k_scales;
+  a.p.table = page_table;
+  a.p.q_starts = q_starts;
+  a.p.kv_lens = kv_lens;
+  a.p.sk_p = strides[0];
+  a.p.sk_h = strides[1];
+  a.p.sk_s = strides[2];
+  a.p.table_s = strides[3];
+  a.p.seqs = seqs;
+  a.p.tokens = tokens;
+  a.p.kv_heads = kv_heads;
+  a.p.group = 1;
+  a.p.pages = pages;
+  a.p.page = page_size;
+  a.p.page_shift = log2_of(page_size);
+  a.p.max_q = tokens;
+  a.p.max_kv = (int)((int64_t)table_width * page_size);
+  a.p.kv_heads_div = bd3::FastDiv::of(kv_heads);
+  a.bounds = static_cast<uint16_t*>(bounds);
+  const int64_t slots = chunk_blocks(seqs, tokens, page_size);
+  if (slots * kv_heads > 4 * (int64_t)kMaxWorkgroups) return fail(BD3_EINVAL, "batch too large (limit 2^26 pages and heads)");
+  a.slots = (int)slots;
+  return hip_status(bd3::launch_page_bounds(a, pool_type, static_cast<hipStream_t>(stream)), "page_bounds launch");
+}
+
+// Columns within max_kv, whole groups of 16.
+static int64_t select_width(int32_t page_size, int32_t max_kv) {
+  return (((int64_t)max_kv + page_size - 1) / page_size + 15) / 16 * 16;
+}
+
+size_t bd3_select_pages_workspace_bytes(int32_t seqs, int32_t tokens, int32_t kv_heads, int32_t page_size,
+                                        int32_t max_kv, int32_t block_size) {
+  if (seqs < 1 || tokens < 1 || kv_heads < 1 || page_size < 16 || max_kv < 1 || max_kv > bd3::kPagedMaxKeys || block_size < 1)
+    return 0;
+  const int64_t items = chunk_blocks(seqs, tokens, block_size) * kv_heads, width = select_width(page_size, max_kv);
+  if (items >= kPagedItems || items * width >= ((int64_t)1 << 40)) return 0;
+  return (size_t)(items * width) * 12 + (size_t)(items * (width / 16)) * 4;
+}
+
+int bd3_select_pages(const void* q, const void* bounds, const int32_t* page_table, const int32_t* q_starts,
+                     const int32_t* kv_lens, int32_t* out, int32_t seqs, int32_t tokens, int32_t heads,
+                     int32_t kv_heads, int32_t head_dim, int32_t pages, int32_t page_size, int32_t table_width,
+                     int32_t max_q, int32_t max_kv, int32_t block_size, int32_t top, int32_t first, int32_t recent,
+                     const int64_t* strides, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int st = check_paged(seqs, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, page_table, q_starts,
+                           kv_lens, strides))
+    return st;
+  if (block_size < 1) return fail(BD3_EINVAL, "block_size must be >= 1");
+  if (max_q < 0 || max_kv < 0) return fail(BD3_EINVAL, "max_q and max_kv must be >= 0");
+  if (max_kv > (int64_t)table_width * page_size)
+    return fail(BD3_EINVAL, "max_kv (%d) exceeds the page table's %lld keys a sequence", max_kv,
+                (long long)table_width * page_size);
+  if (first < 0 || recent < 0) return fail(BD3_EINVAL, "first and recent must be >= 0");
+  if (seqs == 0 || tokens == 0 || max_q == 0) return BD3_OK;
+  if (max_kv == 0) max_kv = 1;  // no columns: every list is empty
+  max_q = std::min(max_q, tokens);
+  if (!paged_fits(heads, kv_heads, max_q))
+    return fail(BD3_EINVAL, "max_q * heads / kv_heads too large (limit 2^29 rows a chunk)");
+  const int64_t cols = ((int64_t)max_kv + page_size - 1) / page_size;
+  // the most columns that a block lies in: it begins at a multiple of what its size shares with a page's
+  const int64_t lie = (2 * (int64_t)page_size - std::gcd(page_size, block_size) + block_size - 1) / page_size;
+  const int64_t own = std::min(lie, cols);
+  if (top < std::min(first + (int64_t)recent + own, cols))
+    return fail(BD3_EINVAL, "top (%d) is less than the columns always taken: first + recent + %lld of a block", top,
+                (long long)own);
+  if (top < 1) return fail(BD3_EINVAL, "top must be >= 1");
+  if (int st = check_rows(q, strides, 2, "q")) return st;
+  if (strides[2] < 0) return fail(BD3_EINVAL, "page_table stride must be >= 0");
+  if (bounds == nullptr || !aligned16(bounds)) return fail(BD3_EINVAL, "bounds must be a 16-byte aligned device pointer");
+  if (out == nullptr || reinterpret_cast<uintptr_t>(out) % 4 != 0)
+    return fail(BD3_EINVAL, "out must be a 4-byte aligned device pointer");
+  const int64_t slots = chunk_blocks(seqs, tokens, block_size), items = slots * kv_heads;
+  const int64_t width = select_width(page_size, max_kv);
+  if (items >= kPagedItems || items * ((width + 63) / 64) > kMaxWorkgroups)
+    return fail(BD3_EINVAL, "batch too large (limit 2^24 workgroups of 64 columns of a block and KV head)");
+  const size_t need = bd3_select_pages_workspace_bytes(seqs, tokens, kv_heads, page_size, max_kv, block_size);
+  if (workspace_bytes < need) return fail(BD3_EINVAL, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
+  if (workspace == nullptr || !aligned16(workspace))
+    return fail(BD3_EINVAL, "workspace must be a 16-byte aligned device pointer");
+  bd3::SelectArgs a = {};
+  a.p.q = static_cast<const uint16_t*>(q);
+  a.p.table = page_table;
+  a.p.q_starts = q_starts;
+  a.p.kv_lens = kv_lens;
+  a.p.sq_t = strides[0];
+  a.p.sq_h = strides[1];
+  a.p.table_s = strides[2];
+  a.p.seqs = seqs;
+  a.p.tokens = tokens;
+  a.p.kv_heads = kv_heads;
+  a.p.group = heads / kv_heads;
+  a.p.pages = pages;
+  a.p.page = page_size;
+  a.p.page_shift = log2_of(page_size);
+  a.p.top = top;
+  a.p.max_q = max_q;
+  a.p.max_kv = max_kv;
+  a.p.bs = std::min(block_size, bd3::kPagedMaxKeys);
+  a.p.bs_div = bd3::FastDiv::of(a.p.bs);
+  a.p.group_div = bd3::FastDiv::of(a.p.group);
+  a.p.kv_heads_div = bd3::FastDiv::of(kv_heads);
+  a.bounds = static_cast<uint16_t*>(const_cast<void*>(bounds));
+  a.out = out;
+  a.slots = (int)slots;
+  a.width = (int)width;
+  a.first = first;
+  a.recent = recent;
+  a.sums = static_cast<double*>(workspace);
+  a.scores = reinterpret_cast<float*>(a.sums + items * width);
+  a.error = a.scores + items * width;
+  return hip_status(bd3::launch_select_pages(a, static_cast<hipStream_t>(stream)), "select_pages launch");
+}
+
 
 int bd3_adjust_logits(const void* logits, int32_t logits_fp32, void* out, int32_t batch, int32_t rows, int32_t vocab,
                       const int64_t* tokens, int32_t history, const int32_t* lengths, const float* penalties,

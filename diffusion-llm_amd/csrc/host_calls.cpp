@@ -52,9 +52,14 @@ struct Library {
   decltype(&bd3_qkv_rope) qkv_rope;
   decltype(&bd3_subs_sample_ws) subs_sample_ws;
   decltype(&bd3_subs_sample_workspace_bytes) subs_sample_workspace_bytes;
-  decltype(&bd3_paged_attn_workspace_bytes) paged_attn_workspace_bytes;
-  decltype(&bd3_paged_attn) paged_attn;
+  decltype(&bd3_paged_attn_pool_workspace_bytes) paged_attn_workspace_bytes;
+  decltype(&bd3_paged_attn_pool) paged_attn;
   decltype(&bd3_paged_qkv_rope) paged_qkv_rope;
+  decltype(&bd3_paged_qkv_rope8) paged_qkv_rope8;
+  decltype(&bd3_page_values) page_values;
+  decltype(&bd3_page_bounds) page_bounds;
+  decltype(&bd3_select_pages_workspace_bytes) select_pages_workspace_bytes;
+  decltype(&bd3_select_pages) select_pages;
   decltype(&bd3_adjust_logits) adjust_logits;
   decltype(&bd3_ln_modulate) ln_modulate;
   decltype(&bd3_gate_residual) gate_residual;
@@ -361,19 +366,39 @@ int32_t is_f32(const Tensor& t) {
   throw Refused{PyExc_KeyError, std::string("bf16 or fp32 tensors only, got ") + c10::toString(t.scalar_type())};
 }
 
-// The tensors that describe a ragged batch and its pool, checked (the kernels take
-// their addresses and sizes as they are).
-struct PagedBatch {
-  Tensor k, v, table, starts, lens;
-  int32_t seqs, pages, kv_heads, page, width;
-  PagedBatch(Args& a) : k(a.tensor()), v(a.tensor()), table(a.tensor()), starts(a.tensor()), lens(a.tensor()) {}
-  void check(const Tensor& first, int64_t heads) {
-    on_one_gpu(first, k, v, table, starts, lens);
-    require(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16, "bf16 inputs only");
-    require(k.dim() == 4 && k.sizes() == v.sizes() && k.size(3) == kHeadDim,
-            "k_pages and v_pages must be (pages, kv_heads, page_size, 64)");
-    require(vec_ready(k) && vec_ready(v), "k_pages and v_pages must have 16-byte aligned rows (they are not copied)");
-    require(k.size(1) >= 1 && heads % k.size(1) == 0, "heads must be a multiple of k_pages' kv_heads");
+// The pages of a pool and, of an 8-bit one, their scales.
+int32_t pool_type(const Tensor& pages) {
+  if (pages.scalar_type() == at::kBFloat16) return BD3_POOL_BF16;
+  if (pages.scalar_type() == at::kChar) return BD3_POOL_INT8;
+  require(pages.scalar_type() == at::kFloat8_e4m3fn, "bf16 inputs only (pages may be int8 or float8_e4m3fn, with scales)");
+  return BD3_POOL_E4M3;
+}
+
+bool pages_ready(const Tensor& t) {
+  if (!vec_ready(t)) return false;
+  for (int64_t i = 0; i < 3; ++i)
+    if (t.stride(i) * t.element_size() % 16 != 0) return false;
+  return true;
+}
+
+void check_scales(const Tensor& pages, const Tensor& scales) {
+  require(scales.defined() == (pool_type(pages) != BD3_POOL_BF16), "8-bit pages need scales, bf16 pages take none");
+  if (!scales.defined()) return;
+  on_one_gpu(pages, scales);
+  require(scales.scalar_type() == at::kFloat && scales.dim() == 3 && scales.size(0) == pages.size(0) &&
+              scales.size(1) == pages.size(1) && scales.size(2) == pages.size(2) / 16 && scales.is_contiguous(),
+          "scales must be contiguous float32 (pages, kv_heads, page_size / 16)");
+}
+
+const float* scales_p(const Tensor& t) { return t.defined() ? static_cast<const float*>(t.data_ptr()) : nullptr; }
+
+// The arrays that describe a ragged batch.
+struct BatchArrays {
+  Tensor table, starts, lens;
+  int32_t seqs, width;
+  BatchArrays(Args& a) : table(a.tensor()), starts(a.tensor()), lens(a.tensor()) {}
+  void check(const Tensor& first) {
+    on_one_gpu(first, table, starts, lens);
     require(table.scalar_type() == at::kInt && starts.scalar_type() == at::kInt && lens.scalar_type() == at::kInt,
             "page_table, q_starts and kv_lens must be int32");
     require(table.dim() == 2 && (table.size(1) == 1 || table.stride(1) == 1),
@@ -381,17 +406,38 @@ struct PagedBatch {
     require(starts.dim() == 1 && lens.dim() == 1 && starts.size(0) == table.size(0) + 1 &&
                 lens.size(0) == table.size(0) && starts.is_contiguous() && lens.is_contiguous(),
             "q_starts must be (seqs + 1) and kv_lens (seqs), contiguous");
-    require(table.size(0) <= INT32_MAX - 1 && table.size(1) <= INT32_MAX && k.size(0) <= INT32_MAX,
-            "batch or pool too large");
+    require(table.size(0) <= INT32_MAX - 1 && table.size(1) <= INT32_MAX, "batch or pool too large");
     seqs = dim32(table, 0);
     width = dim32(table, 1);
-    pages = dim32(k, 0);
-    kv_heads = dim32(k, 1);
-    page = k.size(2) <= INT32_MAX ? dim32(k, 2) : 0;
   }
   const int32_t* table_p() const { return static_cast<const int32_t*>(ptr(table)); }
   const int32_t* starts_p() const { return static_cast<const int32_t*>(ptr(starts)); }
   const int32_t* lens_p() const { return static_cast<const int32_t*>(ptr(lens)); }
+};
+
+// The tensors that describe a ragged batch and its pool, checked (the kernels take
+// their addresses and sizes as they are).
+struct PagedPool {
+  Tensor k, v;
+  int32_t pages, kv_heads, page, type;
+  PagedPool(Args& a) : k(a.tensor()), v(a.tensor()) {}
+};
+struct PagedBatch : PagedPool, BatchArrays {
+  PagedBatch(Args& a) : PagedPool(a), BatchArrays(a) {}
+  void check(const Tensor& first, int64_t heads) {
+    on_one_gpu(first, k, v, table, starts, lens);
+    type = pool_type(k);
+    require(v.scalar_type() == k.scalar_type(), "k_pages and v_pages must have one dtype");
+    require(k.dim() == 4 && k.sizes() == v.sizes() && k.size(3) == kHeadDim,
+            "k_pages and v_pages must be (pages, kv_heads, page_size, 64)");
+    require(pages_ready(k) && pages_ready(v), "k_pages and v_pages must have 16-byte aligned rows (they are not copied)");
+    require(k.size(1) >= 1 && heads % k.size(1) == 0, "heads must be a multiple of k_pages' kv_heads");
+    BatchArrays::check(first);
+    require(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX, "batch or pool too large");
+    pages = dim32(k, 0);
+    kv_heads = dim32(k, 1);
+    page = k.size(2) <= INT32_MAX ? dim32(k, 2) : 0;
+  }
 };
 
 // Written tensors: no element twice (an expanded one would be a race).
@@ -439,54 +485,73 @@ Tensor token_rows(const Tensor& out, int64_t tokens, int64_t heads, const Tensor
 }
 
 // paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv, total_kv,
-// out or None) -> O; max_kv, total_kv < 0: the table's, seqs * max_kv
+// out or None, k_scales or None, v_scales or None, columns or None) -> O; max_kv, total_kv < 0: the table's,
+// seqs * max_kv
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&] {
-    Args a(args, n, 11);
+    Args a(args, n, 14);
     Tensor q = a.tensor();
     PagedBatch b(a);
     const int32_t bs = a.int32(), max_q = a.int32();
     int32_t max_kv = a.int32();
     int64_t total = a.integer();
     Tensor out = a.maybe_tensor();
+    const Tensor k_scales = a.maybe_tensor(), v_scales = a.maybe_tensor();
+    Tensor columns = a.maybe_tensor();
     require(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(2) == kHeadDim,
             "q must be a (tokens, heads, 64) bf16 tensor");
     require(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX, "q is too large");
     b.check(q, q.size(1));
+    check_scales(b.k, k_scales);
+    check_scales(b.v, v_scales);
+    if (columns.defined()) {
+      on_one_gpu(q, columns);
+      require(columns.dim() == 3 && columns.scalar_type() == at::kInt && columns.size(0) == q.size(0) &&
+                  columns.size(1) == b.kv_heads && columns.size(2) >= 1 && columns.size(2) <= INT32_MAX &&
+                  (columns.size(2) == 1 || columns.stride(2) == 1),
+              "columns must be int32 (tokens, kv_heads, top) with last stride 1");
+    }
     {
       NoGil nogil;
       const c10::DeviceGuard device(q.device());
       q = ready_tokens(q);
-      const int32_t T = dim32(q, 0), H = dim32(q, 1);
+      const int32_t T = dim32(q, 0), H = dim32(q, 1), top = columns.defined() ? dim32(columns, 2) : 0;
       out = token_rows(out, T, H, q);
-      require(apart(out, q, b.k, b.v, b.table, b.starts, b.lens), "out must not overlap an input");
+      require(apart(out, q, b.k, b.v, b.table, b.starts, b.lens, k_scales, v_scales, columns), "out must not overlap an input");
       if (max_kv < 0) max_kv = (int32_t)std::min<int64_t>((int64_t)b.width * b.page, INT32_MAX);
       if (total < 0) total = (int64_t)b.seqs * max_kv;
-      const size_t bytes = g_lib.paged_attn_workspace_bytes(b.seqs, T, H, b.kv_heads, max_q, max_kv, total);
+      const size_t bytes =
+          g_lib.paged_attn_workspace_bytes(b.type, b.seqs, T, H, b.kv_heads, b.page, max_q, max_kv, total, bs, top);
       const Tensor ws = bytes ? workspace(bytes, q) : Tensor();
-      const int64_t st[11] = {q.stride(0),   q.stride(1),   b.k.stride(0),   b.k.stride(1),   b.k.stride(2), b.v.stride(0),
-                              b.v.stride(1), b.v.stride(2), out.stride(0), out.stride(1), b.table.stride(0)};
-      check(g_lib.paged_attn(ptr(q), ptr(b.k), ptr(b.v), ptr(out), b.table_p(), b.starts_p(), b.lens_p(), b.seqs, T, H,
-                             b.kv_heads, kHeadDim, b.pages, b.page, b.width, max_q, max_kv, total, bs, st, kScale,
+      const int64_t st[13] = {q.stride(0),   q.stride(1),   b.k.stride(0), b.k.stride(1),   b.k.stride(2),
+                              b.v.stride(0), b.v.stride(1), b.v.stride(2), out.stride(0),   out.stride(1),
+                              b.table.stride(0), top ? columns.stride(0) : 0, top ? columns.stride(1) : 0};
+      check(g_lib.paged_attn(ptr(q), ptr(b.k), ptr(b.v), scales_p(k_scales), scales_p(v_scales), b.type, ptr(out),
+                             b.table_p(), b.starts_p(), b.lens_p(), static_cast<const int32_t*>(ptr(columns)), top, b.seqs,
+                             T, H, b.kv_heads, kHeadDim, b.pages, b.page, b.width, max_q, max_kv, total, bs, st, kScale,
                              ptr(ws), bytes, stream_of(q)));
     }
     return THPVariable_Wrap(out);
   });
 }
 
-// paged_attention_inputs(qkv, heads, sin, cos, k_pages, v_pages, page_table, q_starts, kv_lens, out or None) -> q
+// paged_attention_inputs(qkv, heads, sin, cos, k_pages, v_pages, page_table, q_starts, kv_lens, out or None,
+// k_scales or None, v_scales or None) -> q
 PyObject* paged_attention_inputs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&] {
-    Args a(args, n, 10);
+    Args a(args, n, 12);
     Tensor qkv = a.tensor();
     const int32_t heads = a.int32();
     Tensor sin = a.tensor(), cos = a.tensor();
     PagedBatch b(a);
     Tensor out = a.maybe_tensor();
+    const Tensor k_scales = a.maybe_tensor(), v_scales = a.maybe_tensor();
     require(qkv.dim() == 2 && qkv.scalar_type() == at::kBFloat16, "qkv must be a (tokens, width) bf16 tensor");
     require(heads >= 1, "n_heads must be >= 1");
     b.check(qkv, heads);
     on_one_gpu(qkv, sin, cos);
+    check_scales(b.k, k_scales);
+    check_scales(b.v, v_scales);
     require(writable(b.k) && writable(b.v), "k_pages and v_pages are written: no element may occur twice");
     require(qkv.size(1) == ((int64_t)heads + 2 * (int64_t)b.kv_heads) * kHeadDim,
             "projection width must be (n_heads + 2 * kv_heads) * 64");
@@ -507,10 +572,129 @@ PyObject* paged_attention_inputs(PyObject*, PyObject* const* args, Py_ssize_t n)
         require(apart(*t, sin, cos, b.table, b.starts, b.lens), "out and the pages must not overlap an input");
       const int64_t st[10] = {qkv.stride(0), out.stride(0), out.stride(1), b.k.stride(0), b.k.stride(1), b.k.stride(2),
                               b.v.stride(0), b.v.stride(1), b.v.stride(2), b.table.stride(0)};
-      check(g_lib.paged_qkv_rope(ptr(qkv), static_cast<const float*>(ptr(sin)), static_cast<const float*>(ptr(cos)),
-                                 dim32(sin, 0), ptr(out), ptr(b.k), ptr(b.v), b.table_p(), b.starts_p(), b.lens_p(),
-                                 b.seqs, dim32(qkv, 0), heads, b.kv_heads, kHeadDim, b.pages, b.page, b.width, st,
-                                 stream_of(qkv)));
+      if (b.type == BD3_POOL_BF16) {
+        check(g_lib.paged_qkv_rope(ptr(qkv), static_cast<const float*>(ptr(sin)), static_cast<const float*>(ptr(cos)),
+                                   dim32(sin, 0), ptr(out), ptr(b.k), ptr(b.v), b.table_p(), b.starts_p(), b.lens_p(),
+                                   b.seqs, dim32(qkv, 0), heads, b.kv_heads, kHeadDim, b.pages, b.page, b.width, st,
+                                   stream_of(qkv)));
+      } else {
+        for (const Tensor* t : {&k_scales, &v_scales})
+          require(apart(*t, qkv, out, b.k, b.v, sin, cos, b.table, b.starts, b.lens), "the scales must not overlap another argument");
+        require(apart(k_scales, v_scales), "the scales must not overlap another argument");
+        check(g_lib.paged_qkv_rope8(ptr(qkv), static_cast<const float*>(ptr(sin)), static_cast<const float*>(ptr(cos)),
+                                    dim32(sin, 0), ptr(out), ptr(b.k), ptr(b.v), static_cast<float*>(ptr(k_scales)),
+                                    static_cast<float*>(ptr(v_scales)), b.type, b.table_p(), b.starts_p(), b.lens_p(),
+                                    b.seqs, dim32(qkv, 0), heads, b.kv_heads, kHeadDim, b.pages, b.page, b.width, st,
+                                    stream_of(qkv)));
+      }
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// page_values(k_pages, v_pages, k_scales, v_scales) -> (k, v) bf16
+PyObject* page_values(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] {
+    Args a(args, n, 4);
+    const Tensor k = a.tensor(), v = a.tensor(), k_scales = a.tensor(), v_scales = a.tensor();
+    on_one_gpu(k, v);
+    const int32_t type = pool_type(k);
+    require(type != BD3_POOL_BF16, "k_pages and v_pages must be int8 or float8_e4m3fn");
+    require(v.scalar_type() == k.scalar_type(), "k_pages and v_pages must have one dtype");
+    require(k.dim() == 4 && k.sizes() == v.sizes() && k.size(3) == kHeadDim,
+            "k_pages and v_pages must be (pages, kv_heads, page_size, 64)");
+    require(pages_ready(k) && pages_ready(v), "k_pages and v_pages must have 16-byte aligned rows (they are not copied)");
+    require(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX, "pool too large");
+    check_scales(k, k_scales);
+    check_scales(v, v_scales);
+    Tensor k_out, v_out;
+    {
+      NoGil nogil;
+      const c10::DeviceGuard device(k.device());
+      k_out = at::empty(k.sizes(), k.options().dtype(at::kBFloat16));
+      v_out = at::empty(k.sizes(), k.options().dtype(at::kBFloat16));
+      const int64_t st[6] = {k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2)};
+      check(g_lib.page_values(ptr(k), ptr(v), scales_p(k_scales), scales_p(v_scales), type, ptr(k_out), ptr(v_out),
+                              dim32(k, 0), dim32(k, 1), dim32(k, 2), kHeadDim, st, stream_of(k)));
+    }
+    return pack(k_out, v_out);
+  });
+}
+
+void check_bounds(const Tensor& bounds, int64_t pages, int64_t kv_heads) {
+  require(bounds.dim() == 4 && bounds.scalar_type() == at::kBFloat16 && (pages < 0 || bounds.size(0) == pages) &&
+              (kv_heads < 0 || bounds.size(1) == kv_heads) && bounds.size(2) == 2 && bounds.size(3) == kHeadDim &&
+              bounds.is_contiguous() && vec_ready(bounds),
+          "bounds must be contiguous bf16 (pages, kv_heads, 2, 64)");
+}
+
+// page_bounds(k_pages, bounds, page_table, q_starts, kv_lens, tokens, k_scales or None) -> bounds
+PyObject* page_bounds(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] {
+    Args a(args, n, 7);
+    const Tensor k = a.tensor(), bounds = a.tensor();
+    BatchArrays b(a);
+    const int32_t tokens = a.int32();
+    const Tensor k_scales = a.maybe_tensor();
+    on_one_gpu(k, bounds);
+    b.check(k);
+    const int32_t type = pool_type(k);
+    require(k.dim() == 4 && k.size(3) == kHeadDim && k.size(1) >= 1, "k_pages must be (pages, kv_heads, page_size, 64)");
+    require(pages_ready(k), "k_pages must have 16-byte aligned rows (they are not copied)");
+    require(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX, "pool too large");
+    check_scales(k, k_scales);
+    check_bounds(bounds, k.size(0), k.size(1));
+    {
+      NoGil nogil;
+      const c10::DeviceGuard device(k.device());
+      require(apart(bounds, k, b.table, b.starts, b.lens, k_scales), "bounds must not overlap an input");
+      const int64_t st[4] = {k.stride(0), k.stride(1), k.stride(2), b.table.stride(0)};
+      check(g_lib.page_bounds(ptr(k), scales_p(k_scales), type, ptr(bounds), b.table_p(), b.starts_p(), b.lens_p(), b.seqs,
+                              tokens, dim32(k, 1), kHeadDim, dim32(k, 0), dim32(k, 2), b.width, st, stream_of(k)));
+    }
+    return THPVariable_Wrap(bounds);
+  });
+}
+
+// select_pages(q, bounds, page_table, q_starts, kv_lens, block_size, page_size, top, max_q, max_kv, first, recent,
+// out or None) -> columns; max_kv < 0: the table's
+PyObject* select_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] {
+    Args a(args, n, 13);
+    Tensor q = a.tensor();
+    const Tensor bounds = a.tensor();
+    BatchArrays b(a);
+    const int32_t bs = a.int32(), page = a.int32(), top = a.int32(), max_q = a.int32();
+    int32_t max_kv = a.int32();
+    const int32_t first = a.int32(), recent = a.int32();
+    Tensor out = a.maybe_tensor();
+    require(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(2) == kHeadDim,
+            "q must be a (tokens, heads, 64) bf16 tensor");
+    require(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX, "q is too large");
+    on_one_gpu(q, bounds);
+    b.check(q);
+    check_bounds(bounds, -1, -1);
+    require(bounds.size(0) <= INT32_MAX && bounds.size(1) >= 1 && q.size(1) % bounds.size(1) == 0,
+            "heads must be a multiple of the bounds' kv_heads");
+    require(page >= 1, "page_size must be a power of two in [16, 1024]");
+    {
+      NoGil nogil;
+      const c10::DeviceGuard device(q.device());
+      q = ready_tokens(q);
+      const int32_t T = dim32(q, 0), H = dim32(q, 1), KH = dim32(bounds, 1);
+      require(top >= 1, "top must be >= 1");
+      if (!out.defined()) out = at::empty({T, KH, top}, q.options().dtype(at::kInt));
+      require(out.dim() == 3 && out.size(0) == T && out.size(1) == KH && out.size(2) == top && out.scalar_type() == at::kInt &&
+                  out.device() == q.device() && out.is_contiguous(),
+              "out must be contiguous int32 (tokens, kv_heads, top)");
+      require(apart(out, q, bounds, b.table, b.starts, b.lens), "out must not overlap an input");
+      if (max_kv < 0) max_kv = (int32_t)std::min<int64_t>((int64_t)b.width * page, INT32_MAX);
+      const size_t bytes = g_lib.select_pages_workspace_bytes(b.seqs, T, KH, page, std::max(max_kv, 1), bs);
+      const Tensor ws = bytes ? workspace(bytes, q) : Tensor();
+      const int64_t st[3] = {q.stride(0), q.stride(1), b.table.stride(0)};
+      check(g_lib.select_pages(ptr(q), ptr(bounds), b.table_p(), b.starts_p(), b.lens_p(), static_cast<int32_t*>(ptr(out)),
+                               b.seqs, T, H, KH, kHeadDim, dim32(bounds, 0), page, b.width, max_q, max_kv, bs, top, first,
+                               recent, st, ptr(ws), bytes, stream_of(q)));
     }
     return THPVariable_Wrap(out);
   });
@@ -739,9 +923,14 @@ PyObject* bind(PyObject*, PyObject* dict) {
     set("bd3_qkv_rope", l.qkv_rope);
     set("bd3_subs_sample_ws", l.subs_sample_ws);
     set("bd3_subs_sample_workspace_bytes", l.subs_sample_workspace_bytes);
-    set("bd3_paged_attn_workspace_bytes", l.paged_attn_workspace_bytes);
-    set("bd3_paged_attn", l.paged_attn);
+    set("bd3_paged_attn_pool_workspace_bytes", l.paged_attn_workspace_bytes);
+    set("bd3_paged_attn_pool", l.paged_attn);
     set("bd3_paged_qkv_rope", l.paged_qkv_rope);
+    set("bd3_paged_qkv_rope8", l.paged_qkv_rope8);
+    set("bd3_page_values", l.page_values);
+    set("bd3_page_bounds", l.page_bounds);
+    set("bd3_select_pages_workspace_bytes", l.select_pages_workspace_bytes);
+    set("bd3_select_pages", l.select_pages);
     set("bd3_adjust_logits", l.adjust_logits);
     set("bd3_ln_modulate", l.ln_modulate);
     set("bd3_gate_residual", l.gate_residual);
@@ -761,6 +950,9 @@ PyMethodDef methods[] = {
     BD3_FAST(subs_sample),
     BD3_FAST(paged_attention),
     BD3_FAST(paged_attention_inputs),
+    BD3_FAST(page_values),
+    BD3_FAST(page_bounds),
+    BD3_FAST(select_pages),
     BD3_FAST(adjust_logits),
     BD3_FAST(ln_modulate),
     BD3_FAST(gate_residual),

@@ -69,6 +69,19 @@ SIGNATURES: dict[str, tuple] = {
                                       _i32, _i32, _i32, _i32, ctypes.c_int64, _i32, _i64p, _f32, _c_p, _sz, _c_p]),
     "bd3_paged_qkv_rope": (ctypes.c_int, [_c_p, _c_p, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32,
                                           _i32, _i32, _i32, _i32, _i32, _i32, _i64p, _c_p]),
+    "bd3_paged_attn_pool_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.c_int64, _i32,
+                                                  _i32]),
+    "bd3_paged_attn_pool": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32,
+                                           _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.c_int64, _i32,
+                                           _i64p, _f32, _c_p, _sz, _c_p]),
+    "bd3_paged_qkv_rope8": (ctypes.c_int, [_c_p, _c_p, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _c_p,
+                                           _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64p, _c_p]),
+    "bd3_page_values": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _i32, _i32, _i32, _i32, _i64p, _c_p]),
+    "bd3_page_bounds": (ctypes.c_int, [_c_p, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _i32, _i32, _i32, _i32, _i32, _i32,
+                                       _i32, _i64p, _c_p]),
+    "bd3_select_pages_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "bd3_select_pages": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64p, _c_p, _sz, _c_p]),
     "bd3_adjust_logits": (ctypes.c_int, [_c_p, _i32, _c_p, _i32, _i32, _i32, _c_p, _i32, _c_p,
                                          ctypes.POINTER(_f32), _c_p, _c_p, _c_p, _c_p, _c_p, _f32, _i64p, _c_p]),
     "bd3_ln_modulate": (ctypes.c_int, [_c_p, _i32, _c_p, _i32, _c_p, _c_p, _i32, _c_p, _i32, _i32, _i32, _i32,

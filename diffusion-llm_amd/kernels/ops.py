@@ -18,8 +18,21 @@ carries its backward (register_autograd).
     torch.ops.bd3.paged_attn(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv=-1,
                              total_kv=-1) -> O
         kernels.paged.paged_attention; -1: the defaults
+    torch.ops.bd3.paged_qkv_rope8(qkv, n_heads, sin, cos, k_pages, v_pages, k_scales, v_scales, page_table, q_starts,
+                                  kv_lens) -> q
+        kernels.paged.paged_attention_inputs8; writes the pages and scales
+    torch.ops.bd3.paged_attn_pool(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv=-1,
+                                  total_kv=-1, k_scales=None, v_scales=None, columns=None) -> O
+        kernels.paged.paged_attention_pool
+    torch.ops.bd3.page_bounds(k_pages, bounds, page_table, q_starts, kv_lens, tokens, k_scales=None)
+        kernels.paged.page_bounds; writes bounds
+    torch.ops.bd3.select_pages(q, bounds, page_table, q_starts, kv_lens, block_size, page_size, top, max_q, max_kv=-1,
+                               first=1, recent=1) -> columns
+        kernels.paged.select_pages
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 from torch import Tensor
@@ -113,7 +126,7 @@ def paged_qkv_rope(qkv: Tensor, n_heads: int, sin_table: Tensor, cos_table: Tens
                    page_table: Tensor, q_starts: Tensor, kv_lens: Tensor) -> Tensor:
     """The attention inputs of a ragged batch, keys and values into their pages."""
     return host().paged_attention_inputs(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, page_table, q_starts,
-                                         kv_lens, None)
+                                         kv_lens, None, None, None)
 
 
 @paged_qkv_rope.register_fake
@@ -126,9 +139,64 @@ def paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, 
                block_size: int, max_q: int, max_kv: int = -1, total_kv: int = -1) -> Tensor:
     """Attention of a ragged batch over its pages."""
     return host().paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv,
-                                  total_kv, None)
+                                  total_kv, None, None, None, None)
 
 
 @paged_attn.register_fake
 def _paged_attn_fake(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv=-1, total_kv=-1):
     return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("bd3::paged_qkv_rope8", mutates_args=("k_pages", "v_pages", "k_scales", "v_scales"))
+def paged_qkv_rope8(qkv: Tensor, n_heads: int, sin_table: Tensor, cos_table: Tensor, k_pages: Tensor, v_pages: Tensor,
+                    k_scales: Tensor, v_scales: Tensor, page_table: Tensor, q_starts: Tensor, kv_lens: Tensor) -> Tensor:
+    """The attention inputs of a ragged batch, keys and values into 8-bit pages."""
+    return host().paged_attention_inputs(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, page_table, q_starts,
+                                         kv_lens, None, k_scales, v_scales)
+
+
+@paged_qkv_rope8.register_fake
+def _paged_qkv_rope8_fake(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, k_scales, v_scales, page_table, q_starts,
+                          kv_lens):
+    return qkv.new_empty((qkv.shape[0], n_heads, D))
+
+
+@torch.library.custom_op("bd3::paged_attn_pool", mutates_args=())
+def paged_attn_pool(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, q_starts: Tensor, kv_lens: Tensor,
+                    block_size: int, max_q: int, max_kv: int = -1, total_kv: int = -1, k_scales: Optional[Tensor] = None,
+                    v_scales: Optional[Tensor] = None, columns: Optional[Tensor] = None) -> Tensor:
+    """Attention of a ragged batch over pages of any kind, all or those of a list."""
+    return host().paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv,
+                                  total_kv, None, k_scales, v_scales, columns)
+
+
+@paged_attn_pool.register_fake
+def _paged_attn_pool_fake(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q, max_kv=-1, total_kv=-1,
+                          k_scales=None, v_scales=None, columns=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("bd3::page_bounds", mutates_args=("bounds",))
+def page_bounds(k_pages: Tensor, bounds: Tensor, page_table: Tensor, q_starts: Tensor, kv_lens: Tensor, tokens: int,
+                k_scales: Optional[Tensor] = None) -> None:
+    """The bounds of the pages that hold tokens of the chunks."""
+    host().page_bounds(k_pages, bounds, page_table, q_starts, kv_lens, tokens, k_scales)
+
+
+@page_bounds.register_fake
+def _page_bounds_fake(k_pages, bounds, page_table, q_starts, kv_lens, tokens, k_scales=None):
+    return None
+
+
+@torch.library.custom_op("bd3::select_pages", mutates_args=())
+def select_pages(q: Tensor, bounds: Tensor, page_table: Tensor, q_starts: Tensor, kv_lens: Tensor, block_size: int,
+                 page_size: int, top: int, max_q: int, max_kv: int = -1, first: int = 1, recent: int = 1) -> Tensor:
+    """The pages that the attention of a batch is to read."""
+    return host().select_pages(q, bounds, page_table, q_starts, kv_lens, block_size, page_size, top, max_q, max_kv, first,
+                               recent, None)
+
+
+@select_pages.register_fake
+def _select_pages_fake(q, bounds, page_table, q_starts, kv_lens, block_size, page_size, top, max_q, max_kv=-1, first=1,
+                       recent=1):
+    return q.new_empty((q.shape[0], bounds.shape[1], top), dtype=torch.int32)

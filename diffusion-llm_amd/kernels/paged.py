@@ -13,6 +13,11 @@ run a layer's attention for all of them, in two launches (three where the keys
 are cut over workgroups). `paged_attention_inputs` and `paged_attention` are the
 same calls on a caller's own pool, tables and lengths.
 
+The pages may hold 8-bit codes with scales (`paged_attention_inputs8`, `paged_attention_pool`): half the
+memory, half the bytes that the attention reads. And a step may read only the pages that promise
+most for its queries, by bounds of each page's keys (`page_bounds`, `select_pages`,
+`batch.attention(..., top=)`): its time no longer grows with the cache.
+
 Tokens are packed: sequence b owns rows q_starts[b] .. q_starts[b + 1] - 1 of
 every (tokens, ...) tensor. Its token i is at position kv_lens[b] - n + i, n the
 chunk's tokens, and sees the keys up to the end of its block of block_size
@@ -32,6 +37,7 @@ from torch import Tensor
 from kernels._native import host
 
 D = 64
+BLOCK = 16  # slots that share a scale
 
 
 def paged_attention(
@@ -55,7 +61,8 @@ def paged_attention(
     finite, also those that only later tokens of the chunk see (their weights are
     zeros that multiply them). `out` overlaps no input."""
     return host().paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q,
-                                  -1 if max_kv is None else max_kv, -1 if total_kv is None else total_kv, out)
+                                  -1 if max_kv is None else max_kv, -1 if total_kv is None else total_kv, out,
+                                  None, None, None)
 
 
 def paged_attention_inputs(
@@ -77,27 +84,156 @@ def paged_attention_inputs(
     use their last row; nothing is written where the table has no page. out,
     k_pages and v_pages overlap neither each other nor another argument."""
     return host().paged_attention_inputs(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, page_table, q_starts,
-                                         kv_lens, out)
+                                         kv_lens, out, None, None)
+
+
+def paged_attention_pool(
+    q: Tensor,           # (tokens, heads, 64) bf16
+    k_pages: Tensor,     # (pages, kv_heads, page_size, 64) bf16, int8 or float8_e4m3fn
+    v_pages: Tensor,
+    page_table: Tensor,
+    q_starts: Tensor,
+    kv_lens: Tensor,
+    block_size: int,
+    max_q: int,
+    max_kv: int | None = None,
+    total_kv: int | None = None,
+    out: Tensor | None = None,
+    k_scales: Tensor | None = None,  # of 8-bit pages: (pages, kv_heads, page_size // 16) float32, contiguous
+    v_scales: Tensor | None = None,
+    columns: Tensor | None = None,   # (tokens, kv_heads, top) int32 (select_pages)
+) -> Tensor:
+    """paged_attention over any kind of pool, and over selected pages.
+
+    8-bit pages hold codes, value = scale * code with a scale for each 16 slots and
+    head (paged_attention_inputs8 writes them); the scales of blocks that hold keys must
+    be finite and at least 2 ** -100. Codes enter the products exactly, scales multiply
+    scores and probabilities in fp32: the result is as near to the values as
+    paged_attention's is to its bf16 ones.
+
+    With `columns` the tokens of one block of block_size positions read, as far as they see them,
+    only the pages in the table's columns columns[first of them in the chunk, KV head]. No column may
+    occur twice, so of a list only as many entries are read as the sequence has columns with keys;
+    entries that are none of these (-1) name nothing."""
+    return host().paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q,
+                                  -1 if max_kv is None else max_kv, -1 if total_kv is None else total_kv, out,
+                                  k_scales, v_scales, columns)
+
+
+def paged_attention_inputs8(
+    qkv: Tensor,         # as in paged_attention_inputs
+    n_heads: int,
+    sin_table: Tensor,
+    cos_table: Tensor,
+    k_pages: Tensor,     # (pages, kv_heads, page_size, 64) int8 or float8_e4m3fn; written
+    v_pages: Tensor,
+    k_scales: Tensor,    # (pages, kv_heads, page_size // 16) float32, contiguous; written
+    v_scales: Tensor,
+    page_table: Tensor,
+    q_starts: Tensor,
+    kv_lens: Tensor,
+    out: Tensor | None = None,
+) -> Tensor:
+    """paged_attention_inputs into 8-bit pages. Each 16 slots (a block: slots 16 i to
+    16 i + 15 of a page) and head take a scale: the one that their new values need
+    (max|x| / 127, or for float8_e4m3fn the least power of two with 448 * scale >=
+    max|x|; at least 2 ** -100), or, if the block holds earlier tokens of the sequence, its
+    scale times the least power of two with which the new values fit; the block's
+    other codes are then rounded to the new scale. A new value is off by at most half
+    a step (the scale, or the spacing of e4m3 there); an earlier one in the
+    end by less than one step.
+
+    A block that holds earlier tokens keeps a scale that uncommitted ones, since overwritten,
+    have raised. Values must be finite. Blocks are written whole: no two sequences of a
+    call may write into the same one. No written tensor overlaps another argument."""
+    return host().paged_attention_inputs(qkv, n_heads, sin_table, cos_table, k_pages, v_pages, page_table, q_starts,
+                                         kv_lens, out, k_scales, v_scales)
+
+
+def page_values(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor) -> tuple[Tensor, Tensor]:
+    """The values that 8-bit pages hold, as bf16 (pages, kv_heads, page_size, 64) each."""
+    return host().page_values(k_pages, v_pages, k_scales, v_scales)
+
+
+def page_bounds(
+    k_pages: Tensor,     # as in paged_attention_pool
+    bounds: Tensor,      # (pages, kv_heads, 2, 64) bf16, contiguous: the lowest, the highest key of each channel; written
+    page_table: Tensor,
+    q_starts: Tensor,
+    kv_lens: Tensor,
+    tokens: int,         # packed tokens of the batch
+    k_scales: Tensor | None = None,
+) -> Tensor:
+    """Form the bounds of the pages that hold tokens of the chunks anew, over all
+    keys that the sequence has in them; returns `bounds`. Other pages' stay, so after the
+    call that writes a chunk's final keys this keeps the bounds of a sequence's pages."""
+    return host().page_bounds(k_pages, bounds, page_table, q_starts, kv_lens, tokens, k_scales)
+
+
+def select_pages(
+    q: Tensor,           # (tokens, heads, 64) bf16
+    bounds: Tensor,      # (pages, kv_heads, 2, 64) bf16 (page_bounds)
+    page_table: Tensor,
+    q_starts: Tensor,
+    kv_lens: Tensor,
+    block_size: int,
+    page_size: int,
+    top: int,            # pages for each block of queries and KV head
+    max_q: int,
+    max_kv: int | None = None,
+    first: int = 1,      # columns always taken: the first ones,
+    recent: int = 1,     # and those before the block's own
+    out: Tensor | None = None,
+) -> Tensor:
+    """The pages that paged_attention_pool is to read, (tokens, kv_heads, top) int32
+    columns of the page table, ascending, then -1. The tokens of one block of
+    block_size positions choose together for each KV head: the first `first` columns,
+    those that hold positions of the block and the `recent` before them, and of the others
+    that they see the ones with the largest
+
+        max over the block's tokens and the KV head's query heads of
+        sum_d max(q_d * lowest_d, q_d * highest_d),
+
+    which no key of the page exceeds in q . k; equals by the lower column. The
+    scores' order is exact. `top` must leave room for the columns always taken. Rows behind the last
+    sequence are left as they are (without `out` undefined). Bounds of the columns always taken are
+    not read; those of the others must be finite."""
+    return host().select_pages(q, bounds, page_table, q_starts, kv_lens, block_size, page_size, top, max_q,
+                               -1 if max_kv is None else max_kv, first, recent, out)
 
 
 class PagedKVCache:
     """A pool of pages for the post-RoPE keys and values of many sequences, the
-    same page numbers in every layer. Host-side bookkeeping: a sequence is the
-    int that `add` returned, until `free`."""
+    same page numbers in every layer, in bf16 or in 8 bits (`dtype`: int8 or
+    float8_e4m3fn, with scales), with bounds of each page's keys for attention over selected
+    pages (`bounds`). Host-side bookkeeping: a sequence is the int that `add`
+    returned, until `free`."""
 
     def __init__(self, n_layers: int, n_pages: int, kv_heads: int, page_size: int = 64,
-                 device: torch.device | str = "cuda"):
+                 device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16, bounds: bool = False):
         assert n_layers >= 1 and n_pages >= 1 and kv_heads >= 1, "need at least one layer, page and KV head"
         assert 16 <= page_size <= 1024 and page_size & (page_size - 1) == 0, \
             "page_size must be a power of two in [16, 1024]"
         self.page_size = page_size
         shape = (n_layers, n_pages, kv_heads, page_size, D)
-        self.k_pages = torch.empty(shape, device=device, dtype=torch.bfloat16)
-        self.v_pages = torch.empty(shape, device=device, dtype=torch.bfloat16)
+        assert dtype in (torch.bfloat16, torch.int8, torch.float8_e4m3fn), \
+            "pages hold bfloat16, int8 or float8_e4m3fn"
+        self.k_pages = torch.empty(shape, device=device, dtype=dtype)
+        self.v_pages = torch.empty(shape, device=device, dtype=dtype)
+        self.k_scales = self.v_scales = self.bounds = None
+        if dtype != torch.bfloat16:  # 0: no scale yet
+            self.k_scales = torch.zeros((*shape[:3], page_size // BLOCK), device=device)
+            self.v_scales = torch.zeros_like(self.k_scales)
+        if bounds:
+            self.bounds = torch.zeros((*shape[:3], 2, D), device=device, dtype=torch.bfloat16)
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages: dict[int, list[int]] = {}
         self._length: dict[int, int] = {}
         self._next = 0
+
+    def scales(self, layer: int) -> tuple[Tensor | None, Tensor | None]:
+        """(k_scales, v_scales) of a layer's 8-bit pages; (None, None) in bf16."""
+        return (None, None) if self.k_scales is None else (self.k_scales[layer], self.v_scales[layer])
 
     @property
     def free_pages(self) -> int:
@@ -160,16 +296,34 @@ class PagedBatch:
 
     def attention_inputs(self, qkv: Tensor, n_heads: int, sin_table: Tensor, cos_table: Tensor, layer: int,
                          out: Tensor | None = None) -> Tensor:
-        """paged_attention_inputs into this layer's pages."""
+        """paged_attention_inputs, or paged_attention_inputs8, into this layer's pages."""
         c = self.cache
-        return paged_attention_inputs(qkv, n_heads, sin_table, cos_table, c.k_pages[layer], c.v_pages[layer],
-                                      self.page_table, self.q_starts, self.kv_lens, out)
+        k_scales, v_scales = c.scales(layer)
+        return host().paged_attention_inputs(qkv, n_heads, sin_table, cos_table, c.k_pages[layer], c.v_pages[layer],
+                                             self.page_table, self.q_starts, self.kv_lens, out, k_scales, v_scales)
 
-    def attention(self, q: Tensor, layer: int, block_size: int, out: Tensor | None = None) -> Tensor:
-        """paged_attention over this layer's pages."""
+    def update_bounds(self, layer: int) -> None:
+        """page_bounds of the pages that hold this step's tokens: after the attention_inputs
+        whose tokens are committed, and before an attention over selected pages
+        if the step has more than one block of a sequence. (The pages of a query's own block are
+        taken whatever their bounds.)"""
         c = self.cache
-        return paged_attention(q, c.k_pages[layer], c.v_pages[layer], self.page_table, self.q_starts, self.kv_lens,
-                               block_size, self.max_q, self.max_kv, self.total_kv, out)
+        assert c.bounds is not None, "the cache keeps no bounds: PagedKVCache(..., bounds=True)"
+        page_bounds(c.k_pages[layer], c.bounds[layer], self.page_table, self.q_starts, self.kv_lens, self.tokens,
+                    c.scales(layer)[0])
+
+    def attention(self, q: Tensor, layer: int, block_size: int, out: Tensor | None = None, top: int | None = None,
+                  first: int = 1, recent: int = 1) -> Tensor:
+        """paged_attention over this layer's pages; with `top` over those that select_pages
+        takes by the cache's bounds."""
+        c = self.cache
+        columns = None
+        if top is not None:
+            assert c.bounds is not None, "the cache keeps no bounds: PagedKVCache(..., bounds=True)"
+            columns = select_pages(q, c.bounds[layer], self.page_table, self.q_starts, self.kv_lens, block_size,
+                                   c.page_size, top, self.max_q, self.max_kv, first, recent)
+        return paged_attention_pool(q, c.k_pages[layer], c.v_pages[layer], self.page_table, self.q_starts, self.kv_lens,
+                                    block_size, self.max_q, self.max_kv, self.total_kv, out, *c.scales(layer), columns)
 
     def commit(self) -> None:
         """Count the step's tokens as committed, in every layer. Once a batch,

@@ -293,10 +293,11 @@ def generate(cfg, p, tables, batch, n_blocks, steps, backend, check=None, graph=
 # serving: sequences of different lengths in one batch, their cache in pages
 
 
-def backbone_paged(cfg, p, tables, tokens, batch, ada):
+def backbone_paged(cfg, p, tables, tokens, batch, ada, top=None, final=False):
     """Logits (tokens, vocab) of a ragged batch's packed tokens (kernels.paged.
     PagedBatch); their keys and values go to the batch's pages. `ada`:
-    ada_params for one sequence (the conditioning is the same for all)."""
+    ada_params for one sequence (the conditioning is the same for all). `top`: the pages that a
+    block's attention reads for a head; `final`: the tokens are those to be committed."""
     from kernels.dit_glue import gate_residual_ln_modulate, ln_modulate
     T = tokens.shape[0]
     ada_layers, ada_final = ada
@@ -306,7 +307,9 @@ def backbone_paged(cfg, p, tables, tokens, batch, ada):
     for li, L in enumerate(layers):
         _, _, g1, sh2, sc2, g2 = ada_layers[li]
         q = batch.attention_inputs(linear(h[0], L["qkv"]), cfg.heads, *tables, li)
-        o = batch.attention(q, li, cfg.bs).view(1, T, cfg.d)
+        if top is not None and final:
+            batch.update_bounds(li)
+        o = batch.attention(q, li, cfg.bs, top=top).view(1, T, cfg.d)
         x, h = gate_residual_ln_modulate(x, g1, linear(o, L["out"]), L["ln2"], sh2, sc2, cfg.eps)
         y = linear(F.gelu(linear(h, L["fc1"]), approximate="tanh"), L["fc2"])
         if li + 1 < len(layers):
@@ -318,7 +321,7 @@ def backbone_paged(cfg, p, tables, tokens, batch, ada):
 
 
 def serve(cfg, p, tables, prompts, n_blocks, steps, n_pages, page_size=64, repetition=1.0, allowed=None, seed=0,
-          check=None):
+          check=None, cache_dtype=torch.bfloat16, top=None):
     """Continue each prompt (1-D token tensors of whole blocks) by n_blocks[i]
     blocks, as many sequences at a time as the pool of n_pages holds: a waiting
     one joins as soon as the pages it will need are free. Every round runs one
@@ -326,11 +329,13 @@ def serve(cfg, p, tables, prompts, n_blocks, steps, n_pages, page_size=64, repet
     all live sequences, with a repetition penalty over what each holds so far
     and a mask of allowed tokens, and the pass that commits the block. `check`:
     optional callback(tokens before the block, block, logits) of each sequence's
-    first step. Returns the sequences' tokens."""
+    first step. `cache_dtype`: what the pages hold (bf16, int8 or float8_e4m3fn); `top`: pages that a block's
+    attention reads for a head, chosen by their keys' bounds (None: all). Returns the sequences' tokens."""
     from kernels.paged import PagedKVCache
     from kernels.sampling import PhiloxStream, adjust_logits, subs_sample_step
     device = p["emb"].device
-    cache = PagedKVCache(cfg.layers, n_pages, cfg.heads, page_size, device=device)
+    cache = PagedKVCache(cfg.layers, n_pages, cfg.heads, page_size, device=device, dtype=cache_dtype,
+                         bounds=top is not None)
     gen = PhiloxStream(seed=seed)
     ada = ada_params(cfg, p, 1, device)
     assert all(len(t) % cfg.bs == 0 for t in prompts), "prompts must be whole blocks"
@@ -348,7 +353,7 @@ def serve(cfg, p, tables, prompts, n_blocks, steps, n_pages, page_size=64, repet
                 joined.append(i)
         if joined:
             batch = cache.batch([live[i][0] for i in joined], [len(out[i]) for i in joined])
-            backbone_paged(cfg, p, tables, torch.cat([out[i] for i in joined]), batch, ada)
+            backbone_paged(cfg, p, tables, torch.cat([out[i] for i in joined]), batch, ada, top, True)
             batch.commit()
         for i in [i for i, (_, left) in live.items() if left == 0]:
             cache.free(live.pop(i)[0])
@@ -362,13 +367,13 @@ def serve(cfg, p, tables, prompts, n_blocks, steps, n_pages, page_size=64, repet
         block = torch.full((len(ids), cfg.bs), cfg.mask, device=device, dtype=torch.long)
         for step in range(steps):
             t, s = 1 - step / steps, 1 - (step + 1) / steps
-            logits = backbone_paged(cfg, p, tables, block.flatten(), batch, ada).view(len(ids), cfg.bs, -1)
+            logits = backbone_paged(cfg, p, tables, block.flatten(), batch, ada, top).view(len(ids), cfg.bs, -1)
             if check is not None and step == 0:
                 for k, i in enumerate(ids):
                     check(out[i], block[k], logits[k])
             logits = adjust_logits(logits, history, lengths, repetition=repetition, allowed=allowed)
             block = subs_sample_step(logits, block, cfg.mask, s / t, generator=gen)
-        backbone_paged(cfg, p, tables, block.flatten(), batch, ada)
+        backbone_paged(cfg, p, tables, block.flatten(), batch, ada, top, True)
         batch.commit()
         for i, new in zip(ids, block):
             out[i] = torch.cat([out[i], new])

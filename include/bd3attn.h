@@ -389,6 +389,108 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
                        const int64_t* strides, void* stream);
 
 /*
+ * Pools held in 8 bits, and attention over the pages of a list. pool_type: what the
+ * pages hold. With BD3_POOL_INT8 or BD3_POOL_E4M3 (OCP e4m3, finite codes) an
+ * element is a code, and each 16 slots (16 i .. 16 i + 15 of a page) of a KV head share
+ * an fp32 scale, value = scale * code: k_scales, v_scales (pages, kv_heads, page_size /
+ * 16), contiguous; those of blocks that hold keys must be finite and at least 2^-100. Strides of such
+ * pages are multiples of 16. BD3_POOL_BF16: the pools of bd3_paged_attn, scales NULL.
+ */
+#define BD3_POOL_BF16 0
+#define BD3_POOL_INT8 1
+#define BD3_POOL_E4M3 2
+
+/*
+ * bd3_paged_attn over any kind of pool; scales multiply scores and probabilities in
+ * fp32, codes are exact operands, so a result is as near to the pool's values as
+ * bd3_paged_attn's to its bf16 ones.
+ *   columns: NULL, or device int32 (tokens, kv_heads, top), last stride 1: lists of
+ *     columns of the page table. The tokens of one block of block_size positions read, for
+ *     the heads of KV head h, only the keys in columns[first token of the block
+ *     in its chunk][h][...], as far as they see them. No column may occur twice, so of
+ *     a list only as many entries are read as the sequence has columns with keys; entries
+ *     outside those that the block sees (-1) name nothing.
+ *   strides: bd3_paged_attn's 11, then columns (token, KV head).
+ * The workspace is bd3_paged_attn_pool_workspace_bytes of the same arguments (top 0: no
+ * columns). Everything else as for bd3_paged_attn. No reference counterpart.
+ */
+size_t bd3_paged_attn_pool_workspace_bytes(int32_t pool_type, int32_t seqs, int32_t tokens, int32_t heads,
+                                           int32_t kv_heads, int32_t page_size, int32_t max_q, int32_t max_kv,
+                                           int64_t total_kv, int32_t block_size, int32_t top);
+int bd3_paged_attn_pool(const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
+                        const float* v_scales, int32_t pool_type, void* o, const int32_t* page_table,
+                        const int32_t* q_starts, const int32_t* kv_lens, const int32_t* columns, int32_t top,
+                        int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                        int32_t pages, int32_t page_size, int32_t table_width, int32_t max_q, int32_t max_kv,
+                        int64_t total_kv, int32_t block_size, const int64_t* strides, float scale,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * bd3_paged_qkv_rope into a pool of 8-bit codes; scales are written with them. A block of
+ * 16 slots whose first token is of this call gets the scale that its new values need:
+ * max|x| / 127 (int8) or the least power of two with 448 scale >= max|x| (e4m3), at least
+ * 2^-100. In a block that holds earlier tokens of the sequence the scale stays, or grows
+ * by the least power of two 2^k with which the new values fit; then the block's
+ * other codes become round(code / 2^k). code = round(x / scale), ties to even, x the fp32
+ * rotated key or the value. Values must be finite (an infinite one counts as the largest
+ * finite one). Blocks are written whole, so no two sequences of a call may write into
+ * one. Strides of the pages are multiples of 16.
+ */
+int bd3_paged_qkv_rope8(const void* qkv, const float* sin_table, const float* cos_table,
+                        int32_t max_pos, void* q_out, void* k_pages, void* v_pages, float* k_scales,
+                        float* v_scales, int32_t pool_type, const int32_t* page_table,
+                        const int32_t* q_starts, const int32_t* kv_lens, int32_t seqs, int32_t tokens,
+                        int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                        int32_t page_size, int32_t table_width, const int64_t* strides, void* stream);
+
+/*
+ * The values of two 8-bit pools as bf16 (rounded once): k_out, v_out (pages, kv_heads,
+ * page_size, 64), contiguous. strides: k_pages (page, head, slot), v_pages (page, head,
+ * slot). The results overlap neither each other nor an input.
+ */
+int bd3_page_values(const void* k_pages, const void* v_pages, const float* k_scales,
+                    const float* v_scales, int32_t pool_type, void* k_out, void* v_out, int32_t pages,
+                    int32_t kv_heads, int32_t page_size, int32_t head_dim, const int64_t* strides,
+                    void* stream);
+
+/*
+ * The bounds of the pages that hold tokens of the batch's chunks, over the keys that the
+ * sequence has in them: bounds (pages, kv_heads, 2, 64) bf16, contiguous, the lowest and
+ * the highest key of each channel (values of 8-bit pools rounded to bf16). Other pages'
+ * bounds stay. Batch and pool as for bd3_paged_attn_pool (K pages only).
+ *   strides: k_pages (page, head, slot), page_table (row).
+ */
+int bd3_page_bounds(const void* k_pages, const float* k_scales, int32_t pool_type, void* bounds,
+                    const int32_t* page_table, const int32_t* q_starts, const int32_t* kv_lens,
+                    int32_t seqs, int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                    int32_t page_size, int32_t table_width, const int64_t* strides, void* stream);
+
+/*
+ * The pages that the attention of a batch is to read, as lists for bd3_paged_attn_pool:
+ * out (tokens, kv_heads, top) int32, contiguous. The tokens of one block of
+ * block_size positions get the same list for a KV head: of the columns that hold keys they see
+ * and whose entry is a page, the first `first` ones, those from the column of the
+ * block's first position less `recent` on, and of the others those of the largest
+ *   max over the block's tokens in the chunk and the KV head's query heads of
+ *   sum_d (q_d > 0 ? q_d * highest_d : q_d * lowest_d)
+ * (exactly: equals by the lower column), `top` in all, ascending, then -1. Rows of out
+ * behind the last sequence, and of tokens beyond max_q, stay as they are; a token before
+ * position 0 gets none.
+ *   q: (tokens, heads, 64) bf16; bounds: (pages, kv_heads, 2, 64) bf16, contiguous, as
+ *     bd3_page_bounds writes them; finite. strides: q (token, head), page_table (row).
+ * Preconditions: top >= first + recent + the most columns that a block can lie in
+ * (within max_kv). workspace: bd3_select_pages_workspace_bytes of the same arguments.
+ */
+size_t bd3_select_pages_workspace_bytes(int32_t seqs, int32_t tokens, int32_t kv_heads, int32_t page_size,
+                                        int32_t max_kv, int32_t block_size);
+int bd3_select_pages(const void* q, const void* bounds, const int32_t* page_table,
+                     const int32_t* q_starts, const int32_t* kv_lens, int32_t* out, int32_t seqs,
+                     int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                     int32_t page_size, int32_t table_width, int32_t max_q, int32_t max_kv,
+                     int32_t block_size, int32_t top, int32_t first, int32_t recent,
+                     const int64_t* strides, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Penalties for repeated tokens, biases and a grammar mask on logits before the
  * draw. For logit x of token v in a row of sequence b, with c the count of v
  * among tokens[b][0 .. lengths[b]):
