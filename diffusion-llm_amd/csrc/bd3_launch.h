@@ -186,7 +186,7 @@ struct PagedArgs {
   int max_q;      // most tokens of a chunk: the caller's bound
   int max_kv;     // most keys of a sequence: the caller's bound, at most the table's
   int bs;
-  FastDiv bs_div, group_div, kv_heads_div;
+  FastDiv bs_div, group_div, kv_heads_div, tile_div;
   int tile;       // query rows per workgroup
   int subs;       // sets of 4 waves per workgroup: 1, 2 or (128-row tiles) 4
   int q_tiles;    // tiles of the longest chunk
@@ -230,6 +230,9 @@ struct PageValuesArgs {
   int64_t total;             // blocks of 16 rows of one of the two
 };
 
+constexpr int kPickColumns = 2048;  // most that one workgroup scores and chooses from
+// Whether a selection goes through a workspace: scored first, then chosen from.
+inline bool select_in_two(int64_t items, int64_t width) { return width > kPickColumns || (items < 128 && width > 256); }
 struct SelectArgs {
   PagedArgs p;               // batch, pool (bounds) and queries (selection)
   uint16_t* bounds;          // (pages, kv_heads, 2, 64): lowest and highest key
@@ -237,6 +240,7 @@ struct SelectArgs {
   int slots;                 // most pages that the chunks touch (bounds), most blocks of the chunks (selection)
   int width;                 // columns within max_kv
   int first, recent;         // columns always taken
+  // Where select_in_two:
   float* scores;             // (slots, kv_heads, width)
   float* error;              // (slots, kv_heads, ceil(width / 16)): bound of the scores' distance from the exact sums
   double* sums;              // (slots, kv_heads, width)

@@ -924,20 +924,34 @@ static_assert(kPagedPartRows * bd3::kHeadDim <= INT32_MAX, "32-bit indices of th
 // sequences of 12 heads over 6004 keys 92, 76). Fitted to batches drawn over 1-64
 // sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV heads and groups of 1-12;
 // over 1500 others the rms error is 9% for up to 16 rows, 12% for 17-256, 10% for more.
-double paged_us(int tile, int subs, double longest, double keys, double items, double busiest, bool split, bool even) {
-  struct Cost {
-    double chain0, chain, load0, load, item, merge, merge_item;
-  };
-  static constexpr Cost kRows16 = {5.7, 0.32, 0.0, 0.64, 1.6, 3.1, 0.0};  // two sets
-  static constexpr Cost kRows32[2] = {{5.7, 0.62, 1.1, 0.54, 1.7, 3.1, 0.37}, {5.9, 0.33, 0.5, 0.52, 4.7, 3.6, 0.0}};
-  static constexpr Cost kRows128[3] = {{4.6, 1.0, 5.2, 0.68, 1.4, 3.2, 1.7},
-                                       {5.5, 0.66, 4.8, 0.70, 2.9, 3.2, 1.9},
-                                       {8.0, 0.52, 0.0, 0.69, 9.5, 0.0, 0.0}};  // four sets: never with ranges
-  const Cost& c = tile == 16 ? kRows16 : tile == 32 ? kRows32[subs - 1] : kRows128[subs >> 1];
-  const double chain =
-      c.chain0 + std::max(c.chain * longest, tile == 16 && even ? 0.36 * busiest : 0.0) / 64.0;
+//
+// 8-bit pools and lists have their own, fitted to 520 batches of 8-bit pools drawn the same way: rms error 9-10%; the plan
+// takes 1.2% more than the best of all plans on average for up to 16 rows, 1.8% for more (at worst 24%). Over 200
+// batches of lists 3% (bf16 pools 2%), at worst 67%.
+struct PagedCost {
+  double chain0, chain, busy, load0, load, item, merge, merge_item, e_even, e;
+};
+const PagedCost& paged_cost(bool codes, int tile, int subs) {
+  static constexpr PagedCost kRows16 = {5.7, 0.32, 0.36, 0.0, 0.64, 1.6, 3.1, 0.0, 3.0, 1.5};  // two sets
+  static constexpr PagedCost kRows32[2] = {{5.7, 0.62, 0.0, 1.1, 0.54, 1.7, 3.1, 0.37, 3.0, 1.5},
+                                           {5.9, 0.33, 0.0, 0.5, 0.52, 4.7, 3.6, 0.0, 3.0, 1.5}};
+  static constexpr PagedCost kRows128[3] = {{4.6, 1.0, 0.0, 5.2, 0.68, 1.4, 3.2, 1.7, 3.0, 3.0},
+                                            {5.5, 0.66, 0.0, 4.8, 0.70, 2.9, 3.2, 1.9, 3.0, 3.0},
+                                            {8.0, 0.52, 0.0, 0.0, 0.69, 9.5, 0.0, 0.0, 3.0, 3.0}};  // four sets: never with ranges
+  static constexpr PagedCost kCodes16[2] = {{0.0, 0.59, 0.25, 5.74, 0.235, 0.29, 2.7, 0.79, 1.27, 1.06},
+                                            {5.7, 0.34, 0.35, 0.0, 0.228, 1.28, 2.4, 1.16, 1.71, 1.0}};
+  static constexpr PagedCost kCodes32[2] = {{5.8, 0.58, 0.22, 5.65, 0.438, 2.75, 2.4, 0.14, 2.92, 2.4},
+                                            {6.8, 0.43, 0.28, 4.8, 0.529, 5.2, 2.75, 0.0, 5.0, 3.9}};
+  static constexpr PagedCost kCodes48 = {6.8, 0.64, 0.57, 7.2, 0.523, 3.27, 2.4, 0.19, 3.64, 2.58};
+  static constexpr PagedCost kCodes128[2] = {{5.16, 1.264, 0.106, 2.2, 0.504, 2.86, 1.3, 1.87, 1.21, 1.21},
+                                             {5.68, 0.897, 0.012, 4.7, 0.683, 4.93, 1.8, 1.37, 1.83, 1.83}};
+  if (codes) return tile == 16 ? kCodes16[subs - 1] : tile == 32 ? kCodes32[subs - 1] : tile == 48 ? kCodes48 : kCodes128[subs - 1];
+  return tile == 16 ? kRows16 : tile == 32 ? kRows32[subs - 1] : kRows128[subs >> 1];
+}
+double paged_us(const PagedCost& c, double longest, double keys, double items, double busiest, bool split, bool even) {
+  const double chain = c.chain0 + std::max(c.chain * longest, even ? c.busy * busiest : 0.0) / 64.0;
   const double load = c.load0 + c.load * keys / (64.0 * 256.0) + c.item * items / 256.0;
-  const double e = even || tile == 128 ? 3.0 : 1.5;
+  const double e = even ? c.e_even : c.e;
   return std::pow(std::pow(chain, e) + std::pow(load, e), 1.0 / e) +
          (split ? c.merge + c.merge_item * items / 256.0 : 0.0);
 }
@@ -968,9 +982,10 @@ PagedPlan paged_plan(int pool_type, int32_t seqs, int32_t tokens, int32_t heads,
   PagedPlan p = {};
   p.split_shift = 30;
   double best = INFINITY;
-  for (int tile : {16, 32, 128}) {
-    if (tile == 16 ? rows > 16 : rows <= 16 || (tile == 32 && rows > 256 && pool_type == BD3_POOL_BF16)) continue;
-    if (tile == 128 && pool_type != BD3_POOL_BF16) continue;
+  const bool codes = pool_type != BD3_POOL_BF16;
+  for (int tile : {16, 32, 48, 128}) {
+    if (tile == 16 ? rows > 16 : rows <= 16 || (tile < 128 && rows > (codes ? 400 : 256))) continue;
+    if (codes ? tile > 32 && rows <= 32 : tile == 48) continue;
     const int q_tiles = (int)((rows + tile - 1) / tile);
     // items without ranges: not every chunk is as long as the longest
     const double units = kv_heads * std::max(1.0, std::min((double)seqs * q_tiles,
@@ -994,13 +1009,18 @@ PagedPlan paged_plan(int pool_type, int32_t seqs, int32_t tokens, int32_t heads,
       p.split_shift = shift;
     };
     if (!fits(1)) continue;
-    for (int subs = tile == 16 ? 2 : 1; subs <= (tile == 128 ? 4 : 2); subs *= 2) {
-      take(paged_us(tile, subs, max_kv, units * seen, units, busiest(1), false, even), subs, 30);
+    const int most = codes ? (tile == 48 ? 1 : 2) : (tile == 128 ? 4 : 2);
+    for (int subs = tile == 16 && !codes ? 2 : 1; subs <= most; subs *= 2) {
+      const PagedCost& c = paged_cost(codes, tile, subs);
+      take(paged_us(c, max_kv, units * seen, units, busiest(1), false, even), subs, 30);
+      // Prompts of 8-bit pools that fill the chip are not cut: their longest tiles go first, which the estimate does
+      // not know (4 of 1500-4096 tokens, 12 heads: 78 us whole, 109 cut).
+      if (codes && tile == 128 && units >= 256.0 && total < 3.0 * tokens) continue;
       for (int shift = 8; subs < 4 && 3 * ((int64_t)1 << shift) <= 2 * (int64_t)max_kv; ++shift) {
         const int ranges = paged_ranges(max_kv, shift);
         if (ranges > 64 || part_rows * ranges > kPagedPartRows || !fits(ranges)) continue;
         const double len = (double)((int64_t)1 << shift), items = std::max(units, units * (seen / len + 0.3));
-        take(paged_us(tile, subs, std::min((double)max_kv, 1.25 * len), units * seen, items,
+        take(paged_us(c, std::min((double)max_kv, 1.25 * len), units * seen, items,
                       busiest(std::max(1.0, std::floor(max_kv / len + 0.5))), true, even),
              subs, shift);
       }
@@ -1018,35 +1038,45 @@ int32_t listed_keys(int32_t page_size, int32_t max_kv, int32_t top) {
   return (int32_t)std::min((int64_t)top * page_size, ((int64_t)max_kv + page_size - 1) / page_size * page_size);
 }
 
-// The plan over lists: tiles hold the rows of one block; ranges as above.
-PagedPlan columns_plan(int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t page_size, int32_t max_q,
-                       int32_t max_kv, int32_t block_size, int32_t top, int32_t* block_tiles) {
+// The plan over lists: tiles hold the rows of one block; ranges as above. The costs of 8-bit pools order the
+// bf16 ones' plans as well.
+PagedPlan columns_plan(int pool_type, int32_t seqs, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t page_size,
+                       int32_t max_q, int32_t max_kv, int32_t block_size, int32_t top, int32_t* block_tiles) {
   const int64_t group = heads / kv_heads, rows = std::min(block_size, max_q) * group;
   const int32_t keys = listed_keys(page_size, max_kv, top);
+  const int64_t blocks = chunk_blocks(seqs, tokens, block_size);
+  const double likely = std::max(1.0, std::min((double)blocks, (double)tokens / block_size + 0.5 * seqs));
+  const int64_t part_rows = std::min((int64_t)tokens * heads, kPagedPartRows + 1);
   PagedPlan p = {};
   p.split_shift = 30;
-  const int tile = rows <= 16 ? 16 : 32;
-  *block_tiles = (int32_t)((rows + tile - 1) / tile);
-  const int64_t tiles = chunk_blocks(seqs, tokens, block_size) * *block_tiles;
-  const double units = (double)kv_heads * *block_tiles * std::max(1.0, std::min((double)tiles, (double)tokens / block_size + 0.5 * seqs));
-  const int64_t part_rows = std::min((int64_t)tokens * heads, kPagedPartRows + 1);
-  if (tiles >= kPagedItems || tiles * kv_heads >= kPagedItems) return p;
+  *block_tiles = 0;
   double best = INFINITY;
-  for (int subs = tile == 16 ? 2 : 1; subs <= 2; subs *= 2) {
-    const auto take = [&](double us, int shift) {
+  for (int tile : {16, 32, 48}) {
+    if (tile == 16 ? rows > 16 : rows <= 16 || (tile == 48 && (rows <= 32 || pool_type == BD3_POOL_BF16))) continue;
+    const int64_t per_block = (rows + tile - 1) / tile;
+    if (blocks * per_block >= kPagedItems || blocks * per_block * kv_heads >= kPagedItems) continue;
+    const int64_t tiles = blocks * per_block;
+    const double units = (double)kv_heads * per_block * likely;
+    const auto busiest = [&](double ranges) { return std::ceil(units * ranges / 256.0) * keys / ranges; };
+    const auto take = [&](double us, int subs, int shift) {
       if (!(us < best)) return;
       best = us;
       p.tile = tile;
       p.tiles = tiles;
       p.subs = subs;
       p.split_shift = shift;
+      *block_tiles = (int32_t)per_block;
     };
-    const auto busiest = [&](double ranges) { return std::ceil(units * ranges / 256.0) * keys / ranges; };
-    take(paged_us(tile, subs, keys, units * keys, units, busiest(1), false, true), 30);
-    for (int shift = 8; 3 * ((int64_t)1 << shift) <= 2 * (int64_t)keys; ++shift) {
-      const int ranges = paged_ranges(keys, shift);
-      if (ranges > 64 || part_rows * ranges > kPagedPartRows || tiles * ranges * kv_heads >= kPagedItems) continue;
-      take(paged_us(tile, subs, 1.25 * (1 << shift), units * keys, units * ranges, busiest(ranges), true, true), shift);
+    // bf16 pools have one kernel of 16 rows, for two sets
+    for (int subs = tile == 16 && pool_type == BD3_POOL_BF16 ? 2 : 1; subs <= (tile == 48 ? 1 : 2); subs *= 2) {
+      const PagedCost& c = paged_cost(true, tile, subs);
+      take(paged_us(c, keys, units * keys, units, busiest(1), false, true), subs, 30);
+      for (int shift = 8; 3 * ((int64_t)1 << shift) <= 2 * (int64_t)keys; ++shift) {
+        const int ranges = paged_ranges(keys, shift);
+        if (ranges > 64 || part_rows * ranges > kPagedPartRows || tiles * ranges * kv_heads >= kPagedItems) continue;
+        take(paged_us(c, std::min((double)keys, 1.25 * (1 << shift)), units * keys, units * ranges, busiest(ranges), true, true),
+             subs, shift);
+      }
     }
   }
   p.n_splits = paged_ranges(keys, p.split_shift);
@@ -1077,7 +1107,7 @@ size_t bd3_paged_attn_pool_workspace_bytes(int32_t pool_type, int32_t seqs, int3
   max_kv = std::max(max_kv, 1);
   total_kv = std::min(total_kv, (int64_t)seqs * max_kv);
   int32_t block_tiles;
-  const PagedPlan plan = top > 0 ? columns_plan(seqs, tokens, heads, kv_heads, page_size, max_q, max_kv,
+  const PagedPlan plan = top > 0 ? columns_plan(pool_type, seqs, tokens, heads, kv_heads, page_size, max_q, max_kv,
                                                 std::min(block_size, bd3::kPagedMaxKeys), top, &block_tiles)
                                  : paged_plan(pool_type, seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
   const size_t rows = paged_part_rows(plan, tokens, heads);
@@ -1114,7 +1144,7 @@ int bd3_paged_attn_pool(const void* q, const void* k_pages, const void* v_pages,
     return fail(BD3_EINVAL, "max_q * heads / kv_heads too large (limit 2^29 rows a chunk)");
   block_size = std::min(block_size, bd3::kPagedMaxKeys);  // as good as any larger one
   int32_t block_tiles = 0;
-  const PagedPlan plan = columns != nullptr ? columns_plan(seqs, tokens, heads, kv_heads, page_size, max_q, max_kv,
+  const PagedPlan plan = columns != nullptr ? columns_plan(pool_type, seqs, tokens, heads, kv_heads, page_size, max_q, max_kv,
                                                            block_size, top, &block_tiles)
                                             : paged_plan(pool_type, seqs, tokens, heads, kv_heads, max_q, max_kv, total_kv);
   if (plan.tile == 0)
@@ -1189,6 +1219,7 @@ int bd3_paged_attn_pool(const void* q, const void* k_pages, const void* v_pages,
   a.bs_div = bd3::FastDiv::of(a.bs);
   a.group_div = bd3::FastDiv::of(a.group);
   a.kv_heads_div = bd3::FastDiv::of(kv_heads);
+  a.tile_div = bd3::FastDiv::of(plan.tile);
   if (plan.tile == 128) {  // the most tiles and ranges that the chunks can have
     a.workgroups = (int)(plan.tiles * plan.n_splits * kv_heads);
     const int unit = std::max(1, 128 / a.group);  // tokens of a tile
@@ -1381,7 +1412,7 @@ size_t bd3_select_pages_workspace_bytes(int32_t seqs, int32_t tokens, int32_t kv
   if (seqs < 1 || tokens < 1 || kv_heads < 1 || page_size < 16 || max_kv < 1 || max_kv > bd3::kPagedMaxKeys || block_size < 1)
     return 0;
   const int64_t items = chunk_blocks(seqs, tokens, block_size) * kv_heads, width = select_width(page_size, max_kv);
-  if (items >= kPagedItems || items * width >= ((int64_t)1 << 40)) return 0;
+  if (!bd3::select_in_two(items, width) || items >= kPagedItems || items * width >= ((int64_t)1 << 40)) return 0;
   return (size_t)(items * width) * 12 + (size_t)(items * (width / 16)) * 4;
 }
 
@@ -1419,11 +1450,11 @@ int bd3_select_pages(const void* q, const void* bounds, const int32_t* page_tabl
     return fail(BD3_EINVAL, "out must be a 4-byte aligned device pointer");
   const int64_t slots = chunk_blocks(seqs, tokens, block_size), items = slots * kv_heads;
   const int64_t width = select_width(page_size, max_kv);
-  if (items >= kPagedItems || items * ((width + 63) / 64) > kMaxWorkgroups)
-    return fail(BD3_EINVAL, "batch too large (limit 2^24 workgroups of 64 columns of a block and KV head)");
+  if (2 * items > kMaxWorkgroups || (bd3::select_in_two(items, width) && items * ((width + 63) / 64) > kMaxWorkgroups))
+    return fail(BD3_EINVAL, "batch too large (limit 2^23 blocks and KV heads, 2^24 times 64 columns of long tables)");
   const size_t need = bd3_select_pages_workspace_bytes(seqs, tokens, kv_heads, page_size, max_kv, block_size);
   if (workspace_bytes < need) return fail(BD3_EINVAL, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
-  if (workspace == nullptr || !aligned16(workspace))
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace)))
     return fail(BD3_EINVAL, "workspace must be a 16-byte aligned device pointer");
   bd3::SelectArgs a = {};
   a.p.q = static_cast<const uint16_t*>(q);
@@ -1453,9 +1484,11 @@ int bd3_select_pages(const void* q, const void* bounds, const int32_t* page_tabl
   a.width = (int)width;
   a.first = first;
   a.recent = recent;
-  a.sums = static_cast<double*>(workspace);
-  a.scores = reinterpret_cast<float*>(a.sums + items * width);
-  a.error = a.scores + items * width;
+  if (need > 0) {
+    a.sums = static_cast<double*>(workspace);
+    a.scores = reinterpret_cast<float*>(a.sums + items * width);
+    a.error = a.scores + items * width;
+  }
   return hip_status(bd3::launch_select_pages(a, static_cast<hipStream_t>(stream)), "select_pages launch");
 }
 

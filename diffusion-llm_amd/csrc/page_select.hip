@@ -10,12 +10,10 @@
 // the block sees, `top` of them, the first ones and those around the block's own
 // tokens always, equals by the lowest column.
 //
-// The order is that of the exact scores: bf16 products are exact in fp32, and their
-// fp32 sum is off by at most 128 * 2^-23 sum |q_d b_d| <= 2^-16 |q|_1 max |b|, whatever
-// the matrix cores' order and rounding (a bound, four times a rounding to nearest's
-// for 128 terms). Where the border between taken and left pages is nearer
-// than that, the scores in doubt are summed again in 64 bits, where bf16 products of any
-// but extreme ratios add without a rounding.
+// The order is that of the exact scores: bf16 products are exact in fp32, and their fp32
+// sum is off by at most 2^-17 sum |q_d b_d| whatever the matrix cores' order and rounding.
+// Where the border between taken and left pages is nearer than that, the scores in doubt are
+// summed again in 64 bits, where bf16 products of any but extreme ratios add without a rounding.
 #include "paged_seq.h"
 
 namespace bd3 {
@@ -120,75 +118,79 @@ __device__ __forceinline__ bf16x8 negative(u32x4 x) {
   return __builtin_bit_cast(bf16x8, __builtin_elementwise_min(v, (i16x8)(short)0));
 }
 
-// Scores of 16 columns a wave: S^T (16 columns x 16 rows) = bounds . [q+ q-]^T, the largest
-// of each column over the rows, and the bound of their error.
-__global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs s, int chunks) {
-  const PagedArgs& a = s.p;
-  const int lane = wi_x() & 63, l16 = lane & 15, hq = lane >> 4;
-  const int wave = wave_uniform(wi_x() >> 6);
-  const int jh = wg_x() / chunks;
-  const int col0 = 16 * (4 * (wg_x() - jh * chunks) + wave);
-  const int j = fast_div(jh, a.kv_heads_div);
-  const int h = jh - j * a.kv_heads;
-  const SeqPiece<PagedSeq> it(
-      a.seqs, j, [&](int b) { return PagedSeq(a, b); }, [&](const PagedSeq& q) { return q.blocks(a); });
-  if (!it.found) return;
-  const QueryBlock blk(a, it.sq, it.at);
-  if (col0 >= blk.cols) return;
+// Scores of 16 columns: S (16 rows x 16 columns) = [q+ q-] . bounds^T on v_mfma_f32_16x16x32_bf16, the largest of
+// each column over the rows, and the same product of the absolute values. Lane (l16, hq): a row's and a column's
+// channels; then, in all four quarters, column l16. The first 16 rows stay in registers. (With the columns as rows of the
+// product the maximum took 32 more instructions, and a call on one token over 1000 pages 2 us.)
+struct ColumnScores {
+  int h, rows, row0;      // the block's rows, the first one's place in the chunk
+  const uint16_t* q;      // the chunk's first token, the KV head's first query head
+  const uint16_t* bounds;  // the KV head's of page 0
+  int64_t sq_t, sq_h, page_step;
+  int pages, group;
+  FastDiv group_div;
+  int lane;
+  u32x4 q0, q1;           // of row l16, channels 8 hq .. + 7 and 32 + 8 hq .. + 7
+  struct Box {
+    bf16x8 x[4];          // high, low: the same channels
+  };
+  float most;             // largest sum of absolute values so far (of the lane's columns)
 
-  const int col = col0 + l16 < blk.cols ? col0 + l16 : blk.cols - 1;
-  int page = a.table[(int64_t)it.b * a.table_s + col];
-  page = (unsigned)page < (unsigned)a.pages ? page : 0;  // no page: left out by the selection
-  const uint16_t* bp = s.bounds + ((int64_t)page * a.kv_heads + h) * (2 * kHeadDim) + 8 * hq;
-  bf16x8 box[4];  // high, low: channels 32 c + 8 hq .. +7
-#pragma unroll
-  for (int c = 0; c < 4; ++c) box[c] = __builtin_bit_cast(bf16x8, ld16(bp + (c < 2 ? kHeadDim : 0) + 32 * (c & 1)));
-  float bmax = 0.f;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bmax = fmaxf(bmax, fabsf((float)box[c][i]));
-
-  f32x4 best = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  float q1 = 0.f;
-  const int rows = (blk.hi - blk.lo) * a.group;
-  for (int r0 = 0; r0 < rows; r0 += 16) {
-    const int row = blk.lo * a.group + (r0 + l16 < rows ? r0 + l16 : rows - 1);
-    const int tok = fast_div(row, a.group_div);
-    const uint16_t* qp =
-        a.q + (int64_t)(it.sq.q0 + tok) * a.sq_t + (int64_t)(h * a.group + row - tok * a.group) * a.sq_h + 8 * hq;
-    const u32x4 x0 = ld16(qp), x1 = ld16(qp + 32);
-    f32x4 acc = mfma16(box[0], positive(x0), f32x4{});
-    acc = mfma16(box[1], positive(x1), acc);
-    acc = mfma16(box[2], negative(x0), acc);
-    acc = mfma16(box[3], negative(x1), acc);
-    const bf16x8 b0 = __builtin_bit_cast(bf16x8, x0), b1 = __builtin_bit_cast(bf16x8, x1);
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += fabsf((float)b0[i]) + fabsf((float)b1[i]);
-    q1 = fmaxf(q1, sum);  // of this lane's channels: the four lanes of a row add up to at least its norm
-#pragma unroll
-    for (int r = 0; r < 4; ++r) best[r] = fmaxf(best[r], acc[r]);
+  __device__ __forceinline__ ColumnScores(const SelectArgs& s, const PagedSeq& sq, const QueryBlock& blk, int h_)
+      : h(h_), rows((blk.hi - blk.lo) * s.p.group), row0(blk.lo * s.p.group),
+        q(s.p.q + (int64_t)sq.q0 * s.p.sq_t + (int64_t)(h_ * s.p.group) * s.p.sq_h),
+        bounds(s.bounds + (int64_t)h_ * (2 * kHeadDim)), sq_t(s.p.sq_t), sq_h(s.p.sq_h),
+        page_step((int64_t)s.p.kv_heads * (2 * kHeadDim)), pages(s.p.pages), group(s.p.group), group_div(s.p.group_div),
+        lane(wi_x() & 63), most(0.f) {
+    const uint16_t* qp = row(0);
+    q0 = ld16(qp);
+    q1 = ld16(qp + 32);
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {  // over the 16 rows: lanes of one quarter
-    float v = best[r];
-    v = fmaxf(v, dpp_move<0xB1>(v));
-    v = fmaxf(v, dpp_move<0x4E>(v));
-    v = fmaxf(v, dpp_move<0x141>(v));
-    best[r] = fmaxf(v, dpp_move<0x140>(v));
+  __device__ __forceinline__ const uint16_t* row(int r0) const {
+    const int r = row0 + (r0 + (lane & 15) < rows ? r0 + (lane & 15) : rows - 1);
+    const int tok = fast_div(r, group_div);
+    return q + tok * sq_t + (r - tok * group) * sq_h + 8 * (lane >> 4);
   }
-  q1 = fmaxf(q1, dpp_move<0xB1>(q1));
-  q1 = fmaxf(q1, dpp_move<0x4E>(q1));
-  q1 = fmaxf(q1, dpp_move<0x141>(q1));
-  q1 = fmaxf(q1, dpp_move<0x140>(q1));
-  q1 += shfl_xor(q1, 16);
-  q1 = sum_xor32(q1);
-  bmax = wave_max(bmax);
-  const int64_t at = (int64_t)jh * s.width;
-  if (l16 == 0) *reinterpret_cast<f32x4*>(s.scores + at + col0 + 4 * hq) = best;
-  if (lane == 0) s.error[(int64_t)jh * (s.width >> 4) + (col0 >> 4)] = q1 * bmax * 0x1p-16f;
-}
+  __device__ __forceinline__ const uint16_t* bounds_of(int page) const {
+    return bounds + page * page_step + 8 * (lane >> 4);
+  }
+  __device__ __forceinline__ Box load(int page) const {
+    // no page: left out by the selection
+    const uint16_t* bp = bounds_of((unsigned)page < (unsigned)pages ? page : 0);
+    Box b;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) b.x[c] = __builtin_bit_cast(bf16x8, ld16(bp + (c < 2 ? kHeadDim : 0) + 32 * (c & 1)));
+    return b;
+  }
+  __device__ __forceinline__ static bf16x8 size(bf16x8 x) {
+    return __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, x) & 0x7fff7fffu);
+  }
+  __device__ __forceinline__ float scores(const Box& box) {
+    float best = -INFINITY;
+    u32x4 x0 = q0, x1 = q1;
+    for (int r0 = 0;;) {
+      const bf16x8 part[4] = {positive(x0), positive(x1), negative(x0), negative(x1)};
+      f32x4 acc = {}, sum = {};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        acc = mfma16(part[c], box.x[c], acc);
+        sum = mfma16(c < 2 ? part[c] : size(part[c]), size(box.x[c]), sum);
+      }
+      best = fmaxf(fmaxf(best, fmaxf(acc[0], acc[1])), fmaxf(acc[2], acc[3]));
+      most = fmaxf(fmaxf(most, fmaxf(sum[0], sum[1])), fmaxf(sum[2], sum[3]));
+      r0 += 16;
+      if (r0 >= rows) break;
+      const uint16_t* qp = row(r0);
+      x0 = ld16(qp);
+      x1 = ld16(qp + 32);
+    }
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(best), __float_as_uint(best), false, false);
+    return max_xor32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  }
+  // Bound of the scores' distance from the exact sums: 64 additions of terms that are not zeros, each off by at most
+  // 2^-23 of the terms' absolute sum whatever their order and rounding; 2^-16 for 2^-17, which covers that sum's own.
+  __device__ __forceinline__ float error() const { return wave_max(most) * 0x1p-16f; }
+};
 
 // Floats in the order of unsigned integers; 0 is below all, kForced above.
 constexpr uint32_t kForced = 0xffffffffu;
@@ -199,174 +201,387 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)v, m, 64);
-    v = v < o ? v : o;
-  }
-  return v;
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {  // as wave_max
+  const auto least = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
+  v = least(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+  v = least(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+  v = least(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+  v = least(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = least(r[0], r[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return least(q[0], q[1]);
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) { return ~wave_min_u32(~v); }
 
-// The exact score of a page: rows to lanes, channels in turn, in 64 bits.
-__device__ double exact_score(const SelectArgs& s, const PagedSeq& sq, const QueryBlock& blk, int h, int page) {
-  const PagedArgs& a = s.p;
-  const int lane = wi_x() & 63;
-  const uint16_t* box = s.bounds + ((int64_t)page * a.kv_heads + h) * (2 * kHeadDim);
+// The exact score of a page: 16 rows at a time, 16 channels to a lane, in 64 bits. (Every lane's sums run in one
+// order, so equal bounds have equal scores.)
+__device__ __forceinline__ double exact_score(const ColumnScores& c, int page) {
+  const ColumnScores::Box box = c.load(page);
   double best = -__builtin_huge_val();
-  const int rows = (blk.hi - blk.lo) * a.group;
-  for (int r0 = 0; r0 < rows; r0 += 64) {
-    const int row = blk.lo * a.group + (r0 + lane < rows ? r0 + lane : rows - 1);
-    const int tok = fast_div(row, a.group_div);
-    const uint16_t* qp =
-        a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(h * a.group + row - tok * a.group) * a.sq_h;
+  u32x4 x[2] = {c.q0, c.q1};
+  for (int r0 = 0;;) {
     double sum = 0.0;
-    for (int d = 0; d < kHeadDim; d += 8) {
-      const bf16x8 x = __builtin_bit_cast(bf16x8, ld16(qp + d));
-      const bf16x8 lo = __builtin_bit_cast(bf16x8, ld16(box + d)), hi = __builtin_bit_cast(bf16x8, ld16(box + kHeadDim + d));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += (double)(float)x[i] * (double)(float)((float)x[i] > 0.f ? hi[i] : lo[i]);
+    for (int k = 0; k < 2; ++k) {
+      const bf16x8 q = __builtin_bit_cast(bf16x8, x[k]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += (double)(float)q[i] * (double)((float)q[i] > 0.f ? (float)box.x[k][i] : (float)box.x[2 + k][i]);
     }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
     best = sum > best ? sum : best;
+    r0 += 16;
+    if (r0 >= c.rows) break;
+    const uint16_t* qp = c.row(r0);
+    x[0] = ld16(qp);
+    x[1] = ld16(qp + 32);
   }
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
+  for (int m = 1; m < 16; m <<= 1) {
     const double o = __shfl_xor(best, m, 64);
     best = o > best ? o : best;
   }
   return best;
 }
 
-// The selection of one block and KV head, a wave each. R: 64 R columns at most, their keys
-// in registers; 0: any number, their keys formed again from the scores each time.
-template <int R>
-__global__ __launch_bounds__(64) void page_select_kernel(SelectArgs s) {
+// What the waves of a workgroup tell each other.
+constexpr int kBins = 512;
+constexpr int kPasses = 4;  // of 9 bits of a key's 32
+template <int NW>
+struct TeamLds {
+  uint32_t words[2][5][NW];
+  uint32_t bins[kPasses][kBins];
+};
+enum Merge { kSum, kLeast, kMost };
+template <int NW>
+struct Team {
+  TeamLds<NW>& lds;
+  int wave, turn = 0;
+  // Each number merged over the waves.
+  template <Merge... M>
+  __device__ __forceinline__ void join(uint32_t (&v)[sizeof...(M)]) {
+    constexpr Merge how[] = {M...};
+    auto& x = lds.words[turn++ & 1];
+    if ((wi_x() & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < (int)sizeof...(M); ++k) x[k][wave] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < (int)sizeof...(M); ++k) {  // a lane a wave, the same in every NW lanes; then lanes i ^ 1, 2, 4, 8
+      uint32_t r = x[k][wi_x() & (NW - 1)];
+      const auto with = [&](uint32_t o) { r = how[k] == kSum ? r + o : how[k] == kLeast ? (r < o ? r : o) : (r > o ? r : o); };
+      with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)r, 0xB1, 0xF, 0xF, false));
+      with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)r, 0x4E, 0xF, 0xF, false));
+      if constexpr (NW > 4) with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)r, 0x141, 0xF, 0xF, false));
+      if constexpr (NW > 8) with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)r, 0x140, 0xF, 0xF, false));
+      v[k] = wave_uniform_u32(r);
+    }
+  }
+  // Sum over the earlier waves, and over all.
+  __device__ __forceinline__ int before(int v, int& all) {
+    auto& x = lds.words[turn++ & 1];
+    if ((wi_x() & 63) == 0) x[0][wave] = (uint32_t)v;
+    __syncthreads();
+    int r = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      r += w < wave ? (int)x[0][w] : 0;
+      all += (int)x[0][w];
+    }
+    all = wave_uniform(all);
+    return wave_uniform(r);
+  }
+};
+
+// What a wave knows of its columns' keys, in every lane: candidates, those always taken, the least and
+// the largest key of the others, a bound of the scores' errors (positive floats are ordered as their bits).
+struct Known {
+  uint32_t v[5] = {0, 0, kForced, 0, 0};
+  __device__ __forceinline__ void add(uint32_t k) {
+    v[0] += __popcll(__ballot(k > 0));
+    v[1] += __popcll(__ballot(k == kForced));
+    if (k > 0 && k != kForced) {
+      v[2] = k < v[2] ? k : v[2];
+      v[3] = k > v[3] ? k : v[3];
+    }
+  }
+  __device__ __forceinline__ void done(float err) {
+    v[2] = wave_min_u32(v[2]);
+    v[3] = wave_max_u32(v[3]);
+    v[4] = __float_as_uint(err);
+  }
+};
+
+// The selection of one block and KV head by NW waves: wave w has the groups of 64 columns from w * per on, `per` to
+// a wave; their keys stay in registers (per <= R) or, R = 0, are asked for again each time. key(g) is the
+// lane's of group g, after a barrier here: 0 no candidate, kForced always taken. sums: a double for each column.
+//
+// The threshold is found by histograms of 512 bins over the range of keys that it is known to be in (a bit search
+// took 20 passes over the keys and 27 of the 39 us of a call on one token over 1000 pages).
+template <int NW, int R, class Key>
+__device__ __forceinline__ void choose(const SelectArgs& s, const ColumnScores& c, const PagedSeq& sq, const QueryBlock& blk,
+                                       const int32_t* table, Known known, Key key, double* sums, Team<NW> team) {
   const PagedArgs& a = s.p;
   const int lane = wi_x() & 63;
-  const int jh = wg_x();
-  const int j = fast_div(jh, a.kv_heads_div);
-  const int h = jh - j * a.kv_heads;
-  const SeqPiece<PagedSeq> it(
-      a.seqs, j, [&](int b) { return PagedSeq(a, b); }, [&](const PagedSeq& q) { return q.blocks(a); });
-  if (!it.found) return;
-  const QueryBlock blk(a, it.sq, it.at);
-  if (blk.lo >= blk.hi) return;
-  const int32_t* table = a.table + (int64_t)it.b * a.table_s;
-  const float* scores = s.scores + (int64_t)jh * s.width;
-  double* sums = s.sums + (int64_t)jh * s.width;
-  const int n = (blk.cols + 63) >> 6;
-  const auto key_of = [&](int i) -> uint32_t {  // 0: not seen, or no page
-    const int col = 64 * i + lane;
-    if (col >= blk.cols || (unsigned)table[col] >= (unsigned)a.pages) return 0;
-    if (col < s.first || col >= blk.own - s.recent) return kForced;
-    return order_key(scores[col]);
-  };
+  const int groups = (blk.cols + 63) >> 6;
+  const int per = (groups + NW - 1) / NW;
+  const int g0 = team.wave * per;
+  const int n = g0 < groups ? (g0 + per < groups ? per : groups - g0) : 0;
+#pragma unroll
+  for (int b = 0; b < kPasses * kBins; b += 64 * NW) (&team.lds.bins[0][0])[b + wi_x()] = 0;
+  static_assert(kPasses * kBins % (64 * NW) == 0, "whole turns");
+  team.template join<kSum, kSum, kLeast, kMost, kMost>(known.v);
   uint32_t kept[R > 0 ? R : 1];
   const auto reread = [&](auto f) {
-    for (int i = 0; i < n; ++i) f(i, key_of(i));
+    for (int i = 0; i < n; ++i) f(g0 + i, key(g0 + i));
   };
   const auto each = [&](auto f) {
     if constexpr (R > 0) {
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-        if (i < n) f(i, kept[i]);
+      for (int i = 0; i < R; ++i) f(g0 + i, kept[i]);  // keys of groups past the last one are 0
     } else {
       reread(f);
     }
   };
   if constexpr (R > 0) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) kept[i] = i < n ? key_of(i) : 0;
+    for (int i = 0; i < R; ++i) kept[i] = i < n ? key(g0 + i) : 0;
   }
-  float err = 0.f;
-  for (int t = lane; t < (blk.cols + 15) >> 4; t += 64) err = fmaxf(err, s.error[(int64_t)jh * (s.width >> 4) + t]);
-  err = wave_max(err);
-  int there = 0;
-  each([&](int, uint32_t k) { there += __popcll(__ballot(k > 0)); });
+  const int there = (int)known.v[0];
+  const float err = __uint_as_float(known.v[4]);
+  int need = a.top - (int)known.v[1];  // of the others
 
-  // The largest t that at least `top` keys reach.
-  uint32_t t = 1;
-  if (there > a.top) {
-    t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t up = t | 1u << bit;
-      int count = 0;
-      each([&](int, uint32_t k) { count += __popcll(__ballot(k >= up)); });
-      if (count >= a.top) t = up;
-      if (count == a.top) break;
+  // Taken: keys from `sure` on and the best `open` of those from `doubt` on.
+  uint32_t sure = 1, doubt = 1;
+  int open = 0;
+  if (there > a.top && need <= 0) {
+    sure = doubt = kForced;  // the first of those always taken
+  } else if (there > a.top) {
+    uint32_t lo = known.v[2], hi = known.v[3];  // the need-th largest key of the others is in [lo, hi]
+    int in_range = there - (int)known.v[1];     // as are these many
+    for (int pass = 0; in_range > need && lo < hi; ++pass) {
+      const int wide = 32 - __builtin_clz((hi - lo) | 1u);
+      const int shift = wide > 9 ? wide - 9 : 0;
+      uint32_t* bins = team.lds.bins[pass];
+      each([&](int, uint32_t k) {
+        if (k >= lo && k <= hi) atomicAdd(&bins[(k - lo) >> shift], 1u);
+      });
+      __syncthreads();
+      // Lane l: bins 511 - 8 l downwards.
+      uint32_t mine[8], total = 0;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        mine[b] = bins[kBins - 1 - 8 * lane - b];
+        total += mine[b];
+      }
+      const int upto = wave_scan((int)total);
+      const int at = __builtin_ctzll(__ballot(upto >= need));
+      int above = __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane((int)total, at);
+      int bin = 0, count = 0;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const int m = __builtin_amdgcn_readlane((int)mine[b], at);
+        if (count == 0 && above + m >= need) {
+          bin = kBins - 1 - 8 * at - b;
+          count = m;
+        }
+        above += count == 0 ? m : 0;
+      }
+      need -= above;
+      in_range = count;
+      const uint32_t last = lo + ((uint32_t)(bin + 1) << shift) - 1;
+      hi = last < hi && last >= lo ? last : hi;
+      lo += (uint32_t)bin << shift;
     }
-  }
-  // Taken: keys from t on, if exactly `top` reach it and the next one is further below than
-  // their errors; else those above the doubtful ones, and the best of these.
-  uint32_t sure = t, doubt = t;  // taken from `sure` on, left below `doubt`
-  int open = 0;                  // places for those in between
-  if (there > a.top) {
-    uint32_t least = kForced, next = 0;
-    int count = 0;
+    // Keys from lo on: exactly `top` with those always taken, unless equal ones are left. The next one has
+    // to be further below than their errors; else the doubtful ones are those around lo.
+    uint32_t border[2] = {kForced, 0};  // the least taken, the largest left
     each([&](int, uint32_t k) {
-      if (k >= t) least = k < least ? k : least;
-      if (k < t) next = k > next ? k : next;
-      count += __popcll(__ballot(k >= t));
+      if (k >= lo) border[0] = k < border[0] ? k : border[0];
+      if (k < lo) border[1] = k > border[1] ? k : border[1];
     });
-    least = wave_min_u32(least);
-    next = wave_max_u32(next);
-    const float v = key_value(least);
+    border[0] = wave_min_u32(border[0]);
+    border[1] = wave_max_u32(border[1]);
+    team.template join<kLeast, kMost>(border);
+    sure = doubt = lo;
+    const float v = key_value(border[0]);
     const bool bounded = (__float_as_uint(err) & 0x7f800000u) != 0x7f800000u;
-    if (count != a.top || (least != kForced && next > 0 && !(bounded && v - key_value(next) > 2.01f * err))) {
+    if (in_range > need || !(bounded && (border[1] == 0 || v - key_value(border[1]) > 2.01f * err))) {
       // 2.01: these sums round as well, by 2^-24 |v| < 2^-8 err
       sure = bounded ? order_key(v + 2.01f * err) + 1 : kForced;
       doubt = bounded ? order_key(v - 2.01f * err) : 1;
-      if (least == kForced) sure = doubt = kForced;  // more columns always taken than fit: the first ones
-      int above = 0;
-      reread([&](int i, uint32_t k) {
-        above += __popcll(__ballot(k >= sure));
+      uint32_t above[1] = {0};
+      reread([&](int g, uint32_t k) {
+        above[0] += __popcll(__ballot(k >= sure));
         uint64_t in = __ballot(k >= doubt && k < sure);
         while (in != 0) {
-          const int at = 64 * i + __builtin_ctzll(in);
+          const int col = 64 * g + __builtin_ctzll(in);
           in &= in - 1;
-          const double e = exact_score(s, it.sq, blk, h, wave_uniform(table[at]));
-          if (lane == 0) sums[at] = e;
+          const double e = exact_score(c, wave_uniform(table[col]));
+          if (lane == 0) sums[col] = e;
         }
       });
-      open = a.top - above;
-      __threadfence_block();
+      team.template join<kSum>(above);  // its barrier also shows the sums
+      open = a.top - (int)above[0];
     }
   }
-  int base = 0;
-  int32_t* out = s.out + (int64_t)(it.sq.q0 + blk.lo) * a.kv_heads * a.top + (int64_t)h * a.top;
-  const int64_t step = (int64_t)a.kv_heads * a.top;
-  const auto emit = [&](int i, bool take) {
-    const uint64_t all = __ballot(take);
-    const int at = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
-    if (take && at < a.top)
-      for (int tok = 0; tok < blk.hi - blk.lo; ++tok) out[tok * step + at] = 64 * i + lane;
-    base += __popcll(all);
-  };
-  if (open <= 0) {
-    each([&](int i, uint32_t k) { emit(i, k >= sure); });
-  } else {
-    reread([&](int i, uint32_t k) {
-      const bool maybe = k >= doubt && k < sure;
-      int before = 0;  // doubtful ones that are better
-      if (__ballot(maybe) != 0) {
-        const int col = 64 * i + lane;
-        const double mine = maybe ? sums[col] : 0.0;
-        reread([&](int i2, uint32_t k2) {
-          uint64_t in = __ballot(k2 >= doubt && k2 < sure);
-          while (in != 0) {
-            const int at = 64 * i2 + __builtin_ctzll(in);
-            in &= in - 1;
-            const double e = sums[at];
-            before += e > mine || (e == mine && at < col);
-          }
-        });
+  const auto taken = [&](int g, uint32_t k) {
+    bool take = k >= sure;
+    const bool maybe = k >= doubt && k < sure;
+    if (open > 0 && __ballot(maybe) != 0) {
+      const int col = 64 * g + lane;
+      const double mine = maybe ? sums[col] : 0.0;
+      int ahead = 0;  // doubtful ones that are better
+      for (int g2 = 0; g2 < groups; ++g2) {
+        const uint32_t k2 = key(g2);
+        uint64_t in = __ballot(k2 >= doubt && k2 < sure);
+        while (in != 0) {
+          const int at = 64 * g2 + __builtin_ctzll(in);
+          in &= in - 1;
+          const double e = sums[at];
+          ahead += e > mine || (e == mine && at < col);
+        }
       }
-      emit(i, k >= sure || (maybe && before < open));
+      take = take || (maybe && ahead < open);
+    }
+    return take;
+  };
+  // The columns taken, in ascending order, for each token of the block.
+  int mine = 0, all;
+  uint64_t settled = 0;  // of the doubtful: bit i of the lane for its column of the wave's i-th group
+  if (open > 0)
+    reread([&](int g, uint32_t k) {
+      const bool take = taken(g, k);
+      if (g - g0 < 64) settled |= (uint64_t)take << (g - g0);
+      mine += __popcll(__ballot(take));
     });
+  else
+    each([&](int, uint32_t k) { mine += __popcll(__ballot(k >= sure)); });
+  int base = team.before(mine, all);
+  int32_t* out = s.out + (int64_t)(sq.q0 + blk.lo) * a.kv_heads * a.top + (int64_t)c.h * a.top;
+  const int64_t step = (int64_t)a.kv_heads * a.top;
+  const int tokens = blk.hi - blk.lo;
+  const auto emit = [&](int g, bool take) {
+    const uint64_t in = __ballot(take);
+    const int at = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+    if (take && at < a.top)
+      for (int tok = 0; tok < tokens; ++tok) out[tok * step + at] = 64 * g + lane;
+    base += __popcll(in);
+  };
+  if (open > 0)
+    reread([&](int g, uint32_t k) { emit(g, g - g0 < 64 ? (settled >> (g - g0)) & 1 : taken(g, k)); });
+  else
+    each([&](int g, uint32_t k) { emit(g, k >= sure); });
+  for (int at = all + wi_x(); at < a.top; at += 64 * NW)
+    for (int tok = 0; tok < tokens; ++tok) out[tok * step + at] = -1;
+}
+
+__device__ __forceinline__ uint32_t column_key(const SelectArgs& s, const QueryBlock& blk, int col, int page, float score) {
+  if (col >= blk.cols || (unsigned)page >= (unsigned)s.p.pages) return 0;
+  return col < s.first || col >= blk.own - s.recent ? kForced : order_key(score);
+}
+
+struct BlockPiece : SeqPiece<PagedSeq> {
+  int h;
+  __device__ __forceinline__ BlockPiece(const PagedArgs& a, int jh)
+      : BlockPiece(a, jh, wave_uniform(fast_div(jh, a.kv_heads_div))) {}
+  __device__ __forceinline__ BlockPiece(const PagedArgs& a, int jh, int j)
+      : SeqPiece<PagedSeq>(a.seqs, j, [&](int b) { return PagedSeq(a, b); }, [&](const PagedSeq& q) { return q.blocks(a); }),
+        h(jh - j * a.kv_heads) {}
+};
+
+// Up to kPickColumns: the waves of a workgroup score them into LDS, 16 a wave and turn, the
+// next ones' bounds on their way, and choose. Few waves for many items, which then all run at once.
+template <int NW>
+__global__ __launch_bounds__(64 * NW, 4) void page_pick_kernel(SelectArgs s) {
+  const PagedArgs& a = s.p;
+  __shared__ uint32_t keys[kPickColumns];
+  __shared__ double sums[kPickColumns];
+  __shared__ TeamLds<NW> team;
+  const int lane = wi_x() & 63, l16 = lane & 15;
+  const int wave = wave_uniform(wi_x() >> 6);
+  const BlockPiece it(a, wg_x());
+  if (!it.found) return;
+  const QueryBlock blk(a, it.sq, it.at);
+  if (blk.lo >= blk.hi) return;
+  const int32_t* table = a.table + (int64_t)it.b * a.table_s;
+  const int tiles = (blk.cols + 15) >> 4;
+  const auto pages_from = [&](int t) {  // lane 16 k + l16: page of column l16 of tile t + NW k
+    const int col = 16 * (t + NW * (lane >> 4)) + l16;
+    return col < blk.cols ? table[col] : -1;
+  };
+  int t = wave, turn = 0;
+  int pages = pages_from(t), page = __shfl(pages, l16, 64);
+  ColumnScores c(s, it.sq, blk, it.h);
+  Known known;
+  ColumnScores::Box box;
+  if (t < tiles) box = c.load(page);
+  while (t < tiles) {
+    const ColumnScores::Box now = box;
+    const int now_page = page, now_at = 16 * t;
+    t += NW;
+    turn = (turn + 1) & 3;
+    if (turn == 0) pages = pages_from(t);
+    page = __shfl(pages, 16 * turn + l16, 64);
+    if (t < tiles) box = c.load(page);
+    const float score = c.scores(now);
+    const uint32_t key = lane < 16 ? column_key(s, blk, now_at + l16, now_page, score) : 0u;
+    if (lane < 16) keys[now_at + l16] = key;
+    known.add(key);
   }
-  for (int at = base + lane; at < a.top; at += 64)
-    for (int tok = 0; tok < blk.hi - blk.lo; ++tok) out[tok * step + at] = -1;
+  known.done(c.error());
+  const auto key = [&](int g) { return 64 * g + lane < blk.cols ? keys[64 * g + lane] : 0u; };
+  choose<NW, kPickColumns / 64 / NW>(s, c, it.sq, blk, table, known, key, sums, Team<NW>{team, wave});
+}
+
+// Few items, whose bounds few CUs would fetch (55 GB/s each), or more columns: scored by as many workgroups as
+// they fill, then chosen by NW waves.
+__global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs s, int chunks) {
+  const PagedArgs& a = s.p;
+  const int lane = wi_x() & 63, l16 = lane & 15;
+  const int wave = wave_uniform(wi_x() >> 6);
+  const int jh = wg_x() / chunks;
+  const int col0 = 16 * (4 * (wg_x() - jh * chunks) + wave);
+  const BlockPiece it(a, jh);
+  if (!it.found) return;
+  const QueryBlock blk(a, it.sq, it.at);
+  if (col0 >= blk.cols) return;
+  const int col = col0 + l16 < blk.cols ? col0 + l16 : blk.cols - 1;
+  ColumnScores c(s, it.sq, blk, it.h);
+  const float score = c.scores(c.load(a.table[(int64_t)it.b * a.table_s + col]));
+  const float err = c.error();
+  if (lane < 16) s.scores[(int64_t)jh * s.width + col0 + lane] = score;
+  if (lane == 0) s.error[(int64_t)jh * (s.width >> 4) + (col0 >> 4)] = err;
+}
+
+template <int NW, int R>
+__global__ __launch_bounds__(64 * NW) void page_select_kernel(SelectArgs s) {
+  const PagedArgs& a = s.p;
+  __shared__ TeamLds<NW> team;
+  const int lane = wi_x() & 63;
+  const int wave = wave_uniform(wi_x() >> 6);
+  const int jh = wg_x();
+  const BlockPiece it(a, jh);
+  if (!it.found) return;
+  const QueryBlock blk(a, it.sq, it.at);
+  if (blk.lo >= blk.hi) return;
+  const int32_t* table = a.table + (int64_t)it.b * a.table_s;
+  const float* scores = s.scores + (int64_t)jh * s.width;
+  float err = 0.f;
+  for (int t = lane; t < (blk.cols + 15) >> 4; t += 64) err = fmaxf(err, s.error[(int64_t)jh * (s.width >> 4) + t]);
+  err = wave_max(err);
+  const ColumnScores c(s, it.sq, blk, it.h);
+  const auto key = [&](int g) {
+    const int col = 64 * g + lane < blk.cols ? 64 * g + lane : blk.cols - 1;
+    const uint32_t k = column_key(s, blk, col, table[col], scores[col]);
+    return 64 * g + lane < blk.cols ? k : 0u;
+  };
+  Known known;
+  for (int g = wave; g < (blk.cols + 63) >> 6; g += NW) known.add(key(g));
+  known.done(err);
+  choose<NW, R>(s, c, it.sq, blk, table, known, key, s.sums + (int64_t)jh * s.width, Team<NW>{team, wave});
 }
 
 }  // namespace
@@ -383,17 +598,24 @@ hipError_t launch_page_bounds(const SelectArgs& s, int pool, hipStream_t stream)
 }
 
 hipError_t launch_select_pages(const SelectArgs& s, hipStream_t stream) {
-  const int chunks = (s.width + 63) / 64;
   const unsigned items = (unsigned)(s.slots * s.p.kv_heads);
+  if (!select_in_two(items, s.width)) {
+    if (items <= 512)
+      hipLaunchKernelGGL(page_pick_kernel<8>, dim3(items), dim3(512), 0, stream, s);
+    else
+      hipLaunchKernelGGL(page_pick_kernel<4>, dim3(items), dim3(256), 0, stream, s);
+    return hipGetLastError();
+  }
+  const int chunks = (s.width + 63) / 64;
   hipLaunchKernelGGL(page_scores_kernel, dim3(items * chunks), dim3(256), 0, stream, s, chunks);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (s.width <= 64 * 8)
-    hipLaunchKernelGGL(page_select_kernel<8>, dim3(items), dim3(64), 0, stream, s);
-  else if (s.width <= 64 * 24)
-    hipLaunchKernelGGL(page_select_kernel<24>, dim3(items), dim3(64), 0, stream, s);
+  if (s.width <= 4 * 64 * 8)
+    hipLaunchKernelGGL((page_select_kernel<4, 8>), dim3(items), dim3(256), 0, stream, s);
+  else if (s.width <= 16 * 64 * 8)
+    hipLaunchKernelGGL((page_select_kernel<16, 8>), dim3(items), dim3(1024), 0, stream, s);
   else
-    hipLaunchKernelGGL(page_select_kernel<0>, dim3(items), dim3(64), 0, stream, s);
+    hipLaunchKernelGGL((page_select_kernel<16, 0>), dim3(items), dim3(1024), 0, stream, s);
   return hipGetLastError();
 }
 

@@ -311,7 +311,8 @@ struct MergeLds {
   float m[NW][ROWS];
   float l[NW][ROWS];
   template <class Item>
-  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const Item& it, int rt, int d) const {
+  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const Item& it, int rt, int d,
+                                            int first = 0) const {  // first: row of the tile that the states begin with
     float mw[NW], mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
@@ -328,7 +329,7 @@ struct MergeLds {
       ot += wgt * *reinterpret_cast<const f32x4*>(&o[w][rt][d]);
     }
     const float inv = lt > 0.f ? 1.f / lt : 0.f;  // a row that sees no key: 0
-    const int row = it.r0 + rt;
+    const int row = it.r0 + first + rt;
     if (ranges == 1) {
       if (row < it.r1) {
         const int t = fast_div(row, a.group_div);
@@ -344,6 +345,124 @@ struct MergeLds {
     }
   }
 };
+// 8-bit pools: chunks of KC keys (groups of 16, each in one page under one scale) that one of NW waves takes
+// in turn: from the pages to registers, full rows (4 lanes a row of 64 codes), the next chunk's
+// loads in flight while the last one is computed from the wave's LDS tile. Codes stay bytes there:
+// the 16-byte part p of row r lies at part p ^ (r / 4 % 4), so that the row reads (16 rows, one part)
+// and the transposed ones (8 rows, one part, twice) meet every bank once.
+template <int NW, int KC, int POOL, bool COLS>
+struct CodeStream {
+  static constexpr int kGroups = KC / 16;
+  static constexpr int kFound = 64 / kGroups;  // chunks whose pages are looked up at once
+  static constexpr int kTile = KC * kHeadDim;  // bytes
+  const PagedArgs& a;
+  const int32_t* table;
+  const int32_t* list;  // COLS: the block's columns
+  const uint8_t *kh, *vh;  // the head's rows of page 0
+  int h, lo, hi, end, wave, lane, mine;
+  int ids;        // lane kGroups i + g: page of group g of chunk base + i
+  int at_key;     // COLS: position of its first key
+  float k_scale, v_scale;  // K's with the softmax's factor
+  uint64_t ok;    // which of them exist
+  u32x4 kr[kGroups], vr[kGroups];  // row lane / 4 of the group, part lane % 4
+  struct Info {
+    uint32_t there;
+    int base[kGroups];
+    float ks[kGroups], vs[kGroups];
+  } info;  // of the loaded chunk
+
+  __device__ __forceinline__ CodeStream(const PagedArgs& a_, int b, int h_, const int32_t* list_, int lo_, int hi_, int end_,
+                                        int wave_, int lane_)
+      : a(a_), list(list_), h(h_), lo(lo_), hi(hi_), end(end_), wave(wave_), lane(lane_), info() {
+    table = a.table + (int64_t)b * a.table_s;
+    kh = static_cast<const uint8_t*>(a.k) + h * a.sk_h;
+    vh = static_cast<const uint8_t*>(a.v) + h * a.sv_h;
+    const int n = hi > lo ? (hi - lo + KC - 1) / KC : 0;
+    mine = n > wave ? (n - wave + NW - 1) / NW : 0;
+  }
+  __device__ __forceinline__ int first_key(int i) const { return lo + (wave + NW * i) * KC; }
+  __device__ __forceinline__ void find(int i) {
+    int key = first_key(i + lane / kGroups) + 16 * (lane % kGroups);
+    ids = -1;
+    if (key < hi) {
+      if constexpr (COLS) {
+        const int col = list[key >> a.page_shift];
+        const int cols = (int)(((int64_t)end + a.page - 1) >> a.page_shift);
+        const bool is = (unsigned)col < (unsigned)cols;
+        key = ((is ? col : 0) << a.page_shift) + (key & (a.page - 1));
+        if (is && key < end) ids = table[col];
+      } else {
+        ids = table[key >> a.page_shift];
+      }
+    }
+    if constexpr (COLS) at_key = key;
+    const bool is = (unsigned)ids < (unsigned)a.pages;
+    ok = __ballot(is);
+    k_scale = v_scale = 1.f;
+    if (is) {
+      const int64_t at = ((int64_t)ids * a.kv_heads + h) * (a.page >> 4) + ((key & (a.page - 1)) >> 4);
+      k_scale = a.k_scales[at] * a.scale_log2;
+      v_scale = a.v_scales[at];
+    }
+  }
+  __device__ __forceinline__ void load(int i) {
+    const int turn = i % kFound;
+    if (turn == 0) find(i);
+    info.there = (uint32_t)(ok >> (kGroups * turn)) & ((1u << kGroups) - 1);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int at = kGroups * turn + g;
+      const int key = COLS ? __builtin_amdgcn_readlane(at_key, at) : first_key(i) + 16 * g;
+      info.base[g] = key;
+      info.ks[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scale), at));
+      info.vs[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_scale), at));
+      const bool is = (info.there >> g) & 1;
+      const int64_t page = __builtin_amdgcn_readlane(ids, at);
+      const int64_t slot = key & (a.page - 1);
+      const uint64_t kb = (uint64_t)(uintptr_t)(is ? kh + page * a.sk_p + slot * a.sk_s : (const uint8_t*)zero_row);
+      const uint64_t vb = (uint64_t)(uintptr_t)(is ? vh + page * a.sv_p + slot * a.sv_s : (const uint8_t*)zero_row);
+      const int last = is ? (COLS ? end : hi) - 1 - key : 0;  // rows past the last key re-read it
+      const int r = (lane >> 2) < last ? lane >> 2 : last;
+      kr[g] = __builtin_nontemporal_load((global_u32x4*)(kb + (uint32_t)(r * (int)a.sk_s + 16 * (lane & 3))));
+      vr[g] = __builtin_nontemporal_load((global_u32x4*)(vb + (uint32_t)(r * (int)a.sv_s + 16 * (lane & 3))));
+    }
+  }
+  __device__ __forceinline__ void stage(uint8_t* ks, uint8_t* vs) const {
+    const int at = (lane >> 2) * 64 + 16 * ((lane & 3) ^ (lane >> 4));
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      *reinterpret_cast<u32x4*>(&ks[1024 * g + at]) = kr[g];
+      *reinterpret_cast<u32x4*>(&vs[1024 * g + at]) = vr[g];
+    }
+  }
+  // Codes 16 hq .. + 15 of key lane % 16 of group g (hq = lane / 16).
+  __device__ __forceinline__ u32x4 key_codes(const uint8_t* ks, int g) const {
+    const int r = lane & 15;
+    return *reinterpret_cast<const u32x4*>(&ks[1024 * g + 64 * r + 16 * ((lane >> 4) ^ (r >> 2))]);
+  }
+  // Codes of column 16 db + lane % 16 of the keys 4 hq .. + 3 of groups 2 h2 and 2 h2 + 1: the order of the scores in
+  // the registers.
+  __device__ __forceinline__ bf16x8 value_codes(const uint8_t* vs, int h2, int db) const {
+    const int s = lane & 15, hq = lane >> 4;
+    const int r = 4 * hq + ((s >> 1) & 3);  // row of the group, s / 8 the group
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+    const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (lds_i32x2*)(&vs[1024 * (2 * h2 + (s >> 3)) + 64 * r + 16 * (db ^ hq) + 8 * (s & 1)]));
+    return cat8(codes4<POOL>((uint32_t)w[0]), codes4<POOL>((uint32_t)w[1]));
+  }
+  // Whether some row does not see some key of the chunk.
+  __device__ __forceinline__ bool masked(const Info& c, int kfull) const {
+    bool m = c.there != (1u << kGroups) - 1;
+    if constexpr (COLS) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) m = m || c.base[g] + 16 > kfull;
+      return m;
+    }
+    return m || c.base[0] + KC > kfull || c.base[0] + KC > hi;
+  }
+};
+
 template <int NW, int ROWS>
 constexpr size_t chunk_smem() {
   constexpr size_t v = sizeof(__bf16) * NW * 2 * kSub * kStride;
@@ -599,6 +718,154 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
   if (tid < 16 * kRows) ml->write_row(a, keys.ranges, it, tid >> 4, 4 * (tid & 15));
 }
 
+// Rows of 8-bit pools: 16 RT rows, NW waves that share the chunks of a range. S^T of 16 keys x 16 rows on
+// v_mfma_f32_16x16x32_bf16 from 16 codes of a key to a lane: the sums run over d in the order that
+// gives (16 hq + 8 c + e), which Q's operand takes as well. A chunk's codes are converted once for all RT
+// row tiles; its scales enter with the softmax's factor and with P.
+template <int NW, int RT, int KC, int POOL, bool COLS>
+__device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const PagedItem<false, COLS>& it, char* smem) {
+  using Stream = CodeStream<NW, KC, POOL, COLS>;
+  constexpr int kG = KC / 16;
+  const int tid = wi_x();
+  const int lane = tid & 63;
+  const int wave = wave_uniform(tid >> 6);
+  const int l16 = lane & 15;
+  const int hq = lane >> 4;
+  uint8_t* ks = reinterpret_cast<uint8_t*>(smem) + wave * 2 * Stream::kTile;
+  uint8_t* vs = ks + Stream::kTile;
+
+  const PagedSeq& sq = it.sq;
+  const ItemKeys<COLS> keys(a, it);
+  if (!keys.any) return;
+  Stream kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
+  if (kv.mine > 0) kv.load(0);
+
+  bf16x8 qreg[RT][2];
+  int khi[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int row = it.r0 + 16 * t + l16 < it.r1 ? it.r0 + 16 * t + l16 : it.r1 - 1;
+    const int tok = fast_div(row, a.group_div);
+    const uint16_t* qp =
+        a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(it.h * a.group + row - tok * a.group) * a.sq_h + 16 * hq;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) qreg[t][c] = __builtin_bit_cast(bf16x8, ld16(qp + 8 * c));
+    const int ends = sq.key_end(a, tok);
+    khi[t] = COLS || ends < keys.hi ? ends : keys.hi;
+  }
+  const int kfull = wave_uniform(sq.key_end(a, fast_div(it.r0, a.group_div)));  // every row sees these
+
+  f32x4 o[RT][4] = {};  // O^T [16-d block]: lane (row l16, hq) holds d 16 db + 4 hq + r
+  float m[RT], lsum[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    m[t] = -INFINITY;
+    lsum[t] = 0.f;
+  }
+  for (int i = 0; i < kv.mine; ++i) {
+    const typename Stream::Info info = kv.info;
+    kv.stage(ks, vs);
+    if (i + 1 < kv.mine) kv.load(i + 1);
+    bf16x8 kop[kG][2];
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+      const u32x4 w = kv.key_codes(ks, g);
+      kop[g][0] = cat8(codes4<POOL>(w[0]), codes4<POOL>(w[1]));
+      kop[g][1] = cat8(codes4<POOL>(w[2]), codes4<POOL>(w[3]));
+    }
+    const bool masked = kv.masked(info, kfull);
+    bf16x8 pop[RT][kG / 2];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      f32x4 s[kG];
+      float mt = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        s[g] = mfma16(kop[g][0], qreg[t][0], f32x4{});
+        s[g] = mfma16(kop[g][1], qreg[t][1], s[g]);
+      }
+      if (masked) {
+#pragma unroll
+        for (int g = 0; g < kG; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[g][r] = info.base[g] + 4 * hq + r < khi[t] && ((info.there >> g) & 1) ? s[g][r] : -INFINITY;
+      }
+#pragma unroll
+      for (int g = 0; g < kG; ++g)
+        mt = fmaxf(mt, fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3])) * info.ks[g]);
+      mt = fmaxf(mt, shfl_xor(mt, 16));
+      mt = max_xor32(mt);
+      if (__ballot(mt > m[t]) != 0) {
+        const float mn = fmaxf(m[t], mt);
+        const float alpha = (mn == -INFINITY) ? 1.f : fast_exp2(m[t] - mn);
+        m[t] = mn;
+        lsum[t] *= alpha;
+#pragma unroll
+        for (int db = 0; db < 4; ++db) o[t][db] *= alpha;
+      }
+      const float mu = (m[t] == -INFINITY) ? 0.f : m[t];
+      f32x4 p[kG];
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          p[g][r] = fast_exp2(fmaf(s[g][r], info.ks[g], -mu));
+          lsum[t] += p[g][r];
+        }
+        p[g] *= info.vs[g];
+      }
+#pragma unroll
+      for (int h2 = 0; h2 < kG / 2; ++h2)
+        pop[t][h2] = to_bf16x8(p[2 * h2][0], p[2 * h2][1], p[2 * h2][2], p[2 * h2][3], p[2 * h2 + 1][0], p[2 * h2 + 1][1],
+                               p[2 * h2 + 1][2], p[2 * h2 + 1][3]);
+    }
+#pragma unroll
+    for (int h2 = 0; h2 < kG / 2; ++h2)
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        const bf16x8 va = kv.value_codes(vs, h2, db);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) o[t][db] = mfma16(va, pop[t][h2], o[t][db]);
+      }
+  }
+
+  auto* ml = reinterpret_cast<MergeLds<NW, 16>*>(smem);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    lsum[t] += shfl_xor(lsum[t], 16);
+    lsum[t] = sum_xor32(lsum[t]);
+    __syncthreads();  // the tiles, and the last rows' states, are reused
+#pragma unroll
+    for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(&ml->o[wave][l16][16 * db + 4 * hq]) = o[t][db];
+    if (hq == 0) {
+      ml->m[wave][l16] = m[t];
+      ml->l[wave][l16] = lsum[t];
+    }
+    __syncthreads();
+    if (tid < 256) ml->write_row(a, keys.ranges, it, tid >> 4, 4 * (tid & 15), 16 * t);
+  }
+}
+
+template <int NW, int KC>
+constexpr size_t codes_smem() {
+  constexpr size_t v = (size_t)NW * 2 * KC * kHeadDim;
+  return v > sizeof(MergeLds<NW, 16>) ? v : sizeof(MergeLds<NW, 16>);
+}
+
+// WPS: waves per SIMD that the registers leave room for.
+template <int NW, int RT, int KC, int WPS, int POOL, bool COLS>
+__global__ __launch_bounds__(NW * 64, WPS) void paged_codes_kernel(PagedArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[codes_smem<NW, KC>()];
+  for (int id = wg_x();; id += a.workgroups) {  // as in paged_rows_kernel
+    const PagedItem<false, COLS> it(a, id);
+    if (!it.found) return;
+    if (!COLS || it.r0 < it.r1) paged_codes_item<NW, RT, KC, POOL, COLS>(a, it, smem);
+    if (id + a.workgroups >= it.total) return;
+    __syncthreads();
+  }
+}
+
 template <int NW, int ROWS, int POOL, bool COLS>
 __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void paged_rows_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[chunk_smem<NW, ROWS>()];
@@ -635,9 +902,15 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
 // over 727-3871 keys).
 constexpr float kRescale = 8.0f;
 
-template <int SUBS>
+// 8-bit pools: each wave loads the codes of its 16 keys to LDS during the step on the tile before,
+// then converts them to bf16 into the other stage, once for the four waves; the tile's four scales
+// enter as in paged_codes_item. (Held in registers during the step the codes spilled 4 to 40 of
+// those: prompts of 1500-4096 tokens in int8 106 us.)
+template <int SUBS, int POOL>
 __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
+  constexpr bool kCodes = POOL != kPoolBf16;
   __shared__ __attribute__((aligned(1024))) __bf16 smem_all[SUBS][2][2][kSwTile];  // [set][stage][K | V]
+  __shared__ __attribute__((aligned(1024))) uint8_t raw_all[kCodes ? SUBS : 1][kCodes ? 8 : 1][1024];  // [set][2 wave + K | V]
   const int tid = wi_x();
   const int lane = tid & 63;
   const int wave = wave_uniform((tid >> 6) & 3);  // in its set
@@ -684,6 +957,17 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     return key < hi ? table[key >> a.page_shift] : -1;
   };
   int ids = entries(0), ids_next = -1;
+  float k_scale = 1.f, v_scale = 1.f;  // 8-bit pools: of the same tiles' 16-key groups, K's with the softmax's factor
+  auto find_scales = [&](int base) {
+    const int key = lo + (sub + SUBS * (base + (lane >> 2))) * kSwRows + 16 * (lane & 3);
+    k_scale = v_scale = 1.f;
+    if ((unsigned)ids < (unsigned)a.pages) {
+      const int64_t at = ((int64_t)ids * a.kv_heads + h) * (a.page >> 4) + ((key & (a.page - 1)) >> 4);
+      k_scale = a.k_scales[at] * a.scale_log2;
+      v_scale = a.v_scales[at];
+    }
+  };
+  if constexpr (kCodes) find_scales(0);
 
   const int qrow0 = r0 + 32 * wave;
   const int myr = qrow0 + l32;
@@ -710,10 +994,14 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   const uint16_t* kh = static_cast<const uint16_t*>(a.k) + h * a.sk_h;
   const uint16_t* vh = static_cast<const uint16_t*>(a.v) + h * a.sv_h;
   uint32_t there = 0;  // quarters of the tile requested last whose page exists
+  float ks_next[4], vs_next[4];  // and their scales
+  const uint32_t raw_w = lds_addr(&raw_all[kCodes ? sub : 0][kCodes ? 2 * wave : 0][0]);
+  const uint8_t* raw = &raw_all[kCodes ? sub : 0][kCodes ? 2 * wave : 0][16 * lane];
   auto issue = [&](int i) {  // the set's i-th tile
     if ((i & 15) == 0 && i > 0) {
       ids = ids_next;
       ok = __ballot((unsigned)ids < (unsigned)a.pages);
+      if constexpr (kCodes) find_scales(i);
     }
     if ((i & 15) == 8) ids_next = entries((i | 15) + 1);
     const int at = 4 * (i & 15) + wave;
@@ -723,6 +1011,21 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     const int lim = (ok >> at) & 1 ? sq.kv - 1 - key : -1;  // the last of its 16 rows that is a key
     const int64_t page = __builtin_amdgcn_readlane(ids, at);
     const int64_t slot = key & (a.page - 1);
+    if constexpr (kCodes) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        ks_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scale), 4 * (i & 15) + q));
+        vs_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_scale), 4 * (i & 15) + q));
+      }
+      const int top = lim < 0 ? 0 : lim;  // rows past the last key re-read it
+      const int r = (lane >> 2) < top ? lane >> 2 : top;
+      const uint8_t* none = reinterpret_cast<const uint8_t*>(zero_row);
+      const uint8_t* kb = lim >= 0 ? static_cast<const uint8_t*>(a.k) + h * a.sk_h + page * a.sk_p + slot * a.sk_s : none;
+      const uint8_t* vb = lim >= 0 ? static_cast<const uint8_t*>(a.v) + h * a.sv_h + page * a.sv_p + slot * a.sv_s : none;
+      dma16(kb, (uint32_t)(r * (int)a.sk_s + 16 * (lane & 3)), raw_w);
+      dma16(vb, (uint32_t)(r * (int)a.sv_s + 16 * (lane & 3)), raw_w + 1024u);
+      return;
+    }
     const void* kb = lim >= 0 ? kh + page * a.sk_p + slot * a.sk_s : zero_row;
     const void* vb = lim >= 0 ? vh + page * a.sv_p + slot * a.sv_s : zero_row;
     if (lim >= 15) {
@@ -744,9 +1047,23 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
       }
     }
   };
+  auto convert = [&](int i) {  // codes of the set's i-th tile to its stage
+    const int r = 16 * wave + (lane >> 2), p = 2 * (lane & 3);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's codes are there
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(raw + 1024 * kv);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<bf16x8*>(&smem[i & 1][kv][64 * r + 8 * ((p + c) ^ swz(r))]) =
+            cat8(codes4<POOL>(x[2 * c]), codes4<POOL>(x[2 * c + 1]));
+    }
+  };
   if (n_mine > 0) issue(0);
 #pragma unroll
   for (int c = 0; c < 4; ++c) asm volatile("" ::"v"(qreg[c]));  // waits for Q here, not in the loop
+  if constexpr (kCodes)
+    if (n_mine > 0) convert(0);
 
   const int khi = sq.key_end(a, tok);  // the lane's row sees [0, khi)
   const int wave_last = qrow0 + 31 < sq.rows ? qrow0 + 31 : sq.rows - 1;
@@ -757,6 +1074,7 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   float mref = 0.f, lsum = 0.f;
   bool valid = false;  // the row has met a key
   const float c2 = a.scale_log2;
+  float k_factor[4], v_factor[4];  // 8-bit pools: the tile's
   auto step = [&](int k0, uint32_t seen, const __bf16* ks, const __bf16* vs) {
     f32x16 s[2];
 #pragma unroll
@@ -774,12 +1092,24 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
           s[sb][r] = key < khi && ((seen >> (2 * sb + (r >> 3))) & 1) ? s[sb][r] : -INFINITY;
         }
     }
-    float mrow = -INFINITY;
+    float mt;
+    if constexpr (kCodes) {
+      float mrow[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int sb = 0; sb < 2; ++sb)
+      for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) mrow = fmaxf(fmaxf(mrow, s[sb][r]), s[sb][r + 1]);
-    const float mt = fmaf(max_xor32(mrow), c2, -mref);
+        for (int r = 0; r < 16; r += 2)
+          mrow[2 * sb + (r >> 3)] = fmaxf(fmaxf(mrow[2 * sb + (r >> 3)], s[sb][r]), s[sb][r + 1]);
+      mt = max_xor32(fmaxf(fmaxf(mrow[0] * k_factor[0], mrow[1] * k_factor[1]),
+                           fmaxf(mrow[2] * k_factor[2], mrow[3] * k_factor[3]))) - mref;
+    } else {
+      float mrow = -INFINITY;
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) mrow = fmaxf(fmaxf(mrow, s[sb][r]), s[sb][r + 1]);
+      mt = fmaf(max_xor32(mrow), c2, -mref);
+    }
     if (__ballot(!valid || mt > kRescale) != 0) {
       const float delta = valid ? fmaxf(mt, 0.f) : (mt == -INFINITY ? 0.f : mt);
       const float alpha = valid ? fast_exp2(-delta) : 1.f;
@@ -793,11 +1123,14 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     for (int sb = 0; sb < 2; ++sb) {
       float p[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = fast_exp2(fmaf(s[sb][r], c2, -mref));
+      for (int r = 0; r < 16; ++r) p[r] = fast_exp2(fmaf(s[sb][r], kCodes ? k_factor[2 * sb + (r >> 3)] : c2, -mref));
 #pragma unroll
       for (int kc = 0; kc < 2; ++kc) {
-        const bf16x8 pop = to_bf16x8(p[8 * kc], p[8 * kc + 1], p[8 * kc + 2], p[8 * kc + 3], p[8 * kc + 4],
-                                     p[8 * kc + 5], p[8 * kc + 6], p[8 * kc + 7]);
+        const float f = kCodes ? v_factor[2 * sb + kc] : 1.f;
+        const bf16x8 pop = kCodes ? to_bf16x8(p[8 * kc] * f, p[8 * kc + 1] * f, p[8 * kc + 2] * f, p[8 * kc + 3] * f,
+                                              p[8 * kc + 4] * f, p[8 * kc + 5] * f, p[8 * kc + 6] * f, p[8 * kc + 7] * f)
+                                  : to_bf16x8(p[8 * kc], p[8 * kc + 1], p[8 * kc + 2], p[8 * kc + 3], p[8 * kc + 4],
+                                              p[8 * kc + 5], p[8 * kc + 6], p[8 * kc + 7]);
         lsum += ((p[8 * kc] + p[8 * kc + 1]) + (p[8 * kc + 2] + p[8 * kc + 3])) +
                 ((p[8 * kc + 4] + p[8 * kc + 5]) + (p[8 * kc + 6] + p[8 * kc + 7]));
 #pragma unroll
@@ -807,6 +1140,17 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   };
 
   uint32_t seen = there;
+  auto take_factors = [&] {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      k_factor[q] = ks_next[q];
+      v_factor[q] = vs_next[q];
+    }
+  };
+  if constexpr (kCodes) {
+    take_factors();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
   vm_wait_barrier<0>();
   const int steps = (n_tiles + SUBS - 1) / SUBS;  // of the set with the most tiles
   for (int i = 0; i < steps; ++i) {
@@ -814,6 +1158,10 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     const int k0 = lo + (sub + SUBS * i) * kSwRows;
     if (i < n_mine && k0 < emax) step(k0, seen, smem[i & 1][0], smem[i & 1][1]);
     seen = there;
+    if constexpr (kCodes) {
+      if (i + 1 < n_mine) convert(i + 1);
+      take_factors();
+    }
     // The next tile is there, and this wave's reads of this one are done before
     // any wave requests the tile after it into the same stage.
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -920,7 +1268,7 @@ __global__ __launch_bounds__(16 * kMergeRows) void paged_combine_kernel(PagedArg
   }
   const int row = at - sq.q0 * a.group;
   if (row >= sq.rows) return;  // of no sequence, or past the caller's bound
-  const int r0 = row & -a.tile;
+  const int r0 = fast_div(row, a.tile_div) * a.tile;
   const int keys = a.columns != nullptr
                        ? sq.listed_keys(a)
                        : sq.key_end(a, fast_div((r0 + a.tile < sq.rows ? r0 + a.tile : sq.rows) - 1, a.group_div));
@@ -965,16 +1313,28 @@ template <int POOL, bool COLS>
 hipError_t launch_paged_tiles(const PagedArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)a.workgroups);
   if (a.tile == 128) {
-    if constexpr (POOL == kPoolBf16 && !COLS) {
-      if (a.subs == 4)
-        hipLaunchKernelGGL(paged128_kernel<4>, grid, dim3(1024), 0, stream, a);
-      else if (a.subs == 2)
-        hipLaunchKernelGGL(paged128_kernel<2>, grid, dim3(512), 0, stream, a);
-      else
-        hipLaunchKernelGGL(paged128_kernel<1>, grid, dim3(256), 0, stream, a);
+    if constexpr (!COLS) {
+      if constexpr (POOL == kPoolBf16) {
+        if (a.subs == 4) hipLaunchKernelGGL((paged128_kernel<4, POOL>), grid, dim3(1024), 0, stream, a);
+      }
+      if (a.subs == 2)
+        hipLaunchKernelGGL((paged128_kernel<2, POOL>), grid, dim3(512), 0, stream, a);
+      else if (a.subs == 1)
+        hipLaunchKernelGGL((paged128_kernel<1, POOL>), grid, dim3(256), 0, stream, a);
     } else {
       return hipErrorInvalidValue;
     }
+  } else if constexpr (POOL != kPoolBf16) {
+    if (a.tile == 16 && a.subs == 2)
+      hipLaunchKernelGGL((paged_codes_kernel<8, 1, 32, 4, POOL, COLS>), grid, dim3(512), 0, stream, a);
+    else if (a.tile == 16)
+      hipLaunchKernelGGL((paged_codes_kernel<4, 1, 32, 3, POOL, COLS>), grid, dim3(256), 0, stream, a);
+    else if (a.tile == 32 && a.subs == 2)
+      hipLaunchKernelGGL((paged_codes_kernel<8, 2, 32, 3, POOL, COLS>), grid, dim3(512), 0, stream, a);
+    else if (a.tile == 32)
+      hipLaunchKernelGGL((paged_codes_kernel<4, 2, 64, 2, POOL, COLS>), grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((paged_codes_kernel<4, 3, 64, 2, POOL, COLS>), grid, dim3(256), 0, stream, a);
   } else {
     if (a.tile == 16)
       hipLaunchKernelGGL((paged_rows_kernel<8, 16, POOL, COLS>), grid, dim3(512), 0, stream, a);

@@ -479,7 +479,8 @@ int bd3_page_bounds(const void* k_pages, const float* k_scales, int32_t pool_typ
  *   q: (tokens, heads, 64) bf16; bounds: (pages, kv_heads, 2, 64) bf16, contiguous, as
  *     bd3_page_bounds writes them; finite. strides: q (token, head), page_table (row).
  * Preconditions: top >= first + recent + the most columns that a block can lie in
- * (within max_kv). workspace: bd3_select_pages_workspace_bytes of the same arguments.
+ * (within max_kv). workspace: bd3_select_pages_workspace_bytes of the same arguments
+ * (0 up to 256 columns, and up to 2048 of many blocks).
  */
 size_t bd3_select_pages_workspace_bytes(int32_t seqs, int32_t tokens, int32_t kv_heads, int32_t page_size,
                                         int32_t max_kv, int32_t block_size);

@@ -381,6 +381,8 @@ SELECT = [
     ([(40, 500)], 16, 1, 16, 32, 11, 1, 0),
     ([(1, 8300)], 2, 1, 16, 1, 64, 1, 1),     # over 512 columns
     ([(2, 25000), (1, 17000)], 1, 1, 16, 1, 100, 1, 1),  # over 1536
+    ([(1, 32800), (5, 40000), (3, 90)], 1, 1, 16, 4, 130, 1, 1),  # over 2048
+    ([(1, 140000)], 1, 1, 16, 1, 2000, 1, 1),  # over 8192
     ([(100, 50)], 2, 2, 128, 1 << 30, 4, 1, 1),
 ]
 

@@ -279,8 +279,8 @@ def test_bounds_refusals(lib, kw, text):
     (dict(first=-1), "first"), (dict(recent=-1), "recent"), (dict(top=2), "always taken"), (dict(top=3, bs=17), "always taken"),
     (dict(top=0, max_kv=0), "top"), (dict(q=None), "q must"), (dict(bounds=P + 2), "bounds"), (dict(out=None), "out"),
     (dict(out=P + 2), "out"), (dict(st=[256, 60, 4]), "q stride"), (dict(st=[256, 64, -1]), "page_table stride"),
-    (dict(ws_bytes=100), "too small"), (dict(ws=None), "workspace must"), (dict(ws=P + 4), "workspace must"),
-    (dict(seqs=1 << 24, tokens=1 << 24, bs=1), "too large"),
+    (dict(ws_bytes=100, width=2049, max_kv=2049 * 16), "too small"), (dict(ws=None, width=2049, max_kv=2049 * 16), "workspace must"),
+    (dict(ws=P + 4, width=2049, max_kv=2049 * 16), "workspace must"), (dict(seqs=1 << 24, tokens=1 << 24, bs=1), "too large"),
     (dict(seqs=1 << 12, tokens=1 << 12, bs=1, width=1 << 18, max_kv=1 << 22, top=9), "too large")])
 def test_select_refusals(lib, kw, text):
     assert select(lib, **kw) == _native.BD3_EINVAL
@@ -313,9 +313,11 @@ def test_workspaces(lib):
         assert size(*bad) == 0
     size = lib.bd3_select_pages_workspace_bytes
     for bad in ((0, 8, 2, 16, 64, 16), (2, 0, 2, 16, 64, 16), (2, 8, 0, 16, 64, 16), (2, 8, 2, 8, 64, 16), (2, 8, 2, 16, 0, 16),
-                (2, 8, 2, 16, (1 << 30) + 1, 16), (2, 8, 2, 16, 64, 0)):
+                (2, 8, 2, 16, (1 << 30) + 1, 16), (2, 8, 2, 16, 1 << 20, 0)):
         assert size(*bad) == 0
-    assert size(2, 8, 2, 16, 64, 16) > 0
+    assert size(200, 200, 2, 16, 2048 * 16, 16) == 0  # a workgroup's LDS
+    assert size(200, 200, 2, 16, 2048 * 16 + 1, 16) > 0
+    assert size(1, 1, 4, 16, 256 * 16, 1) == 0 and size(1, 1, 4, 16, 1000 * 16, 1) > 0  # few items, spread over the CUs
 
 
 def test_selection_without_room_for_the_columns_always_taken(lib):
