@@ -925,9 +925,9 @@ static_assert(kPagedPartRows * bd3::kHeadDim <= INT32_MAX, "32-bit indices of th
 // sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV heads and groups of 1-12;
 // over 1500 others the rms error is 9% for up to 16 rows, 12% for 17-256, 10% for more.
 //
-// 8-bit pools and lists have their own, fitted to 520 batches of 8-bit pools drawn the same way: rms error 9-10%; the plan
-// takes 1.2% more than the best of all plans on average for up to 16 rows, 1.8% for more (at worst 24%). Over 200
-// batches of lists 3% (bf16 pools 2%), at worst 67%.
+// 8-bit pools and lists have their own, fitted to 700 batches of 8-bit pools and 160 of lists drawn the same way: rms error
+// 9-12%; the plan takes 1.2% more than the best of all plans on average for up to 16 rows, 2.2% for more (at worst
+// 31%), over lists 2% (bf16 pools 1%; at worst 54%).
 struct PagedCost {
   double chain0, chain, busy, load0, load, item, merge, merge_item, e_even, e;
 };
@@ -938,13 +938,13 @@ const PagedCost& paged_cost(bool codes, int tile, int subs) {
   static constexpr PagedCost kRows128[3] = {{4.6, 1.0, 0.0, 5.2, 0.68, 1.4, 3.2, 1.7, 3.0, 3.0},
                                             {5.5, 0.66, 0.0, 4.8, 0.70, 2.9, 3.2, 1.9, 3.0, 3.0},
                                             {8.0, 0.52, 0.0, 0.0, 0.69, 9.5, 0.0, 0.0, 3.0, 3.0}};  // four sets: never with ranges
-  static constexpr PagedCost kCodes16[2] = {{0.0, 0.59, 0.25, 5.74, 0.235, 0.29, 2.7, 0.79, 1.27, 1.06},
-                                            {5.7, 0.34, 0.35, 0.0, 0.228, 1.28, 2.4, 1.16, 1.71, 1.0}};
-  static constexpr PagedCost kCodes32[2] = {{5.8, 0.58, 0.22, 5.65, 0.438, 2.75, 2.4, 0.14, 2.92, 2.4},
-                                            {6.8, 0.43, 0.28, 4.8, 0.529, 5.2, 2.75, 0.0, 5.0, 3.9}};
-  static constexpr PagedCost kCodes48 = {6.8, 0.64, 0.57, 7.2, 0.523, 3.27, 2.4, 0.19, 3.64, 2.58};
-  static constexpr PagedCost kCodes128[2] = {{5.16, 1.264, 0.106, 2.2, 0.504, 2.86, 1.3, 1.87, 1.21, 1.21},
-                                             {5.68, 0.897, 0.012, 4.7, 0.683, 4.93, 1.8, 1.37, 1.83, 1.83}};
+  static constexpr PagedCost kCodes16[2] = {{1.865, 0.407, 0.148, 3.628, 0.127, 0.544, 2.373, 0.755, 1.0, 1.012},
+                                            {1.677, 0.275, 0.191, 3.858, 0.105, 1.761, 2.512, 0.708, 1.0, 1.047}};
+  static constexpr PagedCost kCodes32[2] = {{6.064, 0.542, 0.337, 4.474, 0.401, 2.905, 2.416, 0.191, 2.395, 2.132},
+                                            {6.563, 0.345, 0.422, 5.078, 0.488, 5.257, 3.338, 0.0, 5.0, 4.23}};
+  static constexpr PagedCost kCodes48 = {7.01, 0.615, 0.016, 5.43, 0.469, 3.53, 2.407, 0.413, 2.488, 2.297};
+  static constexpr PagedCost kCodes128[2] = {{4.13, 1.276, 0.043, 3.88, 0.489, 2.922, 1.292, 1.948, 1.358, 1.358},
+                                             {5.538, 0.878, 0.032, 5.463, 0.67, 4.764, 1.779, 1.643, 2.128, 2.128}};
   if (codes) return tile == 16 ? kCodes16[subs - 1] : tile == 32 ? kCodes32[subs - 1] : tile == 48 ? kCodes48 : kCodes128[subs - 1];
   return tile == 16 ? kRows16 : tile == 32 ? kRows32[subs - 1] : kRows128[subs >> 1];
 }

@@ -362,13 +362,13 @@ struct CodeStream {
   int h, lo, hi, end, wave, lane, mine;
   int ids;        // lane kGroups i + g: page of group g of chunk base + i
   int at_key;     // COLS: position of its first key
-  float k_scale, v_scale;  // K's with the softmax's factor
+  float k_scale, v_log, v_inv;
   uint64_t ok;    // which of them exist
   u32x4 kr[kGroups], vr[kGroups];  // row lane / 4 of the group, part lane % 4
   struct Info {
     uint32_t there;
     int base[kGroups];
-    float ks[kGroups], vs[kGroups];
+    float ks[kGroups], v_log[kGroups], v_inv[kGroups];  // K's scales, log2 and inverse of V's
   } info;  // of the loaded chunk
 
   __device__ __forceinline__ CodeStream(const PagedArgs& a_, int b, int h_, const int32_t* list_, int lo_, int hi_, int end_,
@@ -398,12 +398,15 @@ struct CodeStream {
     if constexpr (COLS) at_key = key;
     const bool is = (unsigned)ids < (unsigned)a.pages;
     ok = __ballot(is);
-    k_scale = v_scale = 1.f;
+    k_scale = 1.f;
+    float v_scale = 1.f;
     if (is) {
       const int64_t at = ((int64_t)ids * a.kv_heads + h) * (a.page >> 4) + ((key & (a.page - 1)) >> 4);
-      k_scale = a.k_scales[at] * a.scale_log2;
+      k_scale = a.k_scales[at];
       v_scale = a.v_scales[at];
     }
+    v_log = fast_log2(v_scale);
+    v_inv = __builtin_amdgcn_rcpf(v_scale);
   }
   __device__ __forceinline__ void load(int i) {
     const int turn = i % kFound;
@@ -414,8 +417,6 @@ struct CodeStream {
       const int at = kGroups * turn + g;
       const int key = COLS ? __builtin_amdgcn_readlane(at_key, at) : first_key(i) + 16 * g;
       info.base[g] = key;
-      info.ks[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scale), at));
-      info.vs[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_scale), at));
       const bool is = (info.there >> g) & 1;
       const int64_t page = __builtin_amdgcn_readlane(ids, at);
       const int64_t slot = key & (a.page - 1);
@@ -425,6 +426,14 @@ struct CodeStream {
       const int r = (lane >> 2) < last ? lane >> 2 : last;
       kr[g] = __builtin_nontemporal_load((global_u32x4*)(kb + (uint32_t)(r * (int)a.sk_s + 16 * (lane & 3))));
       vr[g] = __builtin_nontemporal_load((global_u32x4*)(vb + (uint32_t)(r * (int)a.sv_s + 16 * (lane & 3))));
+    }
+    // The scales last: the first chunk's are on their way with its codes.
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      info.ks[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scale), kGroups * turn + g));
+      info.v_log[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_log), kGroups * turn + g));
+      info.v_inv[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_inv), kGroups * turn + g));
     }
   }
   __device__ __forceinline__ void stage(uint8_t* ks, uint8_t* vs) const {
@@ -516,9 +525,6 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
   const PagedSeq& sq = it.sq;
   const ItemKeys<COLS> keys(a, it);
   if (!keys.any) return;
-  ChunkStream<NW, POOL, COLS> kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
-  if (kv.mine > 0) kv.load(0);
-
   // Q^T B operand: lane holds row r0 + l32 (clamped), d = 16c + 8g .. +7.
   const int row = it.r0 + l32 < it.r1 ? it.r0 + l32 : it.r1 - 1;
   const int tok = fast_div(row, a.group_div);
@@ -529,6 +535,11 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
   const int ends = sq.key_end(a, tok);
   const int khi = COLS || ends < keys.hi ? ends : keys.hi;
   const int kfull = wave_uniform(sq.key_end(a, fast_div(it.r0, a.group_div)));  // every row of the tile sees these
+  ChunkStream<NW, POOL, COLS> kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
+  if (kv.mine > 0) kv.load(0);
+  // Q is waited for here: in the loop the wait would be for the next chunk as well.
+#pragma unroll
+  for (int c = 0; c < 4; ++c) asm volatile("" ::"v"(qreg[c]));
 
   f32x16 oacc[2] = {};
   float m = -INFINITY, lsum = 0.f;
@@ -634,9 +645,6 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
   const PagedSeq& sq = it.sq;
   const ItemKeys<COLS> keys(a, it);
   if (!keys.any) return;
-  ChunkStream<NW, POOL, COLS> kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
-  if (kv.mine > 0) kv.load(0);
-
   const int row = it.r0 + l16 < it.r1 ? it.r0 + l16 : it.r1 - 1;
   const int tok = fast_div(row, a.group_div);
   const uint16_t* qp = a.q + (int64_t)(sq.q0 + tok) * a.sq_t + (int64_t)(it.h * a.group + row - tok * a.group) * a.sq_h;
@@ -646,6 +654,11 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
   const int ends = sq.key_end(a, tok);
   const int khi = COLS || ends < keys.hi ? ends : keys.hi;
   const int kfull = wave_uniform(sq.key_end(a, fast_div(it.r0, a.group_div)));  // every row sees these
+  ChunkStream<NW, POOL, COLS> kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
+  if (kv.mine > 0) kv.load(0);
+  // Q is waited for here: in the loop the wait would be for the next chunk as well.
+#pragma unroll
+  for (int c = 0; c < 2; ++c) asm volatile("" ::"v"(qreg[c]));
 
   f32x4 o[4] = {};  // O^T [16-d block]: lane (row l16, hq) holds d 16 db + 4 hq + r
   float m = -INFINITY, lsum = 0.f;
@@ -721,7 +734,8 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
 // Rows of 8-bit pools: 16 RT rows, NW waves that share the chunks of a range. S^T of 16 keys x 16 rows on
 // v_mfma_f32_16x16x32_bf16 from 16 codes of a key to a lane: the sums run over d in the order that
 // gives (16 hq + 8 c + e), which Q's operand takes as well. A chunk's codes are converted once for all RT
-// row tiles; its scales enter with the softmax's factor and with P.
+// row tiles. Its scales enter with the softmax: K's with the factor, V's in the exponent, so that what is
+// rounded to bf16 is P times it; the row sum takes its inverse again, once for 4 of the elements.
 template <int NW, int RT, int KC, int POOL, bool COLS>
 __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const PagedItem<false, COLS>& it, char* smem) {
   using Stream = CodeStream<NW, KC, POOL, COLS>;
@@ -737,8 +751,6 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
   const PagedSeq& sq = it.sq;
   const ItemKeys<COLS> keys(a, it);
   if (!keys.any) return;
-  Stream kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
-  if (kv.mine > 0) kv.load(0);
 
   bf16x8 qreg[RT][2];
   int khi[RT];
@@ -753,6 +765,13 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
     const int ends = sq.key_end(a, tok);
     khi[t] = COLS || ends < keys.hi ? ends : keys.hi;
   }
+  Stream kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
+  if (kv.mine > 0) kv.load(0);
+  // Q is waited for here: in the loop the wait would be for the next chunk's codes as well.
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) asm volatile("" ::"v"(qreg[t][c]));
   const int kfull = wave_uniform(sq.key_end(a, fast_div(it.r0, a.group_div)));  // every row sees these
 
   f32x4 o[RT][4] = {};  // O^T [16-d block]: lane (row l16, hq) holds d 16 db + 4 hq + r
@@ -774,6 +793,9 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
       kop[g][1] = cat8(codes4<POOL>(w[2]), codes4<POOL>(w[3]));
     }
     const bool masked = kv.masked(info, kfull);
+    float c2[kG];
+#pragma unroll
+    for (int g = 0; g < kG; ++g) c2[g] = a.scale_log2 * info.ks[g];
     bf16x8 pop[RT][kG / 2];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -785,6 +807,7 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
         s[g] = mfma16(kop[g][1], qreg[t][1], s[g]);
       }
       if (masked) {
+        asm volatile("");  // a branch: few chunks have any of it
 #pragma unroll
         for (int g = 0; g < kG; ++g)
 #pragma unroll
@@ -792,10 +815,8 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
             s[g][r] = info.base[g] + 4 * hq + r < khi[t] && ((info.there >> g) & 1) ? s[g][r] : -INFINITY;
       }
 #pragma unroll
-      for (int g = 0; g < kG; ++g)
-        mt = fmaxf(mt, fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3])) * info.ks[g]);
-      mt = fmaxf(mt, shfl_xor(mt, 16));
-      mt = max_xor32(mt);
+      for (int g = 0; g < kG; ++g) mt = fmaxf(mt, fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3])) * c2[g]);
+      mt = max_xor16_32(mt);
       if (__ballot(mt > m[t]) != 0) {
         const float mn = fmaxf(m[t], mt);
         const float alpha = (mn == -INFINITY) ? 1.f : fast_exp2(m[t] - mn);
@@ -808,12 +829,10 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
       f32x4 p[kG];
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
+        const float to = info.v_log[g] - mu;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[g][r] = fast_exp2(fmaf(s[g][r], info.ks[g], -mu));
-          lsum[t] += p[g][r];
-        }
-        p[g] *= info.vs[g];
+        for (int r = 0; r < 4; ++r) p[g][r] = fast_exp2(fmaf(s[g][r], c2[g], to));
+        lsum[t] = fmaf((p[g][0] + p[g][1]) + (p[g][2] + p[g][3]), info.v_inv[g], lsum[t]);
       }
 #pragma unroll
       for (int h2 = 0; h2 < kG / 2; ++h2)
@@ -957,15 +976,18 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     return key < hi ? table[key >> a.page_shift] : -1;
   };
   int ids = entries(0), ids_next = -1;
-  float k_scale = 1.f, v_scale = 1.f;  // 8-bit pools: of the same tiles' 16-key groups, K's with the softmax's factor
+  float k_scale = 1.f, v_log = 0.f, v_inv = 1.f;  // 8-bit pools: of the same tiles' 16-key groups, K's with the softmax's factor
   auto find_scales = [&](int base) {
     const int key = lo + (sub + SUBS * (base + (lane >> 2))) * kSwRows + 16 * (lane & 3);
-    k_scale = v_scale = 1.f;
+    k_scale = 1.f;
+    float v_scale = 1.f;
     if ((unsigned)ids < (unsigned)a.pages) {
       const int64_t at = ((int64_t)ids * a.kv_heads + h) * (a.page >> 4) + ((key & (a.page - 1)) >> 4);
       k_scale = a.k_scales[at] * a.scale_log2;
       v_scale = a.v_scales[at];
     }
+    v_log = fast_log2(v_scale);
+    v_inv = __builtin_amdgcn_rcpf(v_scale);
   };
   if constexpr (kCodes) find_scales(0);
 
@@ -994,7 +1016,7 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   const uint16_t* kh = static_cast<const uint16_t*>(a.k) + h * a.sk_h;
   const uint16_t* vh = static_cast<const uint16_t*>(a.v) + h * a.sv_h;
   uint32_t there = 0;  // quarters of the tile requested last whose page exists
-  float ks_next[4], vs_next[4];  // and their scales
+  float ks_next[4], v_log_next[4], v_inv_next[4];  // and their scales
   const uint32_t raw_w = lds_addr(&raw_all[kCodes ? sub : 0][kCodes ? 2 * wave : 0][0]);
   const uint8_t* raw = &raw_all[kCodes ? sub : 0][kCodes ? 2 * wave : 0][16 * lane];
   auto issue = [&](int i) {  // the set's i-th tile
@@ -1015,7 +1037,8 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         ks_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scale), 4 * (i & 15) + q));
-        vs_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_scale), 4 * (i & 15) + q));
+        v_log_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_log), 4 * (i & 15) + q));
+        v_inv_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_inv), 4 * (i & 15) + q));
       }
       const int top = lim < 0 ? 0 : lim;  // rows past the last key re-read it
       const int r = (lane >> 2) < top ? lane >> 2 : top;
@@ -1074,7 +1097,7 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   float mref = 0.f, lsum = 0.f;
   bool valid = false;  // the row has met a key
   const float c2 = a.scale_log2;
-  float k_factor[4], v_factor[4];  // 8-bit pools: the tile's
+  float k_factor[4], v_to[4], v_back[4];  // 8-bit pools: the tile's
   auto step = [&](int k0, uint32_t seen, const __bf16* ks, const __bf16* vs) {
     f32x16 s[2];
 #pragma unroll
@@ -1123,16 +1146,16 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     for (int sb = 0; sb < 2; ++sb) {
       float p[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = fast_exp2(fmaf(s[sb][r], kCodes ? k_factor[2 * sb + (r >> 3)] : c2, -mref));
+      for (int r = 0; r < 16; ++r)
+        p[r] = kCodes ? fast_exp2(fmaf(s[sb][r], k_factor[2 * sb + (r >> 3)], v_to[2 * sb + (r >> 3)] - mref))
+                      : fast_exp2(fmaf(s[sb][r], c2, -mref));
 #pragma unroll
       for (int kc = 0; kc < 2; ++kc) {
-        const float f = kCodes ? v_factor[2 * sb + kc] : 1.f;
-        const bf16x8 pop = kCodes ? to_bf16x8(p[8 * kc] * f, p[8 * kc + 1] * f, p[8 * kc + 2] * f, p[8 * kc + 3] * f,
-                                              p[8 * kc + 4] * f, p[8 * kc + 5] * f, p[8 * kc + 6] * f, p[8 * kc + 7] * f)
-                                  : to_bf16x8(p[8 * kc], p[8 * kc + 1], p[8 * kc + 2], p[8 * kc + 3], p[8 * kc + 4],
-                                              p[8 * kc + 5], p[8 * kc + 6], p[8 * kc + 7]);
-        lsum += ((p[8 * kc] + p[8 * kc + 1]) + (p[8 * kc + 2] + p[8 * kc + 3])) +
-                ((p[8 * kc + 4] + p[8 * kc + 5]) + (p[8 * kc + 6] + p[8 * kc + 7]));
+        const bf16x8 pop = to_bf16x8(p[8 * kc], p[8 * kc + 1], p[8 * kc + 2], p[8 * kc + 3], p[8 * kc + 4],
+                                     p[8 * kc + 5], p[8 * kc + 6], p[8 * kc + 7]);
+        const float sum = ((p[8 * kc] + p[8 * kc + 1]) + (p[8 * kc + 2] + p[8 * kc + 3])) +
+                          ((p[8 * kc + 4] + p[8 * kc + 5]) + (p[8 * kc + 6] + p[8 * kc + 7]));
+        lsum = kCodes ? fmaf(sum, v_back[2 * sb + kc], lsum) : lsum + sum;
 #pragma unroll
         for (int db = 0; db < 2; ++db) o[db] = mfma32(sw_tr_op(vs, 32 * sb + 16 * kc, 32 * db, lane), pop, o[db]);
       }
@@ -1144,7 +1167,8 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       k_factor[q] = ks_next[q];
-      v_factor[q] = vs_next[q];
+      v_to[q] = v_log_next[q];
+      v_back[q] = v_inv_next[q];
     }
   };
   if constexpr (kCodes) {
