@@ -87,11 +87,32 @@ __global__ __launch_bounds__(256) void paged_rope8_kernel(PagedRopeArgs a) {
   const bool mine = pos >= c && pos < it.sq.kv;
   const int tok = it.sq.q0 + pos - c;
 
-  f32x4 y[4] = {};  // [half][4 of the 8]
+  // The page and the block's scale are asked for first, so that their round trips are the rotation's. Nothing
+  // is written where the table has no page for the block.
+  const bool is_q = hh < a.heads, is_k = !is_q && hh < a.heads + a.kv_heads;
+  const int kh = hh - a.heads - (is_k ? 0 : a.kv_heads);
+  const int64_t slot = begin & (a.page - 1);
+  int page = -1;
+  if (!is_q && begin >= 0 && (begin >> a.page_shift) < a.width)
+    page = a.table[(int64_t)it.b * a.table_s + (begin >> a.page_shift)];
+  u32x4 x1 = {}, x2 = {};
   if (mine) {
     const uint16_t* src = a.qkv + (int64_t)tok * a.sx_t + hh * kHeadDim + 8 * j;
-    const bf16x8 b1 = __builtin_bit_cast(bf16x8, ld16(src)), b2 = __builtin_bit_cast(bf16x8, ld16(src + kHeadDim / 2));
-    if (hh < a.heads + a.kv_heads) {
+    x1 = ld16(src);
+    x2 = ld16(src + kHeadDim / 2);
+  }
+  page = wave_uniform(page);
+  const bool there = (unsigned)page < (unsigned)a.pages;
+  float* scale_p =
+      (is_k ? a.k_scales : a.v_scales) + ((int64_t)(there ? page : 0) * a.kv_heads + (is_q ? 0 : kh)) * (a.page >> 4) + (slot >> 4);
+  const bool kept = begin < c;  // the block holds earlier tokens
+  float old_scale = 0.f;
+  if (there && kept) old_scale = *scale_p;
+
+  f32x4 y[4] = {};  // [half][4 of the 8]
+  if (mine) {
+    const bf16x8 b1 = __builtin_bit_cast(bf16x8, x1), b2 = __builtin_bit_cast(bf16x8, x2);
+    if (is_q || is_k) {
       const int64_t tp = pos < 0 ? 0 : (pos >= a.max_pos ? a.max_pos - 1 : pos);
       const float* cp = a.cos_t + tp * (kHeadDim / 2) + 8 * j;
       const float* sp = a.sin_t + tp * (kHeadDim / 2) + 8 * j;
@@ -109,7 +130,7 @@ __global__ __launch_bounds__(256) void paged_rope8_kernel(PagedRopeArgs a) {
       }
     }
   }
-  if (hh < a.heads) {
+  if (is_q) {
     if (!mine) return;
     uint16_t* dst = a.q + (int64_t)tok * a.sq_t + (int64_t)hh * a.sq_h + 8 * j;
 #pragma unroll
@@ -119,27 +140,20 @@ __global__ __launch_bounds__(256) void paged_rope8_kernel(PagedRopeArgs a) {
                     y[2 * h2 + 1][2], y[2 * h2 + 1][3]);
     return;
   }
-  // Nothing is written where the table has no page for the block.
-  if (begin < 0 || (begin >> a.page_shift) >= a.width) return;
-  const int page = wave_uniform(a.table[(int64_t)it.b * a.table_s + (begin >> a.page_shift)]);
-  if ((unsigned)page >= (unsigned)a.pages) return;
-  const bool is_k = hh < a.heads + a.kv_heads;
-  const int kh = hh - a.heads - (is_k ? 0 : a.kv_heads);
-  const int64_t slot = begin & (a.page - 1);
+  if (!there) return;
   const int64_t row_s = is_k ? a.sk_s : a.sv_s;
   uint8_t* dst = static_cast<uint8_t*>(is_k ? a.k : a.v) + (int64_t)page * (is_k ? a.sk_p : a.sv_p) +
                  (int64_t)kh * (is_k ? a.sk_h : a.sv_h) + (slot + r) * row_s + 8 * j;
-  float* scale_p = (is_k ? a.k_scales : a.v_scales) + ((int64_t)page * a.kv_heads + kh) * (a.page >> 4) + (slot >> 4);
 
   float m = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(y[i >> 2][i & 3]));
   m = fminf(wave_max(m), 3.4028235e38f);
   const uint32_t need = wave_uniform_u32(needed_scale<POOL>(m));
-  const uint32_t old = wave_uniform_u32(__float_as_uint(*scale_p));
+  const uint32_t old = wave_uniform_u32(__float_as_uint(old_scale));
   uint32_t scale = need;
   int grow = 0;
-  if (begin < c && old >= kSmallestScale && old < kInf) {  // holds earlier tokens, at a scale that is one
+  if (kept && old >= kSmallestScale && old < kInf) {  // at a scale that is one
     grow = (int)(need >> 23) - (int)(old >> 23) + ((need & 0x7fffffu) > (old & 0x7fffffu));
     grow = grow > 0 ? grow : 0;
     scale = old + ((uint32_t)grow << 23);
@@ -161,7 +175,7 @@ __global__ __launch_bounds__(256) void paged_rope8_kernel(PagedRopeArgs a) {
   }
   *reinterpret_cast<u32x2*>(dst) = codes[0];
   *reinterpret_cast<u32x2*>(dst + 32) = codes[1];
-  if (r == (c > begin ? c - begin : 0) && j == 0) *scale_p = __uint_as_float(scale);  // the first new row's lane
+  if (r == (kept ? c - begin : 0) && j == 0) *scale_p = __uint_as_float(scale);  // the first new row's lane
 }
 
 // Values of whole pools: a wave takes a block of 16 rows of a head, 16 codes a lane.
