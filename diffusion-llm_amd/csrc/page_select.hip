@@ -2,7 +2,7 @@
 // and the pages that promise most.
 //
 // bounds[page][KV head] = the lowest and the highest key of the page, channel by channel.
-// No key k of the page has a larger q . k than
+// No key k of the page has a larger q . k than (values of 8-bit pools: but for the bounds' rounding to bf16, 2^-9)
 //     score = sum_d max(q_d low_d, q_d high_d) = q+ . high + q- . low
 // (q+ = max(q, 0), q- = min(q, 0)), a product of length 128 on the matrix cores. The
 // queries of one block of the chunk (they see the same keys) and the heads of a KV
@@ -189,7 +189,8 @@ struct ColumnScores {
   }
   // Bound of the scores' distance from the exact sums: 64 additions of terms that are not zeros, each off by at most
   // 2^-23 of the terms' absolute sum whatever their order and rounding; 2^-16 for 2^-17, which covers that sum's own.
-  __device__ __forceinline__ float error() const { return wave_max(most) * 0x1p-16f; }
+  // And twice 128 terms and sums that may have lost 2^-126 each: below it numbers may lose their bits.
+  __device__ __forceinline__ float error() const { return fmaf(wave_max(most), 0x1p-16f, 0x1p-118f); }
 };
 
 // Floats in the order of unsigned integers; 0 is below all, kForced above.

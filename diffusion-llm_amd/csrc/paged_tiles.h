@@ -80,46 +80,40 @@ struct KeySplit {
 };
 
 // What a chunk's two halves of 16 keys are: whether their page is there, the position of
-// their first key, their scales (8-bit pools).
+// their first key.
 struct ChunkInfo {
   uint32_t there;
   int base[2];
-  float ks[2], vs[2];
 };
 
 // The 32-key chunks of one key range that one of NW waves takes in turn (chunks
 // wave, wave + NW, ...): from the pages to registers, the next chunk's loads in
 // flight while the last one, staged in the wave's LDS tiles, is computed.
-template <int NW, int POOL, bool COLS>
+template <int NW, bool COLS>
 struct ChunkStream {
-  static constexpr bool kCodes = POOL != kPoolBf16;
-  static constexpr int kLoads = kCodes ? 2 : 4;
-  static constexpr int kBytes = kCodes ? 1 : 2;        // of an element
-  static constexpr int kParts = kCodes ? 4 : 8;        // 16-byte parts of a row
   const PagedArgs& a;
   const int32_t* table;
   const int32_t* list;  // COLS: the block's columns
-  const char *kh, *vh;  // the head's rows of page 0
-  int h, lo, hi, end, wave, lane, mine;
+  const uint16_t *kh, *vh;  // the head's rows of page 0
+  int lo, hi, end, wave, lane, mine;
   int ids;        // lane 2 i + half: page of the half's 16 keys (a page holds at least 16) of chunk base + i
   int at_key;     // COLS: position of the first of them
-  float k_scale, v_scale;  // 8-bit pools: their scales
   uint64_t ok;    // which of them exist
-  u32x4 kr[kLoads], vr[kLoads];  // lane + 64 j -> key row (64 j + lane) / kParts of the chunk, 16-byte part lane % kParts
+  u32x4 kr[4], vr[4];  // lane + 64 j -> key row 8 j + lane / 8 of the chunk, 16-byte part lane % 8
   ChunkInfo info;      // of the loaded chunk
 
   // Keys lo .. hi - 1 of the range (of the list, COLS); none from `end` on is a key of the rows.
   __device__ __forceinline__ ChunkStream(const PagedArgs& a_, int b, int h_, const int32_t* list_, int lo_, int hi_,
                                          int end_, int wave_, int lane_)
-      : a(a_), list(list_), h(h_), lo(lo_), hi(hi_), end(end_), wave(wave_), lane(lane_), info() {
+      : a(a_), list(list_), lo(lo_), hi(hi_), end(end_), wave(wave_), lane(lane_), info() {
     table = a.table + (int64_t)b * a.table_s;
-    kh = reinterpret_cast<const char*>(a.k) + kBytes * h * a.sk_h;
-    vh = reinterpret_cast<const char*>(a.v) + kBytes * h * a.sv_h;
+    kh = static_cast<const uint16_t*>(a.k) + h_ * a.sk_h;
+    vh = static_cast<const uint16_t*>(a.v) + h_ * a.sv_h;
     const int n = hi > lo ? (hi - lo + kSub - 1) / kSub : 0;
     mine = n > wave ? (n - wave + NW - 1) / NW : 0;
   }
   __device__ __forceinline__ int first_key(int i) const { return lo + (wave + NW * i) * kSub; }
-  __device__ __forceinline__ void find(int i) {  // pages and scales of 32 chunks
+  __device__ __forceinline__ void find(int i) {  // pages of 32 chunks
     int key = first_key(i + (lane >> 1)) + 16 * (lane & 1);
     ids = -1;
     if (key < hi) {
@@ -134,16 +128,7 @@ struct ChunkStream {
       }
     }
     if constexpr (COLS) at_key = key;
-    const bool is = (unsigned)ids < (unsigned)a.pages;
-    ok = __ballot(is);
-    if constexpr (kCodes) {
-      k_scale = v_scale = 1.f;
-      if (is) {
-        const int64_t at = ((int64_t)ids * a.kv_heads + h) * (a.page >> 4) + ((key & (a.page - 1)) >> 4);
-        k_scale = a.k_scales[at];
-        v_scale = a.v_scales[at];
-      }
-    }
+    ok = __ballot((unsigned)ids < (unsigned)a.pages);
   }
   __device__ __forceinline__ void load(int i) {
     if ((i & 31) == 0) find(i);
@@ -153,22 +138,18 @@ struct ChunkStream {
       const int at = 2 * (i & 31) + hh;
       const int key = COLS ? __builtin_amdgcn_readlane(at_key, at) : first_key(i) + 16 * hh;
       info.base[hh] = key;
-      if constexpr (kCodes) {
-        info.ks[hh] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scale), at));
-        info.vs[hh] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_scale), at));
-      }
       const bool is = (info.there >> hh) & 1;
       const int64_t page = __builtin_amdgcn_readlane(ids, at);
       const int64_t slot = key & (a.page - 1);
-      const uint64_t kb = (uint64_t)(uintptr_t)(is ? kh + kBytes * (page * a.sk_p + slot * a.sk_s) : (const char*)zero_row);
-      const uint64_t vb = (uint64_t)(uintptr_t)(is ? vh + kBytes * (page * a.sv_p + slot * a.sv_s) : (const char*)zero_row);
+      const uint64_t kb = (uint64_t)(uintptr_t)(is ? kh + page * a.sk_p + slot * a.sk_s : zero_row);
+      const uint64_t vb = (uint64_t)(uintptr_t)(is ? vh + page * a.sv_p + slot * a.sv_s : zero_row);
       const int last = is ? (COLS ? end : hi) - 1 - key : 0;  // rows past the last key re-read it
 #pragma unroll
-      for (int j = 0; j < kLoads / 2; ++j) {
-        const int mine = (lane + 64 * j) / kParts, part = 16 * (lane % kParts);
+      for (int j = 0; j < 2; ++j) {
+        const int mine = (lane >> 3) + 8 * j, part = 16 * (lane & 7);
         const int r = mine < last ? mine : last;
-        kr[kLoads / 2 * hh + j] = __builtin_nontemporal_load((global_u32x4*)(kb + (uint32_t)(kBytes * r * (int)a.sk_s + part)));
-        vr[kLoads / 2 * hh + j] = __builtin_nontemporal_load((global_u32x4*)(vb + (uint32_t)(kBytes * r * (int)a.sv_s + part)));
+        kr[2 * hh + j] = __builtin_nontemporal_load((global_u32x4*)(kb + (uint32_t)(2 * r * (int)a.sk_s + part)));
+        vr[2 * hh + j] = __builtin_nontemporal_load((global_u32x4*)(vb + (uint32_t)(2 * r * (int)a.sv_s + part)));
       }
     }
   }
@@ -177,25 +158,12 @@ struct ChunkStream {
     if constexpr (COLS) return c.base[0] + 16 > kfull || c.base[1] + 16 > kfull || c.there != 3;
     return c.base[0] + kSub > kfull || c.base[0] + kSub > hi || c.there != 3;
   }
-  // From a product of codes to a score times log2(e).
-  __device__ __forceinline__ float factor(const ChunkInfo& c, int hh) const {
-    return kCodes ? a.scale_log2 * c.ks[hh] : a.scale_log2;
-  }
-  __device__ __forceinline__ static void put(__bf16* to, u32x4 x) {  // 16 bytes of a row
-    if constexpr (kCodes) {
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-        *reinterpret_cast<bf16x8*>(to + 8 * w) = cat8(codes4<POOL>(x[2 * w]), codes4<POOL>(x[2 * w + 1]));
-    } else {
-      *reinterpret_cast<u32x4*>(to) = x;
-    }
-  }
   __device__ __forceinline__ void stage(__bf16* ks, __bf16* vs) const {
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int off = (lane + 64 * j) / kParts * kStride + 16 / kBytes * (lane % kParts);
-      put(&ks[off], kr[j]);
-      put(&vs[off], vr[j]);
+    for (int j = 0; j < 4; ++j) {
+      const int off = (8 * j + (lane >> 3)) * kStride + 8 * (lane & 7);
+      *reinterpret_cast<u32x4*>(&ks[off]) = kr[j];
+      *reinterpret_cast<u32x4*>(&vs[off]) = vr[j];
     }
   }
 };
@@ -512,7 +480,7 @@ struct ItemKeys {
 // keys of 8 sequences 13.9 us against 15.1; over 4032 keys of 48 sequences 111, 104.
 // At four waves per SIMD it spills (43 -> 50 us). Full launches are bound by HBM (32
 // sequences x 4128 keys 73 us, 5.6 TB/s; contiguous 65).
-template <int NW, int POOL, bool COLS>
+template <int NW, bool COLS>
 __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem<false, COLS>& it, char* smem) {
   const int tid = wi_x();
   const int lane = tid & 63;
@@ -535,7 +503,7 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
   const int ends = sq.key_end(a, tok);
   const int khi = COLS || ends < keys.hi ? ends : keys.hi;
   const int kfull = wave_uniform(sq.key_end(a, fast_div(it.r0, a.group_div)));  // every row of the tile sees these
-  ChunkStream<NW, POOL, COLS> kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
+  ChunkStream<NW, COLS> kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
   if (kv.mine > 0) kv.load(0);
   // Q is waited for here: in the loop the wait would be for the next chunk as well.
 #pragma unroll
@@ -561,18 +529,10 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
         s[r] = key < khi && ((info.there >> (r >> 3)) & 1) ? s[r] : -INFINITY;
       }
     }
-    const float c2[2] = {kv.factor(info, 0), kv.factor(info, 1)};
     float mt = -INFINITY;
-    if constexpr (POOL == kPoolBf16) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[r]);
-      mt = max_xor32(mt) * a.scale_log2;
-    } else {
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx[r >> 3] = fmaxf(mx[r >> 3], s[r]);
-      mt = max_xor32(fmaxf(mx[0] * c2[0], mx[1] * c2[1]));
-    }
+    for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[r]);
+    mt = max_xor32(mt) * a.scale_log2;
     if (__ballot(mt > m) != 0) {
       const float mn = fmaxf(m, mt);
       const float alpha = (mn == -INFINITY) ? 1.f : fast_exp2(m - mn);
@@ -585,9 +545,8 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
     float p[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      p[r] = fast_exp2(fmaf(s[r], c2[r >> 3], -mu));
+      p[r] = fast_exp2(fmaf(s[r], a.scale_log2, -mu));
       lsum += p[r];
-      if constexpr (POOL != kPoolBf16) p[r] *= info.vs[r >> 3];
     }
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc) {
@@ -631,7 +590,7 @@ __device__ __forceinline__ void paged32_item(const PagedArgs& a, const PagedItem
 // lengths are there after 0.5 us, the first chunk is staged after 2.8, done after 3.4,
 // merged and written after 4.6 of the kernel's 7.8 us. Many are bound by HBM: 32
 // sequences of 100-8192 keys 48 us, 5.5 TB/s.
-template <int NW, int POOL, bool COLS>
+template <int NW, bool COLS>
 __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem<false, COLS>& it, char* smem) {
   constexpr int kRows = 16;
   const int tid = wi_x();
@@ -654,7 +613,7 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
   const int ends = sq.key_end(a, tok);
   const int khi = COLS || ends < keys.hi ? ends : keys.hi;
   const int kfull = wave_uniform(sq.key_end(a, fast_div(it.r0, a.group_div)));  // every row sees these
-  ChunkStream<NW, POOL, COLS> kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
+  ChunkStream<NW, COLS> kv(a, it.b, it.h, it.list, keys.lo, keys.hi, keys.end, wave, lane);
   if (kv.mine > 0) kv.load(0);
   // Q is waited for here: in the loop the wait would be for the next chunk as well.
 #pragma unroll
@@ -682,13 +641,11 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
         for (int r = 0; r < 4; ++r)
           s[kb][r] = info.base[kb] + 4 * hq + r < khi && ((info.there >> kb) & 1) ? s[kb][r] : -INFINITY;
     }
-    const float c2[2] = {kv.factor(info, 0), kv.factor(info, 1)};
     const float mx0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
     const float mx1 = fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]));
-    float mt = POOL == kPoolBf16 ? fmaxf(mx0, mx1) : fmaxf(mx0 * c2[0], mx1 * c2[1]);
+    float mt = fmaxf(mx0, mx1);
     mt = fmaxf(mt, shfl_xor(mt, 16));
-    mt = max_xor32(mt);
-    if constexpr (POOL == kPoolBf16) mt *= a.scale_log2;
+    mt = max_xor32(mt) * a.scale_log2;
     if (__ballot(mt > m) != 0) {
       const float mn = fmaxf(m, mt);
       const float alpha = (mn == -INFINITY) ? 1.f : fast_exp2(m - mn);
@@ -703,9 +660,8 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[kb][r] = fast_exp2(fmaf(s[kb][r], c2[kb], -mu));
+        p[kb][r] = fast_exp2(fmaf(s[kb][r], a.scale_log2, -mu));
         lsum += p[kb][r];
-        if constexpr (POOL != kPoolBf16) p[kb][r] *= info.vs[kb];
       }
     const bf16x8 pop = to_bf16x8(p[0][0], p[0][1], p[0][2], p[0][3], p[1][0], p[1][1], p[1][2], p[1][3]);
     const int vrow = 4 * hq + tr_row;
@@ -735,7 +691,8 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
 // v_mfma_f32_16x16x32_bf16 from 16 codes of a key to a lane: the sums run over d in the order that
 // gives (16 hq + 8 c + e), which Q's operand takes as well. A chunk's codes are converted once for all RT
 // row tiles. Its scales enter with the softmax: K's with the factor, V's in the exponent, so that what is
-// rounded to bf16 is P times it; the row sum takes its inverse again, once for 4 of the elements.
+// rounded to bf16 is P times it; the row sum takes its inverse again, once for 4 of the elements. (log2 scale - maximum
+// is off by 2^-24 of the maximum, no more than the scores' own fp32 sums.)
 template <int NW, int RT, int KC, int POOL, bool COLS>
 __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const PagedItem<false, COLS>& it, char* smem) {
   using Stream = CodeStream<NW, KC, POOL, COLS>;
@@ -885,7 +842,7 @@ __global__ __launch_bounds__(NW * 64, WPS) void paged_codes_kernel(PagedArgs a) 
   }
 }
 
-template <int NW, int ROWS, int POOL, bool COLS>
+template <int NW, int ROWS, bool COLS>
 __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void paged_rows_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[chunk_smem<NW, ROWS>()];
   // The launch has about as many workgroups as there are items; those left over
@@ -895,9 +852,9 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
     if (!it.found) return;
     if (!COLS || it.r0 < it.r1) {
       if constexpr (ROWS == 16)
-        paged16_item<NW, POOL, COLS>(a, it, smem);
+        paged16_item<NW, COLS>(a, it, smem);
       else
-        paged32_item<NW, POOL, COLS>(a, it, smem);
+        paged32_item<NW, COLS>(a, it, smem);
     }
     if (id + a.workgroups >= it.total) return;
     __syncthreads();
@@ -1361,11 +1318,11 @@ hipError_t launch_paged_tiles(const PagedArgs& a, hipStream_t stream) {
       hipLaunchKernelGGL((paged_codes_kernel<4, 3, 64, 2, POOL, COLS>), grid, dim3(256), 0, stream, a);
   } else {
     if (a.tile == 16)
-      hipLaunchKernelGGL((paged_rows_kernel<8, 16, POOL, COLS>), grid, dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((paged_rows_kernel<8, 16, COLS>), grid, dim3(512), 0, stream, a);
     else if (a.subs == 2)
-      hipLaunchKernelGGL((paged_rows_kernel<8, 32, POOL, COLS>), grid, dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((paged_rows_kernel<8, 32, COLS>), grid, dim3(512), 0, stream, a);
     else
-      hipLaunchKernelGGL((paged_rows_kernel<4, 32, POOL, COLS>), grid, dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((paged_rows_kernel<4, 32, COLS>), grid, dim3(256), 0, stream, a);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.n_splits == 1) return e;

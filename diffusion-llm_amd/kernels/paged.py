@@ -194,7 +194,7 @@ def select_pages(
         max over the block's tokens and the KV head's query heads of
         sum_d max(q_d * lowest_d, q_d * highest_d),
 
-    which no key of the page exceeds in q . k; equals by the lower column. The
+    which no key of the page exceeds in q . k (of 8-bit pages but for the bounds' rounding to bf16); equals by the lower column. The
     scores' order is exact. `top` must leave room for the columns always taken. Rows behind the last
     sequence are left as they are (without `out` undefined). Bounds of the columns always taken are
     not read; those of the others must be finite."""

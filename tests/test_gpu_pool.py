@@ -393,7 +393,7 @@ def pick(d, bounds, bs, page, top, first=1, recent=1, **kw):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind", ["random", "equal", "near", "zero", "wide", "huge"])
+@pytest.mark.parametrize("kind", ["random", "equal", "near", "zero", "wide", "huge", "tiny", "subnormal"])
 @pytest.mark.parametrize("lens,heads,kv_heads,page,bs,top,first,recent", SELECT)
 def test_selection_matches_definition(cuda, lens, heads, kv_heads, page, bs, top, first, recent, kind):
     """Columns to the last one, also where scores are equal, or differ by less than fp32 sums do."""
@@ -415,6 +415,10 @@ def test_selection_matches_definition(cuda, lens, heads, kv_heads, page, bs, top
         bounds = (bounds[:1].float() * big + torch.randn(bounds.shape, generator=g) * 2.0 ** -6).to(BF)
     elif kind == "huge":  # fp32 sums overflow
         bounds, c["q"] = (bounds.float() * 2.0 ** 64).to(BF), (c["q"].float() * 2.0 ** 62).to(BF)
+    elif kind == "tiny":  # products about fp32's smallest
+        bounds, c["q"] = (bounds.float() * 2.0 ** -66).to(BF), (c["q"].float() * 2.0 ** -62).to(BF)
+    elif kind == "subnormal":  # bf16's smallest, few bits of them
+        bounds, c["q"] = (bounds.float() * 2.0 ** -130).to(BF), (c["q"].float() * 2.0 ** 100).to(BF)
     c["table"][0, 0] = -1 if len(lens) > 1 else c["table"][0, 0]
     want = orc.select_pages(c["q"], bounds, c["table"], c["starts"], c["kv"], bs, page, top, first, recent)
     d = on(c, cuda)
