@@ -241,7 +241,7 @@ struct SelectArgs {
   int width;                 // columns within max_kv
   int first, recent;         // columns always taken
   // Where select_in_two:
-  float* scores;             // (slots, kv_heads, width)
+  uint32_t* keys;            // (slots, kv_heads, width): the scores as ordered numbers
   float* error;              // (slots, kv_heads, ceil(width / 16)): bound of the scores' distance from the exact sums
   double* sums;              // (slots, kv_heads, width)
 };

@@ -1486,8 +1486,8 @@ int bd3_select_pages(const void* q, const void* bounds, const int32_t* page_tabl
   a.recent = recent;
   if (need > 0) {
     a.sums = static_cast<double*>(workspace);
-    a.scores = reinterpret_cast<float*>(a.sums + items * width);
-    a.error = a.scores + items * width;
+    a.keys = reinterpret_cast<uint32_t*>(a.sums + items * width);
+    a.error = reinterpret_cast<float*>(a.keys + items * width);
   }
   return hip_status(bd3::launch_select_pages(a, static_cast<hipStream_t>(stream)), "select_pages launch");
 }

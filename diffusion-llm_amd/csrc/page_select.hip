@@ -75,13 +75,16 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(SelectArgs s) {
       }
     }
   }
+  // Over the lanes of one part: rotations by 4 and 8 within 16 lanes, then across these.
+  const auto over_rows = [](float x) {
+    if constexpr (kParts == 4) x = fmaxf(x, dpp_move<0x124>(x));
+    return max_xor16_32(fmaxf(x, dpp_move<0x128>(x)));
+  };
 #pragma unroll
-  for (int m = kParts; m < 64; m <<= 1)
-#pragma unroll
-    for (int i = 0; i < kCh; ++i) {
-      lo[i] = fminf(lo[i], shfl_xor(lo[i], m));
-      hi[i] = fmaxf(hi[i], shfl_xor(hi[i], m));
-    }
+  for (int i = 0; i < kCh; ++i) {
+    lo[i] = -over_rows(-lo[i]);
+    hi[i] = over_rows(hi[i]);
+  }
   if (lane >= kParts) return;
   uint16_t* out = s.bounds + ((int64_t)page * a.kv_heads + h) * (2 * kHeadDim) + kCh * part;
 #pragma unroll
@@ -167,8 +170,7 @@ struct ColumnScores {
   }
   __device__ __forceinline__ float scores(const Box& box) {
     float best = -INFINITY;
-    u32x4 x0 = q0, x1 = q1;
-    for (int r0 = 0;;) {
+    const auto add = [&](u32x4 x0, u32x4 x1) {
       const bf16x8 part[4] = {positive(x0), positive(x1), negative(x0), negative(x1)};
       f32x4 acc = {}, sum = {};
 #pragma unroll
@@ -178,11 +180,11 @@ struct ColumnScores {
       }
       best = fmaxf(fmaxf(best, fmaxf(acc[0], acc[1])), fmaxf(acc[2], acc[3]));
       most = fmaxf(fmaxf(most, fmaxf(sum[0], sum[1])), fmaxf(sum[2], sum[3]));
-      r0 += 16;
-      if (r0 >= rows) break;
+    };
+    add(q0, q1);  // before the loop, whose waits are for the next columns' bounds as well
+    for (int r0 = 16; r0 < rows; r0 += 16) {
       const uint16_t* qp = row(r0);
-      x0 = ld16(qp);
-      x1 = ld16(qp + 32);
+      add(ld16(qp), ld16(qp + 32));
     }
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(best), __float_as_uint(best), false, false);
     return max_xor32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
@@ -249,10 +251,14 @@ __device__ __forceinline__ double exact_score(const ColumnScores& c, int page) {
 // What the waves of a workgroup tell each other.
 constexpr int kBins = 512;
 constexpr int kPasses = 4;  // of 9 bits of a key's 32
+constexpr int kFew = 64;    // columns in doubt that are ranked in registers
 template <int NW>
 struct TeamLds {
   uint32_t words[2][5][NW];
   uint32_t bins[kPasses][kBins];
+  double sums[kFew];  // of the columns in doubt
+  int cols[kFew];
+  int doubtful;
 };
 enum Merge { kSum, kLeast, kMost };
 template <int NW>
@@ -317,24 +323,25 @@ struct Known {
 
 // The selection of one block and KV head by NW waves: wave w has the groups of 64 columns from w * per on, `per` to
 // a wave; their keys stay in registers (per <= R) or, R = 0, are asked for again each time. key(g) is the
-// lane's of group g, after a barrier here: 0 no candidate, kForced always taken. sums: a double for each column.
+// lane's of group g: 0 no candidate, kForced always taken. Where the wave has them already (OWN) they come in `kept`,
+// else they are there after a barrier here. sums: a double for each column.
 //
 // The threshold is found by histograms of 512 bins over the range of keys that it is known to be in (a bit search
 // took 20 passes over the keys and 27 of the 39 us of a call on one token over 1000 pages).
-template <int NW, int R, class Key>
+template <int NW, int R, bool OWN, class Key>
 __device__ __forceinline__ void choose(const SelectArgs& s, const ColumnScores& c, const PagedSeq& sq, const QueryBlock& blk,
-                                       const int32_t* table, Known known, Key key, double* sums, Team<NW> team) {
+                                       const int32_t* table, int per, uint32_t (&kept)[R > 0 ? R : 1], Known known, Key key,
+                                       double* sums, Team<NW> team) {
   const PagedArgs& a = s.p;
   const int lane = wi_x() & 63;
   const int groups = (blk.cols + 63) >> 6;
-  const int per = (groups + NW - 1) / NW;
   const int g0 = team.wave * per;
   const int n = g0 < groups ? (g0 + per < groups ? per : groups - g0) : 0;
 #pragma unroll
   for (int b = 0; b < kPasses * kBins; b += 64 * NW) (&team.lds.bins[0][0])[b + wi_x()] = 0;
   static_assert(kPasses * kBins % (64 * NW) == 0, "whole turns");
+  if (wi_x() == 0) team.lds.doubtful = 0;
   team.template join<kSum, kSum, kLeast, kMost, kMost>(known.v);
-  uint32_t kept[R > 0 ? R : 1];
   const auto reread = [&](auto f) {
     for (int i = 0; i < n; ++i) f(g0 + i, key(g0 + i));
   };
@@ -346,7 +353,7 @@ __device__ __forceinline__ void choose(const SelectArgs& s, const ColumnScores& 
       reread(f);
     }
   };
-  if constexpr (R > 0) {
+  if constexpr (R > 0 && !OWN) {
 #pragma unroll
     for (int i = 0; i < R; ++i) kept[i] = i < n ? key(g0 + i) : 0;
   }
@@ -413,19 +420,54 @@ __device__ __forceinline__ void choose(const SelectArgs& s, const ColumnScores& 
       // 2.01: these sums round as well, by 2^-24 |v| < 2^-8 err
       sure = bounded ? order_key(v + 2.01f * err) + 1 : kForced;
       doubt = bounded ? order_key(v - 2.01f * err) : 1;
-      uint32_t above[1] = {0};
-      reread([&](int g, uint32_t k) {
-        above[0] += __popcll(__ballot(k >= sure));
-        uint64_t in = __ballot(k >= doubt && k < sure);
-        while (in != 0) {
-          const int col = 64 * g + __builtin_ctzll(in);
-          in &= in - 1;
-          const double e = exact_score(c, wave_uniform(table[col]));
-          if (lane == 0) sums[col] = e;
-        }
+      uint32_t count[2] = {0, 0};  // sure ones, doubtful ones
+      each([&](int g, uint32_t k) {
+        const bool maybe = k >= doubt && k < sure;
+        const uint64_t in = __ballot(maybe);
+        count[0] += __popcll(__ballot(k >= sure));
+        count[1] += __popcll(in);
+        if (R == 0 || in == 0) return;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&team.lds.doubtful, (int)__popcll(in));
+        at = wave_uniform(at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+        if (maybe && at < kFew) team.lds.cols[at] = 64 * g + lane;
       });
-      team.template join<kSum>(above);  // its barrier also shows the sums
-      open = a.top - (int)above[0];
+      team.template join<kSum, kSum>(count);  // its barrier also shows the columns
+      open = a.top - (int)count[0];
+      const int few = (int)count[1];
+      if (R > 0 && few <= kFew) {  // a lane each
+        for (int i = team.wave; i < few; i += NW) {
+          const double e = exact_score(c, wave_uniform(table[wave_uniform(team.lds.cols[i])]));
+          if (lane == 0) team.lds.sums[i] = e;
+        }
+        __syncthreads();
+        const int col = lane < few ? team.lds.cols[lane] : -1;
+        const double mine = lane < few ? team.lds.sums[lane] : 0.0;
+        int ahead = 0;
+        for (int i = 0; i < few; ++i) {
+          const double e = team.lds.sums[i];
+          ahead += e > mine || (e == mine && __builtin_amdgcn_readlane(col, i) < col);
+        }
+        uint64_t in = __ballot(lane < few && ahead < open);
+        while (in != 0) {
+          const int at = __builtin_amdgcn_readlane(col, __builtin_ctzll(in));
+          in &= in - 1;
+#pragma unroll
+          for (int i = 0; i < R; ++i) kept[i] = i < n && 64 * (g0 + i) + lane == at ? kForced : kept[i];
+        }
+        open = 0;
+      } else {
+        reread([&](int g, uint32_t k) {
+          uint64_t in = __ballot(k >= doubt && k < sure);
+          while (in != 0) {
+            const int col = 64 * g + __builtin_ctzll(in);
+            in &= in - 1;
+            const double e = exact_score(c, wave_uniform(table[col]));
+            if (lane == 0) sums[col] = e;
+          }
+        });
+        __syncthreads();
+      }
     }
   }
   const auto taken = [&](int g, uint32_t k) {
@@ -509,36 +551,49 @@ __global__ __launch_bounds__(64 * NW, 4) void page_pick_kernel(SelectArgs s) {
   if (blk.lo >= blk.hi) return;
   const int32_t* table = a.table + (int64_t)it.b * a.table_s;
   const int tiles = (blk.cols + 15) >> 4;
-  const auto pages_from = [&](int t) {  // lane 16 k + l16: page of column l16 of tile t + NW k
-    const int col = 16 * (t + NW * (lane >> 4)) + l16;
-    return col < blk.cols ? table[col] : -1;
-  };
-  int t = wave, turn = 0;
-  int pages = pages_from(t), page = __shfl(pages, l16, 64);
-  ColumnScores c(s, it.sq, blk, it.h);
-  Known known;
-  ColumnScores::Box box;
-  if (t < tiles) box = c.load(page);
-  while (t < tiles) {
-    const ColumnScores::Box now = box;
-    const int now_page = page, now_at = 16 * t;
-    t += NW;
-    turn = (turn + 1) & 3;
-    if (turn == 0) pages = pages_from(t);
-    page = __shfl(pages, 16 * turn + l16, 64);
-    if (t < tiles) box = c.load(page);
-    const float score = c.scores(now);
-    const uint32_t key = lane < 16 ? column_key(s, blk, now_at + l16, now_page, score) : 0u;
-    if (lane < 16) keys[now_at + l16] = key;
-    known.add(key);
+  // The wave's pages, by way of LDS, where their keys will lie: looked up in the loop they would be
+  // waited for behind the bounds on their way.
+  constexpr int kTurns = kPickColumns / 64 / NW;
+  const auto column = [&](int i) { return 16 * (wave + NW * i) + l16; };  // the lane's of the wave's i-th tile
+  int pages[kTurns];
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j) {
+    const int col = column(4 * j + (lane >> 4));
+    pages[j] = col < blk.cols ? table[col] : -1;
   }
+  ColumnScores c(s, it.sq, blk, it.h);
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j) keys[column(4 * j + (lane >> 4))] = (uint32_t)pages[j];
+  constexpr int kAhead = 2;  // tiles on their way
+  ColumnScores::Box box[kAhead];
+  int page[kAhead];
+  const auto ask = [&](int i, int k) {
+    const int col = column(i);
+    page[k] = col < blk.cols ? (int)keys[col] : -1;
+    box[k] = c.load(page[k]);
+  };
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) ask(k, k);
+  Known known;
+  for (int i = 0; wave + NW * i < tiles; i += kAhead)
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int col = column(i + k);  // past the last one: no page, no key
+      const float score = c.scores(box[k]);
+      const uint32_t key = lane < 16 ? column_key(s, blk, col, page[k], score) : 0u;
+      ask(i + k + kAhead, k);
+      if (lane < 16 && col < blk.cols) keys[col] = key;
+      known.add(key);
+    }
   known.done(c.error());
   const auto key = [&](int g) { return 64 * g + lane < blk.cols ? keys[64 * g + lane] : 0u; };
-  choose<NW, kPickColumns / 64 / NW>(s, c, it.sq, blk, table, known, key, sums, Team<NW>{team, wave});
+  const int per = (((blk.cols + 63) >> 6) + NW - 1) / NW;
+  uint32_t kept[kTurns];
+  choose<NW, kTurns, false>(s, c, it.sq, blk, table, per, kept, known, key, sums, Team<NW>{team, wave});
 }
 
-// Few items, whose bounds few CUs would fetch (55 GB/s each), or more columns: scored by as many workgroups as
-// they fill, then chosen by NW waves.
+// Few items, whose bounds few CUs would fetch (55 GB/s each), or more columns: their keys are formed by as many
+// workgroups as they fill, then chosen from by NW waves.
 __global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs s, int chunks) {
   const PagedArgs& a = s.p;
   const int lane = wi_x() & 63, l16 = lane & 15;
@@ -550,13 +605,15 @@ __global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs s, int chun
   const QueryBlock blk(a, it.sq, it.at);
   if (col0 >= blk.cols) return;
   const int col = col0 + l16 < blk.cols ? col0 + l16 : blk.cols - 1;
+  const int page = a.table[(int64_t)it.b * a.table_s + col];
   ColumnScores c(s, it.sq, blk, it.h);
-  const float score = c.scores(c.load(a.table[(int64_t)it.b * a.table_s + col]));
+  const float score = c.scores(c.load(page));
   const float err = c.error();
-  if (lane < 16) s.scores[(int64_t)jh * s.width + col0 + lane] = score;
+  if (lane < 16) s.keys[(int64_t)jh * s.width + col0 + lane] = column_key(s, blk, col0 + lane, page, score);
   if (lane == 0) s.error[(int64_t)jh * (s.width >> 4) + (col0 >> 4)] = err;
 }
 
+// Keys and errors are asked for before the item is known: what lies behind its columns is not used.
 template <int NW, int R>
 __global__ __launch_bounds__(64 * NW) void page_select_kernel(SelectArgs s) {
   const PagedArgs& a = s.p;
@@ -564,25 +621,42 @@ __global__ __launch_bounds__(64 * NW) void page_select_kernel(SelectArgs s) {
   const int lane = wi_x() & 63;
   const int wave = wave_uniform(wi_x() >> 6);
   const int jh = wg_x();
+  const uint32_t* keys = s.keys + (int64_t)jh * s.width;
+  const float* errors = s.error + (int64_t)jh * (s.width >> 4);
+  const int per = (((s.width + 63) >> 6) + NW - 1) / NW;
+  uint32_t kept[R > 0 ? R : 1];
+  float err = 0.f;
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int col = 64 * (wave * per + i) + lane;
+      kept[i] = i < per && col < s.width ? keys[col] : 0;
+    }
+    if (lane < s.width >> 4) err = errors[lane];
+  }
   const BlockPiece it(a, jh);
   if (!it.found) return;
   const QueryBlock blk(a, it.sq, it.at);
   if (blk.lo >= blk.hi) return;
   const int32_t* table = a.table + (int64_t)it.b * a.table_s;
-  const float* scores = s.scores + (int64_t)jh * s.width;
-  float err = 0.f;
-  for (int t = lane; t < (blk.cols + 15) >> 4; t += 64) err = fmaxf(err, s.error[(int64_t)jh * (s.width >> 4) + t]);
-  err = wave_max(err);
   const ColumnScores c(s, it.sq, blk, it.h);
-  const auto key = [&](int g) {
-    const int col = 64 * g + lane < blk.cols ? 64 * g + lane : blk.cols - 1;
-    const uint32_t k = column_key(s, blk, col, table[col], scores[col]);
-    return 64 * g + lane < blk.cols ? k : 0u;
-  };
+  const int tiles = (blk.cols + 15) >> 4;
+  err = lane < tiles ? err : 0.f;
+  for (int t = lane + (R > 0 ? 64 : 0); t < tiles; t += 64) err = fmaxf(err, errors[t]);
+  err = wave_max(err);
+  const auto key = [&](int g) { return 64 * g + lane < blk.cols ? keys[64 * g + lane] : 0u; };
   Known known;
-  for (int g = wave; g < (blk.cols + 63) >> 6; g += NW) known.add(key(g));
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      kept[i] = 64 * (wave * per + i) + lane < blk.cols ? kept[i] : 0;
+      known.add(kept[i]);
+    }
+  } else {
+    for (int g = wave; g < (blk.cols + 63) >> 6; g += NW) known.add(key(g));
+  }
   known.done(err);
-  choose<NW, R>(s, c, it.sq, blk, table, known, key, s.sums + (int64_t)jh * s.width, Team<NW>{team, wave});
+  choose<NW, R, true>(s, c, it.sq, blk, table, per, kept, known, key, s.sums + (int64_t)jh * s.width, Team<NW>{team, wave});
 }
 
 }  // namespace
