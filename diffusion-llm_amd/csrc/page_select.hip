@@ -19,7 +19,8 @@
 namespace bd3 {
 namespace {
 
-// Bounds of the pages that hold tokens of the chunks: a wave a page and head.
+// Bounds of the pages that hold tokens of the chunks: a wave a page and head. Latency: the lengths, the table's entry
+// and the keys are three round trips, one after the other; 1 page x 4 heads 2.6 us, 64 pages of 32 rows x 12 heads 4.6.
 template <int POOL>
 __global__ __launch_bounds__(256) void page_bounds_kernel(SelectArgs s) {
   const PagedArgs& a = s.p;
@@ -248,6 +249,8 @@ __device__ __forceinline__ double exact_score(const ColumnScores& c, int page) {
   return best;
 }
 
+constexpr int kPickWaves = 4;
+
 // What the waves of a workgroup tell each other.
 constexpr int kBins = 512;
 constexpr int kPasses = 4;  // of 9 bits of a key's 32
@@ -327,7 +330,7 @@ struct Known {
 // else they are there after a barrier here. sums: a double for each column.
 //
 // The threshold is found by histograms of 512 bins over the range of keys that it is known to be in (a bit search
-// took 20 passes over the keys and 27 of the 39 us of a call on one token over 1000 pages).
+// took 20 passes over the keys and 27 of the then 39 us of a call on one token over 1000 pages).
 template <int NW, int R, bool OWN, class Key>
 __device__ __forceinline__ void choose(const SelectArgs& s, const ColumnScores& c, const PagedSeq& sq, const QueryBlock& blk,
                                        const int32_t* table, int per, uint32_t (&kept)[R > 0 ? R : 1], Known known, Key key,
@@ -535,10 +538,13 @@ struct BlockPiece : SeqPiece<PagedSeq> {
         h(jh - j * a.kv_heads) {}
 };
 
-// Up to kPickColumns: the waves of a workgroup score them into LDS, 16 a wave and turn, the
-// next ones' bounds on their way, and choose. Few waves for many items, which then all run at once.
-template <int NW>
-__global__ __launch_bounds__(64 * NW, 4) void page_pick_kernel(SelectArgs s) {
+// Up to kPickColumns: the waves of a workgroup score them into LDS, 16 a wave and turn, the next two turns' bounds
+// on their way, and choose. A CU's fetches bound it (1875 columns, 480 KB, 22 us; 1000 18.6; 500 15; 187 11; eight waves
+// were as fast within 3%). 32 sequences of 2000-16000 keys, pages of 32, 12 heads, two blocks each: 17.5 us, of
+// which 5 are the first bounds' queue, 4-6 the rest of them, 3 the choice and 2 more that of an item with
+// columns in doubt.
+__global__ __launch_bounds__(64 * kPickWaves, 4) void page_pick_kernel(SelectArgs s) {
+  constexpr int NW = kPickWaves;
   const PagedArgs& a = s.p;
   __shared__ uint32_t keys[kPickColumns];
   __shared__ double sums[kPickColumns];
@@ -593,7 +599,8 @@ __global__ __launch_bounds__(64 * NW, 4) void page_pick_kernel(SelectArgs s) {
 }
 
 // Few items, whose bounds few CUs would fetch (55 GB/s each), or more columns: their keys are formed by as many
-// workgroups as they fill, then chosen from by NW waves.
+// workgroups as they fill, then chosen from by NW waves. One token, 1000 columns, 4 KV heads: 4.2 + 6.2 us, the second
+// launch 1.4 us until the keys are there and 3 of the choice's barriers.
 __global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs s, int chunks) {
   const PagedArgs& a = s.p;
   const int lane = wi_x() & 63, l16 = lane & 15;
@@ -675,10 +682,7 @@ hipError_t launch_page_bounds(const SelectArgs& s, int pool, hipStream_t stream)
 hipError_t launch_select_pages(const SelectArgs& s, hipStream_t stream) {
   const unsigned items = (unsigned)(s.slots * s.p.kv_heads);
   if (!select_in_two(items, s.width)) {
-    if (items <= 512)
-      hipLaunchKernelGGL(page_pick_kernel<8>, dim3(items), dim3(512), 0, stream, s);
-    else
-      hipLaunchKernelGGL(page_pick_kernel<4>, dim3(items), dim3(256), 0, stream, s);
+    hipLaunchKernelGGL(page_pick_kernel, dim3(items), dim3(64 * kPickWaves), 0, stream, s);
     return hipGetLastError();
   }
   const int chunks = (s.width + 63) / 64;
