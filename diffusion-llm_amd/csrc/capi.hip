@@ -927,7 +927,9 @@ static_assert(kPagedPartRows * bd3::kHeadDim <= INT32_MAX, "32-bit indices of th
 //
 // 8-bit pools and lists have their own, fitted to 700 batches of 8-bit pools and 160 of lists drawn the same way: rms error
 // 9-12%; the plan takes 1.2% more than the best of all plans on average for up to 16 rows, 2.2% for more (at worst
-// 31%), over lists 2% (bf16 pools 1%; at worst 54%).
+// 31%), over lists 2% (bf16 pools 1%; at worst 54%). What each is for, us at its best ranges: 16 rows of 32 sequences
+// over 100-8192 keys 30.5 with one set of four waves, 31.7 with two; of one over 3600 keys 11.2, 10.8; 96 rows of 24
+// sequences over 500-4000 keys 26.1 with 128-row tiles, 25.4 with 32-row ones; 48-row tiles over lists 28.1, 32-row 32.7.
 struct PagedCost {
   double chain0, chain, busy, load0, load, item, merge, merge_item, e_even, e;
 };

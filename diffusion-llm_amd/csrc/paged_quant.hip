@@ -61,7 +61,10 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
 // A wave: a block of 16 positions of one sequence and one head of q | k | v. Lane (row
 // lane / 4, part j = lane % 4) holds the coordinate pairs (8 j + i, 32 + 8 j + i) of its
 // row, so the rotation is lane-local and the block's maximum one wave reduction. The
-// rotation is paged_rope_kernel's; keys are encoded from its fp32 results.
+// rotation is paged_rope_kernel's; keys are encoded from its fp32 results. Bound by memory for chunks (13000 tokens, 16 heads
+// on 4: 18.2 us, 75 MB, 4.1 TB/s; 19.4 before the page and the scale were asked for first), by three
+// round trips else (lengths; page; old scale, with the rotation between: 4 tokens 4.4 us, 1024 4.6). Four
+// heads a wave gained nothing.
 template <int POOL>
 __global__ __launch_bounds__(256) void paged_rope8_kernel(PagedRopeArgs a) {
   const int lane = wi_x() & 63;
@@ -178,7 +181,8 @@ __global__ __launch_bounds__(256) void paged_rope8_kernel(PagedRopeArgs a) {
   if (r == (kept ? c - begin : 0) && j == 0) *scale_p = __uint_as_float(scale);  // the first new row's lane
 }
 
-// Values of whole pools: a wave takes a block of 16 rows of a head, 16 codes a lane.
+// Values of whole pools: a wave takes a block of 16 rows of a head, 16 codes a lane. Bound by memory: 29 MB of codes to 58
+// of values 16.6 us, 5.2 TB/s.
 template <int POOL>
 __global__ __launch_bounds__(256) void page_values_kernel(PageValuesArgs a) {
   const int lane = wi_x() & 63;

@@ -693,6 +693,12 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
 // row tiles. Its scales enter with the softmax: K's with the factor, V's in the exponent, so that what is
 // rounded to bf16 is P times it; the row sum takes its inverse again, once for 4 of the elements. (log2 scale - maximum
 // is off by 2^-24 of the maximum, no more than the scores' own fp32 sums.)
+// 16 rows: 4 waves where many items are bound by HBM (32 sequences of 100-8192 keys, 12 heads: 27 us, 4.3 TB/s of
+// codes, of which 5.5 us until the first are there; 48 of 8192 keys 110, 5.6 TB/s), 8 for few, long ones. 32
+// and 48 rows: a conversion serves 2 or 3 row tiles, one wave a SIMD at 64-key chunks (209 and 253 registers); lists of 40
+// pages of 32, 280 items: 28 us with 48 rows, 33 with 32; bound by what one wave issues (48 products,
+// ~400 VALU instructions a chunk). Codes stay bytes in LDS because a bf16 tile would be twice the writes
+// and the room of half the waves (the first form, 32-key chunks staged in bf16: batch 50.6 -> 37 us).
 template <int NW, int RT, int KC, int POOL, bool COLS>
 __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const PagedItem<false, COLS>& it, char* smem) {
   using Stream = CodeStream<NW, KC, POOL, COLS>;
@@ -881,7 +887,10 @@ constexpr float kRescale = 8.0f;
 // 8-bit pools: each wave loads the codes of its 16 keys to LDS during the step on the tile before,
 // then converts them to bf16 into the other stage, once for the four waves; the tile's four scales
 // enter as in paged_codes_item. (Held in registers during the step the codes spilled 4 to 40 of
-// those: prompts of 1500-4096 tokens in int8 106 us.)
+// those: prompts of 1500-4096 tokens in int8 106 us.) The codes are there when a step ends (8 clocks of waiting); prompts of
+// 1500-4096 tokens, 12 heads 75 us, 560 TFLOP/s, bound by VALU work: exponentials, and ~50 instructions of
+// conversion a wave and tile. 24 sequences of 500-4000 keys, 32 tokens, 12 heads on 4: 23 us, 284 items of 3.5 us start-up
+// and 3-6 steps of 1.4 us, the last of those that share a CU.
 template <int SUBS, int POOL>
 __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   constexpr bool kCodes = POOL != kPoolBf16;

@@ -33,7 +33,9 @@ blocks, and the logits' max-abs difference between the two backbones at
 sampled denoising steps (same tokens, same committed prefix).
 
 With --serve: the same backbone over a paged cache (`serve`), sequences of
-different lengths in one batch that join and leave as the pool's pages allow.
+different lengths in one batch that join and leave as the pool's pages allow;
+--cache int8 or e4m3 keeps the pages in 8 bits, --top N reads the N pages a head
+that promise most for a block.
 """
 from __future__ import annotations
 
@@ -382,7 +384,10 @@ def serve(cfg, p, tables, prompts, n_blocks, steps, n_pages, page_size=64, repet
     return out
 
 
-def run_serving(sequences: int = 32, steps: int = 8, seed: int = 0) -> dict:
+CACHES = {"bf16": torch.bfloat16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+def run_serving(sequences: int = 32, steps: int = 8, seed: int = 0, cache: str = "bf16", top: int | None = None) -> dict:
     """Tokens/s of `serve`: prompts of 32 to 1024 tokens, each continued by 4 to
     16 blocks of 32, through a pool of half the pages that all of them need."""
     import random
@@ -398,14 +403,16 @@ def run_serving(sequences: int = 32, steps: int = 8, seed: int = 0) -> dict:
     n_blocks = [rng.randint(4, 16) for _ in prompts]
     pages = sum(-(-(len(t) + n * cfg.bs) // 64) for t, n in zip(prompts, n_blocks)) // 2
     with torch.no_grad():
-        serve(cfg, p, tables, prompts[:2], [1, 1], 2, pages)  # warm-up
+        kind = {"cache_dtype": CACHES[cache], "top": top}
+        serve(cfg, p, tables, prompts[:2], [1, 1], 2, pages, **kind)  # warm-up
         torch.cuda.synchronize()
         t0 = time.perf_counter()
-        serve(cfg, p, tables, prompts, n_blocks, steps, pages, repetition=1.1)
+        serve(cfg, p, tables, prompts, n_blocks, steps, pages, repetition=1.1, **kind)
         torch.cuda.synchronize()
         seconds = time.perf_counter() - t0
     return {"workload": f"{sequences} prompts of 32-1024 tokens continued by 4-16 blocks of {cfg.bs}, {steps} steps per "
-                        f"block, 12L / 768 / 12H, vocab 50258, paged cache of {pages} x 64 tokens (random init)",
+                        f"block, 12L / 768 / 12H, vocab 50258, paged cache of {pages} x 64 tokens in {cache}"
+                        f"{f', {top} pages read' if top is not None else ''} (random init)",
             "tokens_per_s": sum(n_blocks) * cfg.bs / seconds, "seconds": seconds}
 
 
@@ -491,9 +498,11 @@ def main(argv=None) -> int:
     ap.add_argument("--eager-blocks", type=int, default=2)
     ap.add_argument("--check-steps", type=int, default=4)
     ap.add_argument("--serve", action="store_true", help="the ragged serving loop instead")
+    ap.add_argument("--cache", choices=list(CACHES), default="bf16", help="with --serve: what the pages hold")
+    ap.add_argument("--top", type=int, default=None, help="with --serve: pages that a block's attention reads for a head")
     args = ap.parse_args(argv)
     if args.serve:
-        print(json.dumps(run_serving()), flush=True)
+        print(json.dumps(run_serving(cache=args.cache, top=args.top)), flush=True)
         return 0
     print(json.dumps(run(args.blocks, args.eager_blocks, args.check_steps)), flush=True)
     return 0
