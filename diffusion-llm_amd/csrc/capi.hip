@@ -925,11 +925,13 @@ static_assert(kPagedPartRows * bd3::kHeadDim <= INT32_MAX, "32-bit indices of th
 // sequences, 1-3000 tokens a chunk, 20-10000 keys, 1-16 KV heads and groups of 1-12;
 // over 1500 others the rms error is 9% for up to 16 rows, 12% for 17-256, 10% for more.
 //
-// 8-bit pools and lists have their own, fitted to 700 batches of 8-bit pools and 160 of lists drawn the same way: rms error
-// 9-12%; the plan takes 1.2% more than the best of all plans on average for up to 16 rows, 2.2% for more (at worst
-// 31%), over lists 2% (bf16 pools 1%; at worst 54%). What each is for, us at its best ranges: 16 rows of 32 sequences
-// over 100-8192 keys 30.5 with one set of four waves, 31.7 with two; of one over 3600 keys 11.2, 10.8; 96 rows of 24
-// sequences over 500-4000 keys 26.1 with 128-row tiles, 25.4 with 32-row ones; 48-row tiles over lists 28.1, 32-row 32.7.
+// 8-bit pools and lists have their own, fitted to 2200 batches of 8-bit pools and 400 of lists drawn the same way (16 rows: to
+// 860, whose constants choose better where the lengths differ, 0.9% above the best plan instead of 1.1): rms error
+// 9-12%, also over 700 others; there the plan takes 1.4% more than the best of all plans on average for up to 16 rows, 1.4-3.9%
+// for more (at worst 32%), over lists 2.2% (bf16 pools 1.1%; at worst 34%). Without the kernel of one set of
+// four waves 16 rows take 2.1%, of two 4.3%; without one of the 32-row ones 33-64 rows 6.5 and 7.9%; without
+// 48 rows lists of more than 256 10% instead of 7.8%; without one, two or four sets of 128 rows whole prompts 5.4, 5.2
+// and 2.1% instead of 1.4 (one prompt of 4096 tokens, 12 heads: 54 us with four, 67 with two).
 struct PagedCost {
   double chain0, chain, busy, load0, load, item, merge, merge_item, e_even, e;
 };
@@ -942,12 +944,13 @@ const PagedCost& paged_cost(bool codes, int tile, int subs) {
                                             {8.0, 0.52, 0.0, 0.0, 0.69, 9.5, 0.0, 0.0, 3.0, 3.0}};  // four sets: never with ranges
   static constexpr PagedCost kCodes16[2] = {{1.865, 0.407, 0.148, 3.628, 0.127, 0.544, 2.373, 0.755, 1.0, 1.012},
                                             {1.677, 0.275, 0.191, 3.858, 0.105, 1.761, 2.512, 0.708, 1.0, 1.047}};
-  static constexpr PagedCost kCodes32[2] = {{6.064, 0.542, 0.337, 4.474, 0.401, 2.905, 2.416, 0.191, 2.395, 2.132},
-                                            {6.563, 0.345, 0.422, 5.078, 0.488, 5.257, 3.338, 0.0, 5.0, 4.23}};
-  static constexpr PagedCost kCodes48 = {7.01, 0.615, 0.016, 5.43, 0.469, 3.53, 2.407, 0.413, 2.488, 2.297};
-  static constexpr PagedCost kCodes128[2] = {{4.13, 1.276, 0.043, 3.88, 0.489, 2.922, 1.292, 1.948, 1.358, 1.358},
-                                             {5.538, 0.878, 0.032, 5.463, 0.67, 4.764, 1.779, 1.643, 2.128, 2.128}};
-  if (codes) return tile == 16 ? kCodes16[subs - 1] : tile == 32 ? kCodes32[subs - 1] : tile == 48 ? kCodes48 : kCodes128[subs - 1];
+  static constexpr PagedCost kCodes32[2] = {{6.467, 0.538, 0.353, 5.656, 0.417, 2.72, 2.664, 0.031, 3.852, 3.144},
+                                            {6.616, 0.35, 0.409, 4.777, 0.478, 5.019, 3.077, 0.05, 5.0, 4.179}};
+  static constexpr PagedCost kCodes48 = {7.432, 0.603, 0.404, 5.877, 0.507, 3.343, 2.531, 0.134, 3.319, 2.681};
+  static constexpr PagedCost kCodes128[3] = {{5.151, 1.254, 0.036, 1.967, 0.393, 3.15, 1.416, 1.878, 1.233, 1.233},
+                                             {5.704, 0.868, 0.001, 4.571, 0.605, 5.227, 1.934, 1.292, 1.959, 1.959},
+                                             {8.957, 0.682, 0.682, 3.541, 0.619, 12.27, 0.0, 0.0, 3.46, 3.46}};
+  if (codes) return tile == 16 ? kCodes16[subs - 1] : tile == 32 ? kCodes32[subs - 1] : tile == 48 ? kCodes48 : kCodes128[subs >> 1];
   return tile == 16 ? kRows16 : tile == 32 ? kRows32[subs - 1] : kRows128[subs >> 1];
 }
 double paged_us(const PagedCost& c, double longest, double keys, double items, double busiest, bool split, bool even) {
@@ -1011,7 +1014,7 @@ PagedPlan paged_plan(int pool_type, int32_t seqs, int32_t tokens, int32_t heads,
       p.split_shift = shift;
     };
     if (!fits(1)) continue;
-    const int most = codes ? (tile == 48 ? 1 : 2) : (tile == 128 ? 4 : 2);
+    const int most = tile == 128 ? 4 : tile == 48 ? 1 : 2;
     for (int subs = tile == 16 && !codes ? 2 : 1; subs <= most; subs *= 2) {
       const PagedCost& c = paged_cost(codes, tile, subs);
       take(paged_us(c, max_kv, units * seen, units, busiest(1), false, even), subs, 30);

@@ -1304,10 +1304,9 @@ hipError_t launch_paged_tiles(const PagedArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)a.workgroups);
   if (a.tile == 128) {
     if constexpr (!COLS) {
-      if constexpr (POOL == kPoolBf16) {
-        if (a.subs == 4) hipLaunchKernelGGL((paged128_kernel<4, POOL>), grid, dim3(1024), 0, stream, a);
-      }
-      if (a.subs == 2)
+      if (a.subs == 4)
+        hipLaunchKernelGGL((paged128_kernel<4, POOL>), grid, dim3(1024), 0, stream, a);
+      else if (a.subs == 2)
         hipLaunchKernelGGL((paged128_kernel<2, POOL>), grid, dim3(512), 0, stream, a);
       else if (a.subs == 1)
         hipLaunchKernelGGL((paged128_kernel<1, POOL>), grid, dim3(256), 0, stream, a);
