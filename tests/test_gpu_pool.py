@@ -47,6 +47,8 @@ CASES = [
     ([(1, 700), (2, 30), (16, 256)], 16, 2, 64, 16),
     ([(40, 333), (90, 12)], 12, 1, 64, 8),
     ([(7, 100), (50, 200)], 6, 2, 64, 1 << 30),
+    ([(1024, 0), (900, 100)], 12, 12, 64, 16),  # few, long items: four sets of waves
+    ([(2049, 0), (0, 40)], 12, 6, 16, 1),
 ]
 
 
