@@ -279,8 +279,7 @@ struct MergeLds {
   float m[NW][ROWS];
   float l[NW][ROWS];
   template <class Item>
-  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const Item& it, int rt, int d,
-                                            int first = 0) const {  // first: row of the tile that the states begin with
+  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const Item& it, int rt, int d) const {
     float mw[NW], mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
@@ -297,7 +296,7 @@ struct MergeLds {
       ot += wgt * *reinterpret_cast<const f32x4*>(&o[w][rt][d]);
     }
     const float inv = lt > 0.f ? 1.f / lt : 0.f;  // a row that sees no key: 0
-    const int row = it.r0 + first + rt;
+    const int row = it.r0 + rt;
     if (ranges == 1) {
       if (row < it.r1) {
         const int t = fast_div(row, a.group_div);
@@ -812,33 +811,39 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
       }
   }
 
-  auto* ml = reinterpret_cast<MergeLds<NW, 16>*>(smem);
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     lsum[t] += shfl_xor(lsum[t], 16);
     lsum[t] = sum_xor32(lsum[t]);
-    __syncthreads();  // the tiles, and the last rows' states, are reused
-#pragma unroll
-    for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(&ml->o[wave][l16][16 * db + 4 * hq]) = o[t][db];
-    if (hq == 0) {
-      ml->m[wave][l16] = m[t];
-      ml->l[wave][l16] = lsum[t];
-    }
-    __syncthreads();
-    if (tid < 256) ml->write_row(a, keys.ranges, it, tid >> 4, 4 * (tid & 15), 16 * t);
   }
+  __syncthreads();  // the tiles are reused below
+  auto* ml = reinterpret_cast<MergeLds<NW, 16 * RT>*>(smem);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = 16 * t + l16;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(&ml->o[wave][r][16 * db + 4 * hq]) = o[t][db];
+    if (hq == 0) {
+      ml->m[wave][r] = m[t];
+      ml->l[wave][r] = lsum[t];
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int r0 = 0; r0 < 16 * RT; r0 += 4 * NW)
+    if (r0 + (tid >> 4) < 16 * RT) ml->write_row(a, keys.ranges, it, r0 + (tid >> 4), 4 * (tid & 15));
 }
 
-template <int NW, int KC>
+template <int NW, int RT, int KC>
 constexpr size_t codes_smem() {
   constexpr size_t v = (size_t)NW * 2 * KC * kHeadDim;
-  return v > sizeof(MergeLds<NW, 16>) ? v : sizeof(MergeLds<NW, 16>);
+  return v > sizeof(MergeLds<NW, 16 * RT>) ? v : sizeof(MergeLds<NW, 16 * RT>);
 }
 
 // WPS: waves per SIMD that the registers leave room for.
 template <int NW, int RT, int KC, int WPS, int POOL, bool COLS>
 __global__ __launch_bounds__(NW * 64, WPS) void paged_codes_kernel(PagedArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[codes_smem<NW, KC>()];
+  __shared__ __attribute__((aligned(16))) char smem[codes_smem<NW, RT, KC>()];
   for (int id = wg_x();; id += a.workgroups) {  // as in paged_rows_kernel
     const PagedItem<false, COLS> it(a, id);
     if (!it.found) return;
