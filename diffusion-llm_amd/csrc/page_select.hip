@@ -203,6 +203,10 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
   return k < 1u ? 1u : (k > kForced - 1 ? kForced - 1 : k);
 }
+__device__ __forceinline__ uint64_t order_key(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  return u >> 63 ? ~u : u | (uint64_t)1 << 63;
+}
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {  // as wave_max
@@ -367,6 +371,8 @@ __device__ __forceinline__ void choose(const SelectArgs& s, const ColumnScores& 
   // Taken: keys from `sure` on and the best `open` of those from `doubt` on.
   uint32_t sure = 1, doubt = 1;
   int open = 0;
+  uint64_t level = 0;  // sums above it are taken, of those equal to it the first `room` columns
+  int room = 0, equal_before = 0;
   if (there > a.top && need <= 0) {
     sure = doubt = kForced;  // the first of those always taken
   } else if (there > a.top) {
@@ -470,39 +476,47 @@ __device__ __forceinline__ void choose(const SelectArgs& s, const ColumnScores& 
           }
         });
         __syncthreads();
+        // The open-th largest of the sums, bit by bit (pages that are all alike: 30000 of them 3.6 ms, each one
+        // against each 124).
+        const auto count_sums = [&](auto of) {
+          uint32_t m = 0;
+          reread([&](int g, uint32_t k) {
+            m += __popcll(__ballot(k >= doubt && k < sure && of(order_key(sums[64 * g + lane]))));
+          });
+          return m;
+        };
+        for (int bit = 63; bit >= 0; --bit) {
+          const uint64_t from = level | (uint64_t)1 << bit;
+          uint32_t m[1] = {count_sums([&](uint64_t x) { return x >= from; })};
+          team.template join<kSum>(m);
+          if ((int)m[0] >= open) level = from;
+          if ((int)m[0] == open) break;
+        }
+        uint32_t m[1] = {count_sums([&](uint64_t x) { return x > level; })};
+        team.template join<kSum>(m);
+        room = open - (int)m[0];
+        int all;
+        equal_before = team.before((int)count_sums([&](uint64_t x) { return x == level; }), all);
       }
     }
   }
-  const auto taken = [&](int g, uint32_t k) {
+  const auto taken = [&](int g, uint32_t k, int& equal) {
     bool take = k >= sure;
-    const bool maybe = k >= doubt && k < sure;
-    if (open > 0 && __ballot(maybe) != 0) {
-      const int col = 64 * g + lane;
-      const double mine = maybe ? sums[col] : 0.0;
-      int ahead = 0;  // doubtful ones that are better
-      for (int g2 = 0; g2 < groups; ++g2) {
-        const uint32_t k2 = key(g2);
-        uint64_t in = __ballot(k2 >= doubt && k2 < sure);
-        while (in != 0) {
-          const int at = 64 * g2 + __builtin_ctzll(in);
-          in &= in - 1;
-          const double e = sums[at];
-          ahead += e > mine || (e == mine && at < col);
-        }
-      }
-      take = take || (maybe && ahead < open);
+    if (open > 0) {
+      const bool maybe = k >= doubt && k < sure;
+      const uint64_t x = maybe ? order_key(sums[64 * g + lane]) : 0;
+      const uint64_t at = __ballot(maybe && x == level);
+      const int nth = equal + __builtin_amdgcn_mbcnt_hi((uint32_t)(at >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)at, 0));
+      take = take || (maybe && (x > level || (x == level && nth < room)));
+      equal += __popcll(at);
     }
     return take;
   };
   // The columns taken, in ascending order, for each token of the block.
   int mine = 0, all;
-  uint64_t settled = 0;  // of the doubtful: bit i of the lane for its column of the wave's i-th group
+  int equal = equal_before;
   if (open > 0)
-    reread([&](int g, uint32_t k) {
-      const bool take = taken(g, k);
-      if (g - g0 < 64) settled |= (uint64_t)take << (g - g0);
-      mine += __popcll(__ballot(take));
-    });
+    reread([&](int g, uint32_t k) { mine += __popcll(__ballot(taken(g, k, equal))); });
   else
     each([&](int, uint32_t k) { mine += __popcll(__ballot(k >= sure)); });
   int base = team.before(mine, all);
@@ -516,8 +530,9 @@ __device__ __forceinline__ void choose(const SelectArgs& s, const ColumnScores& 
       for (int tok = 0; tok < tokens; ++tok) out[tok * step + at] = 64 * g + lane;
     base += __popcll(in);
   };
+  equal = equal_before;
   if (open > 0)
-    reread([&](int g, uint32_t k) { emit(g, g - g0 < 64 ? (settled >> (g - g0)) & 1 : taken(g, k)); });
+    reread([&](int g, uint32_t k) { emit(g, taken(g, k, equal)); });
   else
     each([&](int g, uint32_t k) { emit(g, k >= sure); });
   for (int at = all + wi_x(); at < a.top; at += 64 * NW)

@@ -695,7 +695,7 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
 // 16 rows: 4 waves where many items are bound by HBM (32 sequences of 100-8192 keys, 12 heads: 27 us, 4.3 TB/s of
 // codes, of which 5.5 us until the first are there; 48 of 8192 keys 110, 5.6 TB/s), 8 for few, long ones. 32
 // and 48 rows: a conversion serves 2 or 3 row tiles, one wave a SIMD at 64-key chunks (209 and 253 registers); lists of 40
-// pages of 32, 280 items: 28 us with 48 rows, 33 with 32; bound by what one wave issues (48 products,
+// pages of 32, 280 items: 28.7 us with 48 rows, 33 with 32; bound by what one wave issues (48 products,
 // ~400 VALU instructions a chunk). Codes stay bytes in LDS because a bf16 tile would be twice the writes
 // and the room of half the waves (the first form, 32-key chunks staged in bf16: batch 50.6 -> 37 us).
 template <int NW, int RT, int KC, int POOL, bool COLS>

@@ -9,7 +9,9 @@
  *     KV cache of kv_len positions (block-causal);
  *   - split-KV decode attention (partials + LSE merge);
  *   - attention of ragged batches over a paged KV cache, with the inputs written
- *     into its pages, and penalties, biases and grammar masks on the logits.
+ *     into its pages, and penalties, biases and grammar masks on the logits;
+ *   - the same over pages of 8-bit codes with scales, and over the pages that
+ *     promise most for a block's queries by bounds of their keys.
  *
  * Conventions shared by every entry point:
  *   - All tensor pointers are DEVICE pointers to bf16 data (uint16 bit
