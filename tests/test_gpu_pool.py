@@ -285,6 +285,54 @@ def test_page_values(cuda):
             assert torch.equal(x, want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk", [1, 16, 40, 150])
+@pytest.mark.parametrize("dtype", POOLS)
+def test_pages_past_32_bit_offsets(cuda, dtype, chunk):
+    """A step of every operator over pages whose element offsets pass 2^32, beside the first ones, against the same step
+    over a small pool, to the bit."""
+    lens, heads, kv_heads, page, bs, top = [(chunk, 200), (chunk, 90)], 4, 2, 64, 16, 5
+    tables = [t.to(cuda) for t in rope_tables(D, 512)]
+    g = torch.Generator().manual_seed(chunk)
+    need = [-(-(n + x) // page) for n, x in lens]
+    n = sum(need)
+    far = (1 << 32) // (kv_heads * page * D) + 100
+    table = torch.full((2, max(need)), -1, dtype=torch.int32)
+    for b, ids in enumerate(torch.randperm(n, generator=g).split(need)):
+        table[b, :need[b]] = ids
+    starts = torch.tensor([0, chunk, 2 * chunk], dtype=torch.int32, device=cuda)
+    kv = torch.tensor([a + b for a, b in lens], dtype=torch.int32, device=cuda)
+    before = torch.tensor([0, 200, 290], dtype=torch.int32, device=cuda), torch.tensor([200, 90], dtype=torch.int32, device=cuda)
+    first = torch.randn((290, (heads + 2 * kv_heads) * D), generator=g).to(BF).to(cuda)
+    qkv = torch.randn((2 * chunk, (heads + 2 * kv_heads) * D), generator=g).to(BF).to(cuda)
+
+    def step(pages, table):
+        k, v = (torch.empty((pages, kv_heads, page, D), device=cuda, dtype=dtype) for _ in range(2))
+        bounds = torch.empty((pages, kv_heads, 2, D), device=cuda, dtype=BF)
+        scales = [torch.empty((pages, kv_heads, page // 16), device=cuda) for _ in range(2)] if dtype != BF else [None] * 2
+        ids = torch.cat([t[t >= 0] for t in table]).long()
+        for t in (k, v, *scales):  # slots that no call writes
+            if t is not None:
+                t.view(torch.uint8)[ids] = 0
+        for x, s, e in ((first, *before), (qkv, starts, kv)):
+            if dtype == BF:
+                q = paged_attention_inputs(x, heads, *tables, k, v, table, s, e)
+            else:
+                q = paged_attention_inputs8(x, heads, *tables, k, v, *scales, table, s, e)
+            page_bounds(k, bounds, table, s, e, x.shape[0], scales[0])
+        columns = select_pages(q, bounds, table, starts, kv, bs, page, top, chunk)
+        batch = q, k, v, table, starts, kv, bs, chunk
+        o = paged_attention_pool(*batch, k_scales=scales[0], v_scales=scales[1])
+        listed = paged_attention_pool(*batch, k_scales=scales[0], v_scales=scales[1], columns=columns)
+        values = [x[ids] for x in (page_values(k, v, *scales) if dtype != BF and chunk == 16 else ())]
+        return [q, o, columns, listed, bounds[ids], k.view(torch.uint8)[ids], v.view(torch.uint8)[ids], *values] + \
+            [t[ids] for t in scales if t is not None]
+
+    small = step(n, table.to(cuda))
+    large = step(far, torch.where(table >= n // 2, table + far - n, table).to(cuda))
+    assert all(same(a.contiguous(), b.contiguous()) for a, b in zip(small, large))
+
+
 # -- lists of pages --------------------------------------------------------------
 
 LISTED = [
@@ -315,6 +363,23 @@ def test_listed_pages_match_definition(cuda, record_error, lens, heads, kv_heads
         wide[:, :, :top] = columns.to(cuda)
         for given in (columns.to(cuda), wide[:, :, :top]):
             record_error("listed pages / bound", worst(attend(on(c, cuda), bs, given), ref, tol), 1.0)
+
+
+@pytest.mark.gpu
+def test_lists_in_other_layouts(cuda):
+    """One list for all tokens (stride 0), the front of longer lists, KV heads first."""
+    c = pool_case([(16, 900), (7, 300)], 4, 2, 32, I8, seed=3)
+    d = on(c, cuda)
+    g = torch.Generator().manual_seed(1)
+    one = torch.stack([torch.randperm(20, generator=g)[:12].sort().values for _ in range(2)]).to(torch.int32).to(cuda)
+    T = d["q"].shape[0]
+    want = attend(d, 16, one.expand(T, 2, 12).contiguous())
+    assert torch.equal(attend(d, 16, one.expand(T, 2, 12)), want)
+    longer = torch.full((T, 2, 40), 3, dtype=torch.int32, device=cuda)
+    longer[:, :, :12] = one
+    assert torch.equal(attend(d, 16, longer[:, :, :12]), want)
+    heads_first = one[:, None].expand(2, T, 12).contiguous().transpose(0, 1)
+    assert torch.equal(attend(d, 16, heads_first), want)
 
 
 @pytest.mark.gpu
