@@ -279,7 +279,8 @@ struct MergeLds {
   float m[NW][ROWS];
   float l[NW][ROWS];
   template <class Item>
-  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const Item& it, int rt, int d) const {
+  __device__ __forceinline__ void write_row(const PagedArgs& a, int ranges, const Item& it, int rt, int d,
+                                            int first = 0) const {  // first: row of the tile that the states begin with
     float mw[NW], mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
@@ -296,7 +297,7 @@ struct MergeLds {
       ot += wgt * *reinterpret_cast<const f32x4*>(&o[w][rt][d]);
     }
     const float inv = lt > 0.f ? 1.f / lt : 0.f;  // a row that sees no key: 0
-    const int row = it.r0 + rt;
+    const int row = it.r0 + first + rt;
     if (ranges == 1) {
       if (row < it.r1) {
         const int t = fast_div(row, a.group_div);
@@ -686,6 +687,11 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
   if (tid < 16 * kRows) ml->write_row(a, keys.ranges, it, tid >> 4, 4 * (tid & 15));
 }
 
+// Row tiles whose states are merged in one stage: both of 32 rows (1 sequence 7.9 -> 7.6 us, 4 of them 11.6 -> 11.2), one of 48
+// rows (lists 28.1 us, all three at once 28.7).
+template <int RT>
+constexpr int codes_stage = RT == 2 ? 2 : 1;
+
 // Rows of 8-bit pools: 16 RT rows, NW waves that share the chunks of a range. S^T of 16 keys x 16 rows on
 // v_mfma_f32_16x16x32_bf16 from 16 codes of a key to a lane: the sums run over d in the order that
 // gives (16 hq + 8 c + e), which Q's operand takes as well. A chunk's codes are converted once for all RT
@@ -695,7 +701,7 @@ __device__ __forceinline__ void paged16_item(const PagedArgs& a, const PagedItem
 // 16 rows: 4 waves where many items are bound by HBM (32 sequences of 100-8192 keys, 12 heads: 27 us, 4.3 TB/s of
 // codes, of which 5.5 us until the first are there; 48 of 8192 keys 110, 5.6 TB/s), 8 for few, long ones. 32
 // and 48 rows: a conversion serves 2 or 3 row tiles, one wave a SIMD at 64-key chunks (209 and 253 registers); lists of 40
-// pages of 32, 280 items: 28.7 us with 48 rows, 33 with 32; bound by what one wave issues (48 products,
+// pages of 32, 280 items: 28.1 us with 48 rows, 33 with 32; bound by what one wave issues (48 products,
 // ~400 VALU instructions a chunk). Codes stay bytes in LDS because a bf16 tile would be twice the writes
 // and the room of half the waves (the first form, 32-key chunks staged in bf16: batch 50.6 -> 37 us).
 template <int NW, int RT, int KC, int POOL, bool COLS>
@@ -816,28 +822,32 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
     lsum[t] += shfl_xor(lsum[t], 16);
     lsum[t] = sum_xor32(lsum[t]);
   }
-  __syncthreads();  // the tiles are reused below
-  auto* ml = reinterpret_cast<MergeLds<NW, 16 * RT>*>(smem);
+  constexpr int kStage = codes_stage<RT>;
+  auto* ml = reinterpret_cast<MergeLds<NW, 16 * kStage>*>(smem);
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int r = 16 * t + l16;
+  for (int t0 = 0; t0 < RT; t0 += kStage) {
+    __syncthreads();  // the tiles, or the last stage's states, are reused
 #pragma unroll
-    for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(&ml->o[wave][r][16 * db + 4 * hq]) = o[t][db];
-    if (hq == 0) {
-      ml->m[wave][r] = m[t];
-      ml->l[wave][r] = lsum[t];
+    for (int t = t0; t < t0 + kStage; ++t) {
+      const int r = 16 * (t - t0) + l16;
+#pragma unroll
+      for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(&ml->o[wave][r][16 * db + 4 * hq]) = o[t][db];
+      if (hq == 0) {
+        ml->m[wave][r] = m[t];
+        ml->l[wave][r] = lsum[t];
+      }
     }
-  }
-  __syncthreads();
+    __syncthreads();
 #pragma unroll 1
-  for (int r0 = 0; r0 < 16 * RT; r0 += 4 * NW)
-    if (r0 + (tid >> 4) < 16 * RT) ml->write_row(a, keys.ranges, it, r0 + (tid >> 4), 4 * (tid & 15));
+    for (int r0 = 0; r0 < 16 * kStage; r0 += 4 * NW)
+      if (r0 + (tid >> 4) < 16 * kStage) ml->write_row(a, keys.ranges, it, r0 + (tid >> 4), 4 * (tid & 15), 16 * t0);
+  }
 }
 
 template <int NW, int RT, int KC>
 constexpr size_t codes_smem() {
   constexpr size_t v = (size_t)NW * 2 * KC * kHeadDim;
-  return v > sizeof(MergeLds<NW, 16 * RT>) ? v : sizeof(MergeLds<NW, 16 * RT>);
+  return v > sizeof(MergeLds<NW, 16 * codes_stage<RT>>) ? v : sizeof(MergeLds<NW, 16 * codes_stage<RT>>);
 }
 
 // WPS: waves per SIMD that the registers leave room for.
