@@ -970,7 +970,6 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     v_log = fast_log2(v_scale);
     v_inv = __builtin_amdgcn_rcpf(v_scale);
   };
-  if constexpr (kCodes) find_scales(0);
 
   const int qrow0 = r0 + 32 * wave;
   const int myr = qrow0 + l32;
@@ -1000,6 +999,14 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   float ks_next[4], v_log_next[4], v_inv_next[4];  // and their scales
   const uint32_t raw_w = lds_addr(&raw_all[kCodes ? sub : 0][kCodes ? 2 * wave : 0][0]);
   const uint8_t* raw = &raw_all[kCodes ? sub : 0][kCodes ? 2 * wave : 0][16 * lane];
+  auto read_scales = [&](int i) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      ks_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scale), 4 * (i & 15) + q));
+      v_log_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_log), 4 * (i & 15) + q));
+      v_inv_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_inv), 4 * (i & 15) + q));
+    }
+  };
   auto issue = [&](int i) {  // the set's i-th tile
     if ((i & 15) == 0 && i > 0) {
       ids = ids_next;
@@ -1015,12 +1022,7 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     const int64_t page = __builtin_amdgcn_readlane(ids, at);
     const int64_t slot = key & (a.page - 1);
     if constexpr (kCodes) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        ks_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k_scale), 4 * (i & 15) + q));
-        v_log_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_log), 4 * (i & 15) + q));
-        v_inv_next[q] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v_inv), 4 * (i & 15) + q));
-      }
+      if (i > 0) read_scales(i);
       const int top = lim < 0 ? 0 : lim;  // rows past the last key re-read it
       const int r = (lane >> 2) < top ? lane >> 2 : top;
       const uint8_t* none = reinterpret_cast<const uint8_t*>(zero_row);
@@ -1064,6 +1066,10 @@ __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
     }
   };
   if (n_mine > 0) issue(0);
+  if constexpr (kCodes) {  // the first tile's scales after its codes: asked for before them they were waited for first
+    find_scales(0);
+    read_scales(0);
+  }
 #pragma unroll
   for (int c = 0; c < 4; ++c) asm volatile("" ::"v"(qreg[c]));  // waits for Q here, not in the loop
   if constexpr (kCodes)
