@@ -903,7 +903,7 @@ constexpr float kRescale = 8.0f;
 // then converts them to bf16 into the other stage, once for the four waves; the tile's four scales
 // enter as in paged_codes_item. (Held in registers during the step the codes spilled 4 to 40 of
 // those: prompts of 1500-4096 tokens in int8 106 us.) The codes are there when a step ends (8 clocks of waiting); prompts of
-// 1500-4096 tokens, 12 heads 75 us, 560 TFLOP/s, bound by VALU work: exponentials, and ~50 instructions of
+// 1500-4096 tokens, 12 heads 74 us, 565 TFLOP/s, bound by VALU work: exponentials, and ~50 instructions of
 // conversion a wave and tile. 24 sequences of 500-4000 keys, 32 tokens, 12 heads on 4: 23 us, 284 items of 3.5 us start-up
 // and 3-6 steps of 1.4 us, the last of those that share a CU.
 template <int SUBS, int POOL>
