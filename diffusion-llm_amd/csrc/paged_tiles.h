@@ -44,6 +44,7 @@ constexpr int kQT = 32;       // rows of the 32-row tile
 constexpr int kSub = 32;      // keys per wave step
 constexpr int kStride = 72;   // padded LDS row (bf16)
 constexpr int kMergeRow = kHeadDim + 4;
+constexpr float kRescale = 8.0f;  // log2: growth of a running maximum that is let pass
 
 __device__ __attribute__((aligned(128))) uint16_t zero_row[kHeadDim];
 
@@ -697,11 +698,12 @@ constexpr int codes_stage = RT == 2 ? 2 : 1;
 // gives (16 hq + 8 c + e), which Q's operand takes as well. A chunk's codes are converted once for all RT
 // row tiles. Its scales enter with the softmax: K's with the factor, V's in the exponent, so that what is
 // rounded to bf16 is P times it; the row sum takes its inverse again, once for 4 of the elements. (log2 scale - maximum
-// is off by 2^-24 of the maximum, no more than the scores' own fp32 sums.)
-// 16 rows: 4 waves where many items are bound by HBM (32 sequences of 100-8192 keys, 12 heads: 27 us, 4.3 TB/s of
+// is off by 2^-24 of the maximum, no more than the scores' own fp32 sums.) The running maximum is updated when it grew by more
+// than kRescale: among 16 rows some maximum grows in most chunks (lists 28.1 -> 27.3 us, 12 sequences of 32 rows 15.4 -> 14.9).
+// 16 rows: 4 waves where many items are bound by HBM (32 sequences of 100-8192 keys, 12 heads: 26 us, 4.4 TB/s of
 // codes, of which 5.5 us until the first are there; 48 of 8192 keys 110, 5.6 TB/s), 8 for few, long ones. 32
 // and 48 rows: a conversion serves 2 or 3 row tiles, one wave a SIMD at 64-key chunks (209 and 253 registers); lists of 40
-// pages of 32, 280 items: 28.1 us with 48 rows, 33 with 32; bound by what one wave issues (48 products,
+// pages of 32, 280 items: 27.3 us with 48 rows, 33 with 32; bound by what one wave issues (48 products,
 // ~400 VALU instructions a chunk). Codes stay bytes in LDS because a bf16 tile would be twice the writes
 // and the room of half the waves (the first form, 32-key chunks staged in bf16: batch 50.6 -> 37 us).
 template <int NW, int RT, int KC, int POOL, bool COLS>
@@ -785,7 +787,7 @@ __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const Paged
 #pragma unroll
       for (int g = 0; g < kG; ++g) mt = fmaxf(mt, fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3])) * c2[g]);
       mt = max_xor16_32(mt);
-      if (__ballot(mt > m[t]) != 0) {
+      if (__ballot(mt > m[t] + kRescale) != 0) {
         const float mn = fmaxf(m[t], mt);
         const float alpha = (mn == -INFINITY) ? 1.f : fast_exp2(m[t] - mn);
         m[t] = mn;
@@ -897,8 +899,6 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
 // chain, ~1 us for a workgroup alone on its CU: three and four stages only cost
 // occupancy (84 -> 95-107 us for prompts of 1507-4034 tokens, 28.5 -> 31-37 for 96 rows
 // over 727-3871 keys).
-constexpr float kRescale = 8.0f;
-
 // 8-bit pools: each wave loads the codes of its 16 keys to LDS during the step on the tile before,
 // then converts them to bf16 into the other stage, once for the four waves; the tile's four scales
 // enter as in paged_codes_item. (Held in registers during the step the codes spilled 4 to 40 of
