@@ -107,7 +107,7 @@ def paged_attention_pool(
 
     8-bit pages hold codes, value = scale * code with a scale for each 16 slots and
     head (paged_attention_inputs8 writes them); the scales of blocks that hold keys must
-    be finite and at least 2 ** -100. Codes enter the products exactly, scales multiply
+    be finite and at least 2 ** -100 (and values below about 2 ** 100: the sums over keys are fp32). Codes enter the products exactly, scales multiply
     scores and probabilities in fp32: the result is as near to the values as
     paged_attention's is to its bf16 ones.
 

@@ -395,7 +395,8 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
  * pages hold. With BD3_POOL_INT8 or BD3_POOL_E4M3 (OCP e4m3, finite codes) an
  * element is a code, and each 16 slots (16 i .. 16 i + 15 of a page) of a KV head share
  * an fp32 scale, value = scale * code: k_scales, v_scales (pages, kv_heads, page_size /
- * 16), contiguous; those of blocks that hold keys must be finite and at least 2^-100. Strides of such
+ * 16), contiguous; those of blocks that hold keys must be finite and at least 2^-100 (and values
+ * below about 2^100: the sums over keys are fp32). Strides of such
  * pages are multiples of 16. BD3_POOL_BF16: the pools of bd3_paged_attn, scales NULL.
  */
 #define BD3_POOL_BF16 0
