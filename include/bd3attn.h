@@ -434,7 +434,7 @@ int bd3_paged_attn_pool(const void* q, const void* k_pages, const void* v_pages,
  * max|x| / 127 (int8) or the least power of two with 448 scale >= max|x| (e4m3), at least
  * 2^-100. In a block that holds earlier tokens of the sequence the scale stays, or grows
  * by the least power of two 2^k with which the new values fit; then the block's
- * other codes become round(code / 2^k). code = round(x / scale), ties to even, x the fp32
+ * other codes become round(code / 2^k). code = round(x / scale), the quotient in fp32, ties to even, x the fp32
  * rotated key or the value. Values must be finite (an infinite one counts as the largest
  * finite one). Blocks are written whole, so no two sequences of a call may write into
  * one. Strides of the pages are multiples of 16.
