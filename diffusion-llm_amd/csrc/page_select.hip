@@ -138,14 +138,15 @@ struct ColumnScores {
   struct Box {
     bf16x8 x[4];          // high, low: the same channels
   };
-  float most;             // largest sum of absolute values so far (of the lane's columns)
+  int ranked_from, ranked_to;  // columns that are not always taken
+  float most;             // largest sum of absolute values so far (of the lane's ranked columns)
 
   __device__ __forceinline__ ColumnScores(const SelectArgs& s, const PagedSeq& sq, const QueryBlock& blk, int h_)
       : h(h_), rows((blk.hi - blk.lo) * s.p.group), row0(blk.lo * s.p.group),
         q(s.p.q + (int64_t)sq.q0 * s.p.sq_t + (int64_t)(h_ * s.p.group) * s.p.sq_h),
         bounds(s.bounds + (int64_t)h_ * (2 * kHeadDim)), sq_t(s.p.sq_t), sq_h(s.p.sq_h),
         page_step((int64_t)s.p.kv_heads * (2 * kHeadDim)), pages(s.p.pages), group(s.p.group), group_div(s.p.group_div),
-        lane(wi_x() & 63), most(0.f) {
+        lane(wi_x() & 63), ranked_from(s.first), ranked_to(blk.own - s.recent), most(0.f) {
     const uint16_t* qp = row(0);
     q0 = ld16(qp);
     q1 = ld16(qp + 32);
@@ -166,18 +167,23 @@ struct ColumnScores {
     for (int c = 0; c < 4; ++c) b.x[c] = __builtin_bit_cast(bf16x8, ld16(bp + (c < 2 ? kHeadDim : 0) + 32 * (c & 1)));
     return b;
   }
-  __device__ __forceinline__ static bf16x8 size(bf16x8 x) {
-    return __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, x) & 0x7fff7fffu);
+  __device__ __forceinline__ static bf16x8 size(bf16x8 x, uint32_t bits = 0x7fff7fffu) {
+    return __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, x) & bits);
   }
-  __device__ __forceinline__ float scores(const Box& box) {
+  // The bounds of a column that is not ranked (always taken, or without a page) count as zeros in the sums of absolute
+  // values: they are no part of any error, and may be anything (a large first page, bounds not formed yet, page 0).
+  // Those past the last column are not ranked either.
+  __device__ __forceinline__ float scores(const Box& box, int col, int page) {
     float best = -INFINITY;
+    const bool ranked = col >= ranked_from && col < ranked_to && (unsigned)page < (unsigned)pages;
+    const uint32_t bits = ranked ? 0x7fff7fffu : 0u;
     const auto add = [&](u32x4 x0, u32x4 x1) {
       const bf16x8 part[4] = {positive(x0), positive(x1), negative(x0), negative(x1)};
       f32x4 acc = {}, sum = {};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         acc = mfma16(part[c], box.x[c], acc);
-        sum = mfma16(c < 2 ? part[c] : size(part[c]), size(box.x[c]), sum);
+        sum = mfma16(c < 2 ? part[c] : size(part[c]), size(box.x[c], bits), sum);
       }
       best = fmaxf(fmaxf(best, fmaxf(acc[0], acc[1])), fmaxf(acc[2], acc[3]));
       most = fmaxf(fmaxf(most, fmaxf(sum[0], sum[1])), fmaxf(sum[2], sum[3]));
@@ -190,7 +196,7 @@ struct ColumnScores {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(best), __float_as_uint(best), false, false);
     return max_xor32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
   }
-  // Bound of the scores' distance from the exact sums: 64 additions of terms that are not zeros, each off by at most
+  // Bound of the ranked scores' distance from the exact sums: 64 additions of terms that are not zeros, each off by at most
   // 2^-23 of the terms' absolute sum whatever their order and rounding; 2^-16 for 2^-17, which covers that sum's own.
   // And twice 128 terms and sums that may have lost 2^-126 each: below it numbers may lose their bits.
   __device__ __forceinline__ float error() const { return fmaf(wave_max(most), 0x1p-16f, 0x1p-118f); }
@@ -600,7 +606,7 @@ __global__ __launch_bounds__(64 * kPickWaves, 4) void page_pick_kernel(SelectArg
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int col = column(i + k);  // past the last one: no page, no key
-      const float score = c.scores(box[k]);
+      const float score = c.scores(box[k], col, page[k]);
       const uint32_t key = lane < 16 ? column_key(s, blk, col, page[k], score) : 0u;
       ask(i + k + kAhead, k);
       if (lane < 16 && col < blk.cols) keys[col] = key;
@@ -629,7 +635,7 @@ __global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs s, int chun
   const int col = col0 + l16 < blk.cols ? col0 + l16 : blk.cols - 1;
   const int page = a.table[(int64_t)it.b * a.table_s + col];
   ColumnScores c(s, it.sq, blk, it.h);
-  const float score = c.scores(c.load(page));
+  const float score = c.scores(c.load(page), col0 + l16, page);
   const float err = c.error();
   if (lane < 16) s.keys[(int64_t)jh * s.width + col0 + lane] = column_key(s, blk, col0 + lane, page, score);
   if (lane == 0) s.error[(int64_t)jh * (s.width >> 4) + (col0 >> 4)] = err;

@@ -196,8 +196,8 @@ def select_pages(
 
     which no key of the page exceeds in q . k (of 8-bit pages but for the bounds' rounding to bf16); equals by the lower column. The
     scores' order is exact. `top` must leave room for the columns always taken. Rows behind the last
-    sequence are left as they are (without `out` undefined). Bounds of the columns always taken are
-    not read; those of the others must be finite."""
+    sequence are left as they are (without `out` undefined). Bounds of the columns always taken may
+    be anything; those of the others must be finite."""
     return host().select_pages(q, bounds, page_table, q_starts, kv_lens, block_size, page_size, top, max_q,
                                -1 if max_kv is None else max_kv, first, recent, out)
 

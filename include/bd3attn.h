@@ -480,7 +480,8 @@ int bd3_page_bounds(const void* k_pages, const float* k_scales, int32_t pool_typ
  * behind the last sequence, and of tokens beyond max_q, stay as they are; a token before
  * position 0 gets none.
  *   q: (tokens, heads, 64) bf16; bounds: (pages, kv_heads, 2, 64) bf16, contiguous, as
- *     bd3_page_bounds writes them; finite. strides: q (token, head), page_table (row).
+ *     bd3_page_bounds writes them; finite, but for the columns always taken, whose bounds may be anything.
+ *     strides: q (token, head), page_table (row).
  * Preconditions: top >= first + recent + the most columns that a block can lie in
  * (within max_kv). workspace: bd3_select_pages_workspace_bytes of the same arguments
  * (0 up to 256 columns, and up to 2048 of many blocks).
