@@ -226,6 +226,8 @@ class PagedKVCache:
             self.v_scales = torch.zeros_like(self.k_scales)
         if bounds:
             self.bounds = torch.zeros((*shape[:3], 2, D), device=device, dtype=torch.bfloat16)
+        # of each layer: how many of a sequence's first tokens the bounds of its pages cover
+        self._bounded: list[dict[int, int]] = [{} for _ in range(n_layers)]
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages: dict[int, list[int]] = {}
         self._length: dict[int, int] = {}
@@ -255,6 +257,8 @@ class PagedKVCache:
         still runs on them must be before it in stream order."""
         self._free.extend(reversed(self._pages.pop(seq)))
         del self._length[seq]
+        for covered in self._bounded:
+            covered.pop(seq, None)
 
     def batch(self, seqs: list[int], new_tokens: list[int]) -> "PagedBatch":
         """One step of these sequences, new_tokens[i] tokens of seqs[i] after its
@@ -293,6 +297,9 @@ class PagedBatch:
         n = len(seqs)
         self.q_starts, self.kv_lens = data[:n + 1], data[n + 1:2 * n + 1]
         self.page_table = data[2 * n + 1:].view(n, width)
+        self._committed = False
+        self._formed: set[int] = set()  # layers whose bounds cover this step
+        self._checked: set[tuple] = set()  # selections whose bounds are known to be there
 
     def attention_inputs(self, qkv: Tensor, n_heads: int, sin_table: Tensor, cos_table: Tensor, layer: int,
                          out: Tensor | None = None) -> Tensor:
@@ -311,15 +318,52 @@ class PagedBatch:
         assert c.bounds is not None, "the cache keeps no bounds: PagedKVCache(..., bounds=True)"
         page_bounds(c.k_pages[layer], c.bounds[layer], self.page_table, self.q_starts, self.kv_lens, self.tokens,
                     c.scales(layer)[0])
+        self.bounds_formed(layer)
+
+    def bounds_formed(self, layer: int) -> None:
+        """Count this step's bounds in a layer as formed, as update_bounds does. For a caller whose replayed graph, or
+        page_bounds itself, formed them."""
+        self._formed.add(layer)
+        if self._committed:
+            self._count_bounds(layer)
+
+    def _covers(self, layer: int, seq: int, start: int) -> bool:
+        """Whether the pages before the one that holds position `start` have their bounds."""
+        page = self.cache.page_size
+        return self.cache._bounded[layer].get(seq, 0) >= start // page * page
+
+    def _count_bounds(self, layer: int) -> None:
+        c = self.cache
+        for s, n, kv in zip(self.seqs, self.new_tokens, self.lens):
+            if n > 0 and s in c._length and self._covers(layer, s, kv - n):
+                c._bounded[layer][s] = kv  # less than before if later tokens are there: the last page was formed without them
+
+    def _check_bounds(self, layer: int, block_size: int, top: int, first: int, recent: int) -> None:
+        """The pages that the last block of each sequence ranks, and earlier ones a part of, have bounds over all of their keys."""
+        c = self.cache
+        for s, n, kv in zip(self.seqs, self.new_tokens, self.lens):
+            if n == 0 or -(-kv // c.page_size) <= top:
+                continue
+            ranked = (kv - 1) // block_size * block_size // c.page_size - recent  # [first, ranked)
+            have = kv if layer in self._formed and self._covers(layer, s, kv - n) else c._bounded[layer].get(s, 0)
+            assert ranked <= first or have >= ranked * c.page_size, \
+                f"layer {layer}, sequence {s}: page bounds cover {have} of the {ranked * c.page_size} tokens whose pages are to be " \
+                "ranked: update_bounds in every step that is committed, and before a step of several blocks selects"
 
     def attention(self, q: Tensor, layer: int, block_size: int, out: Tensor | None = None, top: int | None = None,
                   first: int = 1, recent: int = 1) -> Tensor:
         """paged_attention over this layer's pages; with `top` over those that select_pages
-        takes by the cache's bounds."""
+        takes by the cache's bounds, refused (AssertionError) while bounds that it ranks by have not been formed
+        (update_bounds)."""
         c = self.cache
         columns = None
         if top is not None:
             assert c.bounds is not None, "the cache keeps no bounds: PagedKVCache(..., bounds=True)"
+            asked = layer, block_size, top, first, recent
+            if asked not in self._checked:
+                if block_size >= 1:  # else the call refuses it
+                    self._check_bounds(*asked)
+                self._checked.add(asked)
             columns = select_pages(q, c.bounds[layer], self.page_table, self.q_starts, self.kv_lens, block_size,
                                    c.page_size, top, self.max_q, self.max_kv, first, recent)
         return paged_attention_pool(q, c.k_pages[layer], c.v_pages[layer], self.page_table, self.q_starts, self.kv_lens,
@@ -333,3 +377,6 @@ class PagedBatch:
             assert c._length.get(s) == kv - n, "the sequence has moved on since this batch was made"
         for s, kv in zip(self.seqs, self.lens):
             c._length[s] = kv
+        self._committed = True
+        for layer in self._formed:
+            self._count_bounds(layer)
