@@ -112,9 +112,10 @@ def paged_attention_pool(
     paged_attention's is to its bf16 ones.
 
     With `columns` the tokens of one block of block_size positions read, as far as they see them,
-    only the pages in the table's columns columns[first of them in the chunk, KV head]. No column may
-    occur twice, so of a list only as many entries are read as the sequence has columns with keys;
-    entries that are none of these (-1) name nothing."""
+    only the pages in the table's columns columns[first of them in the chunk, KV head]. Of a list the
+    first ceil(length / page_size) places are read (the sequence has no more columns with keys, and none
+    may occur twice): a column behind them is not, also where some of them hold none. An entry that is no
+    column that the block sees (-1) names nothing."""
     return host().paged_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, block_size, max_q,
                                   -1 if max_kv is None else max_kv, -1 if total_kv is None else total_kv, out,
                                   k_scales, v_scales, columns)

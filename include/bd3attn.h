@@ -410,9 +410,10 @@ int bd3_paged_qkv_rope(const void* qkv, const float* sin_table, const float* cos
  *   columns: NULL, or device int32 (tokens, kv_heads, top), last stride 1: lists of
  *     columns of the page table. The tokens of one block of block_size positions read, for
  *     the heads of KV head h, only the keys in columns[first token of the block
- *     in its chunk][h][...], as far as they see them. No column may occur twice, so of
- *     a list only as many entries are read as the sequence has columns with keys; entries
- *     outside those that the block sees (-1) name nothing.
+ *     in its chunk][h][...], as far as they see them. Of a list the first ceil(kv_len /
+ *     page_size) places are read (the sequence has no more columns with keys, and none may
+ *     occur twice): a column behind them is not, also where some of them hold none. Entries
+ *     outside the columns that the block sees (-1) name nothing.
  *   strides: bd3_paged_attn's 11, then columns (token, KV head).
  * The workspace is bd3_paged_attn_pool_workspace_bytes of the same arguments (top 0: no
  * columns). Everything else as for bd3_paged_attn. No reference counterpart.

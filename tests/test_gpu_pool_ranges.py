@@ -1,4 +1,4 @@
-"""Lengths and starts out of range against the definitions over what they are bounded to."""
+"""Lengths and starts out of range, and lists past the places that are read, against the definitions over what counts of them."""
 from __future__ import annotations
 
 import pytest
@@ -90,3 +90,22 @@ def test_bounds_and_selections_of_such_batches(cuda, dtype, seqs, chunk):
     out = torch.full((T, 1, 8), -2, dtype=torch.int32, device=cuda)
     select_pages(d["q"], bounds, d["table"], d["starts"], d["kv"], 16, page, 8, chunk, most, out=out)
     assert torch.equal(out.cpu(), orc.select_pages(c["q"], want, c["table"], c["starts"], c["kv"], 16, page, 8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", POOLS)
+@pytest.mark.parametrize("chunk", [1, 16, 48])
+def test_lists_are_read_as_far_as_the_sequence_has_columns(cuda, record_error, dtype, chunk):
+    """Three columns: the first three places are read, whatever stands there. A column behind them is not."""
+    page, max_kv, bs = 16, 48, 48
+    c = full_case(dtype, 2, chunk, 2, 1, page, max_kv, seed=chunk)
+    c["starts"], c["kv"] = torch.tensor([0, chunk, 2 * chunk], dtype=torch.int32), torch.tensor([48, 48], dtype=torch.int32)
+    c["q"] = torch.cat([c["q"][:chunk], c["q"][:chunk]])
+    for row in ([-1, -1, 0, 1, 2], [2, -1, 1, 0, -1], [-1, -1, -1, 0, 1], [0, 1, 2, -1, -1], [1, 7, 1 << 29, 0, 2], [-1, 2, -5, 2, 2]):
+        columns = torch.tensor(row, dtype=torch.int32).expand(2 * chunk, 1, 5).contiguous()
+        ref, tol = pool_reference(c, bs, columns)
+        read = torch.tensor(row[:3] + [-1, -1], dtype=torch.int32).expand(2 * chunk, 1, 5).contiguous()
+        assert torch.equal(pool_reference(c, bs, read)[0], ref), "the definition"
+        o = attend(c, cuda, bs, chunk, max_kv, 96, columns)
+        record_error("lists' places / bound", worst(o, ref, tol), 1.0)
+        assert (o == 0).all() == (row[:3] == [-1, -1, -1])
