@@ -367,8 +367,9 @@ class PagedBatch:
                 self._checked.add(asked)
             columns = select_pages(q, c.bounds[layer], self.page_table, self.q_starts, self.kv_lens, block_size,
                                    c.page_size, top, self.max_q, self.max_kv, first, recent)
-        return paged_attention_pool(q, c.k_pages[layer], c.v_pages[layer], self.page_table, self.q_starts, self.kv_lens,
-                                    block_size, self.max_q, self.max_kv, self.total_kv, out, *c.scales(layer), columns)
+        k_scales, v_scales = c.scales(layer)
+        return host().paged_attention(q, c.k_pages[layer], c.v_pages[layer], self.page_table, self.q_starts, self.kv_lens,
+                                      block_size, self.max_q, self.max_kv, self.total_kv, out, k_scales, v_scales, columns)
 
     def commit(self) -> None:
         """Count the step's tokens as committed, in every layer. Once a batch,
