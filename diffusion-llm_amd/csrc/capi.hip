@@ -927,7 +927,8 @@ static_assert(kPagedPartRows * bd3::kHeadDim <= INT32_MAX, "32-bit indices of th
 //
 // 8-bit pools and lists have their own, fitted to 2200 batches of 8-bit pools and 400 of lists drawn the same way (16 rows: to
 // 860, whose constants choose better where the lengths differ, 0.9% above the best plan instead of 1.1): rms error
-// 9-12%. Over 1100 others the plan takes 1.0% more than the best of all plans on average for up to 16 rows, 1.3-3.2%
+// 9-12%. Over 1100 others the plan takes 1.0% more than the best of the plans tried (every tile, set and range of a power of
+// two) on average for up to 16 rows, 1.3-3.2%
 // for more (at worst 45%), over lists 2.3% (bf16 pools 1.4%; at worst 32%). Without the kernel of one set of
 // four waves 16 rows take 2.1%, of two 4.3%; without one of the 32-row ones 33-64 rows 6.5 and 7.9%; without
 // 48 rows lists of more than 256 10% instead of 7.8%; without one, two or four sets of 128 rows whole prompts 5.4, 5.2

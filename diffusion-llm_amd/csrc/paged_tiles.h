@@ -702,10 +702,11 @@ constexpr int codes_stage = RT == 2 ? 2 : 1;
 // than kRescale: among 16 rows some maximum grows in most chunks (lists 28.1 -> 27.3 us, 12 sequences of 32 rows 15.4 -> 14.9).
 // 16 rows: 4 waves where many items are bound by HBM (32 sequences of 100-8192 keys, 12 heads: 26 us, 4.4 TB/s of
 // codes, of which 5.5 us until the first are there; 48 of 8192 keys 110, 5.6 TB/s), 8 for few, long ones. 32
-// and 48 rows: a conversion serves 2 or 3 row tiles, one wave a SIMD at 64-key chunks (209 and 253 registers); lists of 40
-// pages of 32, 280 items: 27.3 us with 48 rows, 33 with 32; bound by what one wave issues (48 products,
-// ~400 VALU instructions a chunk). Codes stay bytes in LDS because a bf16 tile would be twice the writes
-// and the room of half the waves (the first form, 32-key chunks staged in bf16: batch 50.6 -> 37 us).
+// and 48 rows: a conversion serves 2 or 3 row tiles, at most two waves a SIMD at 64-key chunks (209 and 253 registers);
+// lists of 40 pages of 32, 340 items: 27.3 us with 48 rows, 33 with 32. An item is 5 us until its first chunk is there (2.9 to
+// find it and the end of its list), a chunk 2.9 us (48 products, ~650 VALU instructions, 805 where it is masked), the merge 2; on
+// the 84 CUs that have two a chunk is 3.8, and these end last. Eight waves of 32-key chunks took 38 us, four 29. Codes stay bytes
+// in LDS because a bf16 tile would be twice the writes and the room of half the waves (the first form, 32-key chunks staged in bf16: batch 50.6 -> 37 us).
 template <int NW, int RT, int KC, int POOL, bool COLS>
 __device__ __forceinline__ void paged_codes_item(const PagedArgs& a, const PagedItem<false, COLS>& it, char* smem) {
   using Stream = CodeStream<NW, KC, POOL, COLS>;
@@ -905,7 +906,8 @@ __global__ __launch_bounds__(NW * 64, ROWS == 16 ? 4 : NW == 4 ? 3 : 2) void pag
 // those: prompts of 1500-4096 tokens in int8 106 us.) The codes are there when a step ends (8 clocks of waiting); prompts of
 // 1500-4096 tokens, 12 heads 74 us, 565 TFLOP/s, bound by VALU work: exponentials, and ~50 instructions of
 // conversion a wave and tile. 24 sequences of 500-4000 keys, 32 tokens, 12 heads on 4: 23 us, 284 items of 3.5 us start-up
-// and 3-6 steps of 1.4 us, the last of those that share a CU.
+// and 3-6 steps of two tiles, 2.0 us each where the workgroup has its CU alone: most are done after 13 us, those of 5 and 6 steps
+// on the 28 CUs that have two (up to 3.4 us a step) after 17-21.
 template <int SUBS, int POOL>
 __global__ __launch_bounds__(256 * SUBS, 4) void paged128_kernel(PagedArgs a) {
   constexpr bool kCodes = POOL != kPoolBf16;
