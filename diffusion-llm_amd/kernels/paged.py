@@ -324,6 +324,7 @@ class PagedBatch:
     def bounds_formed(self, layer: int) -> None:
         """Count this step's bounds in a layer as formed, as update_bounds does. For a caller whose replayed graph, or
         page_bounds itself, formed them."""
+        layer = range(len(self.cache._bounded))[layer]  # -1: the last one, as for the tensors
         self._formed.add(layer)
         if self._committed:
             self._count_bounds(layer)
@@ -360,7 +361,7 @@ class PagedBatch:
         columns = None
         if top is not None:
             assert c.bounds is not None, "the cache keeps no bounds: PagedKVCache(..., bounds=True)"
-            asked = layer, block_size, top, first, recent
+            asked = range(len(c._bounded))[layer], block_size, top, first, recent
             if asked not in self._checked:
                 if block_size >= 1:  # else the call refuses it
                     self._check_bounds(*asked)

@@ -132,3 +132,14 @@ def test_every_sequence_counts():
     assert select(c.batch([a, b], [1, 0])), "no tokens, no selection"
     short = c.add()
     assert select(c.batch([a, short], [1, 40]))
+
+
+def test_layers_are_counted_from_either_end():
+    c = cache()
+    a = c.add()
+    batch = step(c, [a], [200], formed=(-1,), commit=False)
+    assert select(batch, 1, bs=16) and select(batch, -1, bs=16) and not select(batch, 0, bs=16) and not select(batch, -2, bs=16)
+    batch.commit()
+    assert select(c.batch([a], [1]), 1) and not select(c.batch([a], [1]), 0)
+    with pytest.raises(IndexError):
+        batch.bounds_formed(2)
